@@ -76,8 +76,8 @@ enum {
     FTX_BF16 = 30
 };
 
-/* KV element types */
-enum { FTX_KV_F32 = 0, FTX_KV_F16 = 1 };
+/* KV element types (FTX_KV_Q8: paged caches only) */
+enum { FTX_KV_F32 = 0, FTX_KV_F16 = 1, FTX_KV_Q8 = 2 };
 
 /* acceptance modes */
 enum {
@@ -90,6 +90,8 @@ typedef struct ftx_ctx ftx_ctx;
 typedef struct ftx_tensor ftx_tensor;
 typedef struct ftx_model ftx_model;
 typedef struct ftx_kv ftx_kv;
+typedef struct ftx_pool ftx_pool;
+typedef struct ftx_plan ftx_plan;
 
 typedef struct {
     char name[64];
@@ -347,6 +349,90 @@ int ftx_accept_batch(ftx_ctx* ctx, const ftx_accept_args* args, int n);
  * Synchronous (the host needs the token for the next step); prob may be
  * NULL. */
 int ftx_argmax_prob(ftx_ctx* ctx, const float* row, int64_t V, int32_t* token, float* prob);
+
+/* ---- paged KV caches (no counterpart in the reference, whose KvCache is one
+ * contiguous fp16 array, include/ft/kv_cache.h:10-47) ----
+ *
+ * A pool holds pages of FTX_PAGE tokens, each with the K and V rows of every
+ * layer; a sequence is a table of pages, position p in slot p % FTX_PAGE of
+ * page table[p / FTX_PAGE].  What a row (head_dim values of one token and kv
+ * head, a = its largest magnitude) stands for once stored:
+ *   FTX_KV_F16  half(x 2^-e) 2^e, e = 0 for 2^-8 <= a <= 65504, else
+ *               e = ilogb(a) - 14 (no value overflows, rows of small values
+ *               keep 11 bits)
+ *   FTX_KV_Q8   q s with the scale s = float(a / 127) and q = 127 x / a
+ *               rounded to the nearest integer, ties to even
+ * A row with a < 2^-100 is stored as zeros; one that holds an infinity or a
+ * NaN is NaN in every element. */
+enum { FTX_PAGE = 64 };
+/* n_pages (<= 2^24) pages for n_layer layers of n_head_kv heads; head_dim 64,
+ * 128 or 256; kv_dtype FTX_KV_F16 or FTX_KV_Q8. */
+int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t head_dim,
+                    int64_t n_pages, int kv_dtype, ftx_pool** out);
+/* Frees the pool; FTX_E_INVALID while a plan or a paged cache of it lives. */
+int ftx_pool_free(ftx_pool* p);
+/* Pages not taken. */
+int64_t ftx_pool_available(const ftx_pool* p);
+/* Take n free pages (lowest ids first) / give taken pages back.  FTX_E_NOMEM
+ * when fewer are free (nothing is taken then); FTX_E_INVALID for a page that
+ * is not taken or named twice (nothing is given then).  Host bookkeeping
+ * only: contents stay. */
+int ftx_pool_take(ftx_pool* p, int64_t n, int32_t* pages);
+int ftx_pool_give(ftx_pool* p, const int32_t* pages, int64_t n);
+
+/* One sequence of a step: npast tokens in its pages, M new ones at positions
+ * npast .. npast + M - 1 (a chain), or a draft tree: parents as in
+ * ftx_verify_args (M <= 256), node i at position npast + depth(i), in slot
+ * npast + i. */
+typedef struct {
+    const int32_t* pages;    /* host: the sequence's pages in order; -1: absent */
+    int64_t n_pages;         /* >= (npast + M) / FTX_PAGE, rounded up */
+    int64_t npast;
+    int64_t M;               /* >= 0 */
+    const int32_t* parents;  /* host [M] or NULL (chain) */
+} ftx_paged_seq;
+typedef struct {
+    const ftx_paged_seq* seqs;  /* host */
+    int64_t nseq;               /* 1 .. 65535 */
+    int64_t n_head;             /* query heads, a multiple of the pool's; 0: no attention */
+    /* window > 0: a token at position p sees the positions above p - window
+     * and the first `sinks` ones only.  0: all before it */
+    int64_t window, sinks;
+} ftx_plan_args;
+/* What the calls of one step share, for every layer: tables, masks and the
+ * division of the attention's work, checked here and copied to the device
+ * (stream-ordered).  Every page must be taken; a page that new tokens go to
+ * may occur once in all tables (pages that are only read may be shared);
+ * pages that no new token sees may be absent.  ftx_plan_set gives the plan
+ * another step's sequences; on an error the plan keeps the old ones, except
+ * that after FTX_E_NOMEM and FTX_E_DEVICE it has none. */
+int ftx_plan_create(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args* a, ftx_plan** out);
+int ftx_plan_set(ftx_plan* pl, const ftx_plan_args* a);
+int ftx_plan_free(ftx_plan* pl);
+
+/* The calls below enqueue on the context's stream and take device memory;
+ * row n of a matrix is ld floats (0: dense) after row n - 1.  They may be
+ * recorded into a HIP graph; ftx_plan_set is then refused for that plan, and
+ * the plan, its pool and the matrices must outlive the graph.  Calls of one
+ * plan share its workspace: they must not overlap. */
+
+/* Store the new tokens' k and v rows ([sum of M][n_head_kv * head_dim],
+ * sequence after sequence) of a layer in their pages. */
+int ftx_paged_write(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v,
+                    int64_t ldv);
+/* Read back what rows stand for, fp32: the new tokens' rows (context = 0), or
+ * positions 0 .. npast + M - 1 of every sequence (context = 1; FTX_E_RANGE
+ * where a page of them is absent). */
+int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v,
+                   int64_t ldv);
+/* out[n][h] = sum_j softmax_j(q[n][h] . k_j / sqrt(head_dim)) v_j over the
+ * slots that new token n sees (its own among them: ftx_paged_write first), kv
+ * head h / (n_head / n_head_kv).  q, out: [sum of M][n_head * head_dim], not
+ * overlapping.  Error against 64 bits some 2^-21 of sum_j p_j |v_j|, plus
+ * 2^-38 of the largest |v_j| for each slot seen.  Rows past the last token stay as they
+ * are. */
+int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out,
+                        int64_t ldo);
 
 /* ---- kernel trace (the reference keeps wall-clock RunStats only,
  * include/ft/engine.h:25-39) ---- */

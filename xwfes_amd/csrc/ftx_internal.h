@@ -30,6 +30,7 @@ enum TraceKind {
     TK_XQ_PREP,
     TK_MOE_ROUTE,
     TK_MOE_COMBINE,
+    TK_PAGED_KV,    // rows into and out of pages
     TK_EVENT_PAIR,  // empty event brackets: the brackets' own time
     TK_COUNT
 };

@@ -1,0 +1,578 @@
+// paged.hip -- paged KV caches: the page pool, a step's plan and the C ABI's
+// calls over them (include/ftx.h).  The kernels are in k_paged.hip.
+#include "paged.h"
+
+#include <algorithm>
+#include <cstdio>
+#include <new>
+
+#include "paged_pool.h"
+
+// ---------------------------------------------------------------- plan tables
+
+int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_t>& mark,
+                 uint32_t& epoch, PagedTables& o, std::string& err) {
+    auto fail = [&](int code, const char* what) {
+        err = std::string("plan: ") + what;
+        return code;
+    };
+    o = PagedTables{};
+    if (!a.seqs) return fail(FTX_E_INVALID, "null argument");
+    if (a.nseq < 1 || a.nseq > 65535) return fail(FTX_E_INVALID, "nseq out of range (1 .. 65535)");
+    if (a.n_head < 0 || a.n_head % g.n_kv || a.n_head > 65535)
+        return fail(FTX_E_INVALID, "n_head must be a multiple of the pool's kv heads");
+    if (a.window < 0 || a.sinks < 0) return fail(FTX_E_INVALID, "negative window or sinks");
+    // (positions stay below 2^30)
+    constexpr int64_t FAR = (int64_t)1 << 30;
+    const int64_t W = std::min(a.window, FAR), sinks = W ? std::min(a.sinks, FAR) : 0;
+    o.n_head = a.n_head;
+    o.window = W;
+    o.sinks = sinks;
+    if ((int64_t)mark.size() != g.n_pages) mark.assign((size_t)g.n_pages, 0u);
+    if (epoch >= 0xFFFFFFF0u) {
+        std::fill(mark.begin(), mark.end(), 0u);
+        epoch = 0;
+    }
+    // marks of this call: named once / written / written and named
+    const uint32_t named = epoch + 1, written = epoch + 2;
+    epoch += 2;
+    const int64_t gqa = a.n_head / g.n_kv;
+    for (int64_t s = 0; s < a.nseq; ++s) {
+        const ftx_paged_seq& q = a.seqs[s];
+        if (q.npast < 0 || q.M < 0 || q.npast > FAR || q.M > FAR || q.npast + q.M > FAR)
+            return fail(FTX_E_RANGE, "npast and M must be >= 0, npast + M <= 2^30");
+        if (q.parents && q.M > 256) return fail(FTX_E_INVALID, "a draft tree has at most 256 nodes");
+        const int64_t ntab = (q.npast + q.M + FTX_PAGE - 1) / FTX_PAGE;
+        if (q.n_pages < ntab || (ntab && !q.pages))
+            return fail(FTX_E_INVALID, "too few pages for npast + M");
+        PagedSeq d{};
+        d.npast = (int32_t)q.npast;
+        d.M = (int32_t)q.M;
+        d.tok0 = (int32_t)o.tokens;
+        d.tab0 = (int32_t)o.table.size();
+        d.ntab = (int32_t)ntab;
+        d.dep0 = -1;
+        d.all0 = o.rows;
+        o.tokens += q.M;
+        o.rows += q.npast + q.M;
+        if (o.tokens * std::max<int64_t>(a.n_head, 1) >= (int64_t)1 << 31 ||
+            (int64_t)o.table.size() + ntab >= (int64_t)1 << 31)
+            return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
+        const int64_t first_new = q.M ? q.npast / FTX_PAGE : ntab;
+        for (int64_t i = 0; i < ntab; ++i) {
+            const int32_t pg = q.pages[i];
+            o.table.push_back(pg);
+            if (pg == -1) {
+                if (i >= first_new) return fail(FTX_E_INVALID, "a page of new tokens is absent");
+                o.absent = true;
+                continue;
+            }
+            if (pg < 0 || pg >= g.n_pages) return fail(FTX_E_RANGE, "page id out of range");
+            if (!g.taken[pg]) return fail(FTX_E_INVALID, "a page is not taken from the pool");
+            uint32_t& mk = mark[(size_t)pg];
+            if (mk == written || (mk == named && i >= first_new))
+                return fail(FTX_E_INVALID, "a page that new tokens go to occurs twice");
+            mk = i >= first_new ? written : named;
+        }
+        if (q.M) o.max_new_pages = std::max(o.max_new_pages, ntab - first_new);
+        o.max_pages = std::max(o.max_pages, ntab);
+        if (q.parents) {
+            d.dep0 = (int32_t)o.depth.size();
+            d.aw = (int32_t)((q.M + 31) / 32);
+            d.anc0 = (int32_t)o.anc.size();
+            o.anc.resize(o.anc.size() + (size_t)(q.M * d.aw), 0u);
+            uint32_t* anc = o.anc.data() + d.anc0;
+            for (int64_t i = 0; i < q.M; ++i) {
+                const int32_t p = q.parents[i];
+                if (p < -1 || p >= i) return fail(FTX_E_INVALID, "parents[i] must be in [-1, i)");
+                o.depth.push_back(p < 0 ? 0 : o.depth[(size_t)(d.dep0 + p)] + 1);
+                if (p >= 0) std::copy(anc + p * d.aw, anc + (p + 1) * d.aw, anc + i * d.aw);
+                anc[i * d.aw + i / 32] |= 1u << (i % 32);
+            }
+            // (the ancestors are complete: what the window hides goes last)
+            const int32_t* dep = o.depth.data() + d.dep0;
+            for (int64_t i = 0; W && i < q.M; ++i)
+                for (int64_t j = 0; j < i; ++j)
+                    if (dep[i] - dep[j] >= W && q.npast + dep[j] >= sinks)
+                        anc[i * d.aw + j / 32] &= ~(1u << (j % 32));
+        }
+        o.seqs.push_back(d);
+    }
+    if (a.n_head == 0) return FTX_OK;
+    // the row tiles and the pages each sees
+    struct Tile {
+        int32_t seq, row0, s, a, n;
+    };
+    std::vector<Tile> tiles;
+    int64_t total = 0;
+    for (int64_t s = 0; s < a.nseq; ++s) {
+        const PagedSeq& d = o.seqs[(size_t)s];
+        const int64_t R = d.M * gqa;
+        int64_t checked_s = 0, checked_a = d.ntab;  // pages seen so far: [0, checked_s), [checked_a, ..)
+        for (int64_t row0 = 0; row0 < R; row0 += PAGED_TR) {
+            const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + PAGED_TR) - 1) / gqa;
+            // (a tree's nodes are all looked at: a node's position is below its slot)
+            int64_t lo = 0;
+            if (W) lo = std::max<int64_t>(0, d.npast + (d.dep0 >= 0 ? 0 : t0) - W + 1);
+            const int64_t pa = lo / FTX_PAGE, pe = (d.npast + t1) / FTX_PAGE + 1;
+            const int64_t ps = std::min((sinks + FTX_PAGE - 1) / FTX_PAGE, pa);
+            tiles.push_back(Tile{(int32_t)s, (int32_t)row0, (int32_t)ps, (int32_t)pa, (int32_t)(ps + pe - pa)});
+            total += ps + pe - pa;
+            for (; checked_s < ps; ++checked_s)
+                if (o.table[(size_t)(d.tab0 + checked_s)] < 0)
+                    return fail(FTX_E_INVALID, "a page that a new token sees is absent");
+            for (; checked_a > pa; --checked_a)
+                if (o.table[(size_t)(d.tab0 + checked_a - 1)] < 0)
+                    return fail(FTX_E_INVALID, "a page that a new token sees is absent");
+        }
+    }
+    o.pages_read = (double)total;
+    // lists long enough to be split so that the launch has some four
+    // workgroups a CU, of at least four pages (one a wave)
+    const int64_t want = 4 * (int64_t)std::max(g.cu, 1);
+    const int64_t per = std::max<int64_t>(4, (total * g.n_kv + want - 1) / want);
+    for (const Tile& t : tiles) {
+        const int64_t np = (t.n + per - 1) / per;
+        for (int64_t k = 0; k < np; ++k)
+            o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
+                                        t.a, np > 1 ? (int32_t)(o.parts + k) : -1, 0});
+        if (np > 1) {
+            o.combs.push_back(PagedComb{t.seq, t.row0, (int32_t)o.parts, (int32_t)np});
+            o.parts += np;
+        }
+    }
+    if ((int64_t)o.items.size() * g.n_kv >= (int64_t)1 << 31 || o.parts >= (int64_t)1 << 31)
+        return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
+    // the longest first
+    std::stable_sort(o.items.begin(), o.items.end(),
+                     [](const PagedItem& x, const PagedItem& y) { return x.i1 - x.i0 > y.i1 - y.i0; });
+    return FTX_OK;
+}
+
+extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int64_t n_pages, const uint8_t* taken,
+                           int cu, PagedItem* items, int64_t* n_items, PagedComb* combs, int64_t* n_combs,
+                           int64_t max_out, char* msg, int64_t msg_bytes) {
+    try {
+        PagedGeom g;
+        g.n_kv = n_kv;
+        g.hd = hd;
+        g.n_pages = n_pages;
+        g.taken = taken;
+        g.cu = cu;
+        std::vector<uint32_t> mark;
+        uint32_t epoch = 0;
+        PagedTables t;
+        std::string err;
+        const int rc = paged_tables(g, *a, mark, epoch, t, err);
+        snprintf(msg, (size_t)msg_bytes, "%s", err.c_str());
+        if (rc) return rc;
+        *n_items = (int64_t)t.items.size();
+        *n_combs = (int64_t)t.combs.size();
+        if (*n_items > max_out || *n_combs > max_out) return FTX_E_RANGE;
+        std::copy(t.items.begin(), t.items.end(), items);
+        std::copy(t.combs.begin(), t.combs.end(), combs);
+        return FTX_OK;
+    } catch (...) {
+        return FTX_E_NOMEM;
+    }
+}
+
+// ---------------------------------------------------------------- pool and plan
+
+namespace {
+
+// the context's device made current for a scope
+struct OnDevice {
+    int prev = -1;
+    bool ok = true;
+    explicit OnDevice(int dev) {
+        if (hipGetDevice(&prev) != hipSuccess) prev = -1;
+        if (prev == dev) {
+            prev = -1;
+            return;
+        }
+        ok = hipSetDevice(dev) == hipSuccess;
+        if (!ok) (void)hipGetLastError();
+    }
+    ~OnDevice() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+};
+
+bool capturing(hipStream_t st) {
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &s) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return s != hipStreamCaptureStatusNone;
+}
+
+// device memory of the context's own device
+bool on_device(const ftx_ctx* ctx, const void* p) {
+    hipPointerAttribute_t at;
+    if (hipPointerGetAttributes(&at, p) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return (at.type == hipMemoryTypeDevice && at.device == ctx->device) || at.type == hipMemoryTypeManaged;
+}
+
+// No events of the trace go into a captured graph
+struct NoTrace {
+    ftx_ctx* ctx;
+    bool was;
+    NoTrace(ftx_ctx* c, bool off) : ctx(c), was(c->trace) { c->trace = was && !off; }
+    ~NoTrace() { ctx->trace = was; }
+};
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+}  // namespace
+
+struct ftx_plan {
+    ftx_ctx* ctx = nullptr;
+    ftx_pool* pool = nullptr;
+    PagedTables t;
+    bool ready = false;     // the device block holds t
+    bool captured = false;  // a graph holds calls of this plan
+    std::vector<uint32_t> mark;
+    uint32_t epoch = 0;
+    uint8_t* dev = nullptr;
+    size_t dev_bytes = 0;
+    float* part = nullptr;
+    size_t part_floats = 0;
+    // the tables' host copies, in turn; an event after each copy guards its reuse
+    static constexpr int RING = 2;
+    uint8_t* pin[RING] = {};
+    size_t pin_bytes[RING] = {};
+    hipEvent_t ev[RING] = {};
+    int next = 0;
+    // the parts of the device block
+    size_t o_seq = 0, o_tab = 0, o_dep = 0, o_anc = 0, o_item = 0, o_comb = 0;
+};
+
+static void plan_release(ftx_plan* pl) {
+    if (pl->dev) (void)hipFree(pl->dev);
+    if (pl->part) (void)hipFree(pl->part);
+    for (int i = 0; i < ftx_plan::RING; ++i) {
+        if (pl->pin[i]) (void)hipHostFree(pl->pin[i]);
+        if (pl->ev[i]) (void)hipEventDestroy(pl->ev[i]);
+    }
+    if (pl->pool) --pl->pool->users;
+    delete pl;
+}
+
+// pl->t to the device
+static int plan_upload(ftx_plan* pl) {
+    ftx_ctx* ctx = pl->ctx;
+    const PagedTables& t = pl->t;
+    pl->ready = false;
+    size_t at = 0;
+    auto place = [&](size_t& off, size_t bytes) {
+        off = at;
+        at += up256(bytes);
+    };
+    place(pl->o_seq, t.seqs.size() * sizeof(PagedSeq));
+    place(pl->o_tab, t.table.size() * 4);
+    place(pl->o_dep, t.depth.size() * 4);
+    place(pl->o_anc, t.anc.size() * 4);
+    place(pl->o_item, t.items.size() * sizeof(PagedItem));
+    place(pl->o_comb, t.combs.size() * sizeof(PagedComb));
+    const size_t bytes = at;
+    const size_t pf = (size_t)t.parts * pl->pool->n_kv * PAGED_TR * (pl->pool->hd + 2);
+    hipStream_t st = ctx->stream;
+    auto grow = [&](void** p, size_t& have, size_t need, size_t unit) -> int {
+        if (need <= have) return FTX_OK;
+        if (*p) {
+            // calls on this block may still run
+            FTX_HIP(ctx, hipDeviceSynchronize());
+            FTX_HIP(ctx, hipFree(*p));
+            *p = nullptr;
+            have = 0;
+        }
+        need += need / 4;
+        if (hipMalloc(p, need * unit + 256) != hipSuccess) {
+            (void)hipGetLastError();
+            *p = nullptr;
+            return ftx_fail(ctx, FTX_E_NOMEM, "plan: device allocation failed");
+        }
+        have = need;
+        return FTX_OK;
+    };
+    int rc = grow((void**)&pl->dev, pl->dev_bytes, bytes, 1);
+    if (!rc) rc = grow((void**)&pl->part, pl->part_floats, pf, sizeof(float));
+    if (rc) return rc;
+    const int k = pl->next;
+    if (pl->ev[k]) FTX_HIP(ctx, hipEventSynchronize(pl->ev[k]));
+    if (!pl->ev[k]) FTX_HIP(ctx, hipEventCreateWithFlags(&pl->ev[k], hipEventDisableTiming));
+    if (bytes > pl->pin_bytes[k]) {
+        if (pl->pin[k]) FTX_HIP(ctx, hipHostFree(pl->pin[k]));
+        pl->pin[k] = nullptr;
+        pl->pin_bytes[k] = 0;
+        if (hipHostMalloc((void**)&pl->pin[k], bytes + bytes / 4, hipHostMallocDefault) != hipSuccess) {
+            (void)hipGetLastError();
+            pl->pin[k] = nullptr;
+            return ftx_fail(ctx, FTX_E_NOMEM, "plan: host allocation failed");
+        }
+        pl->pin_bytes[k] = bytes + bytes / 4;
+    }
+    uint8_t* h = pl->pin[k];
+    auto put = [&](size_t off, const void* src, size_t n) {
+        if (n) memcpy(h + off, src, n);
+    };
+    put(pl->o_seq, t.seqs.data(), t.seqs.size() * sizeof(PagedSeq));
+    put(pl->o_tab, t.table.data(), t.table.size() * 4);
+    put(pl->o_dep, t.depth.data(), t.depth.size() * 4);
+    put(pl->o_anc, t.anc.data(), t.anc.size() * 4);
+    put(pl->o_item, t.items.data(), t.items.size() * sizeof(PagedItem));
+    put(pl->o_comb, t.combs.data(), t.combs.size() * sizeof(PagedComb));
+    FTX_HIP(ctx, hipMemcpyAsync(pl->dev, h, bytes, hipMemcpyHostToDevice, st));
+    FTX_HIP(ctx, hipEventRecord(pl->ev[k], st));
+    pl->next = (k + 1) % ftx_plan::RING;
+    pl->ready = true;
+    return FTX_OK;
+}
+
+static PagedView plan_view(const ftx_plan* pl, int64_t layer) {
+    const ftx_pool* p = pl->pool;
+    PagedView v{};
+    v.block = p->block;
+    v.data = p->data + layer * p->n_pages * p->n_kv * p->block;
+    v.n_kv = (int)p->n_kv;
+    v.hd = (int)p->hd;
+    v.q8 = p->q8;
+    v.seqs = (const PagedSeq*)(pl->dev + pl->o_seq);
+    v.table = (const int32_t*)(pl->dev + pl->o_tab);
+    v.nseq = (int)pl->t.seqs.size();
+    return v;
+}
+
+// what every call of a plan checks; *ld: 0 becomes `width`
+static int plan_call(ftx_plan* pl, int64_t layer, const void* x, int64_t* ldx, int64_t xw, const void* y,
+                     int64_t* ldy, int64_t yw) {
+    ftx_ctx* ctx = pl->ctx;
+    if (!pl->ready) return ftx_fail(ctx, FTX_E_INVALID, "the plan has no sequences");
+    if (layer < 0 || layer >= pl->pool->n_layer) return ftx_fail(ctx, FTX_E_RANGE, "layer out of range");
+    if (!x || !y) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    if (*ldx == 0) *ldx = xw;
+    if (*ldy == 0) *ldy = yw;
+    if (*ldx < xw || *ldy < yw) return ftx_fail(ctx, FTX_E_INVALID, "row stride shorter than a row");
+    if (((uintptr_t)x | (uintptr_t)y) & 3) return ftx_fail(ctx, FTX_E_INVALID, "rows must be 4-byte aligned");
+    if (!on_device(ctx, x) || !on_device(ctx, y))
+        return ftx_fail(ctx, FTX_E_INVALID, "rows must be memory of the context's device");
+    if (capturing(ctx->stream)) pl->captured = true;
+    return FTX_OK;
+}
+
+// whether n rows of w floats, ldx and ldy apart, at x and y share a float
+static bool rows_overlap(const float* x, int64_t ldx, const float* y, int64_t ldy, int64_t w, int64_t n) {
+    const intptr_t x0 = (intptr_t)x / 4, y0 = (intptr_t)y / 4;
+    if (n <= 0 || x0 + (n - 1) * ldx + w <= y0 || y0 + (n - 1) * ldy + w <= x0) return false;
+    if (ldx != ldy) return true;
+    // two column ranges of one matrix
+    const intptr_t r = ((y0 - x0) % ldx + ldx) % ldx;
+    return r < w || r > ldx - w;
+}
+
+extern "C" {
+
+int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t head_dim, int64_t n_pages,
+                    int kv_dtype, ftx_pool** out) {
+    if (!ctx || !out) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    *out = nullptr;
+    if (n_layer < 1 || n_layer > 65535 || n_head_kv < 1 || n_head_kv > 1024 || n_pages < 1 ||
+        n_pages > (int64_t)1 << 24)
+        return ftx_fail(ctx, FTX_E_INVALID, "pool: layers, kv heads or pages out of range");
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return ftx_fail(ctx, FTX_E_UNSUPPORTED, "pool: head_dim must be 64, 128 or 256");
+    if (kv_dtype != FTX_KV_F16 && kv_dtype != FTX_KV_Q8)
+        return ftx_fail(ctx, FTX_E_UNSUPPORTED, "pool: kv dtype must be F16 or Q8");
+    OnDevice od(ctx->device);
+    if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
+    ftx_pool* p = new (std::nothrow) ftx_pool;
+    if (!p) return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    p->ctx = ctx;
+    p->n_layer = n_layer;
+    p->n_kv = n_head_kv;
+    p->hd = head_dim;
+    p->n_pages = n_pages;
+    p->q8 = kv_dtype == FTX_KV_Q8;
+    p->block = paged_block_bytes((int)head_dim, p->q8);
+    p->free_pages = n_pages;
+    try {
+        p->taken.assign((size_t)n_pages, 0);
+    } catch (...) {
+        delete p;
+        return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    }
+    const size_t bytes = (size_t)(n_layer * n_pages * n_head_kv * p->block);
+    if (hipMalloc((void**)&p->data, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        delete p;
+        return ftx_fail(ctx, FTX_E_NOMEM, "pool allocation failed");
+    }
+    // finite values everywhere: slots that a row does not see still meet its P.V product
+    if (hipMemset(p->data, 0, bytes) != hipSuccess || hipDeviceSynchronize() != hipSuccess) {
+        (void)hipGetLastError();
+        (void)hipFree(p->data);
+        delete p;
+        return ftx_fail(ctx, FTX_E_DEVICE, "pool: clearing failed");
+    }
+    *out = p;
+    return FTX_OK;
+}
+
+int ftx_pool_free(ftx_pool* p) {
+    if (!p) return FTX_OK;
+    if (p->users) return ftx_fail(p->ctx, FTX_E_INVALID, "pool: a plan or cache of it lives");
+    OnDevice od(p->ctx->device);
+    (void)hipStreamSynchronize(p->ctx->stream);
+    if (p->data) (void)hipFree(p->data);
+    delete p;
+    return FTX_OK;
+}
+
+int64_t ftx_pool_available(const ftx_pool* p) { return p ? p->free_pages : 0; }
+
+int ftx_pool_take(ftx_pool* p, int64_t n, int32_t* pages) {
+    if (!p) return FTX_E_INVALID;
+    if (n < 0 || (n && !pages)) return ftx_fail(p->ctx, FTX_E_INVALID, "pool_take: bad argument");
+    if (n > p->free_pages) return ftx_fail(p->ctx, FTX_E_NOMEM, "pool_take: not enough free pages");
+    p->take(n, pages);
+    return FTX_OK;
+}
+
+int ftx_pool_give(ftx_pool* p, const int32_t* pages, int64_t n) {
+    if (!p) return FTX_E_INVALID;
+    if (n < 0 || (n && !pages)) return ftx_fail(p->ctx, FTX_E_INVALID, "pool_give: bad argument");
+    return p->give(pages, n) ? FTX_OK
+                             : ftx_fail(p->ctx, FTX_E_INVALID, "pool_give: a page is not taken or named twice");
+}
+
+int ftx_plan_set(ftx_plan* pl, const ftx_plan_args* a) {
+    if (!pl) return FTX_E_INVALID;
+    ftx_ctx* ctx = pl->ctx;
+    if (!a) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    if (pl->captured) return ftx_fail(ctx, FTX_E_INVALID, "plan: a graph holds calls of this plan");
+    if (capturing(ctx->stream)) return ftx_fail(ctx, FTX_E_INVALID, "plan: set while the stream is captured");
+    OnDevice od(ctx->device);
+    if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
+    try {
+        PagedGeom g;
+        g.n_kv = pl->pool->n_kv;
+        g.hd = pl->pool->hd;
+        g.n_pages = pl->pool->n_pages;
+        g.taken = pl->pool->taken.data();
+        g.cu = ctx->cu_count;
+        PagedTables t;
+        std::string err;
+        const int rc = paged_tables(g, *a, pl->mark, pl->epoch, t, err);
+        if (rc) return ftx_fail(ctx, rc, err);
+        std::swap(pl->t, t);
+        return plan_upload(pl);
+    } catch (...) {
+        pl->ready = false;
+        return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    }
+}
+
+int ftx_plan_create(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args* a, ftx_plan** out) {
+    if (!ctx || !p || !a || !out) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    *out = nullptr;
+    if (p->ctx != ctx) return ftx_fail(ctx, FTX_E_INVALID, "plan: the pool is another context's");
+    ftx_plan* pl = new (std::nothrow) ftx_plan;
+    if (!pl) return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    pl->ctx = ctx;
+    pl->pool = p;
+    ++p->users;
+    const int rc = ftx_plan_set(pl, a);
+    if (rc) {
+        plan_release(pl);
+        return rc;
+    }
+    *out = pl;
+    return FTX_OK;
+}
+
+int ftx_plan_free(ftx_plan* pl) {
+    if (!pl) return FTX_OK;
+    OnDevice od(pl->ctx->device);
+    (void)hipStreamSynchronize(pl->ctx->stream);
+    plan_release(pl);
+    return FTX_OK;
+}
+
+int ftx_paged_write(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv) {
+    if (!pl) return FTX_E_INVALID;
+    ftx_ctx* ctx = pl->ctx;
+    const int64_t w = pl->pool->n_kv * pl->pool->hd;
+    if (pl->ready && pl->t.tokens == 0) return FTX_OK;
+    const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
+    if (rc) return rc;
+    OnDevice od(ctx->device);
+    const double n = (double)pl->t.tokens;
+    NoTrace nt(ctx, capturing(ctx->stream));
+    TraceScope ts(ctx);
+    FTX_HIP(ctx, launch_paged_write(ctx->stream, plan_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
+    ts.end(TK_PAGED_KV, 2 * n * pl->pool->n_kv * (4.0 * pl->pool->hd + pl->pool->block / (2.0 * FTX_PAGE)));
+    return FTX_OK;
+}
+
+int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv) {
+    if (!pl) return FTX_E_INVALID;
+    ftx_ctx* ctx = pl->ctx;
+    const int64_t w = pl->pool->n_kv * pl->pool->hd;
+    const int64_t n = context ? pl->t.rows : pl->t.tokens;
+    if (pl->ready && n == 0) return FTX_OK;
+    const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
+    if (rc) return rc;
+    if (context && pl->t.absent) return ftx_fail(ctx, FTX_E_RANGE, "paged_read: a page is absent");
+    if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(ctx, FTX_E_INVALID, "paged_read: k and v overlap");
+    OnDevice od(ctx->device);
+    NoTrace nt(ctx, capturing(ctx->stream));
+    TraceScope ts(ctx);
+    FTX_HIP(ctx, launch_paged_read(ctx->stream, plan_view(pl, layer),
+                                   context ? pl->t.max_pages : pl->t.max_new_pages, context, k, ldk, v, ldv));
+    ts.end(TK_PAGED_KV, 2.0 * n * pl->pool->n_kv * (4.0 * pl->pool->hd + pl->pool->block / (2.0 * FTX_PAGE)));
+    return FTX_OK;
+}
+
+int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo) {
+    if (!pl) return FTX_E_INVALID;
+    ftx_ctx* ctx = pl->ctx;
+    const PagedTables& t = pl->t;
+    const ftx_pool* p = pl->pool;
+    if (pl->ready && t.n_head == 0) return ftx_fail(ctx, FTX_E_INVALID, "the plan has no query heads");
+    if (pl->ready && t.tokens == 0) return FTX_OK;
+    const int64_t w = t.n_head * p->hd;
+    const int rc = plan_call(pl, layer, q, &ldq, w, out, &ldo, w);
+    if (rc) return rc;
+    if (rows_overlap(q, ldq, out, ldo, w, t.tokens))
+        return ftx_fail(ctx, FTX_E_INVALID, "paged_attention: q and out overlap");
+    OnDevice od(ctx->device);
+    PagedAttn a{};
+    a.p = plan_view(pl, layer);
+    a.depth = (const int32_t*)(pl->dev + pl->o_dep);
+    a.anc = (const uint32_t*)(pl->dev + pl->o_anc);
+    a.items = (const PagedItem*)(pl->dev + pl->o_item);
+    a.combs = (const PagedComb*)(pl->dev + pl->o_comb);
+    a.n_items = (int)t.items.size();
+    a.n_combs = (int)t.combs.size();
+    a.gqa = (int)(t.n_head / p->n_kv);
+    a.window = (int)t.window;
+    a.sinks = (int)t.sinks;
+    a.q = q;
+    a.out = out;
+    a.ldq = ldq;
+    a.ldo = ldo;
+    a.part = pl->part;
+    a.pml = pl->part + (size_t)t.parts * p->n_kv * PAGED_TR * p->hd;
+    NoTrace nt(ctx, capturing(ctx->stream));
+    TraceScope ts(ctx);
+    FTX_HIP(ctx, launch_paged_attention(ctx->stream, a));
+    ts.end(TK_ATTENTION, t.pages_read * p->n_kv * (double)p->block + 8.0 * t.tokens * w);
+    return FTX_OK;
+}
+
+}  // extern "C"

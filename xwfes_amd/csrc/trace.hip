@@ -10,7 +10,7 @@ thread_local KernelTimer* g_ktimer = nullptr;
 static const char* kTraceNames[TK_COUNT] = {
     "embed", "rmsnorm", "gemv_qkv", "rope_kv", "attention", "gemv_o",
     "gemv_swiglu", "down", "head", "row_stats", "accept", "xq_prep", "moe_route",
-    "moe_combine", "event_pair"};
+    "moe_combine", "paged_kv", "event_pair"};
 
 static void resolve(ftx_ctx* ctx) {
     if (ctx->pending.empty()) {

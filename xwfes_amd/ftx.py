@@ -17,7 +17,8 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "ftx.h")
 F32, F16, Q4_0, Q4_1, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 2, 3, 8, 12, 14, 30
 BLOCK = {F32: (1, 4), F16: (1, 2), BF16: (1, 2), Q4_0: (32, 18), Q4_1: (32, 20),
          Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+PAGE = 64  # tokens of a page
 # the sampler state of seed 0 (include/ft/sampler.h:19)
 SAMPLER_SEED = 0x9E3779B97F4A7C15
 ACCEPT_GREEDY, ACCEPT_RATIO, ACCEPT_RESIDUAL = 0, 1, 2
@@ -79,6 +80,16 @@ class AcceptArgs(C.Structure):
                 ("top_p", C.c_float)]
 
 
+class PagedSeq(C.Structure):
+    _fields_ = [("pages", _i32p), ("n_pages", _i64), ("npast", _i64), ("M", _i64),
+                ("parents", _i32p)]
+
+
+class PlanArgs(C.Structure):
+    _fields_ = [("seqs", C.POINTER(PagedSeq)), ("nseq", _i64), ("n_head", _i64), ("window", _i64),
+                ("sinks", _i64)]
+
+
 class TraceEntry(C.Structure):
     _fields_ = [("name", C.c_char * 24), ("launches", C.c_int64), ("ms", C.c_double),
                 ("bytes", C.c_double), ("kernel_launches", C.c_int64), ("kernel_ms", C.c_double)]
@@ -133,6 +144,17 @@ def load(path=LIB_PATH):
         "ftx_accept_batch": (C.c_int, [_vp, C.POINTER(AcceptArgs), C.c_int]),
         "ftx_argmax_prob": (C.c_int, [_vp, _vp, _i64, _i32p, _fp]),
         "ftx_fill_normal": (C.c_int, [_vp, _vp, C.c_int, _i64, C.c_uint64, C.c_float]),
+        "ftx_pool_create": (C.c_int, [_vp, _i64, _i64, _i64, _i64, C.c_int, C.POINTER(_vp)]),
+        "ftx_pool_free": (C.c_int, [_vp]),
+        "ftx_pool_available": (_i64, [_vp]),
+        "ftx_pool_take": (C.c_int, [_vp, _i64, _i32p]),
+        "ftx_pool_give": (C.c_int, [_vp, _i32p, _i64]),
+        "ftx_plan_create": (C.c_int, [_vp, _vp, C.POINTER(PlanArgs), C.POINTER(_vp)]),
+        "ftx_plan_set": (C.c_int, [_vp, C.POINTER(PlanArgs)]),
+        "ftx_plan_free": (C.c_int, [_vp]),
+        "ftx_paged_write": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64]),
+        "ftx_paged_read": (C.c_int, [_vp, _i64, C.c_int, _vp, _i64, _vp, _i64]),
+        "ftx_paged_attention": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64]),
         "ftx_trace": (C.c_int, [_vp, C.c_int]),
         "ftx_trace_read": (C.c_int, [_vp, C.POINTER(TraceEntry), C.c_int, C.POINTER(C.c_int)]),
         "ftx_trace_replay": (C.c_int, [_vp, C.c_char_p, C.c_int]),
@@ -307,6 +329,14 @@ class Context:
         self.check(self.lib.ftx_expert_chunk(self.h, C.byref(j)))
         return out
 
+    # ---- paged KV caches ----
+    def pool(self, n_layer, n_head_kv, head_dim, n_pages, kv_dtype=KV_F16):
+        """A pool of n_pages pages of PAGE tokens for paged KV caches."""
+        h = _vp()
+        self.check(self.lib.ftx_pool_create(self.h, n_layer, n_head_kv, head_dim, n_pages,
+                                            kv_dtype, C.byref(h)))
+        return Pool(self, h.value)
+
     # ---- verify path ----
     def model(self, cfg, tensors, max_tokens=64):
         """cfg: dict of hyper-parameters (n_expert / n_expert_used for MoE);
@@ -395,6 +425,82 @@ class Context:
         return [dict(accepted=acc[:na.value].tolist(), bonus=bonus.value, rng=s.value,
                      sampler_state=ss.value, margin=mg.value)
                 for acc, na, bonus, s, ss, mg in outs]
+
+
+def plan_args(seqs, n_head=0, window=0, sinks=0):
+    """(PlanArgs, what it points into) of seqs = [(pages, npast, M[, parents]), ...]."""
+    keep, arr = [], (PagedSeq * max(len(seqs), 1))()
+    for i, (pages, npast, M, *rest) in enumerate(seqs):
+        pg = np.ascontiguousarray(pages, np.int32)
+        par = None if not rest or rest[0] is None else np.ascontiguousarray(rest[0], np.int32)
+        if par is not None and par.size != M:
+            raise ValueError("parents: %d of %d" % (par.size, M))
+        keep += [pg, par]
+        arr[i] = PagedSeq(pg.ctypes.data_as(_i32p), pg.size, npast, M,
+                          None if par is None else par.ctypes.data_as(_i32p))
+    return PlanArgs(arr, len(seqs), n_head, window, sinks), (keep, arr)
+
+
+class Pool:
+    """Pages of a paged KV cache (ftx_pool_*)."""
+
+    def __init__(self, ctx, handle):
+        self.ctx, self.handle = ctx, handle
+
+    @property
+    def available(self):
+        return self.ctx.lib.ftx_pool_available(self.handle)
+
+    def take(self, n):
+        a = np.empty(max(n, 1), np.int32)
+        self.ctx.check(self.ctx.lib.ftx_pool_take(self.handle, n, a.ctypes.data_as(_i32p)))
+        return a[:n].tolist()
+
+    def give(self, pages):
+        a = np.ascontiguousarray(pages, np.int32)
+        self.ctx.check(self.ctx.lib.ftx_pool_give(self.handle, a.ctypes.data_as(_i32p), a.size))
+
+    def plan(self, seqs, n_head=0, window=0, sinks=0):
+        """A step's plan: seqs = [(pages, npast, M[, parents]), ...]; n_head = 0:
+        a plan to write and read back only."""
+        a, keep = plan_args(seqs, n_head, window, sinks)
+        h = _vp()
+        self.ctx.check(self.ctx.lib.ftx_plan_create(self.ctx.h, self.handle, C.byref(a),
+                                                    C.byref(h)))
+        return Plan(self.ctx, h.value)
+
+    def free(self):
+        if self.handle:
+            self.ctx.check(self.ctx.lib.ftx_pool_free(self.handle))
+            self.handle = None
+
+
+class Plan:
+    """One step's calls over a pool (ftx_plan_*, ftx_paged_*): device pointers,
+    row strides in floats (0: dense)."""
+
+    def __init__(self, ctx, handle):
+        self.ctx, self.handle = ctx, handle
+
+    def set(self, seqs, n_head=0, window=0, sinks=0):
+        a, keep = plan_args(seqs, n_head, window, sinks)
+        self.ctx.check(self.ctx.lib.ftx_plan_set(self.handle, C.byref(a)))
+
+    def write(self, layer, k_ptr, v_ptr, ldk=0, ldv=0):
+        self.ctx.check(self.ctx.lib.ftx_paged_write(self.handle, layer, k_ptr, ldk, v_ptr, ldv))
+
+    def read(self, layer, k_ptr, v_ptr, context=False, ldk=0, ldv=0):
+        self.ctx.check(self.ctx.lib.ftx_paged_read(self.handle, layer, int(context), k_ptr, ldk,
+                                                   v_ptr, ldv))
+
+    def attend(self, layer, q_ptr, out_ptr, ldq=0, ldo=0):
+        self.ctx.check(self.ctx.lib.ftx_paged_attention(self.handle, layer, q_ptr, ldq, out_ptr,
+                                                        ldo))
+
+    def free(self):
+        if self.handle:
+            self.ctx.lib.ftx_plan_free(self.handle)
+            self.handle = None
 
 
 class Model:

@@ -434,6 +434,20 @@ int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t l
 int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out,
                         int64_t ldo);
 
+/* A paged cache for verify steps: up to cap tokens in pages that the steps
+ * take from `p` (made for the model's layers, kv heads and head size) as the
+ * sequence grows; FTX_E_NOMEM from a step that finds too few leaves its tokens
+ * as they were.  ftx_kv_truncate gives back pages past the committed tokens,
+ * ftx_kv_free all.  window and sinks as in ftx_plan_args; a step gives back
+ * pages that no later token can see, and a truncation to a length whose
+ * window reaches into them is refused (FTX_E_RANGE; 0 is not).  The sequences
+ * of one ftx_verify_batch are all of one pool, window and sinks, or none is
+ * paged.  ftx_kv_write and ftx_kv_read take fp32 arrays for a paged cache
+ * (write takes pages for all of cap, read leaves zeros where no page is);
+ * ftx_kv_pointers gives NULL for its buffers. */
+int ftx_kv_create_paged(ftx_ctx* ctx, const ftx_model* m, ftx_pool* p, int64_t cap, int64_t window,
+                        int64_t sinks, ftx_kv** out);
+
 /* ---- kernel trace (the reference keeps wall-clock RunStats only,
  * include/ft/engine.h:25-39) ---- */
 typedef struct {

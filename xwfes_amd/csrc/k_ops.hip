@@ -145,7 +145,7 @@ __device__ __forceinline__ void rope_kv_row(const RopeArgs& a, int64_t m, int64_
             a.ql16[o + ib] = (_Float16)(y1 - (float)h1);
         }
     }
-    if (h < a.n_head) return;
+    if (h < a.n_head || !a.kc) return;
     __syncthreads();
     const int64_t kh = h - a.n_head;
     const int64_t slot = npast + m;
@@ -294,6 +294,7 @@ __device__ __forceinline__ void rope_kv_head(const RopeArgs& a, int64_t m, int64
                 }
             } else {
                 if (prow || a.bias) row[off + kdim + t] = v[j][e];
+                if (!a.kc) continue;  // (a paged cache's rows are stored from here)
                 const int64_t idx = slot * kdim + kh * a.hd + t;
                 const int64_t vidx = v_index(slot, kh, t, a.hd, a.cap);
                 if (a.kv_f16) {

@@ -129,6 +129,30 @@ __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, fl
     }
 }
 
+// ---------------------------------------------------------------- moves
+// Thread = one dim of a kv head of a layer; it walks the path in increasing i
+// (dst[i] is never a later source).
+__global__ void __launch_bounds__(256) k_paged_move(PagedMove m) {
+    const int d = threadIdx.x;
+    if (d >= m.hd) return;
+    uint8_t* base = m.data + ((int64_t)blockIdx.y * m.n_pages * m.n_kv + blockIdx.x) * m.block;
+    const int64_t vb = paged_values_bytes(m.hd, m.q8), step = m.block * m.n_kv;
+    for (int i = 0; i < m.n; ++i) {
+        const int ss = m.src[i] % FTX_PAGE, ds = m.dst[i] % FTX_PAGE;
+        const uint8_t* s = base + (m.src[i] / FTX_PAGE) * step;
+        uint8_t* t = base + (m.dst[i] / FTX_PAGE) * step;
+        if (m.src[i] == m.dst[i]) continue;
+        if (m.q8) {
+            t[paged_k_at(ds, d, 1)] = s[paged_k_at(ss, d, 1)];
+            t[vb + paged_v_at(ds, d, 1)] = s[vb + paged_v_at(ss, d, 1)];
+        } else {
+            *(uint16_t*)(t + paged_k_at(ds, d, 0)) = *(const uint16_t*)(s + paged_k_at(ss, d, 0));
+            *(uint16_t*)(t + vb + paged_v_at(ds, d, 0)) = *(const uint16_t*)(s + vb + paged_v_at(ss, d, 0));
+        }
+        if (d < 2) ((float*)(t + 2 * vb))[d * FTX_PAGE + ds] = ((const float*)(s + 2 * vb))[d * FTX_PAGE + ss];
+    }
+}
+
 // ---------------------------------------------------------------- attention
 // 8 biased bytes -> fp16 q (exact): the byte under 0x64 is 1024 + q + 128
 __device__ __forceinline__ v8h u8x8(uint32_t a, uint32_t b) {
@@ -467,5 +491,10 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     const dim3 cg((unsigned)a.n_combs * (unsigned)a.p.n_kv);
     auto* comb = a.p.hd == 64 ? k_paged_combine<64> : a.p.hd == 128 ? k_paged_combine<128> : k_paged_combine<256>;
     hipLaunchKernelGGL(comb, cg, dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_move(hipStream_t st, const PagedMove& m) {
+    hipLaunchKernelGGL(k_paged_move, dim3((unsigned)m.n_kv, (unsigned)m.n_layer), dim3(256), 0, st, m);
     return hipGetLastError();
 }

@@ -118,3 +118,20 @@ struct PagedAttn {
     float* pml;   // [parts][n_kv][PAGED_TR][2]: maximum (base 2), sum
 };
 hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a);
+
+// rows of a committed path: slots src[i] move to dst[i] (page * FTX_PAGE +
+// slot), in order, every layer and kv head
+struct PagedMove {
+    uint8_t* data;
+    int64_t block, n_pages;
+    int n_kv, hd, q8, n_layer, n;
+    int32_t src[256], dst[256];
+};
+hipError_t launch_paged_move(hipStream_t st, const PagedMove& m);
+
+// ---------------------------------------------------------------- the verify step's use
+// The plan of the pool's running step (one a pool, its calls in stream order)
+int paged_step_plan(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args& a, ftx_plan** out);
+int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv);
+int paged_read_rows(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv);
+int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo);

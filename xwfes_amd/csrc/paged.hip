@@ -428,6 +428,10 @@ int ftx_pool_free(ftx_pool* p) {
     if (p->users) return ftx_fail(p->ctx, FTX_E_INVALID, "pool: a plan or cache of it lives");
     OnDevice od(p->ctx->device);
     (void)hipStreamSynchronize(p->ctx->stream);
+    if (p->step) {
+        ++p->users;
+        plan_release(p->step);
+    }
     if (p->data) (void)hipFree(p->data);
     delete p;
     return FTX_OK;
@@ -505,51 +509,70 @@ int ftx_plan_free(ftx_plan* pl) {
 
 int ftx_paged_write(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv) {
     if (!pl) return FTX_E_INVALID;
-    ftx_ctx* ctx = pl->ctx;
     const int64_t w = pl->pool->n_kv * pl->pool->hd;
     if (pl->ready && pl->t.tokens == 0) return FTX_OK;
     const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
-    if (rc) return rc;
-    OnDevice od(ctx->device);
-    const double n = (double)pl->t.tokens;
-    NoTrace nt(ctx, capturing(ctx->stream));
-    TraceScope ts(ctx);
-    FTX_HIP(ctx, launch_paged_write(ctx->stream, plan_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
-    ts.end(TK_PAGED_KV, 2 * n * pl->pool->n_kv * (4.0 * pl->pool->hd + pl->pool->block / (2.0 * FTX_PAGE)));
-    return FTX_OK;
+    return rc ? rc : paged_write_rows(pl, layer, k, ldk, v, ldv);
 }
 
 int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv) {
     if (!pl) return FTX_E_INVALID;
-    ftx_ctx* ctx = pl->ctx;
     const int64_t w = pl->pool->n_kv * pl->pool->hd;
     const int64_t n = context ? pl->t.rows : pl->t.tokens;
     if (pl->ready && n == 0) return FTX_OK;
     const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
     if (rc) return rc;
-    if (context && pl->t.absent) return ftx_fail(ctx, FTX_E_RANGE, "paged_read: a page is absent");
-    if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(ctx, FTX_E_INVALID, "paged_read: k and v overlap");
+    if (context && pl->t.absent) return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: a page is absent");
+    if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_read: k and v overlap");
+    return paged_read_rows(pl, layer, context, k, ldk, v, ldv);
+}
+
+int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo) {
+    if (!pl) return FTX_E_INVALID;
+    if (pl->ready && pl->t.n_head == 0) return ftx_fail(pl->ctx, FTX_E_INVALID, "the plan has no query heads");
+    if (pl->ready && pl->t.tokens == 0) return FTX_OK;
+    const int64_t w = pl->t.n_head * pl->pool->hd;
+    const int rc = plan_call(pl, layer, q, &ldq, w, out, &ldo, w);
+    if (rc) return rc;
+    if (rows_overlap(q, ldq, out, ldo, w, pl->t.tokens))
+        return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_attention: q and out overlap");
+    return paged_attend_rows(pl, layer, q, ldq, out, ldo);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------- launches of a plan
+
+// bytes that n rows of K and V move
+static double rows_bytes(const ftx_pool* p, double n) {
+    return n * p->n_kv * (8.0 * p->hd + (double)p->block / FTX_PAGE);
+}
+
+int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv) {
+    ftx_ctx* ctx = pl->ctx;
+    OnDevice od(ctx->device);
+    NoTrace nt(ctx, capturing(ctx->stream));
+    TraceScope ts(ctx);
+    FTX_HIP(ctx, launch_paged_write(ctx->stream, plan_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
+    ts.end(TK_PAGED_KV, rows_bytes(pl->pool, (double)pl->t.tokens));
+    return FTX_OK;
+}
+
+int paged_read_rows(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv) {
+    ftx_ctx* ctx = pl->ctx;
     OnDevice od(ctx->device);
     NoTrace nt(ctx, capturing(ctx->stream));
     TraceScope ts(ctx);
     FTX_HIP(ctx, launch_paged_read(ctx->stream, plan_view(pl, layer),
                                    context ? pl->t.max_pages : pl->t.max_new_pages, context, k, ldk, v, ldv));
-    ts.end(TK_PAGED_KV, 2.0 * n * pl->pool->n_kv * (4.0 * pl->pool->hd + pl->pool->block / (2.0 * FTX_PAGE)));
+    ts.end(TK_PAGED_KV, rows_bytes(pl->pool, (double)(context ? pl->t.rows : pl->t.tokens)));
     return FTX_OK;
 }
 
-int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo) {
-    if (!pl) return FTX_E_INVALID;
+int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo) {
     ftx_ctx* ctx = pl->ctx;
     const PagedTables& t = pl->t;
     const ftx_pool* p = pl->pool;
-    if (pl->ready && t.n_head == 0) return ftx_fail(ctx, FTX_E_INVALID, "the plan has no query heads");
-    if (pl->ready && t.tokens == 0) return FTX_OK;
-    const int64_t w = t.n_head * p->hd;
-    const int rc = plan_call(pl, layer, q, &ldq, w, out, &ldo, w);
-    if (rc) return rc;
-    if (rows_overlap(q, ldq, out, ldo, w, t.tokens))
-        return ftx_fail(ctx, FTX_E_INVALID, "paged_attention: q and out overlap");
     OnDevice od(ctx->device);
     PagedAttn a{};
     a.p = plan_view(pl, layer);
@@ -571,8 +594,18 @@ int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq
     NoTrace nt(ctx, capturing(ctx->stream));
     TraceScope ts(ctx);
     FTX_HIP(ctx, launch_paged_attention(ctx->stream, a));
-    ts.end(TK_ATTENTION, t.pages_read * p->n_kv * (double)p->block + 8.0 * t.tokens * w);
+    ts.end(TK_ATTENTION, t.pages_read * p->n_kv * (double)p->block + 8.0 * t.tokens * t.n_head * p->hd);
     return FTX_OK;
 }
 
-}  // extern "C"
+int paged_step_plan(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args& a, ftx_plan** out) {
+    if (!p->step) {
+        const int rc = ftx_plan_create(ctx, p, &a, &p->step);
+        if (rc) return rc;
+        --p->users;  // the pool's own
+        *out = p->step;
+        return FTX_OK;
+    }
+    *out = p->step;
+    return ftx_plan_set(p->step, &a);
+}

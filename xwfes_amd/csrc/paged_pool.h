@@ -5,6 +5,7 @@
 #include <vector>
 
 struct ftx_ctx;
+struct ftx_plan;
 
 struct ftx_pool {
     ftx_ctx* ctx = nullptr;
@@ -15,6 +16,7 @@ struct ftx_pool {
     std::vector<uint8_t> taken;
     int64_t free_pages = 0, low = 0;  // no free page below `low`
     int users = 0;  // plans and caches
+    ftx_plan* step = nullptr;  // of the verify steps over the pool
 
     // n <= free_pages of them, the lowest ids
     void take(int64_t n, int32_t* pages) {

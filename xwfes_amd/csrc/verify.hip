@@ -8,6 +8,8 @@
 #include "ftx_internal.h"
 
 #include <cstring>
+#include "paged.h"
+#include "paged_pool.h"
 #include "quant_dev.h"
 
 struct ftx_model {
@@ -135,7 +137,58 @@ struct ftx_kv {
     void* v = nullptr;      // [n_layer][n_kv][hd][cap_alloc]
     float* attn_part = nullptr;  // chunk partials of the MFMA attention
     int64_t npast = 0;
+    // paged caches: the pool, the table of pages (-1: out of the window for
+    // good) and what the model's tokens see; no buffers of their own
+    ftx_pool* pool = nullptr;
+    std::vector<int32_t> pages;
+    int64_t window = 0, sinks = 0;
 };
+
+// pages of a paged cache for `tokens` positions, all or none
+static int kv_grow(ftx_kv* kv, int64_t tokens) {
+    const size_t need = (size_t)((tokens + FTX_PAGE - 1) / FTX_PAGE), have = kv->pages.size();
+    if (need <= have) return FTX_OK;
+    try {
+        kv->pages.resize(need);
+    } catch (...) {
+        return ftx_fail(kv->ctx, FTX_E_NOMEM, "host allocation failed");
+    }
+    const int rc = ftx_pool_take(kv->pool, (int64_t)(need - have), kv->pages.data() + have);
+    if (rc) kv->pages.resize(have);
+    return rc;
+}
+
+// give back table entries [from, to) that hold a page
+static void kv_drop(ftx_kv* kv, int64_t from, int64_t to) {
+    for (int64_t i = std::max<int64_t>(from, 0); i < std::min<int64_t>(to, (int64_t)kv->pages.size()); ++i)
+        if (kv->pages[(size_t)i] >= 0) {
+            (void)ftx_pool_give(kv->pool, &kv->pages[(size_t)i], 1);
+            kv->pages[(size_t)i] = -1;
+        }
+}
+
+// the table entries that no token from position npast on sees: [first, second)
+static std::pair<int64_t, int64_t> kv_unseen(const ftx_kv* kv, int64_t npast) {
+    if (!kv->window) return {0, 0};
+    return {(kv->sinks + FTX_PAGE - 1) / FTX_PAGE, std::max<int64_t>(0, npast - kv->window + 1) / FTX_PAGE};
+}
+
+// Paged caches: pages for the step's new tokens, and its plan (else *plan stays null)
+static int step_pages(ftx_ctx* ctx, int64_t n_head, const ftx_seq_args* sq, int64_t nseq, ftx_plan** plan) {
+    const ftx_kv* k0 = sq[0].kv;
+    if (!k0->pool) return FTX_OK;
+    for (int64_t s = 0; s < nseq; ++s) {
+        const auto un = kv_unseen(sq[s].kv, sq[s].kv->npast);
+        kv_drop(sq[s].kv, un.first, un.second);
+    }
+    ftx_paged_seq ps[FTX_MAX_SEQ];
+    for (int64_t s = 0; s < nseq; ++s) {
+        ftx_kv* kv = sq[s].kv;
+        if (const int rc = kv_grow(kv, kv->npast + sq[s].M)) return rc;
+        ps[s] = ftx_paged_seq{kv->pages.data(), (int64_t)kv->pages.size(), kv->npast, sq[s].M, sq[s].parents};
+    }
+    return paged_step_plan(ctx, k0->pool, ftx_plan_args{ps, nseq, n_head, k0->window, k0->sinks}, plan);
+}
 
 static void model_release(ftx_model* m) {
     if (!m) return;
@@ -230,6 +283,8 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
             }
         }
     }
+    ftx_plan* plan = nullptr;
+    if (const int rc = step_pages(ctx, d.n_head, sq, nseq, &plan)) return rc;
     hipStream_t st = ctx->stream;
     int32_t* d_toks = (int32_t*)m->args;
     int32_t* d_depth = (int32_t*)(m->args + AL.depth);
@@ -449,7 +504,7 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
         // sequence
         int64_t Ms[FTX_MAX_SEQ];
         for (int64_t s = 0; s < nseq; ++s) Ms[s] = sq[s].M;
-        bool all_mattn = nseq > 1;
+        bool all_mattn = nseq > 1 && !plan;
         for (int64_t s = 0; s < nseq && all_mattn; ++s)
             all_mattn = attn_mfma_supported(hd, sq[s].kv->kv_f16, sq[s].M, d.n_head, d.n_head_kv,
                                             sq[s].kv->cap_alloc);
@@ -459,7 +514,7 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
         MmFragDst ofd{};
         {
             MmSeg oseg;
-            bool of = mm_seg((size_t)(lt + FTX_T_O), T[FTX_T_O], oseg);
+            bool of = !plan && mm_seg((size_t)(lt + FTX_T_O), T[FTX_T_O], oseg);
             for (int64_t s = 0; s < nseq && of; ++s)
                 of = attn_mfma_supported(hd, sq[s].kv->kv_f16, sq[s].M, d.n_head, d.n_head_kv,
                                             sq[s].kv->cap_alloc);
@@ -468,6 +523,33 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
                 ofd = MmFragDst{oact.xh, oact.xl, oact.sh, oact.sl, 0, m->qdim,
                                 oseg.dt == FTX_Q4_0_MMT ? 1 : 0};
             }
+        }
+        if (plan) {
+            // rotated rows in qkv, K / V from there into the pages, attention
+            // over the pages
+            RopeArgs ras[FTX_MAX_SEQ];
+            for (int64_t s = 0; s < nseq; ++s) {
+                const int64_t r0 = row0[s];
+                RopeArgs ra{m->qkv + r0 * m->ldq, m->ldq, d.n_head, d.n_head_kv, hd, d_depth + r0, d_np + s,
+                            d.rope_theta, d.rope_neox, nullptr, nullptr, 1, 0};
+                ra.bias = m->attn_bias[l];
+                ra.qnorm = m->qnorm[l];
+                ra.knorm = m->knorm[l];
+                ra.eps = eps;
+                if (qpend.S > 0) {
+                    ra.part = qpend.part + r0 * qpend.ldp;
+                    ra.split_stride = qpend.split_stride;
+                    ra.ldp = qpend.ldp;
+                    ra.S = qpend.S;
+                }
+                ra.cs = d_cs + r0 * hd2 * 2;
+                ras[s] = ra;
+            }
+            TRACED_L(TK_ROPE_KV, 2.0 * Md * m->ldq * f4, launch_rope_kv_batch(st, ras, Ms, (int)nseq));
+            const float* kr = m->qkv + m->qdim;
+            rc = paged_write_rows(plan, l, kr, m->ldq, kr + m->kdim, m->ldq);
+            if (!rc) rc = paged_attend_rows(plan, l, m->qkv, m->ldq, m->att, m->qdim);
+            if (rc) return rc;
         }
         if (all_mattn) {
             RopeArgs ras[FTX_MAX_SEQ];
@@ -523,7 +605,7 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
             TRACED_L(TK_ROPE_KV, rope_b, launch_rope_kv_batch(st, ras, Ms, (int)nseq));
             TRACED_L(TK_ATTENTION, attn_b, launch_attn_mfma_batch(st, ams, parts, (int)nseq));
         }
-        for (int64_t s = 0; s < nseq && !all_mattn; ++s) {
+        for (int64_t s = 0; s < nseq && !all_mattn && !plan; ++s) {
             ftx_kv* kv = sq[s].kv;
             const int64_t r0 = row0[s], M = sq[s].M, npast = kv->npast;
             const size_t kvel = kv->kv_f16 ? 2 : 4;
@@ -1051,9 +1133,42 @@ int ftx_kv_create(ftx_ctx* ctx, const ftx_model* m, int64_t cap, int kv_dtype, f
     return FTX_OK;
 }
 
+int ftx_kv_create_paged(ftx_ctx* ctx, const ftx_model* m, ftx_pool* p, int64_t cap, int64_t window,
+                        int64_t sinks, ftx_kv** out) {
+    if (!ctx || !m || !p || !out) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    *out = nullptr;
+    if (cap < 1 || cap > (int64_t)1 << 30) return ftx_fail(ctx, FTX_E_INVALID, "cap must be in 1 .. 2^30");
+    if (window < 0 || sinks < 0) return ftx_fail(ctx, FTX_E_INVALID, "negative window or sinks");
+    if (p->ctx != ctx || m->ctx != ctx)
+        return ftx_fail(ctx, FTX_E_INVALID, "the pool or the model is another context's");
+    if (p->n_layer != m->d.n_layer || p->n_kv != m->d.n_head_kv || p->hd != m->d.head_dim)
+        return ftx_fail(ctx, FTX_E_INVALID, "the pool does not match the model");
+    ftx_kv* kv = new (std::nothrow) ftx_kv;
+    if (!kv) return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    kv->ctx = ctx;
+    kv->n_layer = m->d.n_layer;
+    kv->cap = cap;
+    kv->kdim = m->kdim;
+    kv->n_kv = m->d.n_head_kv;
+    kv->hd = m->d.head_dim;
+    kv->n_head = m->d.n_head;
+    kv->mmax = m->Mmax;
+    kv->kv_f16 = !p->q8;
+    kv->pool = p;
+    kv->window = window;
+    kv->sinks = window ? std::min(sinks, cap) : 0;
+    ++p->users;
+    *out = kv;
+    return FTX_OK;
+}
+
 int ftx_kv_free(ftx_kv* kv) {
     if (!kv) return FTX_OK;
     if (kv->ctx) (void)hipStreamSynchronize(kv->ctx->stream);
+    if (kv->pool) {
+        kv_drop(kv, 0, (int64_t)kv->pages.size());
+        --kv->pool->users;
+    }
     if (kv->k) (void)hipFree(kv->k);
     if (kv->v) (void)hipFree(kv->v);
     if (kv->attn_part) (void)hipFree(kv->attn_part);
@@ -1098,13 +1213,70 @@ static int kv_copy(ftx_kv* kv, void* kh, void* vh, bool to_device) {
     return FTX_OK;
 }
 
+// The same for a paged cache and fp32 arrays: its held positions, a layer at a
+// time through the workspace and the pool's plan
+static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
+    ftx_ctx* ctx = kv->ctx;
+    if (to_device) {
+        // (a dropped page is held again)
+        kv_drop(kv, 0, (int64_t)kv->pages.size());
+        kv->pages.clear();
+        if (const int rc = kv_grow(kv, kv->cap)) return rc;
+    }
+    const int64_t kdim = kv->kdim, n = std::min<int64_t>((int64_t)kv->pages.size() * FTX_PAGE, kv->cap);
+    const size_t bytes = (size_t)(n * kdim) * sizeof(float);
+    if (!to_device) {
+        memset(kh, 0, (size_t)(kv->n_layer * kv->cap * kdim) * sizeof(float));
+        memset(vh, 0, (size_t)(kv->n_layer * kv->cap * kdim) * sizeof(float));
+    }
+    if (n == 0) return FTX_OK;
+    float* ws;
+    if (const int rc = ftx_workspace(ctx, 2 * bytes, (void**)&ws)) return rc;
+    hipStream_t st = ctx->stream;
+    // runs of held pages, each as a sequence of its own
+    for (int64_t p0 = 0; p0 < (int64_t)kv->pages.size();) {
+        if (kv->pages[(size_t)p0] < 0) {
+            ++p0;
+            continue;
+        }
+        int64_t p1 = p0;
+        while (p1 < (int64_t)kv->pages.size() && kv->pages[(size_t)p1] >= 0) ++p1;
+        const int64_t r0 = p0 * FTX_PAGE, rows = std::min(p1 * FTX_PAGE, n) - r0;
+        const ftx_paged_seq seq{kv->pages.data() + p0, p1 - p0, 0, rows, nullptr};
+        const ftx_plan_args pa{&seq, 1, 0, 0, 0};
+        ftx_plan* plan;
+        int rc = paged_step_plan(ctx, kv->pool, pa, &plan);
+        if (rc) return rc;
+        const size_t b = (size_t)(rows * kdim) * sizeof(float);
+        for (int64_t l = 0; l < kv->n_layer; ++l) {
+            const int64_t at = (l * kv->cap + r0) * kdim;
+            if (to_device) {
+                FTX_HIP(ctx, hipMemcpyAsync(ws, kh + at, b, hipMemcpyHostToDevice, st));
+                FTX_HIP(ctx, hipMemcpyAsync(ws + rows * kdim, vh + at, b, hipMemcpyHostToDevice, st));
+                rc = paged_write_rows(plan, l, ws, kdim, ws + rows * kdim, kdim);
+                if (rc) return rc;
+            } else {
+                rc = paged_read_rows(plan, l, 0, ws, kdim, ws + rows * kdim, kdim);
+                if (rc) return rc;
+                FTX_HIP(ctx, hipMemcpyAsync(kh + at, ws, b, hipMemcpyDeviceToHost, st));
+                FTX_HIP(ctx, hipMemcpyAsync(vh + at, ws + rows * kdim, b, hipMemcpyDeviceToHost, st));
+            }
+        }
+        p0 = p1;
+    }
+    FTX_HIP(ctx, hipStreamSynchronize(st));
+    return FTX_OK;
+}
+
 int ftx_kv_write(ftx_kv* kv, const void* k, const void* v) {
     if (!kv || !k || !v) return FTX_E_INVALID;
+    if (kv->pool) return kv_copy_paged(kv, (float*)k, (float*)v, true);
     return kv_copy(kv, (void*)k, (void*)v, true);
 }
 
 int ftx_kv_read(ftx_kv* kv, void* k, void* v) {
     if (!kv || !k || !v) return FTX_E_INVALID;
+    if (kv->pool) return kv_copy_paged(kv, (float*)k, (float*)v, false);
     return kv_copy(kv, k, v, false);
 }
 
@@ -1119,6 +1291,17 @@ int ftx_kv_pointers(ftx_kv* kv, void** k, void** v, int64_t* npast) {
 int ftx_kv_truncate(ftx_kv* kv, int64_t npast) {
     if (!kv) return FTX_E_INVALID;
     if (npast < 0 || npast > kv->cap) return ftx_fail(kv->ctx, FTX_E_RANGE, "npast out of range");
+    if (kv->pool) {
+        const int64_t held = (npast + FTX_PAGE - 1) / FTX_PAGE;
+        if (held > (int64_t)kv->pages.size())
+            return ftx_fail(kv->ctx, FTX_E_RANGE, "truncate: a paged cache does not hold that many tokens");
+        const auto un = kv_unseen(kv, npast);
+        for (int64_t i = 0; i < held; ++i)
+            if (kv->pages[(size_t)i] < 0 && (i < un.first || i >= un.second))
+                return ftx_fail(kv->ctx, FTX_E_RANGE, "truncate: the window's pages are gone");
+        kv_drop(kv, held, (int64_t)kv->pages.size());
+        kv->pages.resize((size_t)held);
+    }
     kv->npast = npast;
     return FTX_OK;
 }
@@ -1145,7 +1328,29 @@ int ftx_kv_commit(ftx_kv* kv, const int32_t* nodes, int64_t n) {
         a.nodes[i] = j;
         moves |= j != i;
     }
-    if (moves) FTX_HIP(ctx, launch_kv_commit(ctx->stream, a, kv->k, kv->v, kv->kv_f16));
+    if (kv->pool && n > 0 && kv->npast + nodes[n - 1] >= (int64_t)kv->pages.size() * FTX_PAGE)
+        return ftx_fail(ctx, FTX_E_RANGE, "kv_commit: node out of range");
+    if (moves && kv->pool) {
+        PagedMove pm{};
+        pm.data = kv->pool->data;
+        pm.block = kv->pool->block;
+        pm.n_pages = kv->pool->n_pages;
+        pm.n_kv = (int)kv->n_kv;
+        pm.hd = (int)kv->hd;
+        pm.q8 = kv->pool->q8;
+        pm.n_layer = (int)kv->n_layer;
+        pm.n = (int)n;
+        auto at = [&](int64_t pos) {
+            return (int32_t)(kv->pages[(size_t)(pos / FTX_PAGE)] * FTX_PAGE + pos % FTX_PAGE);
+        };
+        for (int64_t i = 0; i < n; ++i) {
+            pm.src[i] = at(kv->npast + nodes[i]);
+            pm.dst[i] = at(kv->npast + i);
+        }
+        FTX_HIP(ctx, launch_paged_move(ctx->stream, pm));
+    } else if (moves) {
+        FTX_HIP(ctx, launch_kv_commit(ctx->stream, a, kv->k, kv->v, kv->kv_f16));
+    }
     kv->npast += n;
     return FTX_OK;
 }
@@ -1168,6 +1373,9 @@ int ftx_verify_batch(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* seqs, int64
         for (int64_t r = 0; r < s; ++r)
             if (seqs[r].kv == seqs[s].kv)
                 return ftx_fail(ctx, FTX_E_INVALID, "two sequences share a kv cache");
+        const ftx_kv *k0 = seqs[0].kv, *ks = seqs[s].kv;
+        if (ks->pool != k0->pool || ks->window != k0->window || ks->sinks != k0->sinks)
+            return ftx_fail(ctx, FTX_E_INVALID, "sequences of one step differ in pool, window or sinks");
         Mt += seqs[s].M;
     }
     if (Mt > m->Mmax) return ftx_fail(ctx, FTX_E_INVALID, "tokens of all sequences above max_tokens");
@@ -1183,10 +1391,8 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
         int rc = check_seq(ctx, m, kv, M, a->tokens);
         if (rc) return rc;
     }
-    if (M > 8 || m->has_ext) {
-        const ftx_seq_args sa{kv, M, a->tokens, a->parents, a->logits, a->advance, 0};
-        return verify_large(ctx, m, &sa, 1);
-    }
+    const ftx_seq_args sa{kv, M, a->tokens, a->parents, a->logits, a->advance, 0};
+    if (M > 8 || m->has_ext) return verify_large(ctx, m, &sa, 1);
     const int64_t npast = kv->npast;
     // host-side argument prep: tokens, depth, ancestor masks, npast
     const int aw = (int)((M + 31) / 32);
@@ -1227,6 +1433,8 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
             cs[(i * hd2 + p) * 2] = (float)cn;
             cs[(i * hd2 + p) * 2 + 1] = (float)sn;
         }
+    ftx_plan* plan = nullptr;
+    if ((rc = step_pages(ctx, d.n_head, &sa, 1, &plan))) return rc;
     hipStream_t st = ctx->stream;
     m->toks = (int32_t*)m->args;
     m->depth = (int32_t*)(m->args + AL.depth);
@@ -1354,8 +1562,8 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
                           seg(T[FTX_T_V], m->qkv + m->qdim + m->kdim, m->ldq)};
         uint8_t* kl = (uint8_t*)kv->k + (size_t)(l * kv->cap_alloc * kv->kdim) * kvel;
         uint8_t* vl = (uint8_t*)kv->v + (size_t)(l * kv->cap_alloc * kv->kdim) * kvel;
-        const bool mattn = attn_mfma_supported(d.head_dim, kv->kv_f16, M, d.n_head, d.n_head_kv,
-                                               kv->cap_alloc);
+        const bool mattn = !plan && attn_mfma_supported(d.head_dim, kv->kv_f16, M, d.n_head,
+                                                        d.n_head_kv, kv->cap_alloc);
         // RoPE and the KV write ride on the projection's epilogue when the
         // MFMA kernels take both (interleaved pairs are adjacent outputs)
         const bool fuse = mattn && !d.rope_neox && mv_all(tqkv, 3, D, M);
@@ -1417,6 +1625,11 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
             am.out = m->att;
             TRACED_IDEM(TK_ATTENTION, attn_b,
                         launch_attn_mfma(st, am, kv->attn_part, o_xq ? m->xq : nullptr, o_rd));
+        } else if (plan) {
+            const float* kr = m->qkv + m->qdim;
+            rc = paged_write_rows(plan, l, kr, m->ldq, kr + m->kdim, m->ldq);
+            if (!rc) rc = paged_attend_rows(plan, l, m->qkv, m->ldq, m->att, m->qdim);
+            if (rc) return rc;
         } else {
             AttnArgs aa{m->qkv,  m->ldq, kl,       vl,          kv->kv_f16, m->npast,
                         m->anc,  aw,     d.n_head, d.n_head_kv, d.head_dim, npast + M,

@@ -132,6 +132,7 @@ def load(path=LIB_PATH):
         "ftx_model_create": (C.c_int, [_vp, C.POINTER(ModelDesc), C.POINTER(_vp)]),
         "ftx_model_free": (C.c_int, [_vp]),
         "ftx_kv_create": (C.c_int, [_vp, _vp, _i64, C.c_int, C.POINTER(_vp)]),
+        "ftx_kv_create_paged": (C.c_int, [_vp, _vp, _vp, _i64, _i64, _i64, C.POINTER(_vp)]),
         "ftx_kv_free": (C.c_int, [_vp]),
         "ftx_kv_pointers": (C.c_int, [_vp, C.POINTER(_vp), C.POINTER(_vp), C.POINTER(_i64)]),
         "ftx_kv_truncate": (C.c_int, [_vp, _i64]),
@@ -335,7 +336,7 @@ class Context:
         h = _vp()
         self.check(self.lib.ftx_pool_create(self.h, n_layer, n_head_kv, head_dim, n_pages,
                                             kv_dtype, C.byref(h)))
-        return Pool(self, h.value)
+        return Pool(self, h.value, kv_dtype)
 
     # ---- verify path ----
     def model(self, cfg, tensors, max_tokens=64):
@@ -444,8 +445,8 @@ def plan_args(seqs, n_head=0, window=0, sinks=0):
 class Pool:
     """Pages of a paged KV cache (ftx_pool_*)."""
 
-    def __init__(self, ctx, handle):
-        self.ctx, self.handle = ctx, handle
+    def __init__(self, ctx, handle, kv_dtype):
+        self.ctx, self.handle, self.kv_dtype = ctx, handle, kv_dtype
 
     @property
     def available(self):
@@ -516,6 +517,13 @@ class Model:
                                                   C.byref(h)))
         return KV(self.ctx, h.value, self.cfg, cap, kv_dtype)
 
+    def kv_paged(self, pool, cap, window=0, sinks=0):
+        """A cache of up to cap tokens in pages of `pool`; its host arrays are fp32."""
+        h = _vp()
+        self.ctx.check(self.ctx.lib.ftx_kv_create_paged(self.ctx.h, self.handle, pool.handle, cap,
+                                                        window, sinks, C.byref(h)))
+        return KV(self.ctx, h.value, self.cfg, cap, pool.kv_dtype, paged=True)
+
     def verify(self, kv, tokens, logits_ptr, parents=None, advance=False):
         toks = np.ascontiguousarray(tokens, np.int32)
         par = None if parents is None else np.ascontiguousarray(parents, np.int32)
@@ -570,8 +578,9 @@ class Model:
 
 
 class KV:
-    def __init__(self, ctx, handle, cfg, cap, kv_dtype):
+    def __init__(self, ctx, handle, cfg, cap, kv_dtype, paged=False):
         self.ctx, self.handle, self.cap, self.kv_dtype = ctx, handle, cap, kv_dtype
+        self.host_dtype = np.float16 if kv_dtype == KV_F16 and not paged else np.float32
         self.shape = (cfg["n_layer"], cap, cfg["n_head_kv"] * cfg["head_dim"])
 
     def pointers(self):
@@ -596,14 +605,14 @@ class KV:
     def write(self, k, v):
         """Copy host arrays shaped like self.shape (the reference layout)
         into the cache."""
-        dt = np.float16 if self.kv_dtype == KV_F16 else np.float32
+        dt = self.host_dtype
         k = np.ascontiguousarray(k, dt)
         v = np.ascontiguousarray(v, dt)
         assert k.shape == self.shape and v.shape == self.shape
         self.ctx.check(self.ctx.lib.ftx_kv_write(self.handle, k.ctypes.data, v.ctypes.data))
 
     def read(self):
-        dt = np.float16 if self.kv_dtype == KV_F16 else np.float32
+        dt = self.host_dtype
         k = np.empty(self.shape, dt)
         v = np.empty(self.shape, dt)
         self.ctx.check(self.ctx.lib.ftx_kv_read(self.handle, k.ctypes.data, v.ctypes.data))

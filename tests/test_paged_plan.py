@@ -11,10 +11,10 @@ I32 = np.int32
 
 
 def probe(seqs, n_kv=2, n_head=4, window=0, sinks=0, n_pages=64, taken=None, cu=256, hd=64, most=100000):
-    """(code, message, items [n][8], joins [n][4]) of a step's tables."""
+    """(code, message, items [n][8] (without their sequences), joins [n][4]) of a step's tables."""
     a, keep = ftx.plan_args(seqs, n_head, window, sinks)
     tk = np.ones(n_pages, np.uint8) if taken is None else np.asarray(taken, np.uint8)
-    items, combs = np.zeros((most, 8), I32), np.zeros((most, 4), I32)
+    items, combs = np.zeros((most, 24), I32), np.zeros((most, 4), I32)
     ni, nc, msg = C.c_int64(0), C.c_int64(0), C.create_string_buffer(256)
     f = ftx.load().paged_probe
     f.restype = C.c_int
@@ -22,7 +22,7 @@ def probe(seqs, n_kv=2, n_head=4, window=0, sinks=0, n_pages=64, taken=None, cu=
                   C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_char_p, C.c_int64]
     rc = f(C.byref(a), n_kv, hd, n_pages, tk.ctypes.data, cu, items.ctypes.data, C.byref(ni),
            combs.ctypes.data, C.byref(nc), most, msg, 256)
-    return rc, msg.value.decode(), items[:ni.value], combs[:nc.value]
+    return rc, msg.value.decode(), items[:ni.value, :8], combs[:nc.value]
 
 
 def tree_mask(par):

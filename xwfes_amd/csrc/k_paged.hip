@@ -1,5 +1,8 @@
 // k_paged.hip -- kernels of the paged KV caches: rows quantised into their
 // pages and read back, and the attention of new tokens over pages.
+#include <algorithm>
+#include <type_traits>
+
 #include "mm_dev.h"
 #include "paged.h"
 
@@ -27,15 +30,44 @@ __device__ __forceinline__ void st4(float* p, v4f v, bool vec) {
     for (int i = 0; i < 4; ++i) p[i] = v[i];
 }
 
-// 127 x / a rounded to the nearest integer, ties to even.  The fp32 quotient
-// is off by less than 2e-5; where that could matter the quotient is formed in
-// 64 bits, whose rounding cannot cross a half: |254 x - (2 n + 1) a| is 0 or
-// at least 2^-31 of its terms.
-__device__ __forceinline__ int q8_round(float x, float a, float inv) {
-    const float f = x * inv;
-    float n = rintf(f);
-    if (fabsf(f - n) > 0.4999f) n = (float)rint((double)x * 127.0 / (double)a);
-    return (int)n;
+// The largest of v over aligned groups of W lanes (16, 32 or 64), in all of
+// them: within 16 lanes by DPP, whose moves cost no LDS round trip
+template <int W>
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+    auto step = [&](auto ctrl) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, false);
+        v = v > o ? v : o;
+    };
+    step(std::integral_constant<int, 0xB1>{});   // quad_perm [1, 0, 3, 2]
+    step(std::integral_constant<int, 0x4E>{});   // quad_perm [2, 3, 0, 1]
+    step(std::integral_constant<int, 0x141>{});  // mirrored in 8 lanes
+    step(std::integral_constant<int, 0x140>{});  // mirrored in 16
+#pragma unroll
+    for (int o = 16; o < W; o <<= 1) {
+        const uint32_t t = (uint32_t)__shfl_xor((int)v, o, 64);
+        v = v > t ? v : t;
+    }
+    return v;
+}
+
+// 127 x / a + 128 rounded to the nearest integer, ties to even, in the low byte
+// of b; inv is 127 / a to 2^-22, so the product is off by less than 4e-5.
+// Nearer than 1e-4 to a half the quotient is formed in 64 bits, whose rounding
+// cannot cross a half: |254 x - (2 n + 1) a| is 0 or at least 2^-31 of its
+// terms.  big: so large a row that its reciprocal is not to be had.
+template <int N>
+__device__ __forceinline__ void q8_bits(const float (&x)[N], float a, float inv, bool big, uint32_t (&b)[N]) {
+    constexpr float MAGIC = 12582912.f + 128.f;  // 1.5 2^23: units in the last place
+    float off = big ? 1.f : 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float t = __builtin_fmaf(x[i], inv, MAGIC);
+        b[i] = __builtin_bit_cast(uint32_t, t);
+        off = fmaxf(off, fabsf(__builtin_fmaf(x[i], inv, MAGIC - t)));
+    }
+    if (off > 0.4999f)
+#pragma unroll
+        for (int i = 0; i < N; ++i) b[i] = (uint32_t)((int)rint((double)x[i] * 127.0 / (double)a) + 128);
 }
 
 // The power of two that a row of halves is stored under
@@ -43,58 +75,181 @@ __device__ __forceinline__ int f16_exp(float a) {
     return a >= 0.00390625f && a <= 65504.f ? 0 : (int)((__builtin_bit_cast(uint32_t, a) >> 23) & 255) - 127 - 14;
 }
 
+// A workgroup of the store and of the read-back takes K or V of one page and kv
+// head (its x: page, then head, then K or V: the heads' pieces of a token's row
+// are written at about the same time, or the pieces of one head, a row apart,
+// meet in a few memory channels: 162 us instead of 121 to read back 57138
+// tokens of 8 heads of 128): slots s0 .. s1 - 1 of it, row by row where
+// they are few, else the page's values as they lie in memory through LDS, so
+// that both sides of the copy are whole runs (32 lanes a row of 128 floats;
+// 16 bytes a thread of the page).
+struct PageRows {
+    uint8_t* vals;  // the page's K or V values
+    float* scale;
+    int s0, s1;
+    int64_t row;  // of slot 0 in the matrix (it may lie before its start)
+    int col;      // the kv head's first float
+    bool isv;
+};
+template <int HD, bool Q8>
+__device__ __forceinline__ PageRows page_rows(const PagedView& p, int context) {
+    const PagedSeq sq = p.seqs[blockIdx.y];
+    const int from = context ? 0 : sq.npast;
+    const int z = blockIdx.x % (2 * p.n_kv);
+    const int first = from / FTX_PAGE + blockIdx.x / (2 * p.n_kv);  // the page's place in the table
+    PageRows r{};
+    r.s0 = max(from - first * FTX_PAGE, 0);
+    r.s1 = min(FTX_PAGE, sq.npast + sq.M - first * FTX_PAGE);
+    if (r.s0 >= r.s1) return r;
+    const int kvh = z >> 1;
+    r.isv = z & 1;
+    uint8_t* blk = page_block(p, p.table[sq.tab0 + first], kvh);
+    r.vals = blk + (r.isv ? paged_values_bytes(HD, Q8) : 0);
+    r.scale = (float*)(blk + 2 * paged_values_bytes(HD, Q8)) + (r.isv ? FTX_PAGE : 0);
+    r.row = (int64_t)first * FTX_PAGE + (context ? sq.all0 : (int64_t)sq.tok0 - sq.npast);
+    r.col = kvh * HD;
+    return r;
+}
+constexpr int ROWS_FEW = 16;  // up to here a wave a row is no slower
+
+// |x| as an integer: ordered as the magnitudes are, infinity and NaN above all
+__device__ __forceinline__ uint32_t mag(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7FFFFFFFu; }
+
+// How a row of largest magnitude `amax` (mag) is stored
+template <bool Q8>
+struct RowForm {
+    float a, by;
+    bool ok, zero;
+    __device__ __forceinline__ explicit RowForm(uint32_t amax) {
+        a = __builtin_bit_cast(float, amax);
+        ok = a <= FLT_BIG;
+        zero = !ok || a < ROW_TINY;
+        if constexpr (Q8)
+            by = zero ? 0.f : 127.f * __builtin_amdgcn_rcpf(a);
+        else
+            by = zero ? 0.f : ldexpf(1.f, -f16_exp(a));
+    }
+    __device__ __forceinline__ float scale() const {
+        if (!ok) return __builtin_nanf("");
+        if constexpr (Q8) return zero ? 0.f : a / 127.f;
+        return zero ? 1.f : ldexpf(1.f, f16_exp(a));
+    }
+    // the values' bits in the page, in the low byte (half) of b; finite
+    // whatever the row holds
+    template <int N>
+    __device__ __forceinline__ void bits(const float (&x)[N], uint32_t (&b)[N]) const {
+        if constexpr (Q8) {
+            q8_bits(x, a, by, !zero && a > 1e36f, b);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                b[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(ok ? x[i] * by : 0.f));
+        }
+    }
+};
+
+// The page's image in LDS: 16-byte unit u at u ^ (4 bits of what lies above
+// it), so that the units of one slot's dims (or one slot group's) lie in
+// different banks: 8- to 16-way conflicts without it
+__device__ __forceinline__ int image_unit(int u) { return u ^ (((u >> 4) ^ (u >> 6)) & 15); }
+__device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4) * 16 + (byte & 15); }
+
 // ---------------------------------------------------------------- write
-// Workgroup (page x of sequence y's new tokens, kv head z); a wave per row.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
-    constexpr int E = HD / 64;  // values a lane
-    const PagedSeq sq = p.seqs[blockIdx.y];
-    const int first = sq.npast / FTX_PAGE + blockIdx.x;  // the page's place in the table
-    const int s0 = max(first * FTX_PAGE, sq.npast), s1 = min(first * FTX_PAGE + FTX_PAGE, sq.npast + sq.M);
-    if (s0 >= s1) return;
-    const int kvh = blockIdx.z, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    uint8_t* blk = page_block(p, p.table[sq.tab0 + first], kvh);
-    const int64_t vb = paged_values_bytes(HD, Q8);
-    float* scale = (float*)(blk + 2 * vb);
-    for (int i = w; i < 2 * (s1 - s0); i += 4) {
-        const bool isv = i & 1;
-        const int pos = s0 + (i >> 1), slot = pos % FTX_PAGE;
-        const int64_t row = sq.tok0 + (pos - sq.npast);
-        const float* src = (isv ? v + row * ldv : k + row * ldk) + (int64_t)kvh * HD + E * lane;
-        float x[E], a = 0.f;
-        bool fin = true;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = src[e];
-            fin = fin && fabsf(x[e]) <= FLT_BIG;
-            a = fmaxf(a, fabsf(x[e]));
-        }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor(a, o, 64));
-        const bool ok = !__builtin_amdgcn_ballot_w64(!fin), zero = !ok || a < ROW_TINY;
-        uint8_t* dst = blk + (isv ? vb : 0);
-        float sc;
-        if constexpr (Q8) {
-            const float inv = 127.f / a;
-            sc = zero ? 0.f : a / 127.f;
+    constexpr int E = HD / 64, D4 = HD / 4, EB = Q8 ? 1 : 2;
+    __shared__ uint4 img[HD * FTX_PAGE * EB / 16];
+    __shared__ uint32_t amax[FTX_PAGE];
+    const PageRows pr = page_rows<HD, Q8>(p, 0);
+    if (pr.s0 >= pr.s1) return;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    const int64_t ld = pr.isv ? ldv : ldk;
+    const float* src = (pr.isv ? v : k) + pr.row * ld + pr.col;
+    if (pr.s1 - pr.s0 < ROWS_FEW) {
+        for (int slot = pr.s0 + w; slot < pr.s1; slot += 4) {
+            float x[E];
+            uint32_t a = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const int q = zero ? 0 : q8_round(x[e], a, inv);
-                const int d = E * lane + e;
-                dst[isv ? paged_v_at(slot, d, 1) : paged_k_at(slot, d, 1)] = (uint8_t)(q + 128);
+                x[e] = src[slot * ld + E * lane + e];
+                a = max(a, mag(x[e]));
             }
+            const RowForm<Q8> f(group_max<64>(a));
+            uint32_t b[E];
+            f.bits(x, b);
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int d = E * lane + e;
+                uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8));
+                if constexpr (Q8)
+                    *t = (uint8_t)b[e];
+                else
+                    *(uint16_t*)t = (uint16_t)b[e];
+            }
+            if (lane == 0) pr.scale[slot] = f.scale();
+        }
+        return;
+    }
+    const bool vec = !(((uintptr_t)src | (uintptr_t)(ld * 4)) & 15);
+    uint8_t* im = (uint8_t*)img;
+    // four dims of four consecutive slots a thread: K's run along the dims, V's
+    // along the slots
+#pragma unroll
+    for (int i0 = 0; i0 < FTX_PAGE / 4 * D4; i0 += 256) {
+        const int i = i0 + tid, g = i / D4, d = i % D4 * 4;
+        v4f x[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int slot = 4 * g + r;
+            x[r] = slot >= pr.s0 && slot < pr.s1 ? ld4(src + slot * ld + d, vec) : v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        uint32_t bits[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint32_t a =
+                group_max<D4>(max(max(mag(x[r][0]), mag(x[r][1])), max(mag(x[r][2]), mag(x[r][3]))));
+            const RowForm<Q8> f(a);
+            const float xr[4] = {x[r][0], x[r][1], x[r][2], x[r][3]};
+            f.bits(xr, bits[r]);
+            if (d == 0) amax[4 * g + r] = a;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            // K: slot 4 g + r, dims d ..+3; V: dim d + r, slots 4 g ..+3
+            uint32_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = pr.isv ? bits[e][r] : bits[r][e];
+            uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, Q8) : paged_k_at(4 * g + r, d, Q8));
+            if constexpr (Q8)
+                *(uint32_t*)t = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u),
+                                                      __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), 0x05040100u);
+            else
+                *(uint2*)t = uint2{b[0] | b[1] << 16, b[2] | b[3] << 16};
+        }
+    }
+    __syncthreads();
+    if (tid >= pr.s0 && tid < pr.s1) pr.scale[tid] = RowForm<Q8>(amax[tid]).scale();
+    const bool full = pr.s0 == 0 && pr.s1 == FTX_PAGE;
+    for (int u = tid; u < HD * FTX_PAGE * EB / 16; u += 256) {
+        if (full) {
+            ((uint4*)pr.vals)[u] = img[image_unit(u)];
+        } else if (!pr.isv) {
+            const int slot = 16 * ((u >> 6) & 3) + (u & 15);
+            if (slot >= pr.s0 && slot < pr.s1) ((uint4*)pr.vals)[u] = img[image_unit(u)];
         } else {
-            const int ex = zero ? 0 : f16_exp(a);
-            sc = ldexpf(1.f, ex);
+            // a unit holds 16 (8) slots: those of other tokens stay
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int d = E * lane + e;
-                *(_Float16*)(dst + (isv ? paged_v_at(slot, d, 0) : paged_k_at(slot, d, 0))) =
-                    zero ? (_Float16)0.f : (_Float16)ldexpf(x[e], -ex);
+            for (int x = 0; x < 16 / EB; ++x) {
+                const int st = Q8 ? x >> 2 : 2 * ((u >> 6) & 1) + (x >> 2);
+                const int slot = 16 * st + 4 * ((u >> 4) & 3) + (x & 3);
+                if (slot < pr.s0 || slot >= pr.s1) continue;
+                if constexpr (Q8)
+                    pr.vals[u * 16 + x] = im[image_unit(u) * 16 + x];
+                else
+                    ((uint16_t*)pr.vals)[u * 8 + x] = ((const uint16_t*)im)[image_unit(u) * 8 + x];
             }
         }
-        if (lane == 0) scale[(isv ? FTX_PAGE : 0) + slot] = ok ? sc : __builtin_nanf("");
     }
 }
 
@@ -102,29 +257,50 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, float* __restrict__ k, int64_t ldk,
                                                     float* __restrict__ v, int64_t ldv) {
-    constexpr int E = HD / 64;
-    const PagedSeq sq = p.seqs[blockIdx.y];
-    const int from = context ? 0 : sq.npast;
-    const int first = from / FTX_PAGE + blockIdx.x;
-    const int s0 = max(first * FTX_PAGE, from), s1 = min(first * FTX_PAGE + FTX_PAGE, sq.npast + sq.M);
-    if (s0 >= s1) return;
-    const int kvh = blockIdx.z, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const uint8_t* blk = page_block(p, p.table[sq.tab0 + first], kvh);
-    const int64_t vb = paged_values_bytes(HD, Q8);
-    const float* scale = (const float*)(blk + 2 * vb);
-    for (int i = w; i < 2 * (s1 - s0); i += 4) {
-        const bool isv = i & 1;
-        const int pos = s0 + (i >> 1), slot = pos % FTX_PAGE;
-        const int64_t row = context ? sq.all0 + pos : (int64_t)sq.tok0 + (pos - sq.npast);
-        float* dst = (isv ? v + row * ldv : k + row * ldk) + (int64_t)kvh * HD + E * lane;
-        const uint8_t* src = blk + (isv ? vb : 0);
-        const float sc = scale[(isv ? FTX_PAGE : 0) + slot];
+    constexpr int E = HD / 64, D4 = HD / 4, EB = Q8 ? 1 : 2;
+    __shared__ uint4 img[HD * FTX_PAGE * EB / 16];
+    const PageRows pr = page_rows<HD, Q8>(p, context);
+    if (pr.s0 >= pr.s1) return;
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
+    const int64_t ld = pr.isv ? ldv : ldk;
+    float* dst = (pr.isv ? v : k) + pr.row * ld + pr.col;
+    if (pr.s1 - pr.s0 < ROWS_FEW) {
+        for (int slot = pr.s0 + w; slot < pr.s1; slot += 4) {
+            const float sc = pr.scale[slot];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = E * lane + e;
-            const int at = isv ? paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8);
-            const float q = Q8 ? (float)((int)src[at] - 128) : (float)*(const _Float16*)(src + at);
-            dst[e] = q * sc;
+            for (int e = 0; e < E; ++e) {
+                const int d = E * lane + e;
+                const uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8));
+                dst[slot * ld + d] = (Q8 ? (float)((int)*t - 128) : (float)*(const _Float16*)t) * sc;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int u = tid; u < HD * FTX_PAGE * EB / 16; u += 256) img[image_unit(u)] = ((const uint4*)pr.vals)[u];
+    __syncthreads();
+    const bool vec = !(((uintptr_t)dst | (uintptr_t)(ld * 4)) & 15);
+    const uint8_t* im = (const uint8_t*)img;
+#pragma unroll
+    for (int i0 = 0; i0 < FTX_PAGE / 4 * D4; i0 += 256) {
+        const int i = i0 + tid, g = i / D4, d = i % D4 * 4;
+        float q[4][4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, Q8) : paged_k_at(4 * g + r, d, Q8));
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                q[r][e] = Q8 ? (float)((*(const uint32_t*)t >> (8 * e)) & 255) : (float)((const _Float16*)t)[e];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int slot = 4 * g + r;
+            if (slot < pr.s0 || slot >= pr.s1) continue;
+            const float sc = pr.scale[slot];
+            v4f y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = ((pr.isv ? q[e][r] : q[r][e]) - (Q8 ? 128.f : 0.f)) * sc;
+            st4(dst + slot * ld + d, y, vec);
         }
     }
 }
@@ -162,6 +338,14 @@ __device__ __forceinline__ v8h u8x8(uint32_t a, uint32_t b) {
     const v2h h2 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, 0x64646464u, 0x00050004u)) + o;
     const v2h h3 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, 0x64646464u, 0x00070006u)) + o;
     return v8h{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+}
+
+// A product rounded once, in a register: converted to halves in two places, it
+// could otherwise be rounded from its exact value in one of them, and a low
+// half would not fit its high half (seen: one weight in some 2^13 off by 2^-11).
+__device__ __forceinline__ float rounded(float x) {
+    asm("" : "+v"(x));
+    return x;
 }
 
 __device__ __forceinline__ int f_exp(float x) {  // floor(log2 x) of a normal x
@@ -213,7 +397,7 @@ struct WaveAttn {
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
                 v2h h, lo;
-                split_hl2(x[dc][i >> 2][i & 3] * qs, x[dc][i >> 2][(i & 3) + 1] * qs, h, lo);
+                split_hl2(rounded(x[dc][i >> 2][i & 3] * qs), rounded(x[dc][i >> 2][(i & 3) + 1] * qs), h, lo);
                 qh[dc][i] = h[0];
                 qh[dc][i + 1] = h[1];
                 ql[dc][i] = lo[0];
@@ -223,53 +407,85 @@ struct WaveAttn {
         for (int dt = 0; dt < NDT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    __device__ __forceinline__ v8h k_frag(const uint8_t* blk, int st, int dc, int lane) const {
-        if constexpr (Q8) {
-            const uint4 u = *(const uint4*)(blk + (((dc >> 1) * 4 + st) * 64 + lane) * 16);
-            return dc & 1 ? u8x8(u.z, u.w) : u8x8(u.x, u.y);
-        } else {
-            return *(const v8h*)(blk + ((dc * 4 + st) * 64 + lane) * 16);
+    // A page's loads, issued together: the values of K (or V) as this lane's
+    // operands, 16 bytes each, and the lane's 16 K and V scales
+    static constexpr int NL = HD / (Q8 ? 16 : 8);  // 16-byte loads of K or of V
+    struct Vals {
+        uint4 u[NL];
+    };
+    struct Scales {
+        v4f k[4], v[4];
+    };
+    static __device__ __forceinline__ void load_vals(Vals& x, const uint8_t* vals, int lane) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
+    }
+    static __device__ __forceinline__ void load_scales(Scales& x, const uint8_t* blk, int kq) {
+        const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            x.k[st] = *(const v4f*)(scale + 16 * st + 4 * kq);
+            x.v[st] = *(const v4f*)(scale + FTX_PAGE + 16 * st + 4 * kq);
         }
     }
-    __device__ __forceinline__ v8h v_frag(const uint8_t* vals, int dt, int sp, int lane) const {
+    static __device__ __forceinline__ v8h k_frag(const Vals& x, int st, int dc) {
         if constexpr (Q8) {
-            const uint4 u = *(const uint4*)(vals + (dt * 64 + lane) * 16);
+            const uint4 u = x.u[(dc >> 1) * 4 + st];
+            return dc & 1 ? u8x8(u.z, u.w) : u8x8(u.x, u.y);
+        } else {
+            return __builtin_bit_cast(v8h, x.u[dc * 4 + st]);
+        }
+    }
+    static __device__ __forceinline__ v8h v_frag(const Vals& x, int dt, int sp) {
+        if constexpr (Q8) {
+            const uint4 u = x.u[dt];
             return sp ? u8x8(u.z, u.w) : u8x8(u.x, u.y);
         } else {
-            return *(const v8h*)(vals + ((dt * 2 + sp) * 64 + lane) * 16);
+            return __builtin_bit_cast(v8h, x.u[dt * 2 + sp]);
         }
     }
 
-    // one page; seen(st, r): whether the row sees the slot (whole: it sees all)
-    template <typename Seen>
-    __device__ __forceinline__ void page(const uint8_t* blk, int lane, bool whole, Seen seen) {
-        const int kq = lane >> 4;
-        const uint8_t* vals = blk + paged_values_bytes(HD, Q8);
-        const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
-        v4f s[4], ks[4], vs[4];
-#pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            ks[st] = *(const v4f*)(scale + 16 * st + 4 * kq);
-            vs[st] = *(const v4f*)(scale + FTX_PAGE + 16 * st + 4 * kq);
-        }
+    __device__ __forceinline__ void scores(v4f (&s)[4], const Vals& k) const {
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
             s[st] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int dc = 0; dc < NDC; ++dc) {
-                const v8h kf = k_frag(blk, st, dc, lane);
+                const v8h kf = k_frag(k, st, dc);
                 s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[dc], s[st], 0, 0, 0);
                 s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[dc], s[st], 0, 0, 0);
             }
         }
+    }
+
+    // The page's weights from its scores; the sums so far brought to the new
+    // maximum and V exponent.  seen(st, r): whether the row sees the slot
+    // (whole: it sees all)
+    template <typename Seen>
+    __device__ __forceinline__ void soften(v4f (&s)[4], const Scales& sc, bool whole, Seen seen, v8h (&ph)[2],
+                                           v8h (&pl)[2]) {
+        v4f vs[4];
         float mx = -INFINITY, vm = 0.f;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const bool ok = whole || seen(st, r);
-                s[st][r] = ok ? (s[st][r] * c2) * ks[st][r] : -INFINITY;
-                vs[st][r] = ok ? vs[st][r] : 0.f;
+                s[st][r] = (s[st][r] * c2) * sc.k[st][r];
+                vs[st][r] = sc.v[st][r];
+            }
+        if (!whole)
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const bool ok = seen(st, r);
+                    s[st][r] = ok ? s[st][r] : -INFINITY;
+                    vs[st][r] = ok ? vs[st][r] : 0.f;
+                }
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
                 mx = fmaxf(mx, s[st][r]);
                 vm = fmaxf(vm, vs[st][r]);
             }
@@ -281,12 +497,11 @@ struct WaveAttn {
         const float mr = mn == -INFINITY ? 0.f : mn;  // (nothing seen yet: every p is 0)
         const float al = __builtin_amdgcn_exp2f(m - mr);
         const int en = max(ev, f_exp(vm));  // (vm = 0: -127)
-        const float vscale = ldexpf(1.f, 14 - min(en, 127));
+        const float vscale = ldexpf(1.f, 14 - en);
         const float oal = ldexpf(al, ev - en);
         m = mn;
         ev = en;
         l *= al;
-        v8h ph[2], pl[2];
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
@@ -294,26 +509,28 @@ struct WaveAttn {
                 const float p0 = __builtin_amdgcn_exp2f(s[st][r] - mr);
                 const float p1 = __builtin_amdgcn_exp2f(s[st][r + 1] - mr);
                 l += p0 + p1;
-                // (split_hl2: a high half formed twice, once from the product
-                // unrounded, would not fit its low half)
                 v2h h, lo;
-                split_hl2(p0 * (vs[st][r] * vscale), p1 * (vs[st][r + 1] * vscale), h, lo);
+                split_hl2(rounded(p0 * (vs[st][r] * vscale)), rounded(p1 * (vs[st][r + 1] * vscale)), h, lo);
                 const int i = 4 * (st & 1) + r;
                 ph[st >> 1][i] = h[0];
                 ph[st >> 1][i + 1] = h[1];
                 pl[st >> 1][i] = lo[0];
                 pl[st >> 1][i + 1] = lo[1];
             }
+        if (__builtin_amdgcn_ballot_w64(oal != 1.f))  // (wave-uniform)
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) {
-            o[dt] *= oal;
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= oal;
+    }
+
+    __device__ __forceinline__ void outputs(const Vals& v, const v8h (&ph)[2], const v8h (&pl)[2]) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int sp = 0; sp < 2; ++sp) {
-                const v8h vf = v_frag(vals, dt, sp, lane);
+                const v8h vf = v_frag(v, dt, sp);
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[sp], o[dt], 0, 0, 0);
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[sp], o[dt], 0, 0, 0);
             }
-        }
     }
 };
 
@@ -345,14 +562,16 @@ struct RowSight {
 // there are 8; the item's pages dealt to its four waves, whose softmaxes meet
 // in LDS.
 template <int HD, bool Q8>
-__global__ void __launch_bounds__(256) k_paged_attn(PagedAttn a) {
+__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
     using W = WaveAttn<HD, Q8>;
+    constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
     __shared__ float so[3][4 * W::NDT][64], sm[4][64], sl[4][64];
     __shared__ int se[4][64];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
-    const PagedSeq sq = a.p.seqs[it.seq];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
+    const PagedSeq sq = it.q;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
     const int R = sq.M * a.gqa, rr = it.row0 + col, r = min(rr, R - 1), t = r / a.gqa;
     const int64_t tok = sq.tok0 + t;
     const int head = kvh * a.gqa + r % a.gqa;
@@ -367,11 +586,46 @@ __global__ void __launch_bounds__(256) k_paged_attn(PagedAttn a) {
         hi = min(hi, __shfl_xor(hi, x, 64));
         lo = max(lo, __shfl_xor(lo, x, 64));
     }
-    for (int i = it.i0 + w; i < it.i1; i += 4) {
-        const int pg = i < it.s ? i : it.a + (i - it.s), p0 = pg * FTX_PAGE;
+    // the wave's pages: entries i0 + w, + 4, ..; their ids 64 at a time in the
+    // lanes.  A page's V loads are issued before its scores are formed, the
+    // next page's K loads and scales (PRE) before its softmax, so that each
+    // wait leaves the later loads in flight.
+    const int n = max(0, (it.i1 - it.i0 - w + 3) >> 2);
+    auto place = [&](int j) {  // in the table
+        const int i = it.i0 + w + 4 * j;
+        return i < it.s ? i : it.a + (i - it.s);
+    };
+    int ids = lane < n ? a.p.table[sq.tab0 + place(lane)] : 0;
+    auto block_of = [&](int j) {
+        if ((j & 63) == 0 && j) ids = j + lane < n ? a.p.table[sq.tab0 + place(j + lane)] : 0;
+        return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
+    };
+    typename W::Vals kv, vv;
+    typename W::Scales sc;
+    const uint8_t* blk = nullptr;
+    if (n) {
+        blk = block_of(0);
+        if (PRE) W::load_vals(kv, blk, lane);
+    }
+    for (int j = 0; j < n; ++j) {
+        if (!PRE) W::load_vals(kv, blk, lane);
+        W::load_scales(sc, blk, kq);
+        if (EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
+        __builtin_amdgcn_sched_barrier(0);
+        v4f s[4];
+        wa.scores(s, kv);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
+        if (j + 1 < n) {
+            blk = block_of(j + 1);
+            if (PRE) W::load_vals(kv, blk, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const int p0 = place(j) * FTX_PAGE;
         const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= sight.sinks);
-        const uint8_t* blk = page_block(a.p, a.p.table[sq.tab0 + pg], kvh);
-        wa.page(blk, lane, whole, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); });
+        v8h ph[2], pl[2];
+        wa.soften(s, sc, whole, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
+        wa.outputs(vv, ph, pl);
     }
     wa.l += __shfl_xor(wa.l, 16, 64);
     wa.l += __shfl_xor(wa.l, 32, 64);
@@ -423,39 +677,50 @@ __global__ void __launch_bounds__(256) k_paged_attn(PagedAttn a) {
     }
 }
 
-// Workgroup (row tile with several partials, kv head):
-// out = sum_i 2^(m_i - M) l_i o_i / sum_i 2^(m_i - M) l_i
+// Workgroup (row of a tile with several partials, kv head):
+// out = sum_i 2^(m_i - M) l_i o_i / sum_i 2^(m_i - M) l_i.  Every wave forms M
+// and the sum itself; thread (g, d) adds the partials g, g + G, .. of dims
+// 4 d .. 4 d + 3, the G sums meet in LDS.
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
-    const int kvh = blockIdx.x % a.p.n_kv;
+    constexpr int D4 = HD / 4, G = 256 / D4;
+    __shared__ v4f red[G][D4];
+    const int kvh = blockIdx.x % a.p.n_kv, col = blockIdx.y;
     const PagedComb c = a.combs[blockIdx.x / a.p.n_kv];
     const PagedSeq sq = a.p.seqs[c.seq];
-    const int R = sq.M * a.gqa;
-    const bool vec = !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
-    for (int e = threadIdx.x; e < PAGED_TR * HD / 4; e += 256) {
-        const int col = e / (HD / 4), d = e % (HD / 4) * 4, rr = c.row0 + col;
-        if (rr >= R) continue;
-        const int64_t step = (int64_t)a.p.n_kv * PAGED_TR;
-        const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
-        float M = -INFINITY;
-        for (int i = 0; i < c.n; ++i) M = fmaxf(M, a.pml[2 * (p0 + i * step)]);
-        float den = 0.f;
-        v4f num = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < c.n; ++i) {
-            const float mi = a.pml[2 * (p0 + i * step)];
-            const float f = (mi == M ? 1.f : __builtin_amdgcn_exp2f(mi - M)) * a.pml[2 * (p0 + i * step) + 1];
-            den += f;
-        }
-        for (int i = 0; i < c.n; ++i) {
-            const float mi = a.pml[2 * (p0 + i * step)];
-            const float f = (mi == M ? 1.f : __builtin_amdgcn_exp2f(mi - M)) * a.pml[2 * (p0 + i * step) + 1] / den;
-            const v4f o = *(const v4f*)(a.part + (p0 + i * step) * HD + d);
+    const int rr = c.row0 + col, lane = threadIdx.x & 63;
+    if (rr >= sq.M * a.gqa) return;
+    const int64_t step = (int64_t)a.p.n_kv * PAGED_TR;
+    const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
+    const float2* ml = (const float2*)a.pml + p0;
+    float M = -INFINITY, den = 0.f;
+    for (int i = lane; i < c.n; i += 64) M = fmaxf(M, ml[i * step].x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) num[x] += f * o[x];
-        }
-        const int64_t tok = sq.tok0 + rr / a.gqa;
-        st4(a.out + tok * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD + d, num, vec);
+    for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    auto weight = [&](int i) {
+        const float2 t = ml[i * step];
+        return (t.x == M ? 1.f : __builtin_amdgcn_exp2f(t.x - M)) * t.y;
+    };
+    for (int i = lane; i < c.n; i += 64) den += weight(i);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
+    const int g = threadIdx.x / D4, d = threadIdx.x % D4;
+    v4f num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = g; i < c.n; i += G) {
+        const float f = weight(i) / den;
+        const v4f o = *(const v4f*)(a.part + (p0 + i * step) * HD + 4 * d);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) num[x] += f * o[x];
     }
+    red[g][d] = num;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int x = 1; x < G; ++x) num += red[x][d];
+    const int64_t tok = sq.tok0 + rr / a.gqa;
+    const bool vec = !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
+    st4(a.out + tok * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD + 4 * d, num, vec);
 }
 
 }  // namespace
@@ -469,7 +734,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
 hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_new_pages, const float* k, int64_t ldk,
                               const float* v, int64_t ldv) {
     if (max_new_pages == 0) return hipSuccess;
-    const dim3 grid((unsigned)max_new_pages, (unsigned)p.nseq, (unsigned)p.n_kv);
+    const dim3 grid((unsigned)(max_new_pages * 2 * p.n_kv), (unsigned)p.nseq);
     ktimed_launch(PAGED_CASE(k_paged_write, p.hd, p.q8), grid, dim3(256), 0, st, p, k, ldk, v, ldv);
     return hipGetLastError();
 }
@@ -477,7 +742,7 @@ hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_ne
 hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pages, int context, float* k, int64_t ldk,
                              float* v, int64_t ldv) {
     if (max_pages == 0) return hipSuccess;
-    const dim3 grid((unsigned)max_pages, (unsigned)p.nseq, (unsigned)p.n_kv);
+    const dim3 grid((unsigned)(max_pages * 2 * p.n_kv), (unsigned)p.nseq);
     ktimed_launch(PAGED_CASE(k_paged_read, p.hd, p.q8), grid, dim3(256), 0, st, p, context, k, ldk, v, ldv);
     return hipGetLastError();
 }
@@ -488,7 +753,7 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     ktimed_launch(PAGED_CASE(k_paged_attn, a.p.hd, a.p.q8), grid, dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.n_combs == 0) return e;
-    const dim3 cg((unsigned)a.n_combs * (unsigned)a.p.n_kv);
+    const dim3 cg((unsigned)a.n_combs * (unsigned)a.p.n_kv, (unsigned)std::min(PAGED_TR, a.rows_max));
     auto* comb = a.p.hd == 64 ? k_paged_combine<64> : a.p.hd == 128 ? k_paged_combine<128> : k_paged_combine<256>;
     hipLaunchKernelGGL(comb, cg, dim3(256), 0, st, a);
     return hipGetLastError();

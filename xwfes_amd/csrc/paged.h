@@ -48,11 +48,14 @@ struct PagedSeq {
 };
 // A row tile (PAGED_TR query rows of a kv head: row r = token r / gqa, head
 // r % gqa) over entries i0 .. i1 - 1 of its page list: pages 0 .. s - 1 (the
-// first tokens'), then pages a, a + 1, ..
+// first tokens'), then pages a, a + 1, ..  q: its sequence, held here so that
+// a workgroup's first page is two loads away and not three
 struct PagedItem {
     int32_t seq, row0, i0, i1, s, a;
     int32_t part;  // its partial's place, or -1: the whole list, results go to out
     int32_t pad;
+    PagedSeq q;
+    int32_t fill[6];  // to 96 bytes
 };
 // the partials part0 .. part0 + n - 1 of one row tile
 struct PagedComb {
@@ -68,6 +71,7 @@ struct PagedGeom {
 struct PagedTables {
     int64_t n_head = 0, window = 0, sinks = 0;
     int64_t tokens = 0, rows = 0;  // new tokens, positions of all contexts
+    int64_t longest = 0;            // new tokens of one sequence
     int64_t max_new_pages = 0, max_pages = 0;  // of one sequence
     int64_t parts = 0;
     bool absent = false;  // a page below npast + M is absent
@@ -108,7 +112,7 @@ struct PagedAttn {
     const uint32_t* anc;
     const PagedItem* items;
     const PagedComb* combs;
-    int n_items, n_combs;
+    int n_items, n_combs, rows_max;  // rows_max: query rows of the longest sequence
     int gqa;
     int window, sinks;
     const float* q;

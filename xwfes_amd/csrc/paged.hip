@@ -54,9 +54,10 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         d.dep0 = -1;
         d.all0 = o.rows;
         o.tokens += q.M;
+        o.longest = std::max(o.longest, q.M);
         o.rows += q.npast + q.M;
         if (o.tokens * std::max<int64_t>(a.n_head, 1) >= (int64_t)1 << 31 ||
-            (int64_t)o.table.size() + ntab >= (int64_t)1 << 31)
+            (int64_t)o.table.size() + ntab >= (int64_t)1 << 31 || ntab * 2 * g.n_kv >= (int64_t)1 << 31)
             return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
         const int64_t first_new = q.M ? q.npast / FTX_PAGE : ntab;
         for (int64_t i = 0; i < ntab; ++i) {
@@ -135,7 +136,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         const int64_t np = (t.n + per - 1) / per;
         for (int64_t k = 0; k < np; ++k)
             o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
-                                        t.a, np > 1 ? (int32_t)(o.parts + k) : -1, 0});
+                                        t.a, np > 1 ? (int32_t)(o.parts + k) : -1, 0, o.seqs[(size_t)t.seq], {}});
         if (np > 1) {
             o.combs.push_back(PagedComb{t.seq, t.row0, (int32_t)o.parts, (int32_t)np});
             o.parts += np;
@@ -583,6 +584,7 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.n_items = (int)t.items.size();
     a.n_combs = (int)t.combs.size();
     a.gqa = (int)(t.n_head / p->n_kv);
+    a.rows_max = (int)(t.longest * a.gqa);
     a.window = (int)t.window;
     a.sinks = (int)t.sinks;
     a.q = q;

@@ -9,10 +9,10 @@ most 2^-18 sum |q_i k_ji| / sqrt(hd) (q's two halves: 2^-22; up to 16 MFMA
 accumulations that round by 2^-23; the products with the row's and slot's
 scale 2^-23), which moves every p by as much, twice (p and the sum).  P's two
 halves: 2^-21; of a p so small that its low half is lost, 2^-25 of what the
-halves are scaled to, 2^14 for the row's largest p and V scale, so up to 2^-39
-(2^-38 with the scale's own factor of two) of the largest |v| for each slot
-seen: a bound relative to sum p |v| alone does not hold where the few large p
-meet v near 0.  The outputs' sums round 4 times a page by 2^-23, the softmax
+halves are scaled to (2^10 to 2^14 for the row's largest p and V scale), so up
+to 2^-35 (2^-34 with the scale's own factor of two) of the largest |v| for each
+slot seen: a bound relative to sum p |v| alone does not hold where the few large
+p meet v near 0.  The outputs' sums round 4 times a page by 2^-23, the softmax
 sum 16 times by 2^-24; a join of partials adds 2^-21.
 """
 import ctypes
@@ -156,7 +156,7 @@ class Cache:
             tol = 2 * 2.0 ** -18 * mag + 2.0 ** -20 + 5 * pages * 2.0 ** -23
             outs.append(o)
             n = see.sum(1)[:, None, None]
-            tols.append(np.expm1(np.minimum(tol, 50)) * b + n * 2.0 ** -38 * np.abs(np.nan_to_num(v64)).max(initial=0))
+            tols.append(np.expm1(np.minimum(tol, 50)) * b + n * 2.0 ** -34 * np.abs(np.nan_to_num(v64)).max(initial=0))
         return np.concatenate(outs), np.concatenate(tols)
 
     def check(self, q, **kw):

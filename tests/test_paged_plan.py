@@ -11,10 +11,10 @@ I32 = np.int32
 
 
 def probe(seqs, n_kv=2, n_head=4, window=0, sinks=0, n_pages=64, taken=None, cu=256, hd=64, most=100000):
-    """(code, message, items [n][8] (without their sequences), joins [n][4]) of a step's tables."""
+    """(code, message, items [n][8] (without their sequences), joins [n][5]) of a step's tables."""
     a, keep = ftx.plan_args(seqs, n_head, window, sinks)
     tk = np.ones(n_pages, np.uint8) if taken is None else np.asarray(taken, np.uint8)
-    items, combs = np.zeros((most, 24), I32), np.zeros((most, 4), I32)
+    items, combs = np.zeros((most, 24), I32), np.zeros((most, 5), I32)
     ni, nc, msg = C.c_int64(0), C.c_int64(0), C.create_string_buffer(256)
     f = ftx.load().paged_probe
     f.restype = C.c_int
@@ -128,13 +128,23 @@ def test_items_cover_every_visible_page_once(case):
     rc, msg, items, combs = probe(seqs, n_kv, n_head, window, sinks, n_pages=pages + 1, cu=case.get("cu", 256))
     assert rc == 0, msg
     gqa = n_head // n_kv
-    assert (np.diff(items[:, 3] - items[:, 2]) <= 0).all()  # the longest first
-    parts = sorted(p for p in items[:, 6] if p >= 0)
-    assert parts == list(range(len(parts)))  # every place once
-    joined = sorted(p for c in combs for p in range(c[2], c[2] + c[3]))
-    assert joined == parts and (combs[:, 3] > 1).all()
-    where = {int(p): (int(s), int(r)) for s, r, _, _, _, _, p, _ in items if p >= 0}
-    assert all(where[p] == (c[0], c[1]) for c in combs for p in range(c[2], c[2] + c[3]))
+    # row tiles of 16, then those of 128 (sequences of 65 rows and more), the
+    # longest first in each
+    many = np.array([seqs[s][2] * gqa >= 65 for s in items[:, 0]], bool)
+    assert (np.diff(many.astype(int)) >= 0).all()
+    for part in (items[~many], items[many]):
+        assert (np.diff(part[:, 3] - part[:, 2]) <= 0).all()
+    # a partial is a block of 16 rows: every place once, each joined once
+    places = {}
+    for (s, row0, _, _, _, _, p, _), mn in zip(items, many):
+        for x in range((8 if mn else 1) if p >= 0 else 0):
+            assert p + x not in places
+            places[p + x] = (s, row0 + 16 * x)
+    assert sorted(places) == list(range(len(places)))
+    joined = {p: (c[0], c[1]) for c in combs for p in range(c[2], c[2] + c[3] * c[4], c[4])}
+    assert (combs[:, 3] > 1).all() and len(joined) == combs[:, 3].sum()
+    live = {p: at for p, at in places.items() if at[1] < seqs[at[0]][2] * gqa}
+    assert joined == live
     for s, (_, npast, M, par) in enumerate(seqs):
         see = visible(npast, M, par, window, sinks)
         n = (npast + M + 63) // 64
@@ -143,10 +153,11 @@ def test_items_cover_every_visible_page_once(case):
         want = np.repeat(pad.reshape(M, n, 64).any(2), gqa, axis=0)
         got = np.zeros((M * gqa, n), int)
         for _, row0, i0, i1, sp, a, _, _ in items[items[:, 0] == s]:
-            assert row0 % 16 == 0 and i0 < i1
+            tr = 128 if M * gqa >= 65 else 16
+            assert row0 % tr == 0 and i0 < i1
             pg = np.array([i if i < sp else a + i - sp for i in range(i0, i1)])
             assert (pg >= 0).all() and (pg < n).all() and sp <= a
-            got[row0:row0 + 16, pg] += 1
+            got[row0:row0 + tr, pg] += 1
         assert got.max(initial=0) <= 1 and (got[want] == 1).all()
 
 

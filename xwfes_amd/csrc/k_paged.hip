@@ -352,23 +352,44 @@ __device__ __forceinline__ int f_exp(float x) {  // floor(log2 x) of a normal x
     return (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255) - 127;
 }
 
-// The lowest exponent that V scales are taken relative to: 2^(14 - ev) is
-// finite.  (The smallest scale is 2^-114.)
-constexpr int EV_MIN = -113;
+// The largest of x over the four lanes of a column (l, l ^ 16, l ^ 32, l ^ 48),
+// by exchanging rows of 16 and halves of the wave in registers
+__device__ __forceinline__ float col_max(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false,
+                                              false);
+    x = fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false,
+                                         false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+
+// Levels that V scales are taken relative to: powers of 2^4.  The lowest: 2^-ev
+// is finite; the smallest scale is 2^-114.
+constexpr int EV_MIN = -112;
+__device__ __forceinline__ int ev_level(float vm) {  // 2^level >= vm
+    return max(EV_MIN, ((f_exp(vm) + 4) >> 2) * 4);
+}
 
 // One wave's online softmax over pages for a tile of 16 query rows.  Lane
 // (col, kq) holds the scores of row col at slots 16 st + 4 kq + r and the
 // outputs of row col at dims 16 dt + 4 kq + r.
-// Scores in units of log2: s2 = ((q 2^eq) . k) (2^-eq log2 e / sqrt(hd)) ks.
-// P.V: p vs 2^(14 - ev) is split in two halves, ev the exponent of the largest
-// V scale that the row has seen, so the outputs stand 2^(14 - ev) over.
-template <int HD, bool Q8>
+// The query row is taken times log2 e / sqrt(hd) and a power of two, 2^e, that
+// brings it to [2^6, 2^7); a score in units of log2 is 2^-e s ks exactly as
+// s ks is, so one fma gives the weight's exponent: p = 2^(s ks 2^-e - off).
+// off, as it was rounded, is the running maximum less 12 when it was last taken:
+// it is taken anew where a page's maximum would bring a weight above 2^15 (the
+// products of the sums so far, a third of a page's arithmetic, then fall to one
+// page in ten).  l = sum p, and P.V of p vs 2^-ev in two halves, ev the level
+// of the largest V scale that the row has seen.  out = 2^ev o / l.
+// STAGED: operands come from LDS and are read ahead of the products by hand.
+template <int HD, bool Q8, bool STAGED>
 struct WaveAttn {
     static constexpr int NDC = HD / 32, NDT = HD / 16;
     v8h qh[NDC], ql[NDC];
     v4f o[NDT];
-    float m = -INFINITY, l = 0.f;  // (l: this lane's slots only)
-    float c2;
+    float off = -INFINITY;  // the weights' offset, -inf: nothing seen
+    float l = 0.f;          // (this lane's slots only)
+    float c2;               // 2^-e
     int ev = EV_MIN;
 
     // the query row at q, this lane's dims
@@ -380,18 +401,20 @@ struct WaveAttn {
             const int d0 = Q8 ? 64 * (dc >> 1) + 16 * kq + 8 * (dc & 1) : 32 * dc + 8 * kq;
             x[dc][0] = ld4(q + d0, vec);
             x[dc][1] = ld4(q + d0 + 4, vec);
+        }
+        const float by = 1.4426950408889634f / sqrtf((float)HD);
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float b = fabsf(x[dc][i >> 2][i & 3]);
-                a = b <= FLT_BIG ? fmaxf(a, b) : a;
+                const float y = rounded(x[dc][i >> 2][i & 3] * by);
+                x[dc][i >> 2][i & 3] = y;
+                a = fabsf(y) <= FLT_BIG ? fmaxf(a, fabsf(y)) : a;
             }
-        }
-        a = fmaxf(a, __shfl_xor(a, 16, 64));
-        a = fmaxf(a, __shfl_xor(a, 32, 64));
-        // the largest to [2^6, 2^7): the halves of the smaller ones keep 2^-31 of it
+        a = col_max(a);
         const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 126) : 0;
         const float qs = ldexpf(1.f, e);
-        c2 = ldexpf(1.4426950408889634f / sqrtf((float)HD), -e);
+        c2 = ldexpf(1.f, -e);
 #pragma unroll
         for (int dc = 0; dc < NDC; ++dc)
 #pragma unroll
@@ -420,12 +443,11 @@ struct WaveAttn {
 #pragma unroll
         for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
     }
-    static __device__ __forceinline__ void load_scales(Scales& x, const uint8_t* blk, int kq) {
-        const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
+    static __device__ __forceinline__ void load_scales(Scales& x, const float* k, const float* v, int kq) {
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
-            x.k[st] = *(const v4f*)(scale + 16 * st + 4 * kq);
-            x.v[st] = *(const v4f*)(scale + FTX_PAGE + 16 * st + 4 * kq);
+            x.k[st] = *(const v4f*)(k + 16 * st + 4 * kq);
+            x.v[st] = *(const v4f*)(v + 16 * st + 4 * kq);
         }
     }
     static __device__ __forceinline__ v8h k_frag(const Vals& x, int st, int dc) {
@@ -445,92 +467,188 @@ struct WaveAttn {
         }
     }
 
-    __device__ __forceinline__ void scores(v4f (&s)[4], const Vals& k) const {
+    // Scores of a page, k(st, dc) its operands: those of four slot tiles are
+    // read while the products of the four before them run, on accumulators
+    // that do not wait for each other (left to itself the compiler reads one
+    // operand, waits and multiplies: 733 us instead of 5xx for three chunks of
+    // 1500 tokens)
+    template <typename K>
+    __device__ __forceinline__ void scores(v4f (&s)[4], K k) const {
+        if constexpr (!STAGED) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            s[st] = v4f{0.f, 0.f, 0.f, 0.f};
+            for (int st = 0; st < 4; ++st) {
+                s[st] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int dc = 0; dc < NDC; ++dc) {
-                const v8h kf = k_frag(k, st, dc);
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[dc], s[st], 0, 0, 0);
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[dc], s[st], 0, 0, 0);
+                for (int dc = 0; dc < NDC; ++dc) {
+                    const v8h kf = k(st, dc);
+                    s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[dc], s[st], 0, 0, 0);
+                    s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[dc], s[st], 0, 0, 0);
+                }
             }
+            return;
+        }
+        v8h f[2][4];
+#pragma unroll
+        for (int st = 0; st < 4; ++st) f[0][st] = k(st, 0);
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) {
+            if (dc + 1 < NDC)
+#pragma unroll
+                for (int st = 0; st < 4; ++st) f[(dc + 1) & 1][st] = k(st, dc + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], ql[dc],
+                                                               dc ? s[st] : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], qh[dc], s[st], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
-    // The page's weights from its scores; the sums so far brought to the new
-    // maximum and V exponent.  seen(st, r): whether the row sees the slot
-    // (whole: it sees all)
+    // outputs to another V level
+    __device__ __forceinline__ void raise(int en) {
+        const float f = ldexpf(1.f, max(ev - en, -126));
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] *= f;
+        ev = en;
+    }
+
+    // the scores' largest of the row
+    static __device__ __forceinline__ float row_max(const v4f (&s)[4]) {
+        float mx = fmaxf(s[0][0], s[0][1]);
+#pragma unroll
+        for (int st = 0; st < 4; ++st) mx = fmaxf(fmaxf(mx, s[st][2 * (st == 0)]), s[st][2 * (st == 0) + 1]);
+#pragma unroll
+        for (int st = 1; st < 4; ++st) mx = fmaxf(fmaxf(mx, s[st][2]), s[st][3]);
+        return col_max(mx);
+    }
+
+    // The page's weights from its scores; the sums so far brought to a new
+    // offset or V level where one is needed.  ones: every scale of the page is 1
+    // (sc is not read).  seen(st, r): whether the row sees the slot (whole: it
+    // sees all).  pe: sc.v stands 2^-pe over, pe the level of the page's largest
+    // V scale (whole pages only: what a row does not see must not set its
+    // level), or NO_LEVEL.
+    static constexpr int NO_LEVEL = 1 << 20;
     template <typename Seen>
-    __device__ __forceinline__ void soften(v4f (&s)[4], const Scales& sc, bool whole, Seen seen, v8h (&ph)[2],
-                                           v8h (&pl)[2]) {
-        v4f vs[4];
-        float mx = -INFINITY, vm = 0.f;
+    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, Seen seen,
+                                           v8h (&ph)[2], v8h (&pl)[2]) {
+        // (the scales' products and the maximum in one basic block: across a
+        // branch the compiler makes every score quiet first)
+        float mx;
+        if (whole) {
+            if (!ones)
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                s[st][r] = (s[st][r] * c2) * sc.k[st][r];
-                vs[st][r] = sc.v[st][r];
-            }
-        if (!whole)
+                for (int st = 0; st < 4; ++st) s[st] *= sc.k[st];
+            mx = row_max(s);
+        } else {
 #pragma unroll
             for (int st = 0; st < 4; ++st)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const bool ok = seen(st, r);
-                    s[st][r] = ok ? s[st][r] : -INFINITY;
-                    vs[st][r] = ok ? vs[st][r] : 0.f;
+                    s[st][r] = ok ? (ones ? s[st][r] : s[st][r] * sc.k[st][r]) : -INFINITY;
+                    if (!ones) sc.v[st][r] = ok ? sc.v[st][r] : 0.f;
                 }
+            mx = row_max(s);
+        }
+        const float cand = __builtin_fmaf(mx, c2, -12.f);
+        if (__builtin_amdgcn_ballot_w64(cand > off + 3.f)) {  // (wave-uniform)
+            const float on = fmaxf(off, cand);
+            const float al = off == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(off - on);
+            off = on;
+            l *= al;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= al;
+        }
+        const float on = off == -INFINITY ? 0.f : off;  // (nothing seen yet: every weight is 0)
+        float vf = 1.f;
+        bool flat = true;
+        if (ones) {
+            if (__builtin_amdgcn_ballot_w64(ev < 0)) raise(max(ev, 0));
+            flat = !__builtin_amdgcn_ballot_w64(ev != 0);
+            if (!flat) vf = ldexpf(1.f, -ev);
+        } else if (pe != NO_LEVEL) {
+            if (__builtin_amdgcn_ballot_w64(ev < pe)) raise(max(ev, pe));
+            if (__builtin_amdgcn_ballot_w64(ev != pe)) {
+                const float f = ldexpf(1.f, pe - ev);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                mx = fmaxf(mx, s[st][r]);
-                vm = fmaxf(vm, vs[st][r]);
+                for (int st = 0; st < 4; ++st) sc.v[st] *= f;
             }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        vm = fmaxf(vm, __shfl_xor(vm, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        vm = fmaxf(vm, __shfl_xor(vm, 32, 64));
-        const float mn = fmaxf(m, mx);
-        const float mr = mn == -INFINITY ? 0.f : mn;  // (nothing seen yet: every p is 0)
-        const float al = __builtin_amdgcn_exp2f(m - mr);
-        const int en = max(ev, f_exp(vm));  // (vm = 0: -127)
-        const float vscale = ldexpf(1.f, 14 - en);
-        const float oal = ldexpf(al, ev - en);
-        m = mn;
-        ev = en;
-        l *= al;
+        } else {
+            const float top = fmaxf(fmaxf(fmaxf(fmaxf(sc.v[0][0], sc.v[0][1]), fmaxf(sc.v[0][2], sc.v[0][3])),
+                                          fmaxf(fmaxf(sc.v[1][0], sc.v[1][1]), fmaxf(sc.v[1][2], sc.v[1][3]))),
+                                    fmaxf(fmaxf(fmaxf(sc.v[2][0], sc.v[2][1]), fmaxf(sc.v[2][2], sc.v[2][3])),
+                                          fmaxf(fmaxf(sc.v[3][0], sc.v[3][1]), fmaxf(sc.v[3][2], sc.v[3][3]))));
+            if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.f, ev))) raise(max(ev, ev_level(col_max(fmaxf(top, 0.f)))));
+            const float f = ldexpf(1.f, -ev);
+#pragma unroll
+            for (int st = 0; st < 4; ++st) sc.v[st] *= f;
+        }
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
             for (int r = 0; r < 4; r += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(s[st][r] - mr);
-                const float p1 = __builtin_amdgcn_exp2f(s[st][r + 1] - mr);
-                l += p0 + p1;
+                float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r], c2, -on));
+                float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r + 1], c2, -on));
+                l += p0;
+                l += p1;
+                if (!ones) {
+                    p0 = rounded(p0 * sc.v[st][r]);
+                    p1 = rounded(p1 * sc.v[st][r + 1]);
+                } else if (!flat) {
+                    p0 = rounded(p0 * vf);
+                    p1 = rounded(p1 * vf);
+                }
                 v2h h, lo;
-                split_hl2(rounded(p0 * (vs[st][r] * vscale)), rounded(p1 * (vs[st][r + 1] * vscale)), h, lo);
+                split_hl2(p0, p1, h, lo);
                 const int i = 4 * (st & 1) + r;
                 ph[st >> 1][i] = h[0];
                 ph[st >> 1][i + 1] = h[1];
                 pl[st >> 1][i] = lo[0];
                 pl[st >> 1][i + 1] = lo[1];
             }
-        if (__builtin_amdgcn_ballot_w64(oal != 1.f))  // (wave-uniform)
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) o[dt] *= oal;
     }
 
-    __device__ __forceinline__ void outputs(const Vals& v, const v8h (&ph)[2], const v8h (&pl)[2]) {
+    // v(dt, sp): the page's V operands
+    template <typename V>
+    __device__ __forceinline__ void outputs(V v, const v8h (&ph)[2], const v8h (&pl)[2]) {
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int sp = 0; sp < 2; ++sp) {
-                const v8h vf = v_frag(v, dt, sp);
+                const v8h vf = v(dt, sp);
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[sp], o[dt], 0, 0, 0);
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[sp], o[dt], 0, 0, 0);
             }
+    }
+    // the same, read as K's are; f: the first four
+    template <typename V>
+    __device__ __forceinline__ void outputs_first(v8h (&f)[2][4], V v) const {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) f[0][x] = v(x, 0);
+    }
+    template <typename V>
+    __device__ __forceinline__ void outputs(v8h (&f)[2][4], V v, const v8h (&ph)[2], const v8h (&pl)[2]) {
+        constexpr int NG = NDT / 2;  // groups: four dim tiles, one half of the slots
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            if (g + 1 < NG)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) f[(g + 1) & 1][x] = v((g + 1) / 2 * 4 + x, (g + 1) & 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                o[g / 2 * 4 + x] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], pl[g & 1], o[g / 2 * 4 + x], 0, 0, 0);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                o[g / 2 * 4 + x] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], ph[g & 1], o[g / 2 * 4 + x], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
 };
 
@@ -563,7 +681,7 @@ struct RowSight {
 // in LDS.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
-    using W = WaveAttn<HD, Q8>;
+    using W = WaveAttn<HD, Q8, false>;
     constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
     __shared__ float so[3][4 * W::NDT][64], sm[4][64], sl[4][64];
     __shared__ int se[4][64];
@@ -586,6 +704,8 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
         hi = min(hi, __shfl_xor(hi, x, 64));
         lo = max(lo, __shfl_xor(lo, x, 64));
     }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
     // the wave's pages: entries i0 + w, + 4, ..; their ids 64 at a time in the
     // lanes.  A page's V loads are issued before its scores are formed, the
     // next page's K loads and scales (PRE) before its softmax, so that each
@@ -609,11 +729,12 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     }
     for (int j = 0; j < n; ++j) {
         if (!PRE) W::load_vals(kv, blk, lane);
-        W::load_scales(sc, blk, kq);
+        const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
+        W::load_scales(sc, scale, scale + FTX_PAGE, kq);
         if (EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
         __builtin_amdgcn_sched_barrier(0);
         v4f s[4];
-        wa.scores(s, kv);
+        wa.scores(s, [&](int st, int dc) { return W::k_frag(kv, st, dc); });
         __builtin_amdgcn_sched_barrier(0);
         if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
         if (j + 1 < n) {
@@ -624,12 +745,12 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
         const int p0 = place(j) * FTX_PAGE;
         const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= sight.sinks);
         v8h ph[2], pl[2];
-        wa.soften(s, sc, whole, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
-        wa.outputs(vv, ph, pl);
+        wa.soften(s, sc, false, whole, W::NO_LEVEL, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
+        wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
     }
     wa.l += __shfl_xor(wa.l, 16, 64);
     wa.l += __shfl_xor(wa.l, 32, 64);
-    sm[w][lane] = wa.m;
+    sm[w][lane] = wa.off;
     sl[w][lane] = wa.l;
     se[w][lane] = wa.ev;
     if (w)
@@ -639,7 +760,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
             for (int x = 0; x < 4; ++x) so[w - 1][4 * dt + x][lane] = wa.o[dt][x];
     __syncthreads();
     if (w) return;
-    float M = wa.m, f[4], L = 0.f;
+    float M = wa.off, f[4], L = 0.f;
     int EV = wa.ev;
 #pragma unroll
     for (int x = 1; x < 4; ++x) {
@@ -667,7 +788,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
             float n = wa.o[dt][x] * f[0];
 #pragma unroll
             for (int u = 1; u < 4; ++u) n += so[u - 1][4 * dt + x][lane] * f[u];
-            y[x] = none ? 0.f : ldexpf(n / L, EV - 14);
+            y[x] = none ? 0.f : ldexpf(n / L, EV);
         }
         st4(dst + 16 * dt + 4 * kq, y, vec);
     }
@@ -677,9 +798,193 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     }
 }
 
-// Workgroup (row of a tile with several partials, kv head):
-// out = sum_i 2^(m_i - M) l_i o_i / sum_i 2^(m_i - M) l_i.  Every wave forms M
-// and the sum itself; thread (g, d) adds the partials g, g + G, .. of dims
+typedef __attribute__((address_space(3))) void lds_void;
+
+// Many rows: workgroup = (item of 128 rows, kv head), eight waves of 16 rows.
+// Each page goes to LDS as the halves that the operands are (8-bit values
+// converted once, by all waves), one page ahead in the other buffer: halves by
+// direct copies, 8-bit values through registers, their loads issued before the
+// current page's work and written after it.
+template <int HD, bool Q8>
+constexpr int many_buf_bytes() {
+    return 2 * FTX_PAGE * HD * 2 + 3 * FTX_PAGE * 4 + 16;  // values, scales of K, V, V by level, its level
+}
+template <int HD, bool Q8>
+__global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
+    using W = WaveAttn<HD, Q8, true>;
+    constexpr int VB = FTX_PAGE * HD * 2;  // bytes of K's (V's) halves in LDS
+    constexpr int BUF = many_buf_bytes<HD, Q8>();
+    constexpr int NC = 2 * VB / 1024;  // KB of both
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    const int kvh = blockIdx.x % a.p.n_kv;
+    const PagedItem it = a.items[a.n_few + blockIdx.x / a.p.n_kv];
+    const PagedSeq sq = it.q;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, col = lane & 15, kq = lane >> 4;
+    const int R = sq.M * a.gqa, rr = it.row0 + 16 * w + col, r = min(rr, R - 1), t = r / a.gqa;
+    const bool live = it.row0 + 16 * w < R;  // (wave-uniform)
+    const int64_t tok = sq.tok0 + t;
+    const int head = kvh * a.gqa + r % a.gqa;
+    const bool vecq = !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15);
+    const int n = it.i1 - it.i0;
+    auto place = [&](int j) {
+        const int i = it.i0 + j;
+        return i < it.s ? i : it.a + (i - it.s);
+    };
+    int ids = lane < n ? a.p.table[sq.tab0 + place(lane)] : 0;
+    auto block_of = [&](int j) {
+        if ((j & 63) == 0 && j) ids = j + lane < n ? a.p.table[sq.tab0 + place(j + lane)] : 0;
+        return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
+    };
+    // the thread's share of the next page
+    constexpr int NQ = Q8 ? NC / 16 : 1;  // 16-byte units of 8-bit values
+    uint4 u[NQ];
+    float sc1 = 0.f;
+    auto stage = [&](int j) {
+        const uint8_t* blk = block_of(j);
+        uint8_t* dst = lds + (j & 1) * BUF;
+        if (tid < 2 * FTX_PAGE) sc1 = ((const float*)(blk + 2 * paged_values_bytes(HD, Q8)))[tid];
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) u[i] = ((const uint4*)blk)[i * 512 + tid];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC / 8; ++i)
+                __builtin_amdgcn_global_load_lds((const void*)(blk + ((i * 8 + w) * 64 + lane) * 16),
+                                                 (lds_void*)(dst + (i * 8 + w) * 1024), 16, 0, 0);
+        }
+    };
+    auto commit = [&](int j) {
+        uint8_t* dst = lds + (j & 1) * BUF;
+        if (tid < 2 * FTX_PAGE) ((float*)(dst + 2 * VB))[tid] = sc1;
+        if (w == 1) {
+            // the page's V level and its V scales by it
+            const int pe = ev_level(__builtin_bit_cast(float, group_max<64>(mag(sc1 <= FLT_BIG ? sc1 : 0.f))));
+            ((float*)(dst + 2 * VB))[FTX_PAGE + tid] = ldexpf(sc1, -pe);
+            if (lane == 0) *(int*)(dst + 2 * VB + 3 * FTX_PAGE * 4) = pe;
+        }
+        if constexpr (Q8) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                // unit x of K: dims' half (dc) and slot tile; of V: dim tile
+                const int x = i * 512 + tid, g = x >> 6;
+                v8h* t;
+                int step;
+                if (g < HD / 16) {
+                    t = (v8h*)dst + ((g >> 2) * 8 + (g & 3)) * 64 + (x & 63);
+                    step = 4 * 64;
+                } else {
+                    t = (v8h*)(dst + VB) + (g - HD / 16) * 128 + (x & 63);
+                    step = 64;
+                }
+                t[0] = u8x8(u[i].x, u[i].y);
+                t[step] = u8x8(u[i].z, u[i].w);
+            }
+        }
+    };
+    stage(0);
+    W wa;
+    wa.query(a.q + tok * a.ldq + (int64_t)head * HD, kq, vecq);
+    const RowSight sight(a, sq, t);
+    // the pages that every row of the wave sees whole, and the last that any sees
+    int hi = sight.hi, lo = sight.lo, last = sight.anc ? sq.npast + t : sight.hi;
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) {
+        hi = min(hi, __shfl_xor(hi, x, 64));
+        lo = max(lo, __shfl_xor(lo, x, 64));
+        last = max(last, __shfl_xor(last, x, 64));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    last = __builtin_amdgcn_readfirstlane(last);
+    commit(0);
+    for (int j = 0; j < n; ++j) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's direct copies of page j
+        __syncthreads();                     // every wave's; the other buffer is free
+        if (j + 1 < n) stage(j + 1);
+        const int p0 = place(j) * FTX_PAGE;
+        if (live && p0 <= last) {
+            const uint8_t* buf = lds + (j & 1) * BUF;
+            const float* scale = (const float*)(buf + 2 * VB);
+            const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (scale[FTX_PAGE + lane] != 1.f));
+            v4f s[4];
+            wa.scores(s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); });
+            typename W::Scales sc;
+            const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= sight.sinks);
+            if (!ones) W::load_scales(sc, scale, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
+            const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
+            v8h ph[2], pl[2], f[2][4];
+            auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
+            wa.outputs_first(f, vf);
+            wa.soften(s, sc, ones, whole, pe, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
+            wa.outputs(f, vf, ph, pl);
+        }
+        if (j + 1 < n) commit(j + 1);
+    }
+    if (!live) return;
+    wa.l += __shfl_xor(wa.l, 16, 64);
+    wa.l += __shfl_xor(wa.l, 32, 64);
+    if (rr >= R) return;
+    const bool part = it.part >= 0;
+    const int64_t prow = ((int64_t)(it.part + w) * a.p.n_kv + kvh) * PAGED_TR + col;
+    float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
+    const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
+    const bool none = wa.l == 0.f;  // no page of this part is seen by the row
+#pragma unroll
+    for (int dt = 0; dt < W::NDT; ++dt) {
+        v4f y;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) y[x] = none ? 0.f : ldexpf(wa.o[dt][x] / wa.l, wa.ev);
+        st4(dst + 16 * dt + 4 * kq, y, vec);
+    }
+    if (part && kq == 0) {
+        a.pml[2 * prow] = wa.off;
+        a.pml[2 * prow + 1] = wa.l;
+    }
+}
+
+// out = sum_i 2^(m_i - M) l_i o_i / sum_i 2^(m_i - M) l_i of up to COMB_FEW
+// partials: G rows a workgroup, HD / 4 threads each
+constexpr int COMB_FEW = 8;
+template <int HD>
+__global__ void __launch_bounds__(256) k_paged_combine_few(PagedAttn a) {
+    constexpr int D4 = HD / 4, G = 256 / D4;
+    const int kvh = blockIdx.x % a.p.n_kv, d = threadIdx.x % D4;
+    const int col = blockIdx.y * G + threadIdx.x / D4;
+    const PagedComb c = a.combs[blockIdx.x / a.p.n_kv];
+    const PagedSeq sq = a.p.seqs[c.seq];
+    const int rr = c.row0 + col;
+    if (col >= PAGED_TR || rr >= sq.M * a.gqa) return;
+    const int64_t step = (int64_t)c.step * a.p.n_kv * PAGED_TR;
+    const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
+    const float2* ml = (const float2*)a.pml + p0;
+    float2 t[COMB_FEW];
+    v4f o[COMB_FEW];
+#pragma unroll
+    for (int i = 0; i < COMB_FEW; ++i) {
+        const int64_t at = min(i, c.n - 1) * step;  // (past the last: its partial again, weight 0)
+        t[i] = ml[at];
+        o[i] = *(const v4f*)(a.part + (p0 + at) * HD + 4 * d);
+    }
+    float M = t[0].x, den = 0.f;
+#pragma unroll
+    for (int i = 1; i < COMB_FEW; ++i) M = fmaxf(M, t[i].x);
+#pragma unroll
+    for (int i = 0; i < COMB_FEW; ++i) {
+        t[i].y *= i < c.n ? (t[i].x == M ? 1.f : __builtin_amdgcn_exp2f(t[i].x - M)) : 0.f;
+        den += i < c.n ? t[i].y : 0.f;
+    }
+    v4f num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < COMB_FEW; ++i)
+        if (i < c.n) num += o[i] * (t[i].y / den);
+    const int64_t tok = sq.tok0 + rr / a.gqa;
+    const bool vec = !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
+    st4(a.out + tok * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD + 4 * d, num, vec);
+}
+
+// The same of any number: workgroup (row, kv head).  Every wave forms M and the
+// sum itself; thread (g, d) adds the partials g, g + G, .. of dims
 // 4 d .. 4 d + 3, the G sums meet in LDS.
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
@@ -690,7 +995,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
     const PagedSeq sq = a.p.seqs[c.seq];
     const int rr = c.row0 + col, lane = threadIdx.x & 63;
     if (rr >= sq.M * a.gqa) return;
-    const int64_t step = (int64_t)a.p.n_kv * PAGED_TR;
+    const int64_t step = (int64_t)c.step * a.p.n_kv * PAGED_TR;
     const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
     const float2* ml = (const float2*)a.pml + p0;
     float M = -INFINITY, den = 0.f;
@@ -747,15 +1052,36 @@ hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pag
     return hipGetLastError();
 }
 
+template <int HD, bool Q8>
+static hipError_t launch_many(hipStream_t st, const PagedAttn& a) {
+    static std::atomic<uint64_t> lds_set{0};
+    constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD, Q8>();
+    const hipError_t e = lds_limit((const void*)k_paged_many<HD, Q8>, bytes, lds_set);
+    if (e != hipSuccess) return e;
+    ktimed_launch(k_paged_many<HD, Q8>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(512), (uint32_t)bytes, st,
+                  a);
+    return hipGetLastError();
+}
+
 hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
-    if (a.n_items == 0) return hipSuccess;
-    const dim3 grid((unsigned)a.n_items * (unsigned)a.p.n_kv);
-    ktimed_launch(PAGED_CASE(k_paged_attn, a.p.hd, a.p.q8), grid, dim3(256), 0, st, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e = hipSuccess;
+    if (a.n_many) e = PAGED_CASE(launch_many, a.p.hd, a.p.q8)(st, a);
+    if (e != hipSuccess) return e;
+    if (a.n_few)
+        ktimed_launch(PAGED_CASE(k_paged_attn, a.p.hd, a.p.q8), dim3((unsigned)a.n_few * (unsigned)a.p.n_kv), dim3(256),
+                      0, st, a);
+    e = hipGetLastError();
     if (e != hipSuccess || a.n_combs == 0) return e;
-    const dim3 cg((unsigned)a.n_combs * (unsigned)a.p.n_kv, (unsigned)std::min(PAGED_TR, a.rows_max));
-    auto* comb = a.p.hd == 64 ? k_paged_combine<64> : a.p.hd == 128 ? k_paged_combine<128> : k_paged_combine<256>;
-    hipLaunchKernelGGL(comb, cg, dim3(256), 0, st, a);
+    const int rows = std::min(PAGED_TR, a.rows_max);
+    const unsigned cx = (unsigned)a.n_combs * (unsigned)a.p.n_kv;
+    if (a.comb_max <= COMB_FEW) {
+        auto* f = a.p.hd == 64 ? k_paged_combine_few<64> : a.p.hd == 128 ? k_paged_combine_few<128> : k_paged_combine_few<256>;
+        const int per = 256 / (a.p.hd / 4);
+        hipLaunchKernelGGL(f, dim3(cx, (unsigned)((rows + per - 1) / per)), dim3(256), 0, st, a);
+    } else {
+        auto* f = a.p.hd == 64 ? k_paged_combine<64> : a.p.hd == 128 ? k_paged_combine<128> : k_paged_combine<256>;
+        hipLaunchKernelGGL(f, dim3(cx, (unsigned)rows), dim3(256), 0, st, a);
+    }
     return hipGetLastError();
 }
 

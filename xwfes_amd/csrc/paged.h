@@ -46,22 +46,23 @@ struct PagedSeq {
     int32_t anc0, aw;    // its mask words in the mask array, words a node
     int64_t all0;        // its first row when contexts are read back
 };
-// A row tile (PAGED_TR query rows of a kv head: row r = token r / gqa, head
-// r % gqa) over entries i0 .. i1 - 1 of its page list: pages 0 .. s - 1 (the
-// first tokens'), then pages a, a + 1, ..  q: its sequence, held here so that
-// a workgroup's first page is two loads away and not three
+// A row tile (query rows of a kv head: row r = token r / gqa, head r % gqa;
+// PAGED_TR or PAGED_TR_MANY of them) over entries i0 .. i1 - 1 of its page
+// list: pages 0 .. s - 1 (the first tokens'), then pages a, a + 1, ..  q: its
+// sequence, held here so that a workgroup's first page is two loads away and
+// not three
 struct PagedItem {
     int32_t seq, row0, i0, i1, s, a;
-    int32_t part;  // its partial's place, or -1: the whole list, results go to out
+    int32_t part;  // its partials' place (in blocks of PAGED_TR rows), or -1: the whole list, results go to out
     int32_t pad;
     PagedSeq q;
     int32_t fill[6];  // to 96 bytes
 };
-// the partials part0 .. part0 + n - 1 of one row tile
+// the partials part0, part0 + step, .. (n of them) of PAGED_TR rows
 struct PagedComb {
-    int32_t seq, row0, part0, n;
+    int32_t seq, row0, part0, n, step;
 };
-constexpr int PAGED_TR = 16;
+constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
 
 struct PagedGeom {
     int64_t n_kv = 0, hd = 0, n_pages = 0;
@@ -73,7 +74,9 @@ struct PagedTables {
     int64_t tokens = 0, rows = 0;  // new tokens, positions of all contexts
     int64_t longest = 0;            // new tokens of one sequence
     int64_t max_new_pages = 0, max_pages = 0;  // of one sequence
-    int64_t parts = 0;
+    int64_t parts = 0;   // in blocks of PAGED_TR rows
+    int64_t comb_max = 0;  // most partials of a row
+    int64_t few = 0;     // items of PAGED_TR rows, before those of PAGED_TR_MANY
     bool absent = false;  // a page below npast + M is absent
     double seen = 0, pages_read = 0;  // visible (row, slot) pairs bound, pages of all items
     std::vector<PagedSeq> seqs;
@@ -112,7 +115,8 @@ struct PagedAttn {
     const uint32_t* anc;
     const PagedItem* items;
     const PagedComb* combs;
-    int n_items, n_combs, rows_max;  // rows_max: query rows of the longest sequence
+    int n_few, n_many, n_combs;
+    int rows_max, comb_max;  // query rows of the longest sequence, most partials of a row
     int gqa;
     int window, sinks;
     const float* q;

@@ -10,6 +10,10 @@
 
 // ---------------------------------------------------------------- plan tables
 
+// Query rows of a kv head from which a sequence goes to the kernel that shares
+// each page among 128 rows
+constexpr int64_t PAGED_MANY = 65;
+
 int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_t>& mark,
                  uint32_t& epoch, PagedTables& o, std::string& err) {
     auto fail = [&](int code, const char* what) {
@@ -102,23 +106,26 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     if (a.n_head == 0) return FTX_OK;
     // the row tiles and the pages each sees
     struct Tile {
-        int32_t seq, row0, s, a, n;
+        int32_t seq, row0, rows, s, a, n;
     };
-    std::vector<Tile> tiles;
-    int64_t total = 0;
+    std::vector<Tile> tiles[2];  // of PAGED_TR rows, of PAGED_TR_MANY
+    int64_t total[2] = {0, 0};
     for (int64_t s = 0; s < a.nseq; ++s) {
         const PagedSeq& d = o.seqs[(size_t)s];
         const int64_t R = d.M * gqa;
+        const int many = R >= PAGED_MANY;
+        const int64_t TR = many ? PAGED_TR_MANY : PAGED_TR;
         int64_t checked_s = 0, checked_a = d.ntab;  // pages seen so far: [0, checked_s), [checked_a, ..)
-        for (int64_t row0 = 0; row0 < R; row0 += PAGED_TR) {
-            const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + PAGED_TR) - 1) / gqa;
+        for (int64_t row0 = 0; row0 < R; row0 += TR) {
+            const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + TR) - 1) / gqa;
             // (a tree's nodes are all looked at: a node's position is below its slot)
             int64_t lo = 0;
             if (W) lo = std::max<int64_t>(0, d.npast + (d.dep0 >= 0 ? 0 : t0) - W + 1);
             const int64_t pa = lo / FTX_PAGE, pe = (d.npast + t1) / FTX_PAGE + 1;
             const int64_t ps = std::min((sinks + FTX_PAGE - 1) / FTX_PAGE, pa);
-            tiles.push_back(Tile{(int32_t)s, (int32_t)row0, (int32_t)ps, (int32_t)pa, (int32_t)(ps + pe - pa)});
-            total += ps + pe - pa;
+            tiles[many].push_back(Tile{(int32_t)s, (int32_t)row0, (int32_t)std::min(R - row0, TR), (int32_t)ps,
+                                       (int32_t)pa, (int32_t)(ps + pe - pa)});
+            total[many] += ps + pe - pa;
             for (; checked_s < ps; ++checked_s)
                 if (o.table[(size_t)(d.tab0 + checked_s)] < 0)
                     return fail(FTX_E_INVALID, "a page that a new token sees is absent");
@@ -127,26 +134,38 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
                     return fail(FTX_E_INVALID, "a page that a new token sees is absent");
         }
     }
-    o.pages_read = (double)total;
-    // lists long enough to be split so that the launch has some four
-    // workgroups a CU, of at least four pages (one a wave)
-    const int64_t want = 4 * (int64_t)std::max(g.cu, 1);
-    const int64_t per = std::max<int64_t>(4, (total * g.n_kv + want - 1) / want);
-    for (const Tile& t : tiles) {
-        const int64_t np = (t.n + per - 1) / per;
-        for (int64_t k = 0; k < np; ++k)
-            o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
-                                        t.a, np > 1 ? (int32_t)(o.parts + k) : -1, 0, o.seqs[(size_t)t.seq], {}});
-        if (np > 1) {
-            o.combs.push_back(PagedComb{t.seq, t.row0, (int32_t)o.parts, (int32_t)np});
-            o.parts += np;
+    o.pages_read = (double)(total[0] + total[1]);
+    const int64_t cu = std::max(g.cu, 1);
+    for (int many = 0; many < 2; ++many) {
+        // Lists are split so that a launch has some four workgroups a CU, no
+        // finer than four pages (one a wave); many rows, where a partial is 64 KB
+        // and one workgroup fills a CU: one, no finer than eight pages
+        const int64_t want = (many ? 1 : 4) * cu;
+        const int64_t least = many ? 8 : 4;
+        int64_t per = std::max(least, (total[many] * g.n_kv + want - 1) / want);
+        if (many && (int64_t)tiles[1].size() * g.n_kv >= want) per = INT32_MAX;
+        for (const Tile& t : tiles[many]) {
+            const int64_t np = (t.n + per - 1) / per, blocks = many ? PAGED_TR_MANY / PAGED_TR : 1;
+            for (int64_t k = 0; k < np; ++k)
+                o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
+                                            t.a, np > 1 ? (int32_t)(o.parts + k * blocks) : -1, 0,
+                                            o.seqs[(size_t)t.seq], {}});
+            if (np == 1) continue;
+            o.comb_max = std::max(o.comb_max, np);
+            for (int64_t r = 0; r < t.rows; r += PAGED_TR)
+                o.combs.push_back(PagedComb{t.seq, (int32_t)(t.row0 + r), (int32_t)(o.parts + r / PAGED_TR), (int32_t)np,
+                                            (int32_t)blocks});
+            o.parts += np * blocks;
         }
+        // the longest first
+        std::stable_sort(o.items.begin() + o.few, o.items.end(), [](const PagedItem& x, const PagedItem& y) {
+            return x.i1 - x.i0 > y.i1 - y.i0;
+        });
+        if (!many) o.few = (int64_t)o.items.size();
     }
-    if ((int64_t)o.items.size() * g.n_kv >= (int64_t)1 << 31 || o.parts >= (int64_t)1 << 31)
+    if ((int64_t)o.items.size() * g.n_kv >= (int64_t)1 << 31 || (int64_t)o.combs.size() * g.n_kv >= (int64_t)1 << 31 ||
+        o.parts >= (int64_t)1 << 31)
         return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
-    // the longest first
-    std::stable_sort(o.items.begin(), o.items.end(),
-                     [](const PagedItem& x, const PagedItem& y) { return x.i1 - x.i0 > y.i1 - y.i0; });
     return FTX_OK;
 }
 
@@ -581,10 +600,12 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.anc = (const uint32_t*)(pl->dev + pl->o_anc);
     a.items = (const PagedItem*)(pl->dev + pl->o_item);
     a.combs = (const PagedComb*)(pl->dev + pl->o_comb);
-    a.n_items = (int)t.items.size();
+    a.n_few = (int)t.few;
+    a.n_many = (int)((int64_t)t.items.size() - t.few);
     a.n_combs = (int)t.combs.size();
     a.gqa = (int)(t.n_head / p->n_kv);
     a.rows_max = (int)(t.longest * a.gqa);
+    a.comb_max = (int)std::min<int64_t>(t.comb_max, INT32_MAX);
     a.window = (int)t.window;
     a.sinks = (int)t.sinks;
     a.q = q;

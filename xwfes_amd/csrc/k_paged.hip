@@ -467,6 +467,23 @@ struct WaveAttn {
         }
     }
 
+    // scores of a page, k(st, dc) its operands, of the query halves hi(dc), lo(dc)
+    template <typename K, typename L, typename H>
+    static __device__ __forceinline__ void scores_of(v4f (&s)[4], K k, L lo, H hi) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st) s[st] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int dc = 0; dc < NDC; ++dc) {
+            const v8h l8 = lo(dc), h8 = hi(dc);
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                const v8h kf = k(st, dc);
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, l8, s[st], 0, 0, 0);
+                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, h8, s[st], 0, 0, 0);
+            }
+        }
+    }
+
     // Scores of a page, k(st, dc) its operands: those of four slot tiles are
     // read while the products of the four before them run, on accumulators
     // that do not wait for each other (left to itself the compiler reads one
@@ -475,16 +492,7 @@ struct WaveAttn {
     template <typename K>
     __device__ __forceinline__ void scores(v4f (&s)[4], K k) const {
         if constexpr (!STAGED) {
-#pragma unroll
-            for (int st = 0; st < 4; ++st) {
-                s[st] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int dc = 0; dc < NDC; ++dc) {
-                    const v8h kf = k(st, dc);
-                    s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[dc], s[st], 0, 0, 0);
-                    s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[dc], s[st], 0, 0, 0);
-                }
-            }
+            scores_of(s, k, [&](int dc) { return ql[dc]; }, [&](int dc) { return qh[dc]; });
             return;
         }
         v8h f[2][4];
@@ -527,13 +535,12 @@ struct WaveAttn {
 
     // The page's weights from its scores; the sums so far brought to a new
     // offset or V level where one is needed.  ones: every scale of the page is 1
-    // (sc is not read).  seen(st, r): whether the row sees the slot (whole: it
-    // sees all).  pe: sc.v stands 2^-pe over, pe the level of the page's largest
+    // (sc is not read).  whole: the row sees every slot, else slot 16 st + 4 kq + r
+    // by bit 16 st + r of seen.  pe: sc.v stands 2^-pe over, pe the level of the page's largest
     // V scale (whole pages only: what a row does not see must not set its
     // level), or NO_LEVEL.
     static constexpr int NO_LEVEL = 1 << 20;
-    template <typename Seen>
-    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, Seen seen,
+    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, uint64_t seen,
                                            v8h (&ph)[2], v8h (&pl)[2]) {
         // (the scales' products and the maximum in one basic block: across a
         // branch the compiler makes every score quiet first)
@@ -548,9 +555,14 @@ struct WaveAttn {
             for (int st = 0; st < 4; ++st)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const bool ok = seen(st, r);
-                    s[st][r] = ok ? (ones ? s[st][r] : s[st][r] * sc.k[st][r]) : -INFINITY;
-                    if (!ones) sc.v[st][r] = ok ? sc.v[st][r] : 0.f;
+                    // all ones or zeros
+                    const uint32_t ok = __builtin_amdgcn_sbfe((int)(seen >> (st >= 2 ? 32 : 0)), 16 * (st & 1) + r, 1);
+                    const float x = ones ? s[st][r] : s[st][r] * sc.k[st][r];
+                    s[st][r] = __builtin_bit_cast(
+                        float, (__builtin_bit_cast(uint32_t, x) & ok) | (0xFF800000u & ~ok));  // -inf
+                    // (a copy: a bit cast of a vector's element takes element 0)
+                    const float y = sc.v[st][r];
+                    if (!ones) sc.v[st][r] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & ok);
                 }
             mx = row_max(s);
         }
@@ -652,27 +664,41 @@ struct WaveAttn {
     }
 };
 
-// What a lane's row (token t of the sequence) may see.
+// What a lane's row (token t of the sequence) may see: slots lo .. hi and those
+// below sinks (a chain: up to its own; a tree: of the context), and of a tree's
+// nodes those of its mask words.
 struct RowSight {
-    int hi;   // context positions (a chain: all positions) up to hi
-    int lo;   // from lo on, or below sinks
-    int node0, M;  // a tree: slot node0 + j is node j, by its mask word
+    int hi, lo, sinks;
+    int node0, aw;
     const uint32_t* anc;  // null: a chain
-    int sinks;
     __device__ __forceinline__ RowSight(const PagedAttn& a, const PagedSeq& sq, int t) {
         const bool tree = sq.dep0 >= 0;
         const int pos = sq.npast + (tree ? a.depth[sq.dep0 + t] : t);
         hi = tree ? sq.npast - 1 : pos;
         lo = a.window ? max(0, pos - a.window + 1) : 0;
+        sinks = min(a.sinks, hi + 1);
         node0 = sq.npast;
-        M = sq.M;
+        aw = sq.aw;
         anc = tree ? a.anc + sq.anc0 + (int64_t)t * sq.aw : nullptr;
-        sinks = a.sinks;
     }
-    __device__ __forceinline__ bool sees(int p) const {
-        if (p <= hi) return p >= lo || p < sinks;
-        const int j = p - node0;
-        return anc && j < M && ((anc[j >> 5] >> (j & 31)) & 1u);
+    static __device__ __forceinline__ uint64_t below(int n) {  // bits 0 .. n - 1
+        return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+    }
+    // bit x: whether slot p0 + x is seen
+    __device__ __forceinline__ uint64_t page(int p0) const {
+        uint64_t v = (below(hi + 1 - p0) & ~below(lo - p0)) | below(sinks - p0);
+        const int j0 = p0 - node0;
+        if (anc && j0 > -FTX_PAGE && j0 < 32 * aw) {
+            const int w = max(j0, 0) >> 5;
+            const uint64_t x = anc[w] | (uint64_t)(w + 1 < aw ? anc[w + 1] : 0u) << 32;
+            if (j0 < 0) {
+                v |= x << -j0;
+            } else {
+                const uint64_t y = w + 2 < aw ? anc[w + 2] : 0u;
+                v |= x >> (j0 & 31) | (j0 & 31 ? y << (64 - (j0 & 31)) : 0);
+            }
+        }
+        return v;
     }
 };
 
@@ -683,6 +709,11 @@ template <int HD, bool Q8>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
     using W = WaveAttn<HD, Q8, false>;
     constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
+    // the query's halves, of which the four waves have the same: in LDS where
+    // they would leave too few registers for the values in flight (halves of
+    // 128 dims: 37 spilled, 129 us for one token over 131072; so 1xx)
+    constexpr bool QLDS = !Q8 && HD >= 128;
+    __shared__ v8h qs[QLDS ? 2 : 1][W::NDC][64];
     __shared__ float so[3][4 * W::NDT][64], sm[4][64], sl[4][64];
     __shared__ int se[4][64];
     const int kvh = blockIdx.x % a.p.n_kv;
@@ -696,6 +727,15 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     const bool vecq = !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15);
     W wa;
     wa.query(a.q + tok * a.ldq + (int64_t)head * HD, kq, vecq);
+    if constexpr (QLDS) {
+        if (w == 0)
+#pragma unroll
+            for (int dc = 0; dc < W::NDC; ++dc) {
+                qs[0][dc][lane] = wa.qh[dc];
+                qs[1][dc][lane] = wa.ql[dc];
+            }
+        __syncthreads();
+    }
     const RowSight sight(a, sq, t);
     // the pages that every row of the tile sees whole
     int hi = sight.hi, lo = sight.lo;
@@ -730,12 +770,28 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     for (int j = 0; j < n; ++j) {
         if (!PRE) W::load_vals(kv, blk, lane);
         const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
-        W::load_scales(sc, scale, scale + FTX_PAGE, kq);
+        float k1 = 0.f, v1 = 0.f;
+        if constexpr (Q8) {
+            W::load_scales(sc, scale, scale + FTX_PAGE, kq);
+        } else {
+            // (a page of halves has scales other than 1 where rows are very
+            // large or small: they are loaded then)
+            k1 = scale[lane];
+            v1 = scale[FTX_PAGE + lane];
+        }
         if (EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
         __builtin_amdgcn_sched_barrier(0);
         v4f s[4];
-        wa.scores(s, [&](int st, int dc) { return W::k_frag(kv, st, dc); });
+        auto kf = [&](int st, int dc) { return W::k_frag(kv, st, dc); };
+        if constexpr (QLDS) {
+            asm volatile("" ::: "memory");  // (read again for every page)
+            W::scores_of(s, kf, [&](int dc) { return qs[1][dc][lane]; }, [&](int dc) { return qs[0][dc][lane]; });
+        } else {
+            wa.scores(s, kf);
+        }
         __builtin_amdgcn_sched_barrier(0);
+        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((k1 != 1.f) | (v1 != 1.f));
+        if (!Q8 && !ones) W::load_scales(sc, scale, scale + FTX_PAGE, kq);
         if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
         if (j + 1 < n) {
             blk = block_of(j + 1);
@@ -743,9 +799,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
         }
         __builtin_amdgcn_sched_barrier(0);
         const int p0 = place(j) * FTX_PAGE;
-        const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= sight.sinks);
+        const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
         v8h ph[2], pl[2];
-        wa.soften(s, sc, false, whole, W::NO_LEVEL, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
+        wa.soften(s, sc, ones, whole, W::NO_LEVEL, whole ? 0 : sight.page(p0) >> (4 * kq), ph, pl);
         wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
     }
     wa.l += __shfl_xor(wa.l, 16, 64);
@@ -805,15 +861,17 @@ typedef __attribute__((address_space(3))) void lds_void;
 // converted once, by all waves), one page ahead in the other buffer: halves by
 // direct copies, 8-bit values through registers, their loads issued before the
 // current page's work and written after it.
-template <int HD, bool Q8>
+template <int HD>
 constexpr int many_buf_bytes() {
     return 2 * FTX_PAGE * HD * 2 + 3 * FTX_PAGE * 4 + 16;  // values, scales of K, V, V by level, its level
 }
+constexpr int NW_MANY = PAGED_TR_MANY / PAGED_TR;
 template <int HD, bool Q8>
-__global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
+__global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
+    constexpr int NW = NW_MANY;
     using W = WaveAttn<HD, Q8, true>;
     constexpr int VB = FTX_PAGE * HD * 2;  // bytes of K's (V's) halves in LDS
-    constexpr int BUF = many_buf_bytes<HD, Q8>();
+    constexpr int BUF = many_buf_bytes<HD>();
     constexpr int NC = 2 * VB / 1024;  // KB of both
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int kvh = blockIdx.x % a.p.n_kv;
@@ -837,7 +895,7 @@ __global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
         return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
     };
     // the thread's share of the next page
-    constexpr int NQ = Q8 ? NC / 16 : 1;  // 16-byte units of 8-bit values
+    constexpr int NQ = Q8 ? NC / (2 * NW) : 1;  // 16-byte units of 8-bit values
     uint4 u[NQ];
     float sc1 = 0.f;
     auto stage = [&](int j) {
@@ -846,12 +904,12 @@ __global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
         if (tid < 2 * FTX_PAGE) sc1 = ((const float*)(blk + 2 * paged_values_bytes(HD, Q8)))[tid];
         if constexpr (Q8) {
 #pragma unroll
-            for (int i = 0; i < NQ; ++i) u[i] = ((const uint4*)blk)[i * 512 + tid];
+            for (int i = 0; i < NQ; ++i) u[i] = ((const uint4*)blk)[i * 64 * NW + tid];
         } else {
 #pragma unroll
-            for (int i = 0; i < NC / 8; ++i)
-                __builtin_amdgcn_global_load_lds((const void*)(blk + ((i * 8 + w) * 64 + lane) * 16),
-                                                 (lds_void*)(dst + (i * 8 + w) * 1024), 16, 0, 0);
+            for (int i = 0; i < NC / NW; ++i)
+                __builtin_amdgcn_global_load_lds((const void*)(blk + ((i * NW + w) * 64 + lane) * 16),
+                                                 (lds_void*)(dst + (i * NW + w) * 1024), 16, 0, 0);
         }
     };
     auto commit = [&](int j) {
@@ -867,7 +925,7 @@ __global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 // unit x of K: dims' half (dc) and slot tile; of V: dim tile
-                const int x = i * 512 + tid, g = x >> 6;
+                const int x = i * 64 * NW + tid, g = x >> 6;
                 v8h* t;
                 int step;
                 if (g < HD / 16) {
@@ -910,13 +968,13 @@ __global__ void __launch_bounds__(512) k_paged_many(PagedAttn a) {
             v4f s[4];
             wa.scores(s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); });
             typename W::Scales sc;
-            const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= sight.sinks);
+            const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
             if (!ones) W::load_scales(sc, scale, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
             const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
             v8h ph[2], pl[2], f[2][4];
             auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
             wa.outputs_first(f, vf);
-            wa.soften(s, sc, ones, whole, pe, [&](int st, int x) { return sight.sees(p0 + 16 * st + 4 * kq + x); }, ph, pl);
+            wa.soften(s, sc, ones, whole, pe, whole ? 0 : sight.page(p0) >> (4 * kq), ph, pl);
             wa.outputs(f, vf, ph, pl);
         }
         if (j + 1 < n) commit(j + 1);
@@ -1055,11 +1113,11 @@ hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pag
 template <int HD, bool Q8>
 static hipError_t launch_many(hipStream_t st, const PagedAttn& a) {
     static std::atomic<uint64_t> lds_set{0};
-    constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD, Q8>();
+    constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD>();
     const hipError_t e = lds_limit((const void*)k_paged_many<HD, Q8>, bytes, lds_set);
     if (e != hipSuccess) return e;
-    ktimed_launch(k_paged_many<HD, Q8>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(512), (uint32_t)bytes, st,
-                  a);
+    ktimed_launch(k_paged_many<HD, Q8>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(64 * NW_MANY),
+                  (uint32_t)bytes, st, a);
     return hipGetLastError();
 }
 

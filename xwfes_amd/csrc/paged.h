@@ -76,7 +76,7 @@ struct PagedTables {
     int64_t max_new_pages = 0, max_pages = 0;  // of one sequence
     int64_t parts = 0;   // in blocks of PAGED_TR rows
     int64_t comb_max = 0;  // most partials of a row
-    int64_t few = 0;     // items of PAGED_TR rows, before those of PAGED_TR_MANY
+    int64_t few = 0;     // items of PAGED_TR rows, before the others
     bool absent = false;  // a page below npast + M is absent
     double seen = 0, pages_read = 0;  // visible (row, slot) pairs bound, pages of all items
     std::vector<PagedSeq> seqs;

@@ -599,29 +599,31 @@ struct WaveAttn {
 #pragma unroll
             for (int st = 0; st < 4; ++st) sc.v[st] *= f;
         }
+        // (one loop for each form: tests inside it would part the exponentials)
+        auto weigh = [&](auto by) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+            for (int st = 0; st < 4; ++st)
 #pragma unroll
-            for (int r = 0; r < 4; r += 2) {
-                float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r], c2, -on));
-                float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r + 1], c2, -on));
-                l += p0;
-                l += p1;
-                if (!ones) {
-                    p0 = rounded(p0 * sc.v[st][r]);
-                    p1 = rounded(p1 * sc.v[st][r + 1]);
-                } else if (!flat) {
-                    p0 = rounded(p0 * vf);
-                    p1 = rounded(p1 * vf);
+                for (int r = 0; r < 4; r += 2) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r], c2, -on));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r + 1], c2, -on));
+                    l += p0;
+                    l += p1;
+                    v2h h, lo;
+                    split_hl2(by(p0, st, r), by(p1, st, r + 1), h, lo);
+                    const int i = 4 * (st & 1) + r;
+                    ph[st >> 1][i] = h[0];
+                    ph[st >> 1][i + 1] = h[1];
+                    pl[st >> 1][i] = lo[0];
+                    pl[st >> 1][i + 1] = lo[1];
                 }
-                v2h h, lo;
-                split_hl2(p0, p1, h, lo);
-                const int i = 4 * (st & 1) + r;
-                ph[st >> 1][i] = h[0];
-                ph[st >> 1][i + 1] = h[1];
-                pl[st >> 1][i] = lo[0];
-                pl[st >> 1][i + 1] = lo[1];
-            }
+        };
+        if (!ones)
+            weigh([&](float p, int st, int r) { return rounded(p * sc.v[st][r]); });
+        else if (flat)
+            weigh([&](float p, int, int) { return p; });
+        else
+            weigh([&](float p, int, int) { return rounded(p * vf); });
     }
 
     // v(dt, sp): the page's V operands
@@ -835,7 +837,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     const int64_t prow = ((int64_t)it.part * a.p.n_kv + kvh) * PAGED_TR + col;
     float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
     const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
-    const bool none = L == 0.f;  // no page of this part is seen by the row
+    const float inv = L == 0.f ? 0.f : 1.f / L;  // (0: no page of this part is seen by the row)
 #pragma unroll
     for (int dt = 0; dt < W::NDT; ++dt) {
         v4f y;
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
             float n = wa.o[dt][x] * f[0];
 #pragma unroll
             for (int u = 1; u < 4; ++u) n += so[u - 1][4 * dt + x][lane] * f[u];
-            y[x] = none ? 0.f : ldexpf(n / L, EV);
+            y[x] = ldexpf(n * inv, EV);
         }
         st4(dst + 16 * dt + 4 * kq, y, vec);
     }
@@ -987,12 +989,12 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     const int64_t prow = ((int64_t)(it.part + w) * a.p.n_kv + kvh) * PAGED_TR + col;
     float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
     const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
-    const bool none = wa.l == 0.f;  // no page of this part is seen by the row
+    const float inv = wa.l == 0.f ? 0.f : 1.f / wa.l;  // (0: no page of this part is seen by the row)
 #pragma unroll
     for (int dt = 0; dt < W::NDT; ++dt) {
         v4f y;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = none ? 0.f : ldexpf(wa.o[dt][x] / wa.l, wa.ev);
+        for (int x = 0; x < 4; ++x) y[x] = ldexpf(wa.o[dt][x] * inv, wa.ev);
         st4(dst + 16 * dt + 4 * kq, y, vec);
     }
     if (part && kq == 0) {

@@ -366,8 +366,11 @@ __device__ __forceinline__ float col_max(float x) {
 // Levels that V scales are taken relative to: powers of 2^4.  The lowest: 2^-ev
 // is finite; the smallest scale is 2^-114.
 constexpr int EV_MIN = -112;
-__device__ __forceinline__ int ev_level(float vm) {  // 2^level >= vm
-    return max(EV_MIN, ((f_exp(vm) + 4) >> 2) * 4);
+// the lowest level with 2^level >= vm (1: 0, so that pages with and without a
+// scale other than 1 weigh alike)
+__device__ __forceinline__ int ev_level(float vm) {
+    const uint32_t below = __builtin_bit_cast(uint32_t, fmaxf(vm, 1e-37f)) - 1u;
+    return max(EV_MIN, (((int)(below >> 23) - 127 + 4) >> 2) * 4);
 }
 
 // One wave's online softmax over pages for a tile of 16 query rows.  Lane

@@ -137,11 +137,13 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     o.pages_read = (double)(total[0] + total[1]);
     const int64_t cu = std::max(g.cu, 1);
     for (int many = 0; many < 2; ++many) {
-        // Lists are split so that a launch has some four workgroups a CU, no
-        // finer than four pages (one a wave); many rows, where a partial is 64 KB
-        // and one workgroup fills a CU: one, no finer than eight pages
+        // Lists are split so that a launch has some four workgroups a CU (1 to 4
+        // are within 5%, 8 are 8% slower for one token over 131072), no finer than
+        // four pages, one a wave.  Many rows, where a partial is 64 KB and one
+        // workgroup fills a CU: one workgroup a CU, no finer than two pages (300
+        // rows over 1000 slots of 8-bit 128: 18 us, by four 20, by eight 23)
         const int64_t want = (many ? 1 : 4) * cu;
-        const int64_t least = many ? 8 : 4;
+        const int64_t least = many ? 2 : 4;
         int64_t per = std::max(least, (total[many] * g.n_kv + want - 1) / want);
         if (many && (int64_t)tiles[1].size() * g.n_kv >= want) per = INT32_MAX;
         for (const Tile& t : tiles[many]) {

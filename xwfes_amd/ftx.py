@@ -482,21 +482,28 @@ class Plan:
 
     def __init__(self, ctx, handle):
         self.ctx, self.handle = ctx, handle
+        L = ctx.lib  # (a step makes a few calls a layer: looked up once)
+        self._write, self._read, self._attend = (L.ftx_paged_write, L.ftx_paged_read,
+                                                 L.ftx_paged_attention)
 
     def set(self, seqs, n_head=0, window=0, sinks=0):
         a, keep = plan_args(seqs, n_head, window, sinks)
         self.ctx.check(self.ctx.lib.ftx_plan_set(self.handle, C.byref(a)))
 
     def write(self, layer, k_ptr, v_ptr, ldk=0, ldv=0):
-        self.ctx.check(self.ctx.lib.ftx_paged_write(self.handle, layer, k_ptr, ldk, v_ptr, ldv))
+        rc = self._write(self.handle, layer, k_ptr, ldk, v_ptr, ldv)
+        if rc:
+            self.ctx.check(rc)
 
     def read(self, layer, k_ptr, v_ptr, context=False, ldk=0, ldv=0):
-        self.ctx.check(self.ctx.lib.ftx_paged_read(self.handle, layer, int(context), k_ptr, ldk,
-                                                   v_ptr, ldv))
+        rc = self._read(self.handle, layer, context, k_ptr, ldk, v_ptr, ldv)
+        if rc:
+            self.ctx.check(rc)
 
     def attend(self, layer, q_ptr, out_ptr, ldq=0, ldo=0):
-        self.ctx.check(self.ctx.lib.ftx_paged_attention(self.handle, layer, q_ptr, ldq, out_ptr,
-                                                        ldo))
+        rc = self._attend(self.handle, layer, q_ptr, ldq, out_ptr, ldo)
+        if rc:
+            self.ctx.check(rc)
 
     def free(self):
         if self.handle:

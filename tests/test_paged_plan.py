@@ -115,8 +115,9 @@ CASES = [
 ]
 
 
+@pytest.mark.parametrize("hd,rows", [(64, 256), (128, 256), (256, 128)])
 @pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
-def test_items_cover_every_visible_page_once(case):
+def test_items_cover_every_visible_page_once(case, hd, rows):
     n_kv, n_head = case.get("n_kv", 2), case.get("n_head", 6)
     window, sinks = case.get("window", 0), case.get("sinks", 0)
     seqs, pages = [], 0
@@ -125,11 +126,11 @@ def test_items_cover_every_visible_page_once(case):
         par = [-1 if i < b[0] else max(i - b[0] - i % 3, 0) for i in range(M)] if b else None
         seqs.append((np.arange(pages, pages + n), npast, M, par))
         pages += n
-    rc, msg, items, combs = probe(seqs, n_kv, n_head, window, sinks, n_pages=pages + 1, cu=case.get("cu", 256))
+    rc, msg, items, combs = probe(seqs, n_kv, n_head, window, sinks, n_pages=pages + 1, cu=case.get("cu", 256), hd=hd)
     assert rc == 0, msg
     gqa = n_head // n_kv
-    # row tiles of 16, then those of 128 (sequences of 65 rows and more), the
-    # longest first in each
+    # row tiles of 16, then those of many rows (sequences of 65 rows and more),
+    # the longest first in each
     many = np.array([seqs[s][2] * gqa >= 65 for s in items[:, 0]], bool)
     assert (np.diff(many.astype(int)) >= 0).all()
     for part in (items[~many], items[many]):
@@ -137,7 +138,7 @@ def test_items_cover_every_visible_page_once(case):
     # a partial is a block of 16 rows: every place once, each joined once
     places = {}
     for (s, row0, _, _, _, _, p, _), mn in zip(items, many):
-        for x in range((8 if mn else 1) if p >= 0 else 0):
+        for x in range((rows // 16 if mn else 1) if p >= 0 else 0):
             assert p + x not in places
             places[p + x] = (s, row0 + 16 * x)
     assert sorted(places) == list(range(len(places)))
@@ -153,7 +154,7 @@ def test_items_cover_every_visible_page_once(case):
         want = np.repeat(pad.reshape(M, n, 64).any(2), gqa, axis=0)
         got = np.zeros((M * gqa, n), int)
         for _, row0, i0, i1, sp, a, _, _ in items[items[:, 0] == s]:
-            tr = 128 if M * gqa >= 65 else 16
+            tr = rows if M * gqa >= 65 else 16
             assert row0 % tr == 0 and i0 < i1
             pg = np.array([i if i < sp else a + i - sp for i in range(i0, i1)])
             assert (pg >= 0).all() and (pg < n).all() and sp <= a

@@ -384,8 +384,7 @@ __device__ __forceinline__ int ev_level(float vm) {
 // products of the sums so far, a third of a page's arithmetic, then fall to one
 // page in ten).  l = sum p, and P.V of p vs 2^-ev in two halves, ev the level
 // of the largest V scale that the row has seen.  out = 2^ev o / l.
-// STAGED: operands come from LDS and are read ahead of the products by hand.
-template <int HD, bool Q8, bool STAGED>
+template <int HD, bool Q8>
 struct WaveAttn {
     static constexpr int NDC = HD / 32, NDT = HD / 16;
     v8h qh[NDC], ql[NDC];
@@ -484,37 +483,6 @@ struct WaveAttn {
                 s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, l8, s[st], 0, 0, 0);
                 s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, h8, s[st], 0, 0, 0);
             }
-        }
-    }
-
-    // Scores of a page, k(st, dc) its operands: those of four slot tiles are
-    // read while the products of the four before them run, on accumulators
-    // that do not wait for each other (left to itself the compiler reads one
-    // operand, waits and multiplies: 733 us instead of 5xx for three chunks of
-    // 1500 tokens)
-    template <typename K>
-    __device__ __forceinline__ void scores(v4f (&s)[4], K k) const {
-        if constexpr (!STAGED) {
-            scores_of(s, k, [&](int dc) { return ql[dc]; }, [&](int dc) { return qh[dc]; });
-            return;
-        }
-        v8h f[2][4];
-#pragma unroll
-        for (int st = 0; st < 4; ++st) f[0][st] = k(st, 0);
-#pragma unroll
-        for (int dc = 0; dc < NDC; ++dc) {
-            if (dc + 1 < NDC)
-#pragma unroll
-                for (int st = 0; st < 4; ++st) f[(dc + 1) & 1][st] = k(st, dc + 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], ql[dc],
-                                                               dc ? s[st] : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-            for (int st = 0; st < 4; ++st)
-                s[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], qh[dc], s[st], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
@@ -641,33 +609,70 @@ struct WaveAttn {
                 o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[sp], o[dt], 0, 0, 0);
             }
     }
-    // the same, read as K's are; f: the first four
-    template <typename V>
-    __device__ __forceinline__ void outputs_first(v8h (&f)[2][4], V v) const {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) f[0][x] = v(x, 0);
-    }
-    template <typename V>
-    __device__ __forceinline__ void outputs(v8h (&f)[2][4], V v, const v8h (&ph)[2], const v8h (&pl)[2]) {
-        constexpr int NG = NDT / 2;  // groups: four dim tiles, one half of the slots
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            if (g + 1 < NG)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) f[(g + 1) & 1][x] = v((g + 1) / 2 * 4 + x, (g + 1) & 1);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-                o[g / 2 * 4 + x] =
-                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], pl[g & 1], o[g / 2 * 4 + x], 0, 0, 0);
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-                o[g / 2 * 4 + x] =
-                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], ph[g & 1], o[g / 2 * 4 + x], 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-    }
 };
+
+// Scores of a page for NT tiles of 16 rows from operands in LDS, k(st, dc) K's,
+// lo(x, dc) and hi(x, dc) tile x's query halves: the operands of four slot tiles
+// are read while the products of the four before them run, on accumulators that
+// do not wait for each other (left to itself the compiler reads one operand,
+// waits and multiplies: three chunks of 1500 tokens of 8-bit 128 took 733 us,
+// in this way 657).
+template <int NDC, int NT, typename K, typename L, typename H>
+__device__ __forceinline__ void staged_scores(v4f (&s)[NT][4], K k, L lo, H hi) {
+    v8h f[2][4], l[2][NT];
+    auto read = [&](int dc) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st) f[dc & 1][st] = k(st, dc);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) l[dc & 1][x] = lo(x, dc);
+    };
+    read(0);
+#pragma unroll
+    for (int dc = 0; dc < NDC; ++dc) {
+        if (dc + 1 < NDC) read(dc + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+                s[x][st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], l[dc & 1][x],
+                                                                  dc ? s[x][st] : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+                s[x][st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[dc & 1][st], hi(x, dc), s[x][st], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+// Outputs of a page, v(dt, sp) its V operands, read in the same way
+template <int NT, typename W, typename V>
+__device__ __forceinline__ void staged_outputs(W* wa, V v, const v8h (&ph)[NT][2], const v8h (&pl)[NT][2]) {
+    v8h f[2][4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) f[0][x] = v(x, 0);
+    constexpr int NG = W::NDT / 2;  // groups: four dim tiles, one half of the slots
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+        if (g + 1 < NG)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) f[(g + 1) & 1][x] = v((g + 1) / 2 * 4 + x, (g + 1) & 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+                wa[y].o[g / 2 * 4 + x] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], pl[y][g & 1], wa[y].o[g / 2 * 4 + x], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int y = 0; y < NT; ++y)
+                wa[y].o[g / 2 * 4 + x] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(f[g & 1][x], ph[y][g & 1], wa[y].o[g / 2 * 4 + x], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
 // What a lane's row (token t of the sequence) may see: slots lo .. hi and those
 // below sinks (a chain: up to its own; a tree: of the context), and of a tree's
@@ -712,7 +717,7 @@ struct RowSight {
 // in LDS.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
-    using W = WaveAttn<HD, Q8, false>;
+    using W = WaveAttn<HD, Q8>;
     constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
     // the query's halves, of which the four waves have the same: in LDS where
     // they would leave too few registers for the values in flight (halves of
@@ -792,7 +797,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
             asm volatile("" ::: "memory");  // (read again for every page)
             W::scores_of(s, kf, [&](int dc) { return qs[1][dc][lane]; }, [&](int dc) { return qs[0][dc][lane]; });
         } else {
-            wa.scores(s, kf);
+            W::scores_of(s, kf, [&](int dc) { return wa.ql[dc]; }, [&](int dc) { return wa.qh[dc]; });
         }
         __builtin_amdgcn_sched_barrier(0);
         const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((k1 != 1.f) | (v1 != 1.f));
@@ -861,7 +866,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-// Many rows: workgroup = (item of 128 rows, kv head), eight waves of 16 rows.
+// Many rows: workgroup = (item of paged_tr_many(HD) rows, kv head), eight waves
+// of two tiles of 16 rows (heads of 256 dims, or at most 128 rows: one), the low
+// halves of the queries in LDS.
 // Each page goes to LDS as the halves that the operands are (8-bit values
 // converted once, by all waves), one page ahead in the other buffer: halves by
 // direct copies, 8-bit values through registers, their loads issued before the
@@ -870,11 +877,16 @@ template <int HD>
 constexpr int many_buf_bytes() {
     return 2 * FTX_PAGE * HD * 2 + 3 * FTX_PAGE * 4 + 16;  // values, scales of K, V, V by level, its level
 }
-constexpr int NW_MANY = PAGED_TR_MANY / PAGED_TR;
+constexpr int NW_MANY = 8;
+template <int HD>
+constexpr int many_lo_bytes() {
+    return HD <= 128 ? paged_tr_many(HD) * HD * 2 : 0;
+}
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
-    constexpr int NW = NW_MANY;
-    using W = WaveAttn<HD, Q8, true>;
+    constexpr int NW = NW_MANY, NT = paged_tr_many(HD) / (NW * PAGED_TR);
+    constexpr bool QLO = many_lo_bytes<HD>() > 0;
+    using W = WaveAttn<HD, Q8>;
     constexpr int VB = FTX_PAGE * HD * 2;  // bytes of K's (V's) halves in LDS
     constexpr int BUF = many_buf_bytes<HD>();
     constexpr int NC = 2 * VB / 1024;  // KB of both
@@ -884,10 +896,12 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     const PagedSeq sq = it.q;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, kq = lane >> 4;
-    const int R = sq.M * a.gqa, rr = it.row0 + 16 * w + col, r = min(rr, R - 1), t = r / a.gqa;
-    const bool live = it.row0 + 16 * w < R;  // (wave-uniform)
-    const int64_t tok = sq.tok0 + t;
-    const int head = kvh * a.gqa + r % a.gqa;
+    const int R = sq.M * a.gqa;
+    // the wave's tiles: NT, or one where that takes all rows (of every wave alike)
+    const int nt = it.row0 + NW * PAGED_TR < R ? NT : 1;
+    auto tile_of = [&](int x) { return w * nt + x; };
+    auto row_of = [&](int x) { return it.row0 + 16 * tile_of(x) + col; };
+    const bool live = it.row0 + 16 * tile_of(0) < R;  // (wave-uniform)
     const bool vecq = !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15);
     const int n = it.i1 - it.i0;
     auto place = [&](int j) {
@@ -946,63 +960,92 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         }
     };
     stage(0);
-    W wa;
-    wa.query(a.q + tok * a.ldq + (int64_t)head * HD, kq, vecq);
-    const RowSight sight(a, sq, t);
-    // the pages that every row of the wave sees whole, and the last that any sees
-    int hi = sight.hi, lo = sight.lo, last = sight.anc ? sq.npast + t : sight.hi;
+    W wa[NT];
+    v8h* const qlo = (v8h*)(lds + 2 * BUF) + (QLO ? w * (NT * W::NDC * 64) + lane : 0);
+    // the pages that every row of a tile sees whole, and the last that any row sees
+    int hi[NT], lo[NT], last = 0;
 #pragma unroll
-    for (int x = 1; x < 16; x <<= 1) {
-        hi = min(hi, __shfl_xor(hi, x, 64));
-        lo = max(lo, __shfl_xor(lo, x, 64));
-        last = max(last, __shfl_xor(last, x, 64));
+    for (int x = 0; x < NT; ++x) {
+        const int r = min(row_of(x), R - 1), t = r / a.gqa;
+        wa[x].query(a.q + (int64_t)(sq.tok0 + t) * a.ldq + (int64_t)(kvh * a.gqa + r % a.gqa) * HD, kq, vecq);
+        if constexpr (QLO)
+#pragma unroll
+            for (int dc = 0; dc < W::NDC; ++dc) qlo[(x * W::NDC + dc) * 64] = wa[x].ql[dc];
+        const RowSight sight(a, sq, t);
+        int h = sight.hi, l = sight.lo, e = sight.anc ? sq.npast + t : sight.hi;
+#pragma unroll
+        for (int y = 1; y < 16; y <<= 1) {
+            h = min(h, __shfl_xor(h, y, 64));
+            l = max(l, __shfl_xor(l, y, 64));
+            e = max(e, __shfl_xor(e, y, 64));
+        }
+        hi[x] = __builtin_amdgcn_readfirstlane(h);
+        lo[x] = __builtin_amdgcn_readfirstlane(l);
+        last = max(last, __builtin_amdgcn_readfirstlane(e));
     }
-    hi = __builtin_amdgcn_readfirstlane(hi);
-    lo = __builtin_amdgcn_readfirstlane(lo);
-    last = __builtin_amdgcn_readfirstlane(last);
-    commit(0);
-    for (int j = 0; j < n; ++j) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's direct copies of page j
-        __syncthreads();                     // every wave's; the other buffer is free
-        if (j + 1 < n) stage(j + 1);
+    // page j for the wave's first N tiles
+    auto work = [&](auto tiles, int j) {
+        constexpr int N = decltype(tiles)::value;
         const int p0 = place(j) * FTX_PAGE;
-        if (live && p0 <= last) {
-            const uint8_t* buf = lds + (j & 1) * BUF;
-            const float* scale = (const float*)(buf + 2 * VB);
-            const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (scale[FTX_PAGE + lane] != 1.f));
-            v4f s[4];
-            wa.scores(s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); });
+        const uint8_t* buf = lds + (j & 1) * BUF;
+        const float* scale = (const float*)(buf + 2 * VB);
+        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (scale[FTX_PAGE + lane] != 1.f));
+        v4f s[N][4];
+        staged_scores<W::NDC>(
+            s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); },
+            [&](int x, int dc) { return QLO ? qlo[(x * W::NDC + dc) * 64] : wa[x].ql[dc]; },
+            [&](int x, int dc) { return wa[x].qh[dc]; });
+        v8h ph[N][2], pl[N][2];
+        auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
             typename W::Scales sc;
-            const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
+            const bool whole = p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
             if (!ones) W::load_scales(sc, scale, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
             const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
-            v8h ph[2], pl[2], f[2][4];
-            auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
-            wa.outputs_first(f, vf);
-            wa.soften(s, sc, ones, whole, pe, whole ? 0 : sight.page(p0) >> (4 * kq), ph, pl);
-            wa.outputs(f, vf, ph, pl);
+            uint64_t seen = 0;
+            if (!whole) seen = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0) >> (4 * kq);
+            wa[x].soften(s[x], sc, ones, whole, pe, seen, ph[x], pl[x]);
         }
-        if (j + 1 < n) commit(j + 1);
-    }
-    if (!live) return;
-    wa.l += __shfl_xor(wa.l, 16, 64);
-    wa.l += __shfl_xor(wa.l, 32, 64);
-    if (rr >= R) return;
-    const bool part = it.part >= 0;
-    const int64_t prow = ((int64_t)(it.part + w) * a.p.n_kv + kvh) * PAGED_TR + col;
-    float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
-    const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
-    const float inv = wa.l == 0.f ? 0.f : 1.f / wa.l;  // (0: no page of this part is seen by the row)
+        staged_outputs<N>(wa, vf, ph, pl);
+    };
+    commit(0);
+    auto pages = [&](auto tiles) {
+        for (int j = 0; j < n; ++j) {
+            __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's direct copies of page j
+            __syncthreads();                     // every wave's; the other buffer is free
+            if (j + 1 < n) stage(j + 1);
+            if (live && place(j) * FTX_PAGE <= last) work(tiles, j);
+            if (j + 1 < n) commit(j + 1);
+        }
+    };
+    if (nt == NT)
+        pages(std::integral_constant<int, NT>{});
+    else
+        pages(std::integral_constant<int, 1>{});
+    const bool part = it.part >= 0, vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
 #pragma unroll
-    for (int dt = 0; dt < W::NDT; ++dt) {
-        v4f y;
+    for (int x = 0; x < NT; ++x) {
+        if (x >= nt) return;
+        wa[x].l += __shfl_xor(wa[x].l, 16, 64);
+        wa[x].l += __shfl_xor(wa[x].l, 32, 64);
+        const int rr = row_of(x);
+        if (rr >= R) return;
+        const int64_t prow = ((int64_t)(it.part + tile_of(x)) * a.p.n_kv + kvh) * PAGED_TR + col;
+        float* dst = part ? a.part + prow * HD
+                          : a.out + (int64_t)(sq.tok0 + rr / a.gqa) * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD;
+        const float inv = wa[x].l == 0.f ? 0.f : 1.f / wa[x].l;  // (0: no page of this part is seen by the row)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) y[x] = ldexpf(wa.o[dt][x] * inv, wa.ev);
-        st4(dst + 16 * dt + 4 * kq, y, vec);
-    }
-    if (part && kq == 0) {
-        a.pml[2 * prow] = wa.off;
-        a.pml[2 * prow + 1] = wa.l;
+        for (int dt = 0; dt < W::NDT; ++dt) {
+            v4f y;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) y[z] = ldexpf(wa[x].o[dt][z] * inv, wa[x].ev);
+            st4(dst + 16 * dt + 4 * kq, y, vec);
+        }
+        if (part && kq == 0) {
+            a.pml[2 * prow] = wa[x].off;
+            a.pml[2 * prow + 1] = wa[x].l;
+        }
     }
 }
 
@@ -1118,7 +1161,7 @@ hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pag
 template <int HD, bool Q8>
 static hipError_t launch_many(hipStream_t st, const PagedAttn& a) {
     static std::atomic<uint64_t> lds_set{0};
-    constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD>();
+    constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD>() + many_lo_bytes<HD>();
     const hipError_t e = lds_limit((const void*)k_paged_many<HD, Q8>, bytes, lds_set);
     if (e != hipSuccess) return e;
     ktimed_launch(k_paged_many<HD, Q8>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(64 * NW_MANY),

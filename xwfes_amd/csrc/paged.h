@@ -47,7 +47,7 @@ struct PagedSeq {
     int64_t all0;        // its first row when contexts are read back
 };
 // A row tile (query rows of a kv head: row r = token r / gqa, head r % gqa;
-// PAGED_TR or PAGED_TR_MANY of them) over entries i0 .. i1 - 1 of its page
+// PAGED_TR or paged_tr_many(hd) of them) over entries i0 .. i1 - 1 of its page
 // list: pages 0 .. s - 1 (the first tokens'), then pages a, a + 1, ..  q: its
 // sequence, held here so that a workgroup's first page is two loads away and
 // not three
@@ -62,7 +62,8 @@ struct PagedItem {
 struct PagedComb {
     int32_t seq, row0, part0, n, step;
 };
-constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
+constexpr int PAGED_TR = 16;
+constexpr int paged_tr_many(int64_t hd) { return hd <= 128 ? 256 : 128; }
 
 struct PagedGeom {
     int64_t n_kv = 0, hd = 0, n_pages = 0;

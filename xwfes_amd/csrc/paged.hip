@@ -108,13 +108,13 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     struct Tile {
         int32_t seq, row0, rows, s, a, n;
     };
-    std::vector<Tile> tiles[2];  // of PAGED_TR rows, of PAGED_TR_MANY
+    std::vector<Tile> tiles[2];  // of PAGED_TR rows, of paged_tr_many
     int64_t total[2] = {0, 0};
     for (int64_t s = 0; s < a.nseq; ++s) {
         const PagedSeq& d = o.seqs[(size_t)s];
         const int64_t R = d.M * gqa;
         const int many = R >= PAGED_MANY;
-        const int64_t TR = many ? PAGED_TR_MANY : PAGED_TR;
+        const int64_t TR = many ? paged_tr_many(g.hd) : PAGED_TR;
         int64_t checked_s = 0, checked_a = d.ntab;  // pages seen so far: [0, checked_s), [checked_a, ..)
         for (int64_t row0 = 0; row0 < R; row0 += TR) {
             const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + TR) - 1) / gqa;
@@ -147,7 +147,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         int64_t per = std::max(least, (total[many] * g.n_kv + want - 1) / want);
         if (many && (int64_t)tiles[1].size() * g.n_kv >= want) per = INT32_MAX;
         for (const Tile& t : tiles[many]) {
-            const int64_t np = (t.n + per - 1) / per, blocks = many ? PAGED_TR_MANY / PAGED_TR : 1;
+            const int64_t np = (t.n + per - 1) / per, blocks = many ? paged_tr_many(g.hd) / PAGED_TR : 1;
             for (int64_t k = 0; k < np; ++k)
                 o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
                                             t.a, np > 1 ? (int32_t)(o.parts + k * blocks) : -1, 0,

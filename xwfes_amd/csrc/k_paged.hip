@@ -445,12 +445,13 @@ struct WaveAttn {
 #pragma unroll
         for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
     }
-    static __device__ __forceinline__ void load_scales(Scales& x, const float* k, const float* v, int kq) {
+    static __device__ __forceinline__ void load_four(v4f (&x)[4], const float* at, int kq) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-            x.k[st] = *(const v4f*)(k + 16 * st + 4 * kq);
-            x.v[st] = *(const v4f*)(v + 16 * st + 4 * kq);
-        }
+        for (int st = 0; st < 4; ++st) x[st] = *(const v4f*)(at + 16 * st + 4 * kq);
+    }
+    static __device__ __forceinline__ void load_scales(Scales& x, const float* k, const float* v, int kq) {
+        load_four(x.k, k, kq);
+        load_four(x.v, v, kq);
     }
     static __device__ __forceinline__ v8h k_frag(const Vals& x, int st, int dc) {
         if constexpr (Q8) {
@@ -494,17 +495,31 @@ struct WaveAttn {
         ev = en;
     }
 
-    // the scores' largest of the row
-    static __device__ __forceinline__ float row_max(const v4f (&s)[4]) {
-        float mx = fmaxf(s[0][0], s[0][1]);
+    // scores by the K scales
+    static __device__ __forceinline__ void by_scale(v4f (&s)[4], const Scales& sc) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st) mx = fmaxf(fmaxf(mx, s[st][2 * (st == 0)]), s[st][2 * (st == 0) + 1]);
-#pragma unroll
-        for (int st = 1; st < 4; ++st) mx = fmaxf(fmaxf(mx, s[st][2]), s[st][3]);
-        return col_max(mx);
+        for (int st = 0; st < 4; ++st) s[st] *= sc.k[st];
     }
 
-    // The page's weights from its scores; the sums so far brought to a new
+    // the scores' largest of the row (by name: from products of another basic
+    // block the compiler makes every score quiet before each fmaxf)
+    static __device__ __forceinline__ float row_max(const v4f (&s)[4]) {
+        auto max3 = [](float x, float y, float z) {
+            float r;
+            asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+            return r;
+        };
+        float mx = max3(s[0][0], s[0][1], s[0][2]);
+        mx = max3(mx, s[0][3], s[1][0]);
+        mx = max3(mx, s[1][1], s[1][2]);
+        mx = max3(mx, s[1][3], s[2][0]);
+        mx = max3(mx, s[2][1], s[2][2]);
+        mx = max3(mx, s[2][3], s[3][0]);
+        mx = max3(mx, s[3][1], s[3][2]);
+        return col_max(max3(mx, s[3][3], s[3][3]));
+    }
+
+    // The page's weights from its scores (by_scale's); the sums so far brought to a new
     // offset or V level where one is needed.  ones: every scale of the page is 1
     // (sc is not read).  whole: the row sees every slot, else slot 16 st + 4 kq + r
     // by bit 16 st + r of seen.  pe: sc.v stands 2^-pe over, pe the level of the page's largest
@@ -513,30 +528,21 @@ struct WaveAttn {
     static constexpr int NO_LEVEL = 1 << 20;
     __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, uint64_t seen,
                                            v8h (&ph)[2], v8h (&pl)[2]) {
-        // (the scales' products and the maximum in one basic block: across a
-        // branch the compiler makes every score quiet first)
-        float mx;
-        if (whole) {
-            if (!ones)
-#pragma unroll
-                for (int st = 0; st < 4; ++st) s[st] *= sc.k[st];
-            mx = row_max(s);
-        } else {
+        if (!whole) {
 #pragma unroll
             for (int st = 0; st < 4; ++st)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     // all ones or zeros
                     const uint32_t ok = __builtin_amdgcn_sbfe((int)(seen >> (st >= 2 ? 32 : 0)), 16 * (st & 1) + r, 1);
-                    const float x = ones ? s[st][r] : s[st][r] * sc.k[st][r];
+                    // (copies: a bit cast of a vector's element takes element 0)
+                    const float x = s[st][r], y = sc.v[st][r];
                     s[st][r] = __builtin_bit_cast(
                         float, (__builtin_bit_cast(uint32_t, x) & ok) | (0xFF800000u & ~ok));  // -inf
-                    // (a copy: a bit cast of a vector's element takes element 0)
-                    const float y = sc.v[st][r];
                     if (!ones) sc.v[st][r] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & ok);
                 }
-            mx = row_max(s);
         }
+        const float mx = row_max(s);
         const float cand = __builtin_fmaf(mx, c2, -12.f);
         if (__builtin_amdgcn_ballot_w64(cand > off + 3.f)) {  // (wave-uniform)
             const float on = fmaxf(off, cand);
@@ -811,6 +817,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
         const int p0 = place(j) * FTX_PAGE;
         const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
         v8h ph[2], pl[2];
+        if (!ones) W::by_scale(s, sc);
         wa.soften(s, sc, ones, whole, W::NO_LEVEL, whole ? 0 : sight.page(p0) >> (4 * kq), ph, pl);
         wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
     }
@@ -996,12 +1003,17 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             [&](int x, int dc) { return QLO ? qlo[(x * W::NDC + dc) * 64] : wa[x].ql[dc]; },
             [&](int x, int dc) { return wa[x].qh[dc]; });
         v8h ph[N][2], pl[N][2];
+        typename W::Scales sc;
+        if (!ones) {
+            W::load_four(sc.k, scale, kq);
+#pragma unroll
+            for (int x = 0; x < N; ++x) W::by_scale(s[x], sc);
+        }
         auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            typename W::Scales sc;
             const bool whole = p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
-            if (!ones) W::load_scales(sc, scale, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
+            if (!ones) W::load_four(sc.v, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
             const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
             uint64_t seen = 0;
             if (!whole) seen = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0) >> (4 * kq);

@@ -30,6 +30,18 @@ F16, Q8 = ftx.KV_F16, ftx.KV_Q8
 TYPES = pytest.mark.parametrize("kvt", [F16, Q8], ids=["f16", "q8"])
 
 
+@pytest.fixture(params=[0, 16, 128, 256], ids=["est", "r16", "r128", "r256"])
+def tiles(request):
+    """The row tiles of sequences of 65 rows and more: by the estimate, or given."""
+    force = ftx.load().paged_force_rows
+    force(request.param)
+    yield request.param
+    force(0)
+
+
+TILES = pytest.mark.usefixtures("tiles")
+
+
 def stored(x, kvt):
     """What rows [..., hd] stand for once stored."""
     x = np.asarray(x, np.float32)
@@ -239,6 +251,7 @@ def test_rows_of_every_size(gctx, kvt):
 # ---------------------------------------------------------------- attention
 
 
+@TILES
 @TYPES
 @pytest.mark.parametrize("hd,kv,heads,seqs", [
     (64, 8, 8, [(128, 1)]), (128, 8, 32, [(0, 1)]), (128, 2, 16, [(63, 1), (64, 1), (65, 1), (700, 1), (0, 1)]),
@@ -252,6 +265,7 @@ def test_chains(gctx, kvt, hd, kv, heads, seqs):
     c.free()
 
 
+@TILES
 @TYPES
 @pytest.mark.parametrize("hd,kv,heads,seqs,window,sinks", [
     (128, 2, 8, [(300, 1), (1000, 1)], 1, 0), (128, 2, 8, [(300, 1), (1000, 3)], 64, 0), (64, 2, 8, [(500, 70)], 65, 4),
@@ -265,6 +279,7 @@ def test_windows(gctx, kvt, hd, kv, heads, seqs, window, sinks):
     c.free()
 
 
+@TILES
 @TYPES
 @pytest.mark.parametrize("hd,kv,heads,seqs,window,sinks", [
     (128, 2, 8, [(300, 52, 4)], 0, 0), (64, 2, 8, [(0, 33, 1), (61, 7, 3)], 0, 0), (128, 1, 8, [(900, 256, 2), (5, 3)], 0, 0),
@@ -278,6 +293,7 @@ def test_trees(gctx, kvt, hd, kv, heads, seqs, window, sinks):
     c.free()
 
 
+@TILES
 @TYPES
 @pytest.mark.parametrize("qs,ks,vs", [(1e30, 1e-30, 1.0), (1e-25, 1e25, 1e30), (1.0, 1.0, 1e-28), (30.0, 3.0, 1.0),
                                       (1e3, 1e2, 1e-3), (0.0, 1.0, 1.0), (1.0, 0.0, 0.0)])
@@ -290,6 +306,7 @@ def test_values_of_every_size(gctx, kvt, qs, ks, vs):
     c.free()
 
 
+@TILES
 @TYPES
 def test_large_values_in_hidden_places_change_nothing(gctx, kvt):
     """Rows that a token does not see may be huge, infinite or NaN: its output
@@ -318,6 +335,7 @@ def test_large_values_in_hidden_places_change_nothing(gctx, kvt):
     assert np.isnan(got[np.nan][20:50, 4:]).all() and np.isnan(got[np.inf][20:50, 4:]).all()
 
 
+@TILES
 @TYPES
 def test_a_row_hidden_by_the_window(gctx, kvt):
     """NaN rows between the first tokens and the window, in pages that are read
@@ -338,6 +356,7 @@ def test_a_row_hidden_by_the_window(gctx, kvt):
     assert np.isfinite(outs[0]).all()
 
 
+@TILES
 @TYPES
 def test_pages_that_held_other_things(gctx, kvt):
     """A page that another sequence left full of NaN, then used for a few tokens."""
@@ -358,6 +377,7 @@ def test_pages_that_held_other_things(gctx, kvt):
     c.free()
 
 
+@TILES
 @TYPES
 @pytest.mark.parametrize("pad,off", [(4, 4), (3, 0), (0, 1), (8, 2)])
 def test_strides_and_alignment(gctx, kvt, pad, off):
@@ -369,6 +389,7 @@ def test_strides_and_alignment(gctx, kvt, pad, off):
     c.free()
 
 
+@TILES
 def test_q_k_v_in_one_matrix(gctx):
     """Rows of q | k | v as a projection leaves them, out over q's place of a
     second matrix's columns."""
@@ -386,6 +407,7 @@ def test_q_k_v_in_one_matrix(gctx):
     c.free()
 
 
+@TILES
 @TYPES
 def test_chunks_give_what_one_chunk_gives(gctx, kvt):
     """A prompt in chunks of uneven length over one growing table: each chunk's
@@ -413,6 +435,7 @@ def test_chunks_give_what_one_chunk_gives(gctx, kvt):
     whole.free()
 
 
+@TILES
 @TYPES
 def test_shared_prefix_pages(gctx, kvt):
     """Two sequences over one sequence's first pages, each with its own last page."""
@@ -524,6 +547,7 @@ def test_sequences_without_new_tokens(gctx):
     c.free()
 
 
+@TILES
 @TYPES
 def test_two_graphs_replayed(gctx, kvt):
     """Two plans of one pool, each step captured on its own stream; replays side

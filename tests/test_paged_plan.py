@@ -112,10 +112,21 @@ CASES = [
     dict(seqs=[(900, 40, 3)], window=30, sinks=2), dict(seqs=[(0, 200, 2), (70, 64, 4)], window=3, sinks=3),
     dict(seqs=[(500, 256, 1)]), dict(seqs=[(1900, 1)], cu=1), dict(seqs=[(1900, 1)], cu=4096),
     dict(seqs=[(1500, 33), (1, 1)], n_kv=8, n_head=8), dict(seqs=[(300, 20)], n_kv=1, n_head=48),
+    dict(seqs=[(1900, 260), (40, 50), (3, 2)], cu=1), dict(seqs=[(1900, 260), (500, 30)], cu=9),
+    dict(seqs=[(3000, 64), (3000, 64), (3000, 70)], n_kv=8, n_head=32), dict(seqs=[(250, 40)], n_kv=8, n_head=32),
 ]
 
 
-@pytest.mark.parametrize("hd,rows", [(64, 256), (128, 256), (256, 128)])
+@pytest.fixture(params=[0, 16, 128, 256], ids=["est", "r16", "r128", "r256"])
+def rows(request):
+    """The row tiles of sequences of 65 rows and more: by the estimate, or given."""
+    force = ftx.load().paged_force_rows
+    force(request.param)
+    yield request.param
+    force(0)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("case", CASES, ids=[str(i) for i in range(len(CASES))])
 def test_items_cover_every_visible_page_once(case, hd, rows):
     n_kv, n_head = case.get("n_kv", 2), case.get("n_head", 6)
@@ -129,16 +140,21 @@ def test_items_cover_every_visible_page_once(case, hd, rows):
     rc, msg, items, combs = probe(seqs, n_kv, n_head, window, sinks, n_pages=pages + 1, cu=case.get("cu", 256), hd=hd)
     assert rc == 0, msg
     gqa = n_head // n_kv
-    # row tiles of 16, then those of many rows (sequences of 65 rows and more),
-    # the longest first in each
-    many = np.array([seqs[s][2] * gqa >= 65 for s in items[:, 0]], bool)
+    # row tiles of 16 (all of sequences of up to 64 rows), then those of 128 or
+    # 256, the longest first in each
+    many = items[:, 7] > 0
+    big = np.array([seqs[s][2] * gqa > 64 for s in items[:, 0]], bool)
+    assert not many[~big].any()
+    if rows:
+        assert (many[big] == (rows > 16)).all() and (items[:, 7] <= max(min(rows, 256 if hd <= 128 else 128) // 128, 0)).all()
     assert (np.diff(many.astype(int)) >= 0).all()
     for part in (items[~many], items[many]):
-        assert (np.diff(part[:, 3] - part[:, 2]) <= 0).all()
+        assert (np.diff((part[:, 3] - part[:, 2]) * np.where(part[:, 7] == 2, 7, 4)) <= 0).all()
     # a partial is a block of 16 rows: every place once, each joined once
     places = {}
-    for (s, row0, _, _, _, _, p, _), mn in zip(items, many):
-        for x in range((rows // 16 if mn else 1) if p >= 0 else 0):
+    for (s, row0, _, _, _, _, p, nt), mn in zip(items, many):
+        assert nt in ((0, 1, 2) if hd <= 128 else (0, 1))
+        for x in range((8 * nt if mn else 1) if p >= 0 else 0):
             assert p + x not in places
             places[p + x] = (s, row0 + 16 * x)
     assert sorted(places) == list(range(len(places)))
@@ -153,13 +169,25 @@ def test_items_cover_every_visible_page_once(case, hd, rows):
         pad[:, :npast + M] = see
         want = np.repeat(pad.reshape(M, n, 64).any(2), gqa, axis=0)
         got = np.zeros((M * gqa, n), int)
-        for _, row0, i0, i1, sp, a, _, _ in items[items[:, 0] == s]:
-            tr = rows if M * gqa >= 65 else 16
+        for _, row0, i0, i1, sp, a, _, nt in items[items[:, 0] == s]:
+            tr = 128 * nt or 16
             assert row0 % tr == 0 and i0 < i1
             pg = np.array([i if i < sp else a + i - sp for i in range(i0, i1)])
             assert (pg >= 0).all() and (pg < n).all() and sp <= a
             got[row0:row0 + tr, pg] += 1
         assert got.max(initial=0) <= 1 and (got[want] == 1).all()
+
+
+@pytest.mark.parametrize("hd,M,npast,nseq,nt", [
+    (128, 256, 4000, 16, {2}), (128, 17, 4000, 4, {1}), (128, 64, 300, 1, {0}), (64, 1, 100000, 1, {0}),
+    (256, 256, 4000, 16, {1}), (128, 80, 4000, 4, {1, 2}), (128, 16, 5000, 8, {0}),
+])
+def test_tiles_by_the_work(hd, M, npast, nseq, nt):
+    n = (npast + M + 63) // 64
+    seqs = [(np.arange(i * n, i * n + n), npast, M) for i in range(nseq)]
+    rc, msg, items, _ = probe(seqs, 8, 32, n_pages=nseq * n, hd=hd)
+    assert rc == 0, msg
+    assert set(items[:, 7]) == nt
 
 
 def test_null_arguments_are_status_codes():

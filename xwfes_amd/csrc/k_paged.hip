@@ -727,7 +727,7 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
     // the query's halves, of which the four waves have the same: in LDS where
     // they would leave too few registers for the values in flight (halves of
-    // 128 dims: 37 spilled, 129 us for one token over 131072; so 1xx)
+    // 128 dims: 37 spilled, 129 us for one token over 131072; so 104)
     constexpr bool QLDS = !Q8 && HD >= 128;
     __shared__ v8h qs[QLDS ? 2 : 1][W::NDC][64];
     __shared__ float so[3][4 * W::NDT][64], sm[4][64], sl[4][64];
@@ -873,9 +873,9 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-// Many rows: workgroup = (item of paged_tr_many(HD) rows, kv head), eight waves
-// of two tiles of 16 rows (heads of 256 dims, or at most 128 rows: one), the low
-// halves of the queries in LDS.
+// Many rows: workgroup = (item of 128 or 256 rows, kv head), eight waves of one
+// or two tiles of 16 rows, the low halves of the queries in LDS (but for heads
+// of 256 dims, where LDS holds the pages alone and a wave has one tile).
 // Each page goes to LDS as the halves that the operands are (8-bit values
 // converted once, by all waves), one page ahead in the other buffer: halves by
 // direct copies, 8-bit values through registers, their loads issued before the
@@ -884,14 +884,18 @@ template <int HD>
 constexpr int many_buf_bytes() {
     return 2 * FTX_PAGE * HD * 2 + 3 * FTX_PAGE * 4 + 16;  // values, scales of K, V, V by level, its level
 }
-constexpr int NW_MANY = 8;
+constexpr int NW_MANY = PAGED_TR_MANY / PAGED_TR;
+template <int HD>
+constexpr int many_tiles() {
+    return HD <= 128 ? 2 : 1;
+}
 template <int HD>
 constexpr int many_lo_bytes() {
-    return HD <= 128 ? paged_tr_many(HD) * HD * 2 : 0;
+    return HD <= 128 ? many_tiles<HD>() * PAGED_TR_MANY * HD * 2 : 0;
 }
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
-    constexpr int NW = NW_MANY, NT = paged_tr_many(HD) / (NW * PAGED_TR);
+    constexpr int NW = NW_MANY, NT = many_tiles<HD>();
     constexpr bool QLO = many_lo_bytes<HD>() > 0;
     using W = WaveAttn<HD, Q8>;
     constexpr int VB = FTX_PAGE * HD * 2;  // bytes of K's (V's) halves in LDS
@@ -904,8 +908,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, kq = lane >> 4;
     const int R = sq.M * a.gqa;
-    // the wave's tiles: NT, or one where that takes all rows (of every wave alike)
-    const int nt = it.row0 + NW * PAGED_TR < R ? NT : 1;
+    const int nt = NT == 1 ? 1 : it.nt;  // the wave's tiles
     auto tile_of = [&](int x) { return w * nt + x; };
     auto row_of = [&](int x) { return it.row0 + 16 * tile_of(x) + col; };
     const bool live = it.row0 + 16 * tile_of(0) < R;  // (wave-uniform)
@@ -973,6 +976,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     int hi[NT], lo[NT], last = 0;
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
+        if (x >= nt) break;
         const int r = min(row_of(x), R - 1), t = r / a.gqa;
         wa[x].query(a.q + (int64_t)(sq.tok0 + t) * a.ldq + (int64_t)(kvh * a.gqa + r % a.gqa) * HD, kq, vecq);
         if constexpr (QLO)
@@ -1031,8 +1035,10 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             if (j + 1 < n) commit(j + 1);
         }
     };
-    if (nt == NT)
-        pages(std::integral_constant<int, NT>{});
+    if constexpr (NT == 1)
+        pages(std::integral_constant<int, 1>{});
+    else if (nt == 2)  // (of every wave alike)
+        pages(std::integral_constant<int, 2>{});
     else
         pages(std::integral_constant<int, 1>{});
     const bool part = it.part >= 0, vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);

@@ -47,14 +47,14 @@ struct PagedSeq {
     int64_t all0;        // its first row when contexts are read back
 };
 // A row tile (query rows of a kv head: row r = token r / gqa, head r % gqa;
-// PAGED_TR or paged_tr_many(hd) of them) over entries i0 .. i1 - 1 of its page
+// PAGED_TR, PAGED_TR_MANY or twice that many of them) over entries i0 .. i1 - 1 of its page
 // list: pages 0 .. s - 1 (the first tokens'), then pages a, a + 1, ..  q: its
 // sequence, held here so that a workgroup's first page is two loads away and
 // not three
 struct PagedItem {
     int32_t seq, row0, i0, i1, s, a;
     int32_t part;  // its partials' place (in blocks of PAGED_TR rows), or -1: the whole list, results go to out
-    int32_t pad;
+    int32_t nt;    // 0: PAGED_TR rows; 1: PAGED_TR_MANY; 2: twice that
     PagedSeq q;
     int32_t fill[6];  // to 96 bytes
 };
@@ -62,8 +62,7 @@ struct PagedItem {
 struct PagedComb {
     int32_t seq, row0, part0, n, step;
 };
-constexpr int PAGED_TR = 16;
-constexpr int paged_tr_many(int64_t hd) { return hd <= 128 ? 256 : 128; }
+constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
 
 struct PagedGeom {
     int64_t n_kv = 0, hd = 0, n_pages = 0;
@@ -96,6 +95,10 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
 extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int64_t n_pages, const uint8_t* taken,
                            int cu, PagedItem* items, int64_t* n_items, PagedComb* combs, int64_t* n_combs,
                            int64_t max_out, char* msg, int64_t msg_bytes);
+
+// For tests: the row tiles of sequences of many rows from now on, 16, 128 or 256
+// (heads of 256 dims: 128), 0: by the estimate
+extern "C" void paged_force_rows(int rows);
 
 // ---------------------------------------------------------------- launches
 struct PagedView {

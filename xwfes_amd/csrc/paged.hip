@@ -8,11 +8,59 @@
 
 #include "paged_pool.h"
 
+#include <atomic>
+
 // ---------------------------------------------------------------- plan tables
 
-// Query rows of a kv head from which a sequence goes to the kernel that shares
-// each page among 128 rows
+// Sequences of at least this many query rows a kv head may go to the kernel
+// that shares each page among 128 or 256 rows
 constexpr int64_t PAGED_MANY = 65;
+// Row tiles beyond which such sequences do so without a look at tiles of 16
+constexpr int64_t FEW_MOST = 4096;
+
+namespace {
+
+std::atomic<int> forced_rows{0};  // (paged_force_rows)
+
+struct Tile {
+    int32_t seq, row0, rows, s, a, n;  // n pages: 0 .. s - 1, then a, a + 1, ..
+    int tiles() const { return rows > PAGED_TR_MANY ? 2 : 1; }  // of many rows: a wave's
+};
+
+// us that a launch takes whose lists are split into parts of up to `per` pages,
+// `slots` workgroups at a time, each `fix` and `page` for a page (1.74 times
+// that for two row tiles a wave); a join's launch, its partials written and read
+// at 6 TB/s, what passes 128 MB slower.  Lists of one length go round by round,
+// others fill the gaps of each other.
+struct LaunchCost {
+    int64_t n_kv, hd, slots;
+    double fix, page;
+    double operator()(const std::vector<Tile>& tiles, int64_t per) const {
+        double total = 0, longest = 0;
+        int64_t n = 0, rows = 0;
+        for (const Tile& t : tiles) {
+            const int64_t np = (t.n + per - 1) / per;
+            const bool two = t.tiles() == 2;
+            const double c = fix + (two ? 3 : 0) + (double)((t.n + np - 1) / np) * page * (two ? 1.74 : 1);
+            total += (double)np * c;
+            longest = std::max(longest, c);
+            n += np;
+            if (np > 1) rows += np * t.rows;
+        }
+        if (n == 0) return 0;
+        const double mean = total / (double)n, whole = total * (double)n_kv / (double)slots;
+        double e = longest;
+        if (n * n_kv > slots) {
+            const double rounds = (double)((n * n_kv + slots - 1) / slots) * mean;
+            e = std::max(e, whole + (rounds - whole) * std::max(0., 1 - 4 * (1 - mean / longest)));
+        }
+        if (rows == 0) return e;
+        const double b = (double)(rows * n_kv * hd) * 8;
+        return e + 4 + b / 6e6 + std::max(0., b - 128e6) / 4e6;
+    }
+};
+
+}  // namespace
 
 int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_t>& mark,
                  uint32_t& epoch, PagedTables& o, std::string& err) {
@@ -104,53 +152,102 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         o.seqs.push_back(d);
     }
     if (a.n_head == 0) return FTX_OK;
-    // the row tiles and the pages each sees
-    struct Tile {
-        int32_t seq, row0, rows, s, a, n;
+    // The row tiles and the pages each sees: of TR rows for the sequences of
+    // PAGED_MANY rows and more (big) or the others.  false: a page is absent.
+    auto tile_all = [&](std::vector<Tile>& tiles, bool big, int64_t TR) -> bool {
+        for (int64_t s = 0; s < a.nseq; ++s) {
+            const PagedSeq& d = o.seqs[(size_t)s];
+            const int64_t R = d.M * gqa;
+            if ((R >= PAGED_MANY) != big) continue;
+            int64_t checked_s = 0, checked_a = d.ntab;  // pages seen so far: [0, checked_s), [checked_a, ..)
+            for (int64_t row0 = 0; row0 < R; row0 += TR) {
+                const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + TR) - 1) / gqa;
+                // (a tree's nodes are all looked at: a node's position is below its slot)
+                int64_t lo = 0;
+                if (W) lo = std::max<int64_t>(0, d.npast + (d.dep0 >= 0 ? 0 : t0) - W + 1);
+                const int64_t pa = lo / FTX_PAGE, pe = (d.npast + t1) / FTX_PAGE + 1;
+                const int64_t ps = std::min((sinks + FTX_PAGE - 1) / FTX_PAGE, pa);
+                tiles.push_back(Tile{(int32_t)s, (int32_t)row0, (int32_t)std::min(R - row0, TR), (int32_t)ps,
+                                     (int32_t)pa, (int32_t)(ps + pe - pa)});
+                for (; checked_s < ps; ++checked_s)
+                    if (o.table[(size_t)(d.tab0 + checked_s)] < 0) return false;
+                for (; checked_a > pa; --checked_a)
+                    if (o.table[(size_t)(d.tab0 + checked_a - 1)] < 0) return false;
+            }
+        }
+        return true;
     };
-    std::vector<Tile> tiles[2];  // of PAGED_TR rows, of paged_tr_many
-    int64_t total[2] = {0, 0};
-    for (int64_t s = 0; s < a.nseq; ++s) {
-        const PagedSeq& d = o.seqs[(size_t)s];
-        const int64_t R = d.M * gqa;
-        const int many = R >= PAGED_MANY;
-        const int64_t TR = many ? paged_tr_many(g.hd) : PAGED_TR;
-        int64_t checked_s = 0, checked_a = d.ntab;  // pages seen so far: [0, checked_s), [checked_a, ..)
-        for (int64_t row0 = 0; row0 < R; row0 += TR) {
-            const int64_t t0 = row0 / gqa, t1 = (std::min(R, row0 + TR) - 1) / gqa;
-            // (a tree's nodes are all looked at: a node's position is below its slot)
-            int64_t lo = 0;
-            if (W) lo = std::max<int64_t>(0, d.npast + (d.dep0 >= 0 ? 0 : t0) - W + 1);
-            const int64_t pa = lo / FTX_PAGE, pe = (d.npast + t1) / FTX_PAGE + 1;
-            const int64_t ps = std::min((sinks + FTX_PAGE - 1) / FTX_PAGE, pa);
-            tiles[many].push_back(Tile{(int32_t)s, (int32_t)row0, (int32_t)std::min(R - row0, TR), (int32_t)ps,
-                                       (int32_t)pa, (int32_t)(ps + pe - pa)});
-            total[many] += ps + pe - pa;
-            for (; checked_s < ps; ++checked_s)
-                if (o.table[(size_t)(d.tab0 + checked_s)] < 0)
-                    return fail(FTX_E_INVALID, "a page that a new token sees is absent");
-            for (; checked_a > pa; --checked_a)
-                if (o.table[(size_t)(d.tab0 + checked_a - 1)] < 0)
-                    return fail(FTX_E_INVALID, "a page that a new token sees is absent");
+    const int64_t cu = std::max(g.cu, 1);
+    // Few rows: lists are split so that a launch has some four workgroups a CU (1
+    // to 4 are within 5%, 8 are 8% slower for one token over 131072), no finer
+    // than four pages, one a wave.
+    auto few_per = [&](const std::vector<Tile>& tiles) {
+        int64_t total = 0;
+        for (const Tile& t : tiles) total += t.n;
+        return std::max<int64_t>(4, (total * g.n_kv + 4 * cu - 1) / (4 * cu));
+    };
+    std::vector<Tile> tiles[2], big;  // of PAGED_TR rows, of many
+    int64_t per[2] = {INT32_MAX, INT32_MAX}, big_rows = 0;
+    bool present = tile_all(tiles[0], false, PAGED_TR);
+    for (const PagedSeq& d : o.seqs)
+        if (d.M * gqa >= PAGED_MANY) big_rows += d.M * gqa;
+    if (present && big_rows) {
+        // Sequences of many rows: tiles of 256, 128 or 16 rows (the kernel of
+        // few), their lists split as it is estimated fastest.  Measured, us, for
+        // rows x context (8-bit, 128 dims, 8 kv heads), by 256 / 128 / 16 rows:
+        // 16 x 1024 over 4000: 508 / 581 / 753; 16 x 768 over 4000 (256 rows
+        // leave a third of the second round empty): 545 / 480 / -; 4 x 68 over
+        // 4000: - / 29 / 34; 256 over 300: 22 / 15 / 11.
+        const double page = 0.75 + 1.5 * (double)g.hd / 128;
+        double best = 1e300;
+        int64_t bestp = 0, chosen = 0;
+        const int force = forced_rows.load(std::memory_order_relaxed);
+        const int64_t most = g.hd <= 128 && (force == 0 || force > PAGED_TR_MANY) ? 2 * PAGED_TR_MANY : PAGED_TR_MANY;
+        for (int64_t TR = most; present && TR >= PAGED_TR_MANY; TR /= 2) {
+            if (force && TR < most) break;
+            big.clear();
+            present = tile_all(big, true, TR);
+            const LaunchCost cost{g.n_kv, g.hd, cu, 8, page};
+            int64_t longest = 0;
+            for (const Tile& t : big) longest = std::max<int64_t>(longest, t.n);
+            const bool full = (int64_t)big.size() * g.n_kv >= 4 * cu;
+            for (int64_t k = 1; k <= 64; k += 1 + k / 6) {
+                const int64_t p = (longest + k - 1) / k;
+                if (k > 1 && (full || p < 2)) break;
+                const double us = cost(big, p);
+                if (us >= best) continue;
+                best = us;
+                bestp = p;
+                chosen = TR;
+            }
+            if (chosen == TR) {
+                tiles[1] = big;
+                per[1] = bestp;
+            }
+        }
+        if (present && (force ? force == PAGED_TR : big_rows / PAGED_TR <= FEW_MOST)) {
+            big = tiles[0];
+            present = tile_all(big, true, PAGED_TR);
+            const LaunchCost cost{g.n_kv, g.hd, 2 * cu, 8, 0.8 * (double)g.hd / 128};
+            const int64_t p = few_per(big);
+            const double others = tiles[0].empty() ? 0 : cost(tiles[0], few_per(tiles[0]));
+            if (present && (force || cost(big, p) - others < best)) {
+                tiles[0] = big;
+                tiles[1].clear();
+            }
         }
     }
-    o.pages_read = (double)(total[0] + total[1]);
-    const int64_t cu = std::max(g.cu, 1);
+    if (!present) return fail(FTX_E_INVALID, "a page that a new token sees is absent");
+    per[0] = few_per(tiles[0]);
+    o.pages_read = 0;
     for (int many = 0; many < 2; ++many) {
-        // Lists are split so that a launch has some four workgroups a CU (1 to 4
-        // are within 5%, 8 are 8% slower for one token over 131072), no finer than
-        // four pages, one a wave.  Many rows, where a partial is 64 KB and one
-        // workgroup fills a CU: one workgroup a CU, no finer than two pages (300
-        // rows over 1000 slots of 8-bit 128: 18 us, by four 20, by eight 23)
-        const int64_t want = (many ? 1 : 4) * cu;
-        const int64_t least = many ? 2 : 4;
-        int64_t per = std::max(least, (total[many] * g.n_kv + want - 1) / want);
-        if (many && (int64_t)tiles[1].size() * g.n_kv >= want) per = INT32_MAX;
         for (const Tile& t : tiles[many]) {
-            const int64_t np = (t.n + per - 1) / per, blocks = many ? paged_tr_many(g.hd) / PAGED_TR : 1;
+            o.pages_read += t.n;
+            const int nt = many ? t.tiles() : 0;
+            const int64_t np = (t.n + per[many] - 1) / per[many], blocks = many ? nt * PAGED_TR_MANY / PAGED_TR : 1;
             for (int64_t k = 0; k < np; ++k)
                 o.items.push_back(PagedItem{t.seq, t.row0, (int32_t)(t.n * k / np), (int32_t)(t.n * (k + 1) / np), t.s,
-                                            t.a, np > 1 ? (int32_t)(o.parts + k * blocks) : -1, 0,
+                                            t.a, np > 1 ? (int32_t)(o.parts + k * blocks) : -1, nt,
                                             o.seqs[(size_t)t.seq], {}});
             if (np == 1) continue;
             o.comb_max = std::max(o.comb_max, np);
@@ -159,10 +256,10 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
                                             (int32_t)blocks});
             o.parts += np * blocks;
         }
-        // the longest first
-        std::stable_sort(o.items.begin() + o.few, o.items.end(), [](const PagedItem& x, const PagedItem& y) {
-            return x.i1 - x.i0 > y.i1 - y.i0;
-        });
+        // the longest first (two row tiles a wave: 7 for 4)
+        auto work = [](const PagedItem& x) { return (x.i1 - x.i0) * (int64_t)(x.nt == 2 ? 7 : 4); };
+        std::stable_sort(o.items.begin() + o.few, o.items.end(),
+                         [&](const PagedItem& x, const PagedItem& y) { return work(x) > work(y); });
         if (!many) o.few = (int64_t)o.items.size();
     }
     if ((int64_t)o.items.size() * g.n_kv >= (int64_t)1 << 31 || (int64_t)o.combs.size() * g.n_kv >= (int64_t)1 << 31 ||
@@ -170,6 +267,8 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
     return FTX_OK;
 }
+
+extern "C" void paged_force_rows(int rows) { forced_rows.store(rows, std::memory_order_relaxed); }
 
 extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int64_t n_pages, const uint8_t* taken,
                            int cu, PagedItem* items, int64_t* n_items, PagedComb* combs, int64_t* n_combs,

@@ -155,6 +155,11 @@ __device__ __forceinline__ int image_unit(int u) { return u ^ (((u >> 4) ^ (u >>
 __device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4) * 16 + (byte & 15); }
 
 // ---------------------------------------------------------------- write
+// q = round(127 x / a) + 128 with scale a / 127, or half(x 2^-e) with scale 2^e,
+// a the row's largest magnitude.  Bound by HBM: 4 bytes read for one or two
+// written.  2000 tokens of 8 heads of 128, 8-bit: 8.0 us (2.6 TB/s; the bytes
+// alone are 4.2 at a copy's rate, a launch that does nothing 2); a kernel
+// without the image in LDS, its values written a row apart, took 24.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
@@ -254,6 +259,9 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
 }
 
 // ---------------------------------------------------------------- read back
+// x = (byte - 128) scale, or half scale.  Bound by HBM, mostly its writes: four
+// contexts of up to 16384 (57138 tokens in all, 8 heads of 128, 8-bit) 120 us,
+// 4.9 TB/s, a large copy's rate.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, float* __restrict__ k, int64_t ldk,
                                                     float* __restrict__ v, int64_t ldv) {
@@ -718,9 +726,14 @@ struct RowSight {
     }
 };
 
-// Workgroup = (item, kv head), neighbours on one XCD's L2 sharing a head where
-// there are 8; the item's pages dealt to its four waves, whose softmaxes meet
-// in LDS.
+// Few rows: workgroup = (item, kv head), neighbours on one XCD's L2 sharing a
+// head where there are 8; the item's pages dealt to its four waves, whose
+// softmaxes meet in LDS.  For one token a sequence bound by HBM, the pages
+// straight to registers: 16 sequences of 820 to 8192 slots (8-bit, 8 kv heads
+// of 128) 35 us, where a kernel of the loads alone takes 31.4 (5.3 TB/s); one
+// of 131072 (halves) 104 us, the loads alone 104.  (Joining the partials in the
+// last workgroup of a list instead of a launch of their own: the same for
+// short lists, 14 us slower for one of 131072; by fences 60 us slower.)
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
     using W = WaveAttn<HD, Q8>;
@@ -880,6 +893,14 @@ typedef __attribute__((address_space(3))) void lds_void;
 // converted once, by all waves), one page ahead in the other buffer: halves by
 // direct copies, 8-bit values through registers, their loads issued before the
 // current page's work and written after it.
+// Bound by the SIMDs' issue: queries and weights in two halves make it two
+// products of 16x16x32 for each of the formula's, 16 cycles each; three chunks
+// of 1500 tokens after 1600 to 4000 (8-bit, 128 dims) take 551 us, the CUs
+// busy for 88% of it, in that time products for 47% and other vector
+// instructions for 43% of the SIMDs' cycles.  One tile a wave reads twice the
+// LDS for a product: 656 us, LDS as busy as the products.  Tried and slower:
+// both tiles' low halves in registers (73 spilled, 680), the waves' halves kept
+// in antiphase, scores beside softmax (690), 64 rows a workgroup (686).
 template <int HD>
 constexpr int many_buf_bytes() {
     return 2 * FTX_PAGE * HD * 2 + 3 * FTX_PAGE * 4 + 16;  // values, scales of K, V, V by level, its level

@@ -414,7 +414,8 @@ int ftx_plan_free(ftx_plan* pl);
  * row n of a matrix is ld floats (0: dense) after row n - 1.  They may be
  * recorded into a HIP graph; ftx_plan_set is then refused for that plan, and
  * the plan, its pool and the matrices must outlive the graph.  Calls of one
- * plan share its workspace: they must not overlap. */
+ * plan share its workspace: they must not overlap.  After ftx_set_stream a
+ * call waits for the plan's tables, ftx_plan_set for the device. */
 
 /* Store the new tokens' k and v rows ([sum of M][n_head_kv * head_dim],
  * sequence after sequence) of a layer in their pages. */

@@ -604,6 +604,81 @@ def test_two_graphs_replayed(gctx, kvt):
         c.free()
 
 
+def test_calls_on_another_stream_than_the_tables(gctx):
+    """A plan set on one stream, behind work there, and called at once on
+    another; then set again while the calls there may still run."""
+    hip = _hip()
+    rng = np.random.default_rng(31)
+    busy = Cache(gctx, rng, Q8, 128, 2, 8, [(3000, 500)])
+    busy.write_new()
+    bq = Rows(gctx, queries(rng, busy))
+    bo = Rows(gctx, np.zeros((busy.new, busy.heads * busy.hd), np.float32))
+    c = Cache(gctx, rng, F16, 128, 2, 8, [(900, 3)])
+    c.write_new()
+    q = queries(rng, c)
+    want = c.check(q)
+    qd, out = Rows(gctx, q), Rows(gctx, np.zeros_like(q))
+    st = ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(st)) == 0
+    try:
+        for k in range(3):
+            out.buf.write(out.host)
+            c.plan.set([([], 0, 0)], 8)
+            for _ in range(20):
+                busy.plan.attend(0, bq.ptr, bo.ptr)
+            c.plan.set(c.seqs, 8)
+            gctx.set_stream(st.value)
+            c.plan.attend(0, qd.ptr, out.ptr)
+            gctx.set_stream(None)
+            c.plan.set([([], 0, 0)], 8)
+            gctx.sync()
+            assert hip.hipStreamSynchronize(st) == 0
+            np.testing.assert_array_equal(out.get().reshape(want.shape), want)
+    finally:
+        gctx.set_stream(None)
+        hip.hipStreamSynchronize(st)
+        hip.hipStreamDestroy(st)
+    for x in (bq, bo, qd, out):
+        x.buf.free()
+    c.free()
+    busy.free()
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2], ids=["global", "thread", "relaxed"])
+def test_capture_modes(gctx, mode):
+    """A plan whose tables went up on another stream, captured in every mode."""
+    hip = _hip()
+    rng = np.random.default_rng(32)
+    c = Cache(gctx, rng, Q8, 64, 2, 8, [(500, 2)])
+    c.write_new()
+    q = queries(rng, c)
+    want = c.check(q)
+    qd, out = Rows(gctx, q), Rows(gctx, np.zeros_like(q))
+    st, graph, exe = (ctypes.c_void_p() for _ in range(3))
+    assert hip.hipStreamCreate(ctypes.byref(st)) == 0
+    gctx.set_stream(st.value)
+    try:
+        assert hip.hipStreamBeginCapture(st, mode) == 0
+        c.plan.attend(0, qd.ptr, out.ptr)
+        assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, 0) == 0
+        for _ in range(3):
+            out.buf.write(out.host)
+            assert hip.hipGraphLaunch(exe, st) == 0
+            assert hip.hipStreamSynchronize(st) == 0
+            np.testing.assert_array_equal(out.get().reshape(want.shape), want)
+    finally:
+        gctx.set_stream(None)
+        hip.hipStreamSynchronize(st)
+        if exe:
+            hip.hipGraphExecDestroy(exe)
+        if graph:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+    qd.buf.free(), out.buf.free()
+    c.free()
+
+
 def test_set_while_captured_is_refused(gctx):
     hip = _hip()
     c = Cache(gctx, np.random.default_rng(23), F16, 64, 1, 1, [(3, 1)])

@@ -206,6 +206,31 @@ def test_a_refused_step_takes_nothing(gctx, orc):
     pool2.free()
 
 
+def test_a_refused_batch_or_write_takes_nothing(gctx, orc):
+    su = Setup(gctx, orc, CFG64, Q4K, pages=6)
+    a, k, v = su.context(60, 128)
+    b, _, _ = su.context(64, 128, seed=41)
+    hog = su.gm.kv_paged(su.pool, 256)
+    su.kvs.append(hog)
+    kb = np.zeros((2,) + hog.shape, np.float16)
+    spare = su.pool.take(su.pool.available - 1)
+    # a grows by the last page, b finds none: neither has it
+    refused(-4, su.step, [(a, [1] * 8, None, False), (b, [2] * 8, None, False)])
+    assert su.pool.available == 1
+    # writing all of cap takes 4 pages: refused, and a's rows stay as they were
+    refused(-4, hog.write, *kb)
+    big, before = su.gm.kv_paged(su.pool, 300), a.read()
+    su.kvs.append(big)
+    refused(-4, big.write, *np.zeros((2,) + big.shape, np.float16))
+    for x, y in zip(a.read(), before):
+        np.testing.assert_array_equal(x, y)
+    assert su.pool.available == 1
+    su.pool.give(spare)
+    got = su.step([(a, [1] * 8, None, False), (b, [2] * 8, None, False)])
+    assert all(np.isfinite(x).all() for x in got)
+    su.free()
+
+
 @pytest.mark.parametrize("M", [1, 30])
 def test_window_steps(gctx, orc, M):
     """What lies outside the window and past the first tokens has no effect,

@@ -369,6 +369,10 @@ struct ftx_plan {
     size_t pin_bytes[RING] = {};
     hipEvent_t ev[RING] = {};
     int next = 0;
+    hipEvent_t up = nullptr;  // the last copy's
+    // of the last set or call outside of captures: another stream waits for the
+    // copy, a set on another for everything
+    hipStream_t stream = nullptr;
     // the parts of the device block
     size_t o_seq = 0, o_tab = 0, o_dep = 0, o_anc = 0, o_item = 0, o_comb = 0;
 };
@@ -424,6 +428,7 @@ static int plan_upload(ftx_plan* pl) {
     int rc = grow((void**)&pl->dev, pl->dev_bytes, bytes, 1);
     if (!rc) rc = grow((void**)&pl->part, pl->part_floats, pf, sizeof(float));
     if (rc) return rc;
+    if (pl->up && pl->stream != st) FTX_HIP(ctx, hipDeviceSynchronize());
     const int k = pl->next;
     if (pl->ev[k]) FTX_HIP(ctx, hipEventSynchronize(pl->ev[k]));
     if (!pl->ev[k]) FTX_HIP(ctx, hipEventCreateWithFlags(&pl->ev[k], hipEventDisableTiming));
@@ -450,6 +455,8 @@ static int plan_upload(ftx_plan* pl) {
     put(pl->o_comb, t.combs.data(), t.combs.size() * sizeof(PagedComb));
     FTX_HIP(ctx, hipMemcpyAsync(pl->dev, h, bytes, hipMemcpyHostToDevice, st));
     FTX_HIP(ctx, hipEventRecord(pl->ev[k], st));
+    pl->up = pl->ev[k];
+    pl->stream = st;
     pl->next = (k + 1) % ftx_plan::RING;
     pl->ready = true;
     return FTX_OK;
@@ -469,6 +476,24 @@ static PagedView plan_view(const ftx_plan* pl, int64_t layer) {
     return v;
 }
 
+// the tables' copy ahead of a call on another stream than its own
+static int plan_order(ftx_plan* pl, bool captures) {
+    ftx_ctx* ctx = pl->ctx;
+    if (ctx->stream == pl->stream) return FTX_OK;
+    if (!captures) {
+        FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
+        pl->stream = ctx->stream;
+        return FTX_OK;
+    }
+    // (an event from outside does not go into a graph: the host waits)
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    FTX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
+    const hipError_t e = hipEventSynchronize(pl->up);
+    FTX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
+    FTX_HIP(ctx, e);
+    return FTX_OK;
+}
+
 // what every call of a plan checks; *ld: 0 becomes `width`
 static int plan_call(ftx_plan* pl, int64_t layer, const void* x, int64_t* ldx, int64_t xw, const void* y,
                      int64_t* ldy, int64_t yw) {
@@ -482,8 +507,9 @@ static int plan_call(ftx_plan* pl, int64_t layer, const void* x, int64_t* ldx, i
     if (((uintptr_t)x | (uintptr_t)y) & 3) return ftx_fail(ctx, FTX_E_INVALID, "rows must be 4-byte aligned");
     if (!on_device(ctx, x) || !on_device(ctx, y))
         return ftx_fail(ctx, FTX_E_INVALID, "rows must be memory of the context's device");
-    if (capturing(ctx->stream)) pl->captured = true;
-    return FTX_OK;
+    const bool captures = capturing(ctx->stream);
+    if (captures) pl->captured = true;
+    return plan_order(pl, captures);
 }
 
 // whether n rows of w floats, ldx and ldy apart, at x and y share a float

@@ -182,9 +182,18 @@ static int step_pages(ftx_ctx* ctx, int64_t n_head, const ftx_seq_args* sq, int6
         kv_drop(sq[s].kv, un.first, un.second);
     }
     ftx_paged_seq ps[FTX_MAX_SEQ];
+    size_t had[FTX_MAX_SEQ];
     for (int64_t s = 0; s < nseq; ++s) {
         ftx_kv* kv = sq[s].kv;
-        if (const int rc = kv_grow(kv, kv->npast + sq[s].M)) return rc;
+        had[s] = kv->pages.size();
+        if (const int rc = kv_grow(kv, kv->npast + sq[s].M)) {
+            // (the others' too)
+            for (int64_t r = 0; r < s; ++r) {
+                kv_drop(sq[r].kv, (int64_t)had[r], (int64_t)sq[r].kv->pages.size());
+                sq[r].kv->pages.resize(had[r]);
+            }
+            return rc;
+        }
         ps[s] = ftx_paged_seq{kv->pages.data(), (int64_t)kv->pages.size(), kv->npast, sq[s].M, sq[s].parents};
     }
     return paged_step_plan(ctx, k0->pool, ftx_plan_args{ps, nseq, n_head, k0->window, k0->sinks}, plan);
@@ -1218,7 +1227,12 @@ static int kv_copy(ftx_kv* kv, void* kh, void* vh, bool to_device) {
 static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
     ftx_ctx* ctx = kv->ctx;
     if (to_device) {
-        // (a dropped page is held again)
+        // (a dropped page is held again; too few pages: the cache stays as it is)
+        const int64_t need = (kv->cap + FTX_PAGE - 1) / FTX_PAGE;
+        int64_t held = 0;
+        for (int32_t pg : kv->pages) held += pg >= 0;
+        if (need > held + kv->pool->free_pages)
+            return ftx_fail(ctx, FTX_E_NOMEM, "kv_write: not enough free pages");
         kv_drop(kv, 0, (int64_t)kv->pages.size());
         kv->pages.clear();
         if (const int rc = kv_grow(kv, kv->cap)) return rc;

@@ -256,7 +256,9 @@ def test_rows_of_every_size(gctx, kvt):
 @pytest.mark.parametrize("hd,kv,heads,seqs", [
     (64, 8, 8, [(128, 1)]), (128, 8, 32, [(0, 1)]), (128, 2, 16, [(63, 1), (64, 1), (65, 1), (700, 1), (0, 1)]),
     (128, 1, 1, [(1900, 1)]), (256, 1, 3, [(100, 5), (0, 0), (3, 70)]), (64, 2, 14, [(33, 17), (1, 1), (0, 130)]),
-    (128, 2, 8, [(200, 8), (59, 8)]), (128, 1, 24, [(300, 30)]), (64, 1, 64, [(5, 3)]), (128, 2, 8, [(70, 333)])])
+    (128, 2, 8, [(200, 8), (59, 8)]), (128, 1, 24, [(300, 30)]), (64, 1, 64, [(5, 3)]), (128, 2, 8, [(70, 333)]),
+    (128, 1, 8, [(4000, 1), (20, 3)]), (64, 1, 2, [(2500, 40)]), (128, 8, 32, [(640, 1), (1, 1), (0, 2)]),
+    (64, 8, 8, [(900, 9)] * 3)])
 def test_chains(gctx, kvt, hd, kv, heads, seqs):
     rng = np.random.default_rng(heads + hd)
     c = Cache(gctx, rng, kvt, hd, kv, heads, seqs)

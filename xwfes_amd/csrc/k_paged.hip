@@ -727,24 +727,25 @@ struct RowSight {
 };
 
 // Few rows: workgroup = (item, kv head), neighbours on one XCD's L2 sharing a
-// head where there are 8; the item's pages dealt to its four waves, whose
-// softmaxes meet in LDS.  For one token a sequence bound by HBM, the pages
+// head where there are 8; the item's pages dealt to its NW waves, whose
+// softmaxes meet in LDS (of eight, the last four with the first four before).
+// Four waves take a part of a list, eight a whole one where that is faster.  For one token a sequence bound by HBM, the pages
 // straight to registers: 16 sequences of 820 to 8192 slots (8-bit, 8 kv heads
 // of 128) 35 us, where a kernel of the loads alone takes 31.4 (5.3 TB/s); one
 // of 131072 (halves) 104 us, the loads alone 104.  (Joining the partials in the
 // last workgroup of a list instead of a launch of their own: the same for
 // short lists, 14 us slower for one of 131072; by fences 60 us slower.)
-template <int HD, bool Q8>
-__global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
+template <int HD, bool Q8, int NW>
+__global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
     using W = WaveAttn<HD, Q8>;
     constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
-    // the query's halves, of which the four waves have the same: in LDS where
+    // the query's halves, of which the waves have the same: in LDS where
     // they would leave too few registers for the values in flight (halves of
     // 128 dims: 37 spilled, 129 us for one token over 131072; so 104)
     constexpr bool QLDS = !Q8 && HD >= 128;
     __shared__ v8h qs[QLDS ? 2 : 1][W::NDC][64];
-    __shared__ float so[3][4 * W::NDT][64], sm[4][64], sl[4][64];
-    __shared__ int se[4][64];
+    __shared__ float so[NW == 4 ? 3 : 4][4 * W::NDT][64], sm[NW][64], sl[NW][64];
+    __shared__ int se[NW][64];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
     const PagedSeq sq = it.q;
@@ -775,13 +776,13 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     }
     hi = __builtin_amdgcn_readfirstlane(hi);
     lo = __builtin_amdgcn_readfirstlane(lo);
-    // the wave's pages: entries i0 + w, + 4, ..; their ids 64 at a time in the
+    // the wave's pages: entries i0 + w, + NW, ..; their ids 64 at a time in the
     // lanes.  A page's V loads are issued before its scores are formed, the
     // next page's K loads and scales (PRE) before its softmax, so that each
     // wait leaves the later loads in flight.
-    const int n = max(0, (it.i1 - it.i0 - w + 3) >> 2);
+    const int n = max(0, (it.i1 - it.i0 - w + NW - 1) / NW);
     auto place = [&](int j) {  // in the table
-        const int i = it.i0 + w + 4 * j;
+        const int i = it.i0 + w + NW * j;
         return i < it.s ? i : it.a + (i - it.s);
     };
     int ids = lane < n ? a.p.table[sq.tab0 + place(lane)] : 0;
@@ -836,10 +837,38 @@ __global__ void __launch_bounds__(256, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn
     }
     wa.l += __shfl_xor(wa.l, 16, 64);
     wa.l += __shfl_xor(wa.l, 32, 64);
+    if constexpr (NW == 8) {
+        // waves 4 to 7 into 0 to 3
+        if (w >= 4) {
+            sm[w][lane] = wa.off;
+            sl[w][lane] = wa.l;
+            se[w][lane] = wa.ev;
+#pragma unroll
+            for (int dt = 0; dt < W::NDT; ++dt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) so[w - 4][4 * dt + x][lane] = wa.o[dt][x];
+        }
+        __syncthreads();
+        if (w < 4) {
+            const float mo = sm[w + 4][lane], M = fmaxf(wa.off, mo);
+            const int eo = se[w + 4][lane], EV = max(wa.ev, eo);
+            const float f0 = wa.off == M ? 1.f : __builtin_amdgcn_exp2f(wa.off - M);
+            const float f1 = mo == M ? 1.f : __builtin_amdgcn_exp2f(mo - M);
+            const float g0 = ldexpf(f0, wa.ev - EV), g1 = ldexpf(f1, eo - EV);
+            wa.l = wa.l * f0 + sl[w + 4][lane] * f1;
+            wa.off = M;
+            wa.ev = EV;
+#pragma unroll
+            for (int dt = 0; dt < W::NDT; ++dt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) wa.o[dt][x] = wa.o[dt][x] * g0 + so[w][4 * dt + x][lane] * g1;
+        }
+        __syncthreads();
+    }
     sm[w][lane] = wa.off;
     sl[w][lane] = wa.l;
     se[w][lane] = wa.ev;
-    if (w)
+    if (w && w < 4)
 #pragma unroll
         for (int dt = 0; dt < W::NDT; ++dt)
 #pragma unroll
@@ -1208,13 +1237,26 @@ static hipError_t launch_many(hipStream_t st, const PagedAttn& a) {
     return hipGetLastError();
 }
 
+template <int HD, bool Q8>
+static auto attn_four() {
+    return k_paged_attn<HD, Q8, 4>;
+}
+template <int HD, bool Q8>
+static auto attn_wide() {
+    return k_paged_attn<HD, Q8, HD <= 128 ? 8 : 4>;
+}
+
 hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     hipError_t e = hipSuccess;
     if (a.n_many) e = PAGED_CASE(launch_many, a.p.hd, a.p.q8)(st, a);
     if (e != hipSuccess) return e;
-    if (a.n_few)
-        ktimed_launch(PAGED_CASE(k_paged_attn, a.p.hd, a.p.q8), dim3((unsigned)a.n_few * (unsigned)a.p.n_kv), dim3(256),
-                      0, st, a);
+    if (a.n_few) {
+        const dim3 grid((unsigned)a.n_few * (unsigned)a.p.n_kv);
+        if (a.wide)
+            ktimed_launch(PAGED_CASE(attn_wide, a.p.hd, a.p.q8)(), grid, dim3(512), 0, st, a);
+        else
+            ktimed_launch(PAGED_CASE(attn_four, a.p.hd, a.p.q8)(), grid, dim3(256), 0, st, a);
+    }
     e = hipGetLastError();
     if (e != hipSuccess || a.n_combs == 0) return e;
     const int rows = std::min(PAGED_TR, a.rows_max);

@@ -77,6 +77,7 @@ struct PagedTables {
     int64_t parts = 0;   // in blocks of PAGED_TR rows
     int64_t comb_max = 0;  // most partials of a row
     int64_t few = 0;     // items of PAGED_TR rows, before the others
+    bool wide = false;   // by workgroups of eight waves
     bool absent = false;  // a page below npast + M is absent
     double seen = 0, pages_read = 0;  // visible (row, slot) pairs bound, pages of all items
     std::vector<PagedSeq> seqs;
@@ -120,6 +121,7 @@ struct PagedAttn {
     const PagedItem* items;
     const PagedComb* combs;
     int n_few, n_many, n_combs;
+    bool wide;  // few: eight waves a workgroup
     int rows_max, comb_max;  // query rows of the longest sequence, most partials of a row
     int gqa;
     int window, sinks;

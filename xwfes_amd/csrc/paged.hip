@@ -17,6 +17,8 @@
 constexpr int64_t PAGED_MANY = 65;
 // Row tiles beyond which such sequences do so without a look at tiles of 16
 constexpr int64_t FEW_MOST = 4096;
+// Pages of a list beyond which few rows are not given to eight waves unsplit
+constexpr int64_t WIDE_MOST = 48;
 
 namespace {
 
@@ -47,7 +49,7 @@ struct LaunchCost {
             n += np;
             if (np > 1) rows += np * t.rows;
         }
-        if (n == 0) return 0;
+        if (n == 0) return 0;  // (no launch)
         const double mean = total / (double)n, whole = total * (double)n_kv / (double)slots;
         double e = longest;
         if (n * n_kv > slots) {
@@ -180,11 +182,29 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     const int64_t cu = std::max(g.cu, 1);
     // Few rows: lists are split so that a launch has some four workgroups a CU (1
     // to 4 are within 5%, 8 are 8% slower for one token over 131072), no finer
-    // than four pages, one a wave.
-    auto few_per = [&](const std::vector<Tile>& tiles) {
-        int64_t total = 0;
-        for (const Tile& t : tiles) total += t.n;
-        return std::max<int64_t>(4, (total * g.n_kv + 4 * cu - 1) / (4 * cu));
+    // than four pages, one a wave; or, where the launch has at most a workgroup a
+    // CU, stay whole for workgroups of eight waves and need no join.  Whole / split,
+    // us, for sequences x pages (one token, 8-bit 128 dims, 8 kv heads): 1 x 7 8.8 /
+    // 9.9, 1 x 17 11.6 / 10.0, 8 x 12 10.1 / 10.5, 8 x 22 14.7 / 12.4, 16 x 46
+    // 23.8 / 27.5, 32 x 17 16.7 / 22.7; 64 dims: 1 x 12 7.2 / 8.8, 8 x 17 8.9 /
+    // 8.8, 16 x 46 17.2 / 17.9.
+    struct Few {
+        bool wide;
+        int64_t per;
+        double us;
+    };
+    auto few_plan = [&](const std::vector<Tile>& tiles) {
+        int64_t total = 0, longest = 0;
+        for (const Tile& t : tiles) {
+            total += t.n;
+            longest = std::max<int64_t>(longest, t.n);
+        }
+        const double load = (double)(total * g.n_kv) / (double)cu;  // pages a CU
+        if (g.hd <= 128 && longest > 4 && longest <= WIDE_MOST && (int64_t)tiles.size() * g.n_kv <= cu &&
+            (double)longest <= (g.hd == 64 ? 15 : 10) + 1.6 * load)
+            return Few{true, INT32_MAX, 6 + std::max((0.17 + 0.17 * (double)g.hd / 128) * (double)longest, 0.6 * load)};
+        const int64_t per = std::max<int64_t>(4, (total * g.n_kv + 4 * cu - 1) / (4 * cu));
+        return Few{false, per, LaunchCost{g.n_kv, g.hd, 2 * cu, 8, 0.8 * (double)g.hd / 128}(tiles, per)};
     };
     std::vector<Tile> tiles[2], big;  // of PAGED_TR rows, of many
     int64_t per[2] = {INT32_MAX, INT32_MAX}, big_rows = 0;
@@ -228,17 +248,16 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         if (present && (force ? force == PAGED_TR : big_rows / PAGED_TR <= FEW_MOST)) {
             big = tiles[0];
             present = tile_all(big, true, PAGED_TR);
-            const LaunchCost cost{g.n_kv, g.hd, 2 * cu, 8, 0.8 * (double)g.hd / 128};
-            const int64_t p = few_per(big);
-            const double others = tiles[0].empty() ? 0 : cost(tiles[0], few_per(tiles[0]));
-            if (present && (force || cost(big, p) - others < best)) {
+            if (present && (force || few_plan(big).us - few_plan(tiles[0]).us < best)) {
                 tiles[0] = big;
                 tiles[1].clear();
             }
         }
     }
     if (!present) return fail(FTX_E_INVALID, "a page that a new token sees is absent");
-    per[0] = few_per(tiles[0]);
+    const Few few = few_plan(tiles[0]);
+    per[0] = few.per;
+    o.wide = few.wide;
     o.pages_read = 0;
     for (int many = 0; many < 2; ++many) {
         for (const Tile& t : tiles[many]) {
@@ -698,7 +717,7 @@ static double rows_bytes(const ftx_pool* p, double n) {
 int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv) {
     ftx_ctx* ctx = pl->ctx;
     OnDevice od(ctx->device);
-    NoTrace nt(ctx, capturing(ctx->stream));
+    NoTrace nt(ctx, ctx->trace && capturing(ctx->stream));
     TraceScope ts(ctx);
     FTX_HIP(ctx, launch_paged_write(ctx->stream, plan_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
     ts.end(TK_PAGED_KV, rows_bytes(pl->pool, (double)pl->t.tokens));
@@ -708,7 +727,7 @@ int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, c
 int paged_read_rows(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv) {
     ftx_ctx* ctx = pl->ctx;
     OnDevice od(ctx->device);
-    NoTrace nt(ctx, capturing(ctx->stream));
+    NoTrace nt(ctx, ctx->trace && capturing(ctx->stream));
     TraceScope ts(ctx);
     FTX_HIP(ctx, launch_paged_read(ctx->stream, plan_view(pl, layer),
                                    context ? pl->t.max_pages : pl->t.max_new_pages, context, k, ldk, v, ldv));
@@ -730,6 +749,7 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.n_few = (int)t.few;
     a.n_many = (int)((int64_t)t.items.size() - t.few);
     a.n_combs = (int)t.combs.size();
+    a.wide = t.wide;
     a.gqa = (int)(t.n_head / p->n_kv);
     a.rows_max = (int)(t.longest * a.gqa);
     a.comb_max = (int)std::min<int64_t>(t.comb_max, INT32_MAX);
@@ -741,7 +761,7 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.ldo = ldo;
     a.part = pl->part;
     a.pml = pl->part + (size_t)t.parts * p->n_kv * PAGED_TR * p->hd;
-    NoTrace nt(ctx, capturing(ctx->stream));
+    NoTrace nt(ctx, ctx->trace && capturing(ctx->stream));
     TraceScope ts(ctx);
     FTX_HIP(ctx, launch_paged_attention(ctx->stream, a));
     ts.end(TK_ATTENTION, t.pages_read * p->n_kv * (double)p->block + 8.0 * t.tokens * t.n_head * p->hd);

@@ -126,6 +126,32 @@ def test_8_bit_rows_near_halves(gctx, orc):
 
 
 @pytest.mark.parametrize("kvt", [ftx.KV_F16, ftx.KV_Q8], ids=["f16", "q8"])
+@pytest.mark.parametrize("cfg,neox,M", [
+    (CFG64, False, 1), (CFG64, True, 15), (CFG128, False, 8), (CFG128, True, 3), (CFG128, False, 16),
+    (P.model_cfg(2, 1024, 4, 2, 256, 512, 300), False, 5), (P.model_cfg(2, 1024, 4, 2, 256, 512, 300), True, 12)])
+def test_rows_of_a_step_are_stored_as_the_store_does(gctx, orc, kvt, cfg, neox, M):
+    """The first layer's rows of a step, over the end of a page, against the fp32
+    rows of the same step over a contiguous fp32 cache: bit for bit."""
+    t = Setup(gctx, orc, dict(cfg, rope_neox=neox), Q8, kvt=kvt)
+    npast, cap, V = 60, 90, cfg["vocab"]
+    kv, k, v = t.context(npast, cap)
+    full = t.gm.kv(cap, ftx.KV_F32)
+    full.write(*(np.float32(x) for x in (k, v)))
+    full.truncate(npast)
+    buf = gctx.buffer(M * V * 4)
+    for c in (kv, full):
+        t.gm.verify(c, list(range(M)), buf.ptr)
+    gctx.sync()
+    hd = cfg["head_dim"]
+    for got, want in zip(kv.read(), full.read()):
+        rows = want[0, npast:npast + M].reshape(M, -1, hd)
+        np.testing.assert_array_equal(got[0, npast:npast + M].reshape(M, -1, hd), stored(rows, kvt))
+    buf.free()
+    full.free()
+    t.free()
+
+
+@pytest.mark.parametrize("kvt", [ftx.KV_F16, ftx.KV_Q8], ids=["f16", "q8"])
 def test_commit_of_a_tree_path(gctx, orc, kvt):
     """A path's rows move to the next slots, across a page's end; the step
     after it is the step after the chain of the path."""

@@ -539,7 +539,10 @@ struct RopeBatch {
     int row0[FTX_MAX_SEQ + 1];  // first token row of each sequence
     int nseq;
 };
-hipError_t launch_rope_kv_batch(hipStream_t st, const RopeArgs* as, const int64_t* M, int nseq);
+// pages: the k and v rows go there (sequence s of the view), not to kc and vc
+struct PagedView;
+hipError_t launch_rope_kv_batch(hipStream_t st, const RopeArgs* as, const int64_t* M, int nseq,
+                                const PagedView* pages = nullptr);
 struct AttnArgs {
     const float* qkv;   // q rows, ldq stride
     int64_t ldq;

@@ -146,6 +146,10 @@ hipError_t launch_paged_move(hipStream_t st, const PagedMove& m);
 // ---------------------------------------------------------------- the verify step's use
 // The plan of the pool's running step (one a pool, its calls in stream order)
 int paged_step_plan(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args& a, ftx_plan** out);
+// the layer as the plan's kernels see it, for steps whose RoPE stores the rows
+// (up to PAGED_ROWS_FEW new tokens a sequence, where rows are stored one by one)
+constexpr int PAGED_ROWS_FEW = 15;
+PagedView paged_view(const ftx_plan* pl, int64_t layer);
 int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, const float* v, int64_t ldv);
 int paged_read_rows(ftx_plan* pl, int64_t layer, int context, float* k, int64_t ldk, float* v, int64_t ldv);
 int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo);

@@ -481,7 +481,7 @@ static int plan_upload(ftx_plan* pl) {
     return FTX_OK;
 }
 
-static PagedView plan_view(const ftx_plan* pl, int64_t layer) {
+PagedView paged_view(const ftx_plan* pl, int64_t layer) {
     const ftx_pool* p = pl->pool;
     PagedView v{};
     v.block = p->block;
@@ -719,7 +719,7 @@ int paged_write_rows(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, c
     OnDevice od(ctx->device);
     NoTrace nt(ctx, ctx->trace && capturing(ctx->stream));
     TraceScope ts(ctx);
-    FTX_HIP(ctx, launch_paged_write(ctx->stream, plan_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
+    FTX_HIP(ctx, launch_paged_write(ctx->stream, paged_view(pl, layer), pl->t.max_new_pages, k, ldk, v, ldv));
     ts.end(TK_PAGED_KV, rows_bytes(pl->pool, (double)pl->t.tokens));
     return FTX_OK;
 }
@@ -729,7 +729,7 @@ int paged_read_rows(ftx_plan* pl, int64_t layer, int context, float* k, int64_t 
     OnDevice od(ctx->device);
     NoTrace nt(ctx, ctx->trace && capturing(ctx->stream));
     TraceScope ts(ctx);
-    FTX_HIP(ctx, launch_paged_read(ctx->stream, plan_view(pl, layer),
+    FTX_HIP(ctx, launch_paged_read(ctx->stream, paged_view(pl, layer),
                                    context ? pl->t.max_pages : pl->t.max_new_pages, context, k, ldk, v, ldv));
     ts.end(TK_PAGED_KV, rows_bytes(pl->pool, (double)(context ? pl->t.rows : pl->t.tokens)));
     return FTX_OK;
@@ -741,7 +741,7 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     const ftx_pool* p = pl->pool;
     OnDevice od(ctx->device);
     PagedAttn a{};
-    a.p = plan_view(pl, layer);
+    a.p = paged_view(pl, layer);
     a.depth = (const int32_t*)(pl->dev + pl->o_dep);
     a.anc = (const uint32_t*)(pl->dev + pl->o_anc);
     a.items = (const PagedItem*)(pl->dev + pl->o_item);

@@ -554,9 +554,13 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
                 ra.cs = d_cs + r0 * hd2 * 2;
                 ras[s] = ra;
             }
-            TRACED_L(TK_ROPE_KV, 2.0 * Md * m->ldq * f4, launch_rope_kv_batch(st, ras, Ms, (int)nseq));
+            bool few = true;
+            for (int64_t s = 0; s < nseq; ++s) few = few && Ms[s] <= PAGED_ROWS_FEW;
+            const PagedView pv = paged_view(plan, l);
+            TRACED_L(TK_ROPE_KV, 2.0 * Md * m->ldq * f4,
+                     launch_rope_kv_batch(st, ras, Ms, (int)nseq, few ? &pv : nullptr));
             const float* kr = m->qkv + m->qdim;
-            rc = paged_write_rows(plan, l, kr, m->ldq, kr + m->kdim, m->ldq);
+            rc = few ? FTX_OK : paged_write_rows(plan, l, kr, m->ldq, kr + m->kdim, m->ldq);
             if (!rc) rc = paged_attend_rows(plan, l, m->qkv, m->ldq, m->att, m->qdim);
             if (rc) return rc;
         }
@@ -1606,9 +1610,14 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
             ra.qh16 = qe.qh;
             ra.ql16 = qe.ql;
         }
-        if (!fuse)
+        if (plan) {
+            const PagedView pv = paged_view(plan, l);
+            TRACED(TK_ROPE_KV, 2 * Md * m->ldq * f4 + 2 * Md * m->kdim * (double)kvel,
+                   launch_rope_kv_batch(st, &ra, &M, 1, &pv));
+        } else if (!fuse) {
             TRACED(TK_ROPE_KV, 2 * Md * m->ldq * f4 + 2 * Md * m->kdim * (double)kvel,
                    launch_rope_kv(st, ra, M));
+        }
         const double attn_b =
             2.0 * (double)(npast + M) * m->kdim * (double)kvel + 2 * Md * m->qdim * f4;
         // the chunk combine writes the output projection's activation operand
@@ -1640,9 +1649,7 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
             TRACED_IDEM(TK_ATTENTION, attn_b,
                         launch_attn_mfma(st, am, kv->attn_part, o_xq ? m->xq : nullptr, o_rd));
         } else if (plan) {
-            const float* kr = m->qkv + m->qdim;
-            rc = paged_write_rows(plan, l, kr, m->ldq, kr + m->kdim, m->ldq);
-            if (!rc) rc = paged_attend_rows(plan, l, m->qkv, m->ldq, m->att, m->qdim);
+            rc = paged_attend_rows(plan, l, m->qkv, m->ldq, m->att, m->qdim);
             if (rc) return rc;
         } else {
             AttnArgs aa{m->qkv,  m->ldq, kl,       vl,          kv->kv_f16, m->npast,

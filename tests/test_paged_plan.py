@@ -11,10 +11,10 @@ I32 = np.int32
 
 
 def probe(seqs, n_kv=2, n_head=4, window=0, sinks=0, n_pages=64, taken=None, cu=256, hd=64, most=100000):
-    """(code, message, items [n][8] (without their sequences), joins [n][5]) of a step's tables."""
+    """(code, message, items [n][8] (without their sequences), joins [n][8]) of a step's tables."""
     a, keep = ftx.plan_args(seqs, n_head, window, sinks)
     tk = np.ones(n_pages, np.uint8) if taken is None else np.asarray(taken, np.uint8)
-    items, combs = np.zeros((most, 24), I32), np.zeros((most, 5), I32)
+    items, combs = np.zeros((most, 24), I32), np.zeros((most, 8), I32)
     ni, nc, msg = C.c_int64(0), C.c_int64(0), C.create_string_buffer(256)
     f = ftx.load().paged_probe
     f.restype = C.c_int

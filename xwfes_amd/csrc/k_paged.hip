@@ -1037,9 +1037,8 @@ __global__ void __launch_bounds__(256) k_paged_combine_few(PagedAttn a) {
     const int kvh = blockIdx.x % a.p.n_kv, d = threadIdx.x % D4;
     const int col = blockIdx.y * G + threadIdx.x / D4;
     const PagedComb c = a.combs[blockIdx.x / a.p.n_kv];
-    const PagedSeq sq = a.p.seqs[c.seq];
     const int rr = c.row0 + col;
-    if (col >= PAGED_TR || rr >= sq.M * a.gqa) return;
+    if (col >= PAGED_TR || rr >= c.M * a.gqa) return;
     const int64_t step = (int64_t)c.step * a.p.n_kv * PAGED_TR;
     const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
     const float2* ml = (const float2*)a.pml + p0;
@@ -1063,7 +1062,7 @@ __global__ void __launch_bounds__(256) k_paged_combine_few(PagedAttn a) {
 #pragma unroll
     for (int i = 0; i < COMB_FEW; ++i)
         if (i < c.n) num += o[i] * (t[i].y / den);
-    const int64_t tok = sq.tok0 + rr / a.gqa;
+    const int64_t tok = c.tok0 + rr / a.gqa;
     const bool vec = !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
     st4(a.out + tok * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD + 4 * d, num, vec);
 }
@@ -1073,16 +1072,21 @@ __global__ void __launch_bounds__(256) k_paged_combine_few(PagedAttn a) {
 // 4 d .. 4 d + 3, the G sums meet in LDS.
 template <int HD>
 __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
-    constexpr int D4 = HD / 4, G = 256 / D4;
+    constexpr int D4 = HD / 4, G = 256 / D4, PRE = 4;
     __shared__ v4f red[G][D4];
     const int kvh = blockIdx.x % a.p.n_kv, col = blockIdx.y;
     const PagedComb c = a.combs[blockIdx.x / a.p.n_kv];
-    const PagedSeq sq = a.p.seqs[c.seq];
     const int rr = c.row0 + col, lane = threadIdx.x & 63;
-    if (rr >= sq.M * a.gqa) return;
+    if (rr >= c.M * a.gqa) return;
     const int64_t step = (int64_t)c.step * a.p.n_kv * PAGED_TR;
     const int64_t p0 = ((int64_t)c.part0 * a.p.n_kv + kvh) * PAGED_TR + col;
     const float2* ml = (const float2*)a.pml + p0;
+    const int g = threadIdx.x / D4, d = threadIdx.x % D4;
+    // the first partials of the thread, loaded beside the maxima and sums
+    v4f first[PRE];
+#pragma unroll
+    for (int x = 0; x < PRE; ++x)
+        first[x] = *(const v4f*)(a.part + (p0 + min(g + x * G, c.n - 1) * step) * HD + 4 * d);
     float M = -INFINITY, den = 0.f;
     for (int i = lane; i < c.n; i += 64) M = fmaxf(M, ml[i * step].x);
 #pragma unroll
@@ -1094,10 +1098,12 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
     for (int i = lane; i < c.n; i += 64) den += weight(i);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o, 64);
-    const int g = threadIdx.x / D4, d = threadIdx.x % D4;
     v4f num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < PRE; ++x)
+        if (g + x * G < c.n) num += first[x] * (weight(g + x * G) / den);
 #pragma unroll 4
-    for (int i = g; i < c.n; i += G) {
+    for (int i = g + PRE * G; i < c.n; i += G) {
         const float f = weight(i) / den;
         const v4f o = *(const v4f*)(a.part + (p0 + i * step) * HD + 4 * d);
 #pragma unroll
@@ -1108,7 +1114,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
     if (g) return;
 #pragma unroll
     for (int x = 1; x < G; ++x) num += red[x][d];
-    const int64_t tok = sq.tok0 + rr / a.gqa;
+    const int64_t tok = c.tok0 + rr / a.gqa;
     const bool vec = !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
     st4(a.out + tok * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD + 4 * d, num, vec);
 }

@@ -58,9 +58,10 @@ struct PagedItem {
     PagedSeq q;
     int32_t fill[6];  // to 96 bytes
 };
-// the partials part0, part0 + step, .. (n of them) of PAGED_TR rows
+// the partials part0, part0 + step, .. (n of them) of PAGED_TR rows; tok0, M:
+// its sequence's
 struct PagedComb {
-    int32_t seq, row0, part0, n, step;
+    int32_t seq, row0, part0, n, step, tok0, M, pad;
 };
 constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
 

@@ -272,7 +272,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
             o.comb_max = std::max(o.comb_max, np);
             for (int64_t r = 0; r < t.rows; r += PAGED_TR)
                 o.combs.push_back(PagedComb{t.seq, (int32_t)(t.row0 + r), (int32_t)(o.parts + r / PAGED_TR), (int32_t)np,
-                                            (int32_t)blocks});
+                                            (int32_t)blocks, o.seqs[(size_t)t.seq].tok0, o.seqs[(size_t)t.seq].M, 0});
             o.parts += np * blocks;
         }
         // the longest first (two row tiles a wave: 7 for 4)

@@ -255,6 +255,25 @@ HipSequence::HipSequence(HipVerifier& ver, int64_t ctx_cap, bool kv_f16) : be_(v
               "kv_create");
 }
 
+HipSequence::HipSequence(HipVerifier& ver, HipPool& pool, int64_t ctx_cap, int64_t window, int64_t sinks)
+    : be_(ver.be_) {
+    be_.check(ftx_kv_create_paged(be_.ctx(), ver.model_, pool.pool_, ctx_cap, window, sinks, &kv_),
+              "kv_create_paged");
+}
+
+HipPool::HipPool(HipVerifier& ver, int64_t n_pages, bool eight_bit) {
+    const ModelConfig& c = ver.config();
+    ver.be_.check(ftx_pool_create(ver.be_.ctx(), c.n_layer, c.n_head_kv, c.head_dim, n_pages,
+                                  eight_bit ? FTX_KV_Q8 : FTX_KV_F16, &pool_),
+                  "pool_create");
+}
+
+HipPool::~HipPool() {
+    if (pool_) ftx_pool_free(pool_);
+}
+
+int64_t HipPool::available() const { return ftx_pool_available(pool_); }
+
 HipSequence::~HipSequence() {
     if (kv_) ftx_kv_free(kv_);
 }

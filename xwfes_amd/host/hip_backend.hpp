@@ -225,12 +225,30 @@ public:
 
 private:
     friend class HipSequence;
+    friend class HipPool;
     HipBackend& be_;
     ModelConfig cfg_;
     ftx_model* model_ = nullptr;
     ftx_kv* kv_ = nullptr;
     float* logits_ = nullptr;
     int64_t max_tokens_ = 0;
+};
+
+// Pages of paged caches for a HipVerifier's model (ftx_pool_create; no
+// counterpart in the reference): rows of K and V in 8 bits or halves.  Must
+// outlive its sequences.
+class HipPool {
+public:
+    HipPool(HipVerifier& ver, int64_t n_pages, bool eight_bit = false);
+    ~HipPool();
+    HipPool(const HipPool&) = delete;
+    HipPool& operator=(const HipPool&) = delete;
+
+    int64_t available() const;
+
+private:
+    friend class HipSequence;
+    ftx_pool* pool_ = nullptr;
 };
 
 // One more sequence over a HipVerifier's model (no counterpart in the
@@ -241,6 +259,10 @@ private:
 class HipSequence {
 public:
     HipSequence(HipVerifier& ver, int64_t ctx_cap, bool kv_f16 = true);
+    // a cache in pages of `pool`, taken as it grows (ftx_kv_create_paged); its
+    // host arrays are fp32.  window > 0: a token sees the last `window`
+    // positions and the first `sinks`
+    HipSequence(HipVerifier& ver, HipPool& pool, int64_t ctx_cap, int64_t window = 0, int64_t sinks = 0);
     ~HipSequence();
     HipSequence(const HipSequence&) = delete;
     HipSequence& operator=(const HipSequence&) = delete;

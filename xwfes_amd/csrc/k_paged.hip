@@ -285,6 +285,13 @@ __device__ __forceinline__ float col_max(float x) {
 // Levels that V scales are taken relative to: powers of 2^4.  The lowest: 2^-ev
 // is finite; the smallest scale is 2^-114.
 constexpr int EV_MIN = -112;
+// Halves come in two kinds: rows kept as they are (scale 1) or larger (2 and up),
+// and small ones, of scales 2^-23 and less whose values reach 2^15 all the same.
+// Under level 0, which a row of scale 1 sets whatever its size from 2^-8 up, a
+// small row's weights would lose their low bits, and more than those: a page of
+// both kinds is taken in two visits, large slots then small ones, and the small
+// ones' level of a row at level 0 is this (the highest that they have).
+constexpr int EV_SMALL = -20;
 // the lowest level with 2^level >= vm (1: 0, so that pages with and without a
 // scale other than 1 weigh alike)
 __device__ __forceinline__ int ev_level(float vm) {
@@ -440,14 +447,15 @@ struct WaveAttn {
 
     // The page's weights from its scores (by_scale's); the sums so far brought to a new
     // offset or V level where one is needed.  ones: every scale of the page is 1
-    // (sc is not read).  whole: the row sees every slot, else slot 16 st + 4 kq + r
-    // by bit 16 st + r of seen.  pe: sc.v stands 2^-pe over, pe the level of the page's largest
-    // V scale (whole pages only: what a row does not see must not set its
-    // level), or NO_LEVEL.
+    // (sc is not read).  whole: the row sees every slot, else slot x by bit x of
+    // sight.  pe: sc.v stands 2^-pe over, pe the level of the page's largest
+    // V scale (whole pages of one kind only: what a row does not see must not set its
+    // level), or NO_LEVEL.  small: the slots of this visit are the page's small ones.
     static constexpr int NO_LEVEL = 1 << 20;
-    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, uint64_t seen,
-                                           v8h (&ph)[2], v8h (&pl)[2]) {
+    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, bool small,
+                                           uint64_t sight, int kq, v8h (&ph)[2], v8h (&pl)[2]) {
         if (!whole) {
+            const uint64_t seen = sight >> (4 * kq);
 #pragma unroll
             for (int st = 0; st < 4; ++st)
 #pragma unroll
@@ -475,11 +483,14 @@ struct WaveAttn {
         float vf = 1.f;
         bool flat = true;
         if (ones) {
-            if (__builtin_amdgcn_ballot_w64(ev < 0)) raise(max(ev, 0));
-            flat = !__builtin_amdgcn_ballot_w64(ev != 0);
+            // (a row that sees nothing here keeps its level: its weights are 0)
+            const bool any = whole || sight;
+            if (__builtin_amdgcn_ballot_w64(any & (ev < 0))) raise(any ? max(ev, 0) : ev);
+            flat = !__builtin_amdgcn_ballot_w64(any & (ev != 0));
             if (!flat) vf = ldexpf(1.f, -ev);
         } else if (pe != NO_LEVEL) {
-            if (__builtin_amdgcn_ballot_w64(ev < pe)) raise(max(ev, pe));
+            const int en = !Q8 && pe < 0 && ev == 0 ? EV_SMALL : max(ev, pe);
+            if (__builtin_amdgcn_ballot_w64(ev != en)) raise(en);
             if (__builtin_amdgcn_ballot_w64(ev != pe)) {
                 const float f = ldexpf(1.f, pe - ev);
 #pragma unroll
@@ -490,7 +501,11 @@ struct WaveAttn {
                                           fmaxf(fmaxf(sc.v[1][0], sc.v[1][1]), fmaxf(sc.v[1][2], sc.v[1][3]))),
                                     fmaxf(fmaxf(fmaxf(sc.v[2][0], sc.v[2][1]), fmaxf(sc.v[2][2], sc.v[2][3])),
                                           fmaxf(fmaxf(sc.v[3][0], sc.v[3][1]), fmaxf(sc.v[3][2], sc.v[3][3]))));
-            if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.f, ev))) raise(max(ev, ev_level(col_max(fmaxf(top, 0.f)))));
+            const bool down = !Q8 && small && ev == 0;
+            if (__builtin_amdgcn_ballot_w64(down | (top > ldexpf(1.f, ev)))) {
+                const int lev = ev_level(col_max(fmaxf(top, 0.f)));
+                raise(down ? EV_SMALL : max(ev, lev));
+            }
             const float f = ldexpf(1.f, -ev);
 #pragma unroll
             for (int st = 0; st < 4; ++st) sc.v[st] *= f;
@@ -637,6 +652,21 @@ struct RowSight {
     }
 };
 
+// Which slots of a page of halves hold large and which small V rows (rows of
+// zeros and slots never written, of scale 0, are neither); v: slot lane's V scale
+struct Kinds {
+    uint64_t large = 0, tiny = 0;
+    __device__ __forceinline__ Kinds(bool one_kind, float v) {
+        if (one_kind) return;
+        large = __builtin_amdgcn_ballot_w64(v >= 1.f);
+        tiny = __builtin_amdgcn_ballot_w64((v > 0.f) & (v < 1.f));
+    }
+    __device__ __forceinline__ bool both() const { return large && tiny; }
+    // the slots of a visit, of the first or the second
+    __device__ __forceinline__ uint64_t part(bool second) const { return !both() ? ~0ull : second ? ~large : large; }
+    __device__ __forceinline__ bool small(bool second) const { return tiny && (second || !large); }
+};
+
 // Few rows: workgroup = (item, kv head), neighbours on one XCD's L2 sharing a
 // head where there are 8; the item's pages dealt to its NW waves, whose
 // softmaxes meet in LDS (of eight, the last four with the first four before).
@@ -708,7 +738,8 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         blk = block_of(0);
         if (PRE) W::load_vals(kv, blk, lane);
     }
-    for (int j = 0; j < n; ++j) {
+    bool second = false;  // a page of large and small rows of halves: its small ones
+    for (int j = 0; j < n;) {
         if (!PRE) W::load_vals(kv, blk, lane);
         const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
         float k1 = 0.f, v1 = 0.f;
@@ -734,17 +765,23 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((k1 != 1.f) | (v1 != 1.f));
         if (!Q8 && !ones) W::load_scales(sc, scale, scale + FTX_PAGE, kq);
         if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
-        if (j + 1 < n) {
-            blk = block_of(j + 1);
+        const int p0 = place(j) * FTX_PAGE;
+        const Kinds kinds(Q8 || ones, v1);
+        const bool again = kinds.both() && !second;
+        if (again) {
+            if (PRE) W::load_vals(kv, blk, lane);
+        } else if (++j < n) {
+            blk = block_of(j);
             if (PRE) W::load_vals(kv, blk, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const int p0 = place(j) * FTX_PAGE;
-        const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
+        const bool whole = !kinds.both() && p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
         v8h ph[2], pl[2];
         if (!ones) W::by_scale(s, sc);
-        wa.soften(s, sc, ones, whole, W::NO_LEVEL, whole ? 0 : sight.page(p0) >> (4 * kq), ph, pl);
+        wa.soften(s, sc, ones, whole, W::NO_LEVEL, kinds.small(second), whole ? 0 : sight.page(p0) & kinds.part(second), kq,
+                  ph, pl);
         wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
+        second = again;
     }
     wa.l += __shfl_xor(wa.l, 16, 64);
     wa.l += __shfl_xor(wa.l, 32, 64);
@@ -955,13 +992,15 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         lo[x] = __builtin_amdgcn_readfirstlane(l);
         last = max(last, __builtin_amdgcn_readfirstlane(e));
     }
-    // page j for the wave's first N tiles
-    auto work = [&](auto tiles, int j) {
+    // page j for the wave's first N tiles; whether it takes a second visit
+    auto work = [&](auto tiles, int j, bool second) -> bool {
         constexpr int N = decltype(tiles)::value;
         const int p0 = place(j) * FTX_PAGE;
         const uint8_t* buf = lds + (j & 1) * BUF;
         const float* scale = (const float*)(buf + 2 * VB);
-        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (scale[FTX_PAGE + lane] != 1.f));
+        const float v1 = Q8 ? 0.f : scale[FTX_PAGE + lane];
+        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (v1 != 1.f));
+        const Kinds kinds(Q8 || ones, v1);
         v4f s[N][4];
         staged_scores<W::NDC>(
             s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); },
@@ -977,14 +1016,15 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            const bool whole = p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
+            const bool whole = !kinds.both() && p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
             if (!ones) W::load_four(sc.v, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
             const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
-            uint64_t seen = 0;
-            if (!whole) seen = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0) >> (4 * kq);
-            wa[x].soften(s[x], sc, ones, whole, pe, seen, ph[x], pl[x]);
+            uint64_t sight = 0;
+            if (!whole) sight = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0) & kinds.part(second);
+            wa[x].soften(s[x], sc, ones, whole, pe, kinds.small(second), sight, kq, ph[x], pl[x]);
         }
         staged_outputs<N>(wa, vf, ph, pl);
+        return kinds.both() && !second;
     };
     commit(0);
     auto pages = [&](auto tiles) {
@@ -992,7 +1032,8 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's direct copies of page j
             __syncthreads();                     // every wave's; the other buffer is free
             if (j + 1 < n) stage(j + 1);
-            if (live && place(j) * FTX_PAGE <= last) work(tiles, j);
+            if (live && place(j) * FTX_PAGE <= last)
+                for (bool second = false; work(tiles, j, second);) second = true;
             if (j + 1 < n) commit(j + 1);
         }
     };

@@ -79,8 +79,9 @@ struct RowForm {
     }
     __device__ __forceinline__ float scale() const {
         if (!ok) return __builtin_nanf("");
-        if constexpr (Q8) return zero ? 0.f : a / 127.f;
-        return zero ? 1.f : ldexpf(1.f, f16_exp(a));
+        if (zero) return 0.f;  // (of no size: it must not set a level)
+        if constexpr (Q8) return a / 127.f;
+        return ldexpf(1.f, f16_exp(a));
     }
     // the values' bits in the page, in the low byte (half) of b; finite
     // whatever the row holds

@@ -444,8 +444,9 @@ int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq
  * window reaches into them is refused (FTX_E_RANGE; 0 is not).  The sequences
  * of one ftx_verify_batch are all of one pool, window and sinks, or none is
  * paged.  ftx_kv_write and ftx_kv_read take fp32 arrays for a paged cache
- * (write takes pages for all of cap, read leaves zeros where no page is);
- * ftx_kv_pointers gives NULL for its buffers. */
+ * (write takes pages for all of cap; read leaves zeros where no page is and past
+ * the last new token); a length or a path that reaches past the rows it was
+ * given is refused (FTX_E_RANGE).  ftx_kv_pointers gives NULL for its buffers. */
 int ftx_kv_create_paged(ftx_ctx* ctx, const ftx_model* m, ftx_pool* p, int64_t cap, int64_t window,
                         int64_t sinks, ftx_kv** out);
 

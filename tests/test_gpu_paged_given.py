@@ -1,0 +1,90 @@
+"""A paged cache shows the rows that it was given, never what its pages held for
+another: reads past the last new tokens are zeros, and a length or a path that
+reaches past them is refused."""
+import numpy as np
+import pytest
+
+from test_gpu_paged import F16, Q8, refused
+from test_gpu_paged_steps import CFG64, Setup
+from test_gpu_paged_steps import Q8 as Q8_0
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def setup(gctx, orc, request):
+    t = Setup(gctx, orc, CFG64, Q8_0, kvt=request.param, pages=4)
+    # both pages of the pool's first take, full of another cache's rows
+    other = t.gm.kv_paged(t.pool, 256)
+    other.write(*np.full((2,) + other.shape, 5.0, np.float32))
+    other.free()
+    yield t
+    t.free()
+
+
+KINDS = pytest.mark.parametrize("setup", [F16, Q8], ids=["f16", "q8"], indirect=True)
+
+
+@KINDS
+@pytest.mark.parametrize("M", [1, 9, 64, 70])
+def test_rows_past_the_new_tokens_read_zero(setup, M):
+    kv = setup.gm.kv_paged(setup.pool, 200)
+    setup.kvs.append(kv)
+    toks = list(range(M))
+    setup.step([(kv, toks, None, True)])
+    for x in kv.read():
+        assert x[:, :M].any((0, 2)).all() and not x[:, M:].any()
+    # tokens that were not committed are the cache's own
+    setup.step([(kv, [7, 8, 9], None, False)])
+    for x in kv.read():
+        assert x[:, :M + 3].any((0, 2)).all() and not x[:, M + 3:].any()
+
+
+@KINDS
+def test_lengths_and_paths_past_the_new_tokens_are_refused(setup):
+    kv = setup.gm.kv_paged(setup.pool, 200)
+    setup.kvs.append(kv)
+    refused(-5, kv.truncate, 1)
+    setup.step([(kv, [1, 2, 3, 4], [-1, 0, 0, 1], False)])
+    refused(-5, kv.truncate, 5)
+    refused(-5, kv.commit, [0, 4])
+    kv.commit([0, 2])
+    assert kv.pointers()[2] == 2
+    refused(-5, kv.truncate, 5)
+    kv.truncate(4)
+    kv.truncate(0)
+    assert setup.pool.available == 4
+    # pages taken anew hold nothing of it
+    setup.step([(kv, [1], None, False)])
+    refused(-5, kv.truncate, 2)
+    for x in kv.read():
+        assert x[:, :1].any() and not x[:, 1:].any()
+
+
+@KINDS
+def test_a_refused_step_gives_nothing(setup):
+    kv, hog = (setup.gm.kv_paged(setup.pool, 256) for _ in range(2))
+    setup.kvs += [kv, hog]
+    setup.step([(kv, [1, 2], None, True)])
+    refused(-4, setup.step, [(kv, [5] * 70, None, False), (hog, [6] * 180, None, False)])
+    refused(-5, kv.truncate, 3)
+    for x in kv.read():
+        assert x[:, :2].any((0, 2)).all() and not x[:, 2:].any()
+
+
+@KINDS
+def test_a_written_cache_is_given_all_of_its_rows(setup):
+    kv = setup.gm.kv_paged(setup.pool, 100)
+    setup.kvs.append(kv)
+    k, v = np.random.default_rng(1).standard_normal((2,) + kv.shape).astype(np.float32)
+    kv.write(k, v)
+    assert all(x.any((0, 2)).all() for x in kv.read())
+    kv.truncate(99)
+    setup.step([(kv, [3], None, True)])
+    refused(-5, kv.truncate, 101)
+    kv.truncate(10)
+    # the rest of the page that length ends in is still its own
+    kv.truncate(64)
+    refused(-5, kv.truncate, 65)
+    for x in kv.read():
+        assert x[:, :64].any((0, 2)).all() and not x[:, 64:].any()

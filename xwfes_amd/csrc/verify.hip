@@ -142,6 +142,7 @@ struct ftx_kv {
     ftx_pool* pool = nullptr;
     std::vector<int32_t> pages;
     int64_t window = 0, sinks = 0;
+    int64_t given = 0;  // positions that it was given rows for: what lies past them in its last page is not its own
 };
 
 // pages of a paged cache for `tokens` positions, all or none
@@ -770,8 +771,10 @@ static int verify_large(ftx_ctx* ctx, ftx_model* m, const ftx_seq_args* sq, int6
         }
     }
 #undef TRACED_L
-    for (int64_t s = 0; s < nseq; ++s)
+    for (int64_t s = 0; s < nseq; ++s) {
+        if (plan) sq[s].kv->given = std::max(sq[s].kv->given, sq[s].kv->npast + sq[s].M);
         if (sq[s].advance) sq[s].kv->npast += sq[s].M;
+    }
     return FTX_OK;
 }
 
@@ -1239,9 +1242,10 @@ static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
             return ftx_fail(ctx, FTX_E_NOMEM, "kv_write: not enough free pages");
         kv_drop(kv, 0, (int64_t)kv->pages.size());
         kv->pages.clear();
+        kv->given = 0;
         if (const int rc = kv_grow(kv, kv->cap)) return rc;
     }
-    const int64_t kdim = kv->kdim, n = std::min<int64_t>((int64_t)kv->pages.size() * FTX_PAGE, kv->cap);
+    const int64_t kdim = kv->kdim, n = to_device ? kv->cap : kv->given;
     const size_t bytes = (size_t)(n * kdim) * sizeof(float);
     if (!to_device) {
         memset(kh, 0, (size_t)(kv->n_layer * kv->cap * kdim) * sizeof(float));
@@ -1252,13 +1256,14 @@ static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
     if (const int rc = ftx_workspace(ctx, 2 * bytes, (void**)&ws)) return rc;
     hipStream_t st = ctx->stream;
     // runs of held pages, each as a sequence of its own
-    for (int64_t p0 = 0; p0 < (int64_t)kv->pages.size();) {
+    const int64_t n_pages = (n + FTX_PAGE - 1) / FTX_PAGE;
+    for (int64_t p0 = 0; p0 < n_pages;) {
         if (kv->pages[(size_t)p0] < 0) {
             ++p0;
             continue;
         }
         int64_t p1 = p0;
-        while (p1 < (int64_t)kv->pages.size() && kv->pages[(size_t)p1] >= 0) ++p1;
+        while (p1 < n_pages && kv->pages[(size_t)p1] >= 0) ++p1;
         const int64_t r0 = p0 * FTX_PAGE, rows = std::min(p1 * FTX_PAGE, n) - r0;
         const ftx_paged_seq seq{kv->pages.data() + p0, p1 - p0, 0, rows, nullptr};
         const ftx_plan_args pa{&seq, 1, 0, 0, 0};
@@ -1283,6 +1288,7 @@ static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
         p0 = p1;
     }
     FTX_HIP(ctx, hipStreamSynchronize(st));
+    if (to_device) kv->given = n;
     return FTX_OK;
 }
 
@@ -1311,7 +1317,7 @@ int ftx_kv_truncate(ftx_kv* kv, int64_t npast) {
     if (npast < 0 || npast > kv->cap) return ftx_fail(kv->ctx, FTX_E_RANGE, "npast out of range");
     if (kv->pool) {
         const int64_t held = (npast + FTX_PAGE - 1) / FTX_PAGE;
-        if (held > (int64_t)kv->pages.size())
+        if (npast > kv->given)
             return ftx_fail(kv->ctx, FTX_E_RANGE, "truncate: a paged cache does not hold that many tokens");
         const auto un = kv_unseen(kv, npast);
         for (int64_t i = 0; i < held; ++i)
@@ -1319,6 +1325,7 @@ int ftx_kv_truncate(ftx_kv* kv, int64_t npast) {
                 return ftx_fail(kv->ctx, FTX_E_RANGE, "truncate: the window's pages are gone");
         kv_drop(kv, held, (int64_t)kv->pages.size());
         kv->pages.resize((size_t)held);
+        kv->given = std::min(kv->given, held * FTX_PAGE);
     }
     kv->npast = npast;
     return FTX_OK;
@@ -1346,7 +1353,7 @@ int ftx_kv_commit(ftx_kv* kv, const int32_t* nodes, int64_t n) {
         a.nodes[i] = j;
         moves |= j != i;
     }
-    if (kv->pool && n > 0 && kv->npast + nodes[n - 1] >= (int64_t)kv->pages.size() * FTX_PAGE)
+    if (kv->pool && n > 0 && kv->npast + nodes[n - 1] >= kv->given)
         return ftx_fail(ctx, FTX_E_RANGE, "kv_commit: node out of range");
     if (moves && kv->pool) {
         PagedMove pm{};
@@ -1695,6 +1702,7 @@ int ftx_verify_step(ftx_ctx* ctx, ftx_model* m, ftx_kv* kv, const ftx_verify_arg
         if (rc) return rc;
     }
 #undef TRACED
+    if (plan) kv->given = std::max(kv->given, npast + M);
     if (a->advance) kv->npast = npast + M;
     return FTX_OK;
 }

@@ -306,7 +306,8 @@ __device__ __forceinline__ int ev_level(float vm) {
 // brings it to [2^6, 2^7); a score in units of log2 is 2^-e s ks exactly as
 // s ks is, so one fma gives the weight's exponent: p = 2^(s ks 2^-e - off).
 // off, as it was rounded, is the running maximum less 12 when it was last taken:
-// it is taken anew where a page's maximum would bring a weight above 2^15 (the
+// it is taken anew where a page's maximum would bring a weight above 2^15 (p is at
+// most that, also where a score's last place is worth more; the
 // products of the sums so far, a third of a page's arithmetic, then fall to one
 // page in ten).  l = sum p, and P.V of p vs 2^-ev in two halves, ev the level
 // of the largest V scale that the row has seen.  out = 2^ev o / l.
@@ -470,9 +471,14 @@ struct WaveAttn {
                 }
         }
         const float mx = row_max(s);
-        const float cand = __builtin_fmaf(mx, c2, -12.f);
-        if (__builtin_amdgcn_ballot_w64(cand > off + 3.f)) {  // (wave-uniform)
-            const float on = fmaxf(off, cand);
+        // (rows that need none keep theirs: a row's bits are its own, not its tile's)
+        const bool over = __builtin_fmaf(mx, c2, -off) > 15.f;
+        if (__builtin_amdgcn_ballot_w64(over)) {
+            float cand = __builtin_fmaf(mx, c2, -12.f);
+            // (from 2^26 on the 12 may round to 16, then to nothing: the score itself)
+            if (__builtin_fmaf(mx, c2, -cand) > 15.f) cand = mx * c2;
+            if (cand > FLT_BIG) cand = __builtin_nanf("");  // (a score past fp32)
+            const float on = over ? cand : off;
             const float al = off == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(off - on);
             off = on;
             l *= al;
@@ -842,7 +848,8 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
     const int64_t prow = ((int64_t)it.part * a.p.n_kv + kvh) * PAGED_TR + col;
     float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
     const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
-    const float inv = L == 0.f ? 0.f : 1.f / L;  // (0: no page of this part is seen by the row)
+    // (0: no page of this part is seen by the row; of a whole list, every score is below fp32: NaN)
+    const float inv = part && L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int dt = 0; dt < W::NDT; ++dt) {
         v4f y;
@@ -1054,7 +1061,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         const int64_t prow = ((int64_t)(it.part + tile_of(x)) * a.p.n_kv + kvh) * PAGED_TR + col;
         float* dst = part ? a.part + prow * HD
                           : a.out + (int64_t)(sq.tok0 + rr / a.gqa) * a.ldo + (int64_t)(kvh * a.gqa + rr % a.gqa) * HD;
-        const float inv = wa[x].l == 0.f ? 0.f : 1.f / wa[x].l;  // (0: no page of this part is seen by the row)
+        const float inv = part && wa[x].l == 0.f ? 0.f : 1.f / wa[x].l;  // (as in k_paged_attn)
 #pragma unroll
         for (int dt = 0; dt < W::NDT; ++dt) {
             v4f y;

@@ -415,7 +415,9 @@ int ftx_plan_free(ftx_plan* pl);
  * recorded into a HIP graph; ftx_plan_set is then refused for that plan, and
  * the plan, its pool and the matrices must outlive the graph.  Calls of one
  * plan share its workspace: they must not overlap.  After ftx_set_stream a
- * call waits for the plan's tables, ftx_plan_set for the device. */
+ * call waits for the plan's tables, ftx_plan_set for the device; the first call
+ * that is recorded after a ftx_plan_set waits on the host until they are there
+ * (a graph may be launched on any stream). */
 
 /* Store the new tokens' k and v rows ([sum of M][n_head_kv * head_dim],
  * sequence after sequence) of a layer in their pages. */

@@ -3,8 +3,11 @@
 #include "paged.h"
 
 #include <algorithm>
+#include <chrono>
 #include <cstdio>
+#include <cstring>
 #include <new>
+#include <thread>
 
 #include "paged_pool.h"
 
@@ -389,11 +392,14 @@ struct ftx_plan {
     hipEvent_t ev[RING] = {};
     int next = 0;
     hipEvent_t up = nullptr;  // the last copy's
+    bool landed = false;      // the host has waited for it
     // of the last set or call outside of captures: another stream waits for the
     // copy, a set on another for everything
     hipStream_t stream = nullptr;
     // the parts of the device block
-    size_t o_seq = 0, o_tab = 0, o_dep = 0, o_anc = 0, o_item = 0, o_comb = 0;
+    size_t o_seq = 0, o_tab = 0, o_dep = 0, o_anc = 0, o_item = 0, o_comb = 0, o_serial = 0;
+    size_t bytes = 0;     // of the last set's tables
+    uint64_t serial = 0;  // its number
 };
 
 static void plan_release(ftx_plan* pl) {
@@ -423,7 +429,9 @@ static int plan_upload(ftx_plan* pl) {
     place(pl->o_anc, t.anc.size() * 4);
     place(pl->o_item, t.items.size() * sizeof(PagedItem));
     place(pl->o_comb, t.combs.size() * sizeof(PagedComb));
-    const size_t bytes = at;
+    place(pl->o_serial, sizeof pl->serial);
+    const size_t bytes = pl->bytes = at;
+    ++pl->serial;
     const size_t pf = (size_t)t.parts * pl->pool->n_kv * PAGED_TR * (pl->pool->hd + 2);
     hipStream_t st = ctx->stream;
     auto grow = [&](void** p, size_t& have, size_t need, size_t unit) -> int {
@@ -472,9 +480,11 @@ static int plan_upload(ftx_plan* pl) {
     put(pl->o_anc, t.anc.data(), t.anc.size() * 4);
     put(pl->o_item, t.items.data(), t.items.size() * sizeof(PagedItem));
     put(pl->o_comb, t.combs.data(), t.combs.size() * sizeof(PagedComb));
+    put(pl->o_serial, &pl->serial, sizeof pl->serial);
     FTX_HIP(ctx, hipMemcpyAsync(pl->dev, h, bytes, hipMemcpyHostToDevice, st));
     FTX_HIP(ctx, hipEventRecord(pl->ev[k], st));
     pl->up = pl->ev[k];
+    pl->landed = false;
     pl->stream = st;
     pl->next = (k + 1) % ftx_plan::RING;
     pl->ready = true;
@@ -495,21 +505,49 @@ PagedView paged_view(const ftx_plan* pl, int64_t layer) {
     return v;
 }
 
-// the tables' copy ahead of a call on another stream than its own
+// The last set's tables in device memory, seen from the host: read back on a
+// stream of its own and compared (their event is no help, HIP refuses one whose
+// stream is being captured).  The serial number tells them from an older set's.
+static hipError_t tables_landed(const ftx_plan* pl) {
+    std::vector<uint8_t> got(pl->bytes);
+    const uint8_t* want = pl->pin[(pl->next + ftx_plan::RING - 1) % ftx_plan::RING];
+    hipStream_t st;
+    hipError_t e = hipStreamCreateWithFlags(&st, hipStreamNonBlocking);
+    if (e != hipSuccess) return e;
+    for (;;) {
+        e = hipMemcpyAsync(got.data(), pl->dev, pl->bytes, hipMemcpyDeviceToHost, st);
+        if (e == hipSuccess) e = hipStreamSynchronize(st);
+        if (e != hipSuccess || memcmp(got.data(), want, pl->bytes) == 0) break;
+        std::this_thread::sleep_for(std::chrono::microseconds(50));
+    }
+    (void)hipStreamDestroy(st);
+    return e;
+}
+
+// the tables' copy ahead of a call on another stream than its own, and of a
+// captured one on any: the copy is not in the graph, which may be launched on
+// another stream than the captured one, so the host waits
 static int plan_order(ftx_plan* pl, bool captures) {
     ftx_ctx* ctx = pl->ctx;
-    if (ctx->stream == pl->stream) return FTX_OK;
     if (!captures) {
+        if (ctx->stream == pl->stream) return FTX_OK;
         FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
         pl->stream = ctx->stream;
         return FTX_OK;
     }
-    // (an event from outside does not go into a graph: the host waits)
+    if (pl->landed) return FTX_OK;
+    OnDevice od(ctx->device);
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
     FTX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
-    const hipError_t e = hipEventSynchronize(pl->up);
+    hipError_t e;
+    try {
+        e = tables_landed(pl);
+    } catch (...) {
+        e = hipErrorOutOfMemory;
+    }
     FTX_HIP(ctx, hipThreadExchangeStreamCaptureMode(&mode));
     FTX_HIP(ctx, e);
+    pl->landed = true;
     return FTX_OK;
 }
 

@@ -103,6 +103,9 @@ extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int
 extern "C" void paged_force_rows(int rows);
 
 // ---------------------------------------------------------------- launches
+// a launch has fewer than 2^32 threads along its x
+inline bool paged_grid_fits(int64_t workgroups, int64_t threads) { return workgroups * threads < (int64_t)1 << 32; }
+
 struct PagedView {
     uint8_t* data;  // the layer's first block
     int64_t block;  // bytes of a block

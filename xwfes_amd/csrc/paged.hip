@@ -156,6 +156,8 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         }
         o.seqs.push_back(d);
     }
+    if (!paged_grid_fits(o.max_new_pages * 2 * g.n_kv, 256))
+        return fail(FTX_E_RANGE, "too many new tokens of one sequence in one plan");
     if (a.n_head == 0) return FTX_OK;
     // The row tiles and the pages each sees: of TR rows for the sequences of
     // PAGED_MANY rows and more (big) or the others.  false: a page is absent.
@@ -284,8 +286,9 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
                          [&](const PagedItem& x, const PagedItem& y) { return work(x) > work(y); });
         if (!many) o.few = (int64_t)o.items.size();
     }
-    if ((int64_t)o.items.size() * g.n_kv >= (int64_t)1 << 31 || (int64_t)o.combs.size() * g.n_kv >= (int64_t)1 << 31 ||
-        o.parts >= (int64_t)1 << 31)
+    if (!paged_grid_fits(o.few * g.n_kv, o.wide ? 512 : 256) ||
+        !paged_grid_fits(((int64_t)o.items.size() - o.few) * g.n_kv, 512) ||
+        !paged_grid_fits((int64_t)o.combs.size() * g.n_kv, 256) || o.parts >= (int64_t)1 << 31)
         return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
     return FTX_OK;
 }
@@ -726,6 +729,8 @@ int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t l
     if (pl->ready && n == 0) return FTX_OK;
     const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
     if (rc) return rc;
+    if (context && !paged_grid_fits(pl->t.max_pages * 2 * pl->pool->n_kv, 256))
+        return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: too many positions of one sequence");
     if (context && pl->t.absent) return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: a page is absent");
     if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_read: k and v overlap");
     return paged_read_rows(pl, layer, context, k, ldk, v, ldv);

@@ -88,3 +88,12 @@ def test_a_written_cache_is_given_all_of_its_rows(setup):
     refused(-5, kv.truncate, 65)
     for x in kv.read():
         assert x[:, :64].any((0, 2)).all() and not x[:, 64:].any()
+
+
+def test_pools_past_64_bits_are_refused(gctx):
+    """Sizes whose product of bytes comes round to some 6 MB in 64 bits."""
+    for layers, kv, pages in ((36359, 900, 8535041), (45133, 709, 8728098)):
+        assert (layers * kv * pages * (4 * 64 * 256 + 8 * 64)) % 2 ** 64 < 10 ** 7
+        refused(-4, gctx.pool, layers, kv, 256, pages, F16)
+    refused(-4, gctx.pool, 65535, 1024, 256, 1 << 24, F16)
+    gctx.pool(3, 2, 256, 5, F16).free()

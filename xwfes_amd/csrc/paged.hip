@@ -613,8 +613,10 @@ int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t he
         delete p;
         return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
     }
-    const size_t bytes = (size_t)(n_layer * n_pages * n_head_kv * p->block);
-    if (hipMalloc((void**)&p->data, bytes) != hipSuccess) {
+    // (up to 2^66: past 64 bits the product would come round to a small size)
+    const int64_t blocks = n_layer * n_pages * n_head_kv;
+    const size_t bytes = blocks <= ((int64_t)1 << 62) / p->block ? (size_t)(blocks * p->block) : 0;
+    if (bytes == 0 || hipMalloc((void**)&p->data, bytes) != hipSuccess) {
         (void)hipGetLastError();
         delete p;
         return ftx_fail(ctx, FTX_E_NOMEM, "pool allocation failed");

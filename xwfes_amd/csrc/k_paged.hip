@@ -428,22 +428,17 @@ struct WaveAttn {
         for (int st = 0; st < 4; ++st) s[st] *= sc.k[st];
     }
 
-    // the scores' largest of the row (by name: from products of another basic
-    // block the compiler makes every score quiet before each fmaxf)
+    // the scores' largest of the row (`maximum`, which hands NaN on: fmaxf, from
+    // products of another basic block, makes every score quiet first.  By the
+    // compiler's own instructions, so that it keeps the products' wait)
     static __device__ __forceinline__ float row_max(const v4f (&s)[4]) {
         auto max3 = [](float x, float y, float z) {
-            float r;
-            asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
-            return r;
+            return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
         };
-        float mx = max3(s[0][0], s[0][1], s[0][2]);
-        mx = max3(mx, s[0][3], s[1][0]);
-        mx = max3(mx, s[1][1], s[1][2]);
-        mx = max3(mx, s[1][3], s[2][0]);
-        mx = max3(mx, s[2][1], s[2][2]);
-        mx = max3(mx, s[2][3], s[3][0]);
-        mx = max3(mx, s[3][1], s[3][2]);
-        return col_max(max3(mx, s[3][3], s[3][3]));
+        const float a = max3(s[0][0], s[0][1], s[0][2]), b = max3(s[0][3], s[1][0], s[1][1]);
+        const float c = max3(s[1][2], s[1][3], s[2][0]), d = max3(s[2][1], s[2][2], s[2][3]);
+        const float e = max3(s[3][0], s[3][1], s[3][2]);
+        return col_max(max3(max3(a, b, c), max3(d, e, s[3][3]), s[3][3]));
     }
 
     // The page's weights from its scores (by_scale's); the sums so far brought to a new

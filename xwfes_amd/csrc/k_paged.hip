@@ -317,7 +317,7 @@ struct WaveAttn {
     v8h qh[NDC], ql[NDC];
     v4f o[NDT];
     float off = -INFINITY;  // the weights' offset, -inf: nothing seen
-    float l = 0.f;          // (this lane's slots only)
+    float l = 0.f, lp = 0.f;  // (this lane's slots only; lp: of the last page)
     float c2;               // 2^-e
     int ev = EV_MIN;
 
@@ -465,6 +465,7 @@ struct WaveAttn {
                     if (!ones) sc.v[st][r] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, y) & ok);
                 }
         }
+        l += lp;
         const float mx = row_max(s);
         // (rows that need none keep theirs: a row's bits are its own, not its tile's)
         const bool over = __builtin_fmaf(mx, c2, -off) > 15.f;
@@ -511,16 +512,21 @@ struct WaveAttn {
 #pragma unroll
             for (int st = 0; st < 4; ++st) sc.v[st] *= f;
         }
-        // (one loop for each form: tests inside it would part the exponentials)
+        // (one loop for each form: tests inside it would part the exponentials.
+        // A page's weights are added up by themselves, lp, so that a long sum
+        // takes one rounding a page where the outputs take four; joined to l at
+        // the next page: here it costs copies of the outputs, 480 -> 495 us for
+        // three chunks of 1500 tokens, there none, 478)
         auto weigh = [&](auto by) {
+            lp = 0.f;
 #pragma unroll
             for (int st = 0; st < 4; ++st)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2) {
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r], c2, -on));
                     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[st][r + 1], c2, -on));
-                    l += p0;
-                    l += p1;
+                    lp += p0;
+                    lp += p1;
                     v2h h, lo;
                     split_hl2(by(p0, st, r), by(p1, st, r + 1), h, lo);
                     const int i = 4 * (st & 1) + r;
@@ -784,6 +790,7 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
         second = again;
     }
+    wa.l += wa.lp;
     wa.l += __shfl_xor(wa.l, 16, 64);
     wa.l += __shfl_xor(wa.l, 32, 64);
     if constexpr (NW == 8) {
@@ -1049,6 +1056,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
         if (x >= nt) return;
+        wa[x].l += wa[x].lp;
         wa[x].l += __shfl_xor(wa[x].l, 16, 64);
         wa[x].l += __shfl_xor(wa[x].l, 32, 64);
         const int rr = row_of(x);

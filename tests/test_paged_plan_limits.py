@@ -57,3 +57,25 @@ def test_long_contexts_are_not_new_pages():
     far[-3:] = [0, 1, 2]
     rc, msg, _, _ = probe([(far, 64 << 20, 1)], 1, 4, window=100)
     assert rc == 0, msg
+
+
+def test_given_row_tiles_are_the_threads_own():
+    """A test's row tiles reach no plan of another thread."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from xwfes_amd import ftx
+
+    def tiles():
+        return set(probe([(np.arange(5), 0, 300)], 2, 8)[2][:, 7])
+
+    force = ftx.load().paged_force_rows
+    with ThreadPoolExecutor(1) as other:
+        mine = tiles()
+        assert mine == {0}
+        force(128)
+        try:
+            assert tiles() == {1} and other.submit(tiles).result() == mine
+        finally:
+            force(0)
+        other.submit(force, 128).result()
+        assert tiles() == mine and other.submit(tiles).result() == {1}

@@ -98,8 +98,8 @@ extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int
                            int cu, PagedItem* items, int64_t* n_items, PagedComb* combs, int64_t* n_combs,
                            int64_t max_out, char* msg, int64_t msg_bytes);
 
-// For tests: the row tiles of sequences of many rows from now on, 16, 128 or 256
-// (heads of 256 dims: 128), 0: by the estimate
+// For tests: the row tiles of sequences of many rows in the calling thread's plans
+// from now on, 16, 128 or 256 (heads of 256 dims: 128), 0: by the estimate
 extern "C" void paged_force_rows(int rows);
 
 // ---------------------------------------------------------------- launches

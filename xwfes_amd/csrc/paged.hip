@@ -11,8 +11,6 @@
 
 #include "paged_pool.h"
 
-#include <atomic>
-
 // ---------------------------------------------------------------- plan tables
 
 // Sequences of at least this many query rows a kv head may go to the kernel
@@ -25,7 +23,7 @@ constexpr int64_t WIDE_MOST = 48;
 
 namespace {
 
-std::atomic<int> forced_rows{0};  // (paged_force_rows)
+thread_local int forced_rows = 0;  // (paged_force_rows)
 
 struct Tile {
     int32_t seq, row0, rows, s, a, n;  // n pages: 0 .. s - 1, then a, a + 1, ..
@@ -226,7 +224,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         const double page = 0.75 + 1.5 * (double)g.hd / 128;
         double best = 1e300;
         int64_t bestp = 0, chosen = 0;
-        const int force = forced_rows.load(std::memory_order_relaxed);
+        const int force = forced_rows;
         const int64_t most = g.hd <= 128 && (force == 0 || force > PAGED_TR_MANY) ? 2 * PAGED_TR_MANY : PAGED_TR_MANY;
         for (int64_t TR = most; present && TR >= PAGED_TR_MANY; TR /= 2) {
             if (force && TR < most) break;
@@ -293,7 +291,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     return FTX_OK;
 }
 
-extern "C" void paged_force_rows(int rows) { forced_rows.store(rows, std::memory_order_relaxed); }
+extern "C" void paged_force_rows(int rows) { forced_rows = rows; }
 
 extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int64_t n_pages, const uint8_t* taken,
                            int cu, PagedItem* items, int64_t* n_items, PagedComb* combs, int64_t* n_combs,

@@ -292,6 +292,12 @@ constexpr int EV_MIN = -112;
 // both kinds is taken in two visits, large slots then small ones, and the small
 // ones' level of a row at level 0 is this (the highest that they have).
 constexpr int EV_SMALL = -20;
+enum Kind { ALL, LARGE, SMALL };
+// whether a page of halves with slot lane's V scale v holds rows of both kinds
+// (rows of zeros and slots never written have scale 0 and are neither)
+__device__ __forceinline__ bool both_kinds(float v) {
+    return __builtin_amdgcn_ballot_w64(v >= 1.f) && __builtin_amdgcn_ballot_w64((v > 0.f) & (v < 1.f));
+}
 // the lowest level with 2^level >= vm (1: 0, so that pages with and without a
 // scale other than 1 weigh alike)
 __device__ __forceinline__ int ev_level(float vm) {
@@ -446,10 +452,20 @@ struct WaveAttn {
     // (sc is not read).  whole: the row sees every slot, else slot x by bit x of
     // sight.  pe: sc.v stands 2^-pe over, pe the level of the page's largest
     // V scale (whole pages of one kind only: what a row does not see must not set its
-    // level), or NO_LEVEL.  small: the slots of this visit are the page's small ones.
+    // level), or NO_LEVEL.  kind: the page's slots, or its large or its small ones.
     static constexpr int NO_LEVEL = 1 << 20;
-    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, bool small,
+    __device__ __forceinline__ void soften(v4f (&s)[4], Scales& sc, bool ones, bool whole, int pe, Kind kind,
                                            uint64_t sight, int kq, v8h (&ph)[2], v8h (&pl)[2]) {
+        if (!Q8 && kind != ALL) {
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if ((sc.v[st][r] < 1.f) == (kind == LARGE)) {
+                        s[st][r] = -INFINITY;
+                        sc.v[st][r] = 0.f;
+                    }
+        }
         if (!whole) {
             const uint64_t seen = sight >> (4 * kq);
 #pragma unroll
@@ -486,9 +502,9 @@ struct WaveAttn {
         bool flat = true;
         if (ones) {
             // (a row that sees nothing here keeps its level: its weights are 0)
-            const bool any = whole || sight;
-            if (__builtin_amdgcn_ballot_w64(any & (ev < 0))) raise(any ? max(ev, 0) : ev);
-            flat = !__builtin_amdgcn_ballot_w64(any & (ev != 0));
+            const uint64_t any = whole ? ~0ull : __builtin_amdgcn_ballot_w64(sight != 0);
+            if (__builtin_amdgcn_ballot_w64(ev < 0) & any) raise(whole || sight ? max(ev, 0) : ev);
+            flat = !(__builtin_amdgcn_ballot_w64(ev != 0) & any);
             if (!flat) vf = ldexpf(1.f, -ev);
         } else if (pe != NO_LEVEL) {
             const int en = !Q8 && pe < 0 && ev == 0 ? EV_SMALL : max(ev, pe);
@@ -503,7 +519,8 @@ struct WaveAttn {
                                           fmaxf(fmaxf(sc.v[1][0], sc.v[1][1]), fmaxf(sc.v[1][2], sc.v[1][3]))),
                                     fmaxf(fmaxf(fmaxf(sc.v[2][0], sc.v[2][1]), fmaxf(sc.v[2][2], sc.v[2][3])),
                                           fmaxf(fmaxf(sc.v[3][0], sc.v[3][1]), fmaxf(sc.v[3][2], sc.v[3][3]))));
-            const bool down = !Q8 && small && ev == 0;
+            // (halves: the scales left are of one kind)
+            const bool down = !Q8 && ev == 0 && __builtin_amdgcn_ballot_w64((top > 0.f) & (top < 1.f));
             if (__builtin_amdgcn_ballot_w64(down | (top > ldexpf(1.f, ev)))) {
                 const int lev = ev_level(col_max(fmaxf(top, 0.f)));
                 raise(down ? EV_SMALL : max(ev, lev));
@@ -659,21 +676,6 @@ struct RowSight {
     }
 };
 
-// Which slots of a page of halves hold large and which small V rows (rows of
-// zeros and slots never written, of scale 0, are neither); v: slot lane's V scale
-struct Kinds {
-    uint64_t large = 0, tiny = 0;
-    __device__ __forceinline__ Kinds(bool one_kind, float v) {
-        if (one_kind) return;
-        large = __builtin_amdgcn_ballot_w64(v >= 1.f);
-        tiny = __builtin_amdgcn_ballot_w64((v > 0.f) & (v < 1.f));
-    }
-    __device__ __forceinline__ bool both() const { return large && tiny; }
-    // the slots of a visit, of the first or the second
-    __device__ __forceinline__ uint64_t part(bool second) const { return !both() ? ~0ull : second ? ~large : large; }
-    __device__ __forceinline__ bool small(bool second) const { return tiny && (second || !large); }
-};
-
 // Few rows: workgroup = (item, kv head), neighbours on one XCD's L2 sharing a
 // head where there are 8; the item's pages dealt to its NW waves, whose
 // softmaxes meet in LDS (of eight, the last four with the first four before).
@@ -773,8 +775,7 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         if (!Q8 && !ones) W::load_scales(sc, scale, scale + FTX_PAGE, kq);
         if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
         const int p0 = place(j) * FTX_PAGE;
-        const Kinds kinds(Q8 || ones, v1);
-        const bool again = kinds.both() && !second;
+        const bool both = !Q8 && !ones && both_kinds(v1), again = both && !second;
         if (again) {
             if (PRE) W::load_vals(kv, blk, lane);
         } else if (++j < n) {
@@ -782,11 +783,11 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
             if (PRE) W::load_vals(kv, blk, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
-        const bool whole = !kinds.both() && p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
+        const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
         v8h ph[2], pl[2];
         if (!ones) W::by_scale(s, sc);
-        wa.soften(s, sc, ones, whole, W::NO_LEVEL, kinds.small(second), whole ? 0 : sight.page(p0) & kinds.part(second), kq,
-                  ph, pl);
+        wa.soften(s, sc, ones, whole, W::NO_LEVEL, !both ? ALL : second ? SMALL : LARGE, whole ? 0 : sight.page(p0), kq, ph,
+                  pl);
         wa.outputs([&](int dt, int sp) { return W::v_frag(vv, dt, sp); }, ph, pl);
         second = again;
     }
@@ -952,10 +953,11 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         uint8_t* dst = lds + (j & 1) * BUF;
         if (tid < 2 * FTX_PAGE) ((float*)(dst + 2 * VB))[tid] = sc1;
         if (w == 1) {
-            // the page's V level and its V scales by it
+            // the page's V level (or that it has none: rows of both kinds) and its V scales by it
             const int pe = ev_level(__builtin_bit_cast(float, group_max<64>(mag(sc1 <= FLT_BIG ? sc1 : 0.f))));
             ((float*)(dst + 2 * VB))[FTX_PAGE + tid] = ldexpf(sc1, -pe);
-            if (lane == 0) *(int*)(dst + 2 * VB + 3 * FTX_PAGE * 4) = pe;
+            const bool both = !Q8 && both_kinds(sc1);
+            if (lane == 0) *(int*)(dst + 2 * VB + 3 * FTX_PAGE * 4) = both ? W::NO_LEVEL : pe;
         }
         if constexpr (Q8) {
 #pragma unroll
@@ -1007,9 +1009,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         const int p0 = place(j) * FTX_PAGE;
         const uint8_t* buf = lds + (j & 1) * BUF;
         const float* scale = (const float*)(buf + 2 * VB);
-        const float v1 = Q8 ? 0.f : scale[FTX_PAGE + lane];
-        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (v1 != 1.f));
-        const Kinds kinds(Q8 || ones, v1);
+        const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((scale[lane] != 1.f) | (scale[FTX_PAGE + lane] != 1.f));
         v4f s[N][4];
         staged_scores<W::NDC>(
             s, [&](int st, int dc) { return *(const v8h*)(buf + ((dc * 4 + st) * 64 + lane) * 16); },
@@ -1017,23 +1017,28 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             [&](int x, int dc) { return wa[x].qh[dc]; });
         v8h ph[N][2], pl[N][2];
         typename W::Scales sc;
+        int lev = 0;
+        Kind kind = ALL;
         if (!ones) {
             W::load_four(sc.k, scale, kq);
+            lev = __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE));
+            if (!Q8 && lev == W::NO_LEVEL) kind = second ? SMALL : LARGE;
 #pragma unroll
             for (int x = 0; x < N; ++x) W::by_scale(s[x], sc);
         }
         auto vf = [&](int dt, int sp) { return *(const v8h*)(buf + VB + ((dt * 2 + sp) * 64 + lane) * 16); };
 #pragma unroll
         for (int x = 0; x < N; ++x) {
-            const bool whole = !kinds.both() && p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
-            if (!ones) W::load_four(sc.v, scale + (whole ? 2 : 1) * FTX_PAGE, kq);
-            const int pe = whole ? __builtin_amdgcn_readfirstlane(*(const int*)(scale + 3 * FTX_PAGE)) : W::NO_LEVEL;
+            const bool whole = p0 + FTX_PAGE - 1 <= hi[x] && (p0 >= lo[x] || p0 + FTX_PAGE <= a.sinks);
+            const bool leveled = whole && (Q8 || kind == ALL);
+            if (!ones) W::load_four(sc.v, scale + (leveled ? 2 : 1) * FTX_PAGE, kq);
+            const int pe = leveled ? lev : W::NO_LEVEL;
             uint64_t sight = 0;
-            if (!whole) sight = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0) & kinds.part(second);
-            wa[x].soften(s[x], sc, ones, whole, pe, kinds.small(second), sight, kq, ph[x], pl[x]);
+            if (!whole) sight = RowSight(a, sq, min(row_of(x), R - 1) / a.gqa).page(p0);
+            wa[x].soften(s[x], sc, ones, whole, pe, kind, sight, kq, ph[x], pl[x]);
         }
         staged_outputs<N>(wa, vf, ph, pl);
-        return kinds.both() && !second;
+        return !Q8 && kind == LARGE;
     };
     commit(0);
     auto pages = [&](auto tiles) {
@@ -1041,8 +1046,10 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's direct copies of page j
             __syncthreads();                     // every wave's; the other buffer is free
             if (j + 1 < n) stage(j + 1);
-            if (live && place(j) * FTX_PAGE <= last)
+            if (live && place(j) * FTX_PAGE <= last) {
+#pragma clang loop unroll(disable)
                 for (bool second = false; work(tiles, j, second);) second = true;
+            }
             if (j + 1 < n) commit(j + 1);
         }
     };

@@ -67,10 +67,11 @@ __device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4)
 
 // ---------------------------------------------------------------- write
 // q = round(127 x / a) + 128 with scale a / 127, or half(x 2^-e) with scale 2^e,
-// a the row's largest magnitude.  Bound by HBM: 4 bytes read for one or two
-// written.  2000 tokens of 8 heads of 128, 8-bit: 8.0 us (2.6 TB/s; the bytes
-// alone are 4.2 at a copy's rate, a launch that does nothing 2); a kernel
-// without the image in LDS, its values written a row apart, took 24.
+// a the row's largest magnitude.  4 bytes read for one or two written; 2000
+// tokens of 8 heads of 128, 8-bit: 8.0 us, where the bytes take 4.2 at a copy's
+// rate and a launch that does nothing 2: bound by the latency of a workgroup's
+// one pass, load, maximum, LDS, barrier and store.  A kernel without the image
+// in LDS, its values written a row apart, took 24.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
@@ -882,9 +883,11 @@ typedef __attribute__((address_space(3))) void lds_void;
 // current page's work and written after it.
 // Bound by the SIMDs' issue: queries and weights in two halves make it two
 // products of 16x16x32 for each of the formula's, 16 cycles each; three chunks
-// of 1500 tokens after 1600 to 4000 (8-bit, 128 dims) take 551 us, the CUs
-// busy for 88% of it, in that time products for 47% and other vector
-// instructions for 43% of the SIMDs' cycles.  One tile a wave reads twice the
+// of 1500 tokens after 1600 to 4000 (8-bit, 128 dims) take 467 us call after
+// call, the CUs busy for 88% of it, in that time products for 48% and other
+// vector instructions for 45% of the SIMDs' cycles (a wave's products run beside
+// another's vector instructions in part).  On the lower clock of a trace, where
+// the kernel takes 539 and took 557: one tile a wave reads twice the
 // LDS for a product: 656 us, LDS as busy as the products.  Tried and slower:
 // both tiles' low halves in registers (73 spilled, 680), the waves' halves kept
 // in antiphase, scores beside softmax (690), 64 rows a workgroup (686).

@@ -190,7 +190,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     // us, for sequences x pages (one token, 8-bit 128 dims, 8 kv heads): 1 x 7 8.8 /
     // 9.9, 1 x 17 11.6 / 10.0, 8 x 12 10.1 / 10.5, 8 x 22 14.7 / 12.4, 16 x 46
     // 23.8 / 27.5, 32 x 17 16.7 / 22.7; 64 dims: 1 x 12 7.2 / 8.8, 8 x 17 8.9 /
-    // 8.8, 16 x 46 17.2 / 17.9.
+    // 8.8, 16 x 46 17.2 / 17.9.  Halves, of twice the bytes a page, go by the same rule.
     struct Few {
         bool wide;
         int64_t per;

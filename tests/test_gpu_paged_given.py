@@ -97,3 +97,39 @@ def test_pools_past_64_bits_are_refused(gctx):
         refused(-4, gctx.pool, layers, kv, 256, pages, F16)
     refused(-4, gctx.pool, 65535, 1024, 256, 1 << 24, F16)
     gctx.pool(3, 2, 256, 5, F16).free()
+
+
+@KINDS
+@pytest.mark.parametrize("window", [0, 70])
+def test_a_refused_write_leaves_the_cache_as_it_was(gctx, setup, window):
+    """A write that its plan refuses (the stream is being captured): the cache's
+    rows, length and pages, and the pool's, are those before."""
+    import ctypes
+
+    from test_zz_no_alloc import _hip
+
+    hip = _hip()
+    kv = setup.gm.kv_paged(setup.pool, 250, window=window)
+    setup.kvs.append(kv)
+    for n in (100, 60):
+        setup.step([(kv, [(7 * i) % 300 for i in range(n)], None, True)])
+    before, free = kv.read(), setup.pool.available
+    rows = np.full((2,) + kv.shape, 3.0, np.float32)
+    st, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(st)) == 0
+    gctx.set_stream(st.value)
+    try:
+        assert hip.hipStreamBeginCapture(st, 2) == 0
+        refused(-1, kv.write, *rows)
+        assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+    finally:
+        gctx.set_stream(None)
+        if graph.value:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+    assert setup.pool.available == free and kv.pointers()[2] == 160
+    for x, y in zip(kv.read(), before):
+        np.testing.assert_array_equal(x, y)
+    setup.step([(kv, [5], None, False)])
+    kv.write(*rows)
+    assert setup.pool.available == 0 and all((x != 0).all() for x in kv.read())

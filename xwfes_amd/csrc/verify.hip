@@ -1229,43 +1229,28 @@ static int kv_copy(ftx_kv* kv, void* kh, void* vh, bool to_device) {
     return FTX_OK;
 }
 
-// The same for a paged cache and fp32 arrays: its held positions, a layer at a
-// time through the workspace and the pool's plan
-static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
+// The same for a paged cache and fp32 arrays: the first n positions of `table`
+// where it holds a page, a layer at a time through the workspace and the
+// pool's plan
+static int kv_copy_pages(ftx_kv* kv, const std::vector<int32_t>& table, int64_t n, float* kh, float* vh,
+                         bool to_device) {
     ftx_ctx* ctx = kv->ctx;
-    if (to_device) {
-        // (a dropped page is held again; too few pages: the cache stays as it is)
-        const int64_t need = (kv->cap + FTX_PAGE - 1) / FTX_PAGE;
-        int64_t held = 0;
-        for (int32_t pg : kv->pages) held += pg >= 0;
-        if (need > held + kv->pool->free_pages)
-            return ftx_fail(ctx, FTX_E_NOMEM, "kv_write: not enough free pages");
-        kv_drop(kv, 0, (int64_t)kv->pages.size());
-        kv->pages.clear();
-        kv->given = 0;
-        if (const int rc = kv_grow(kv, kv->cap)) return rc;
-    }
-    const int64_t kdim = kv->kdim, n = to_device ? kv->cap : kv->given;
-    const size_t bytes = (size_t)(n * kdim) * sizeof(float);
-    if (!to_device) {
-        memset(kh, 0, (size_t)(kv->n_layer * kv->cap * kdim) * sizeof(float));
-        memset(vh, 0, (size_t)(kv->n_layer * kv->cap * kdim) * sizeof(float));
-    }
     if (n == 0) return FTX_OK;
+    const int64_t kdim = kv->kdim;
     float* ws;
-    if (const int rc = ftx_workspace(ctx, 2 * bytes, (void**)&ws)) return rc;
+    if (const int rc = ftx_workspace(ctx, 2 * (size_t)(n * kdim) * sizeof(float), (void**)&ws)) return rc;
     hipStream_t st = ctx->stream;
     // runs of held pages, each as a sequence of its own
     const int64_t n_pages = (n + FTX_PAGE - 1) / FTX_PAGE;
     for (int64_t p0 = 0; p0 < n_pages;) {
-        if (kv->pages[(size_t)p0] < 0) {
+        if (table[(size_t)p0] < 0) {
             ++p0;
             continue;
         }
         int64_t p1 = p0;
-        while (p1 < n_pages && kv->pages[(size_t)p1] >= 0) ++p1;
+        while (p1 < n_pages && table[(size_t)p1] >= 0) ++p1;
         const int64_t r0 = p0 * FTX_PAGE, rows = std::min(p1 * FTX_PAGE, n) - r0;
-        const ftx_paged_seq seq{kv->pages.data() + p0, p1 - p0, 0, rows, nullptr};
+        const ftx_paged_seq seq{table.data() + p0, p1 - p0, 0, rows, nullptr};
         const ftx_plan_args pa{&seq, 1, 0, 0, 0};
         ftx_plan* plan;
         int rc = paged_step_plan(ctx, kv->pool, pa, &plan);
@@ -1288,19 +1273,53 @@ static int kv_copy_paged(ftx_kv* kv, float* kh, float* vh, bool to_device) {
         p0 = p1;
     }
     FTX_HIP(ctx, hipStreamSynchronize(st));
-    if (to_device) kv->given = n;
+    return FTX_OK;
+}
+
+static int kv_read_paged(ftx_kv* kv, float* kh, float* vh) {
+    const size_t bytes = (size_t)(kv->n_layer * kv->cap * kv->kdim) * sizeof(float);
+    memset(kh, 0, bytes);
+    memset(vh, 0, bytes);
+    return kv_copy_pages(kv, kv->pages, kv->given, kh, vh, false);
+}
+
+// Pages for all of cap: those held, and fresh ones elsewhere (for dropped ones
+// too), which go back when the call fails
+static int kv_write_paged(ftx_kv* kv, float* kh, float* vh) {
+    ftx_pool* p = kv->pool;
+    const size_t need = (size_t)((kv->cap + FTX_PAGE - 1) / FTX_PAGE);
+    std::vector<int32_t> table, fresh;
+    try {
+        table = kv->pages;
+        table.resize(need, -1);
+        fresh.resize((size_t)std::count(table.begin(), table.end(), -1));
+    } catch (...) {
+        return ftx_fail(kv->ctx, FTX_E_NOMEM, "host allocation failed");
+    }
+    int rc = ftx_pool_take(p, (int64_t)fresh.size(), fresh.data());
+    if (rc) return rc;
+    size_t used = 0;
+    for (int32_t& pg : table)
+        if (pg < 0) pg = fresh[used++];
+    rc = kv_copy_pages(kv, table, kv->cap, kh, vh, true);
+    if (rc) {
+        (void)ftx_pool_give(p, fresh.data(), (int64_t)fresh.size());
+        return rc;
+    }
+    kv->pages.swap(table);
+    kv->given = kv->cap;
     return FTX_OK;
 }
 
 int ftx_kv_write(ftx_kv* kv, const void* k, const void* v) {
     if (!kv || !k || !v) return FTX_E_INVALID;
-    if (kv->pool) return kv_copy_paged(kv, (float*)k, (float*)v, true);
+    if (kv->pool) return kv_write_paged(kv, (float*)k, (float*)v);
     return kv_copy(kv, (void*)k, (void*)v, true);
 }
 
 int ftx_kv_read(ftx_kv* kv, void* k, void* v) {
     if (!kv || !k || !v) return FTX_E_INVALID;
-    if (kv->pool) return kv_copy_paged(kv, (float*)k, (float*)v, false);
+    if (kv->pool) return kv_read_paged(kv, (float*)k, (float*)v);
     return kv_copy(kv, k, v, false);
 }
 

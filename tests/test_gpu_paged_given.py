@@ -133,3 +133,36 @@ def test_a_refused_write_leaves_the_cache_as_it_was(gctx, setup, window):
     setup.step([(kv, [5], None, False)])
     kv.write(*rows)
     assert setup.pool.available == 0 and all((x != 0).all() for x in kv.read())
+
+
+@KINDS
+@pytest.mark.parametrize("M", [1, 30])
+def test_a_step_that_its_plan_refuses_takes_no_pages(gctx, setup, M):
+    import ctypes
+
+    from test_zz_no_alloc import _hip
+
+    hip = _hip()
+    kv = setup.gm.kv_paged(setup.pool, 200)
+    setup.kvs.append(kv)
+    setup.step([(kv, [1] * 64, None, True)])
+    before = kv.read()
+    buf = gctx.buffer(M * CFG64["vocab"] * 4)
+    st, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(st)) == 0
+    gctx.set_stream(st.value)
+    try:
+        assert hip.hipStreamBeginCapture(st, 2) == 0
+        refused(-1, setup.gm.verify, kv, [2] * M, buf.ptr)
+        assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+    finally:
+        gctx.set_stream(None)
+        if graph.value:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+    assert setup.pool.available == 3 and kv.pointers()[2] == 64
+    for x, y in zip(kv.read(), before):
+        np.testing.assert_array_equal(x, y)
+    setup.step([(kv, [2] * M, None, True)])
+    assert setup.pool.available == 2
+    buf.free()

@@ -184,20 +184,22 @@ static int step_pages(ftx_ctx* ctx, int64_t n_head, const ftx_seq_args* sq, int6
     }
     ftx_paged_seq ps[FTX_MAX_SEQ];
     size_t had[FTX_MAX_SEQ];
-    for (int64_t s = 0; s < nseq; ++s) {
-        ftx_kv* kv = sq[s].kv;
-        had[s] = kv->pages.size();
-        if (const int rc = kv_grow(kv, kv->npast + sq[s].M)) {
-            // (the others' too)
-            for (int64_t r = 0; r < s; ++r) {
-                kv_drop(sq[r].kv, (int64_t)had[r], (int64_t)sq[r].kv->pages.size());
-                sq[r].kv->pages.resize(had[r]);
-            }
-            return rc;
-        }
-        ps[s] = ftx_paged_seq{kv->pages.data(), (int64_t)kv->pages.size(), kv->npast, sq[s].M, sq[s].parents};
+    int64_t grown = 0;
+    int rc = FTX_OK;
+    for (; grown < nseq && !rc; ++grown) {
+        ftx_kv* kv = sq[grown].kv;
+        had[grown] = kv->pages.size();
+        rc = kv_grow(kv, kv->npast + sq[grown].M);
+        ps[grown] =
+            ftx_paged_seq{kv->pages.data(), (int64_t)kv->pages.size(), kv->npast, sq[grown].M, sq[grown].parents};
     }
-    return paged_step_plan(ctx, k0->pool, ftx_plan_args{ps, nseq, n_head, k0->window, k0->sinks}, plan);
+    if (!rc) rc = paged_step_plan(ctx, k0->pool, ftx_plan_args{ps, nseq, n_head, k0->window, k0->sinks}, plan);
+    // (a step that does not run takes no pages)
+    for (int64_t r = 0; rc && r < grown; ++r) {
+        kv_drop(sq[r].kv, (int64_t)had[r], (int64_t)sq[r].kv->pages.size());
+        sq[r].kv->pages.resize(had[r]);
+    }
+    return rc;
 }
 
 static void model_release(ftx_model* m) {

@@ -166,3 +166,19 @@ def test_a_step_that_its_plan_refuses_takes_no_pages(gctx, setup, M):
     setup.step([(kv, [2] * M, None, True)])
     assert setup.pool.available == 2
     buf.free()
+
+
+@KINDS
+def test_one_window_over_caches_of_two_sizes(setup):
+    """More first tokens than one cache can hold: one window, sinks and step."""
+    a, b = (setup.gm.kv_paged(setup.pool, cap, window=8, sinks=100) for cap in (40, 150))
+    whole = setup.gm.kv_paged(setup.pool, 40)
+    setup.kvs += [a, b, whole]
+    toks = list(range(30))
+    got = setup.step([(a, toks, None, True), (b, toks, None, True)])
+    np.testing.assert_array_equal(got[0], got[1])
+    # every position is one of the first 100: no window
+    np.testing.assert_array_equal(setup.step([(whole, toks, None, True), ])[0], got[0])
+    far = setup.gm.kv_paged(setup.pool, 150, window=8, sinks=1 << 40)
+    setup.kvs.append(far)
+    np.testing.assert_array_equal(setup.step([(far, toks, None, True)])[0], got[0])

@@ -1174,7 +1174,8 @@ int ftx_kv_create_paged(ftx_ctx* ctx, const ftx_model* m, ftx_pool* p, int64_t c
     kv->kv_f16 = !p->q8;
     kv->pool = p;
     kv->window = window;
-    kv->sinks = window ? std::min(sinks, cap) : 0;
+    // (positions stay below 2^30; not cut to cap, which caches of one step need not share)
+    kv->sinks = window ? std::min(sinks, (int64_t)1 << 30) : 0;
     ++p->users;
     *out = kv;
     return FTX_OK;

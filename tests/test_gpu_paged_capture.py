@@ -6,7 +6,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from test_gpu_paged import Q8, TYPES, Cache, Rows, queries
+from test_gpu_paged import Q8, TYPES, Cache, Rows, queries, refused
 from test_zz_no_alloc import _hip
 
 pytestmark = pytest.mark.gpu
@@ -66,3 +66,32 @@ def test_set_and_captured_on_one_stream_launched_on_another(gctx, kvt, mode):
         x.buf.free()
     c.free()
     busy.free()
+
+
+def test_refused_calls_of_a_capture_leave_the_plan_free(gctx):
+    """A plan none of whose calls was recorded can be set again."""
+    hip = _hip()
+    c = Cache(gctx, np.random.default_rng(34), Q8, 64, 1, 2, [(70, 5)])
+    c.write_new()
+    far = c.pool.plan([([-1, c.tables[0][1]], 70, 5)], 2, 3)
+    m = Rows(gctx, np.zeros((5, 4 * 128)))
+    st, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamCreate(ctypes.byref(st)) == 0
+    gctx.set_stream(st.value)
+    try:
+        assert hip.hipStreamBeginCapture(st, 2) == 0
+        refused(-1, c.plan.attend, 0, m.ptr, m.ptr)
+        refused(-1, c.plan.read, 0, m.ptr, m.ptr)
+        refused(-5, far.read, 0, m.ptr, m.ptr + 4 * 256, True, 512, 512)
+        assert hip.hipStreamEndCapture(st, ctypes.byref(graph)) == 0
+    finally:
+        gctx.set_stream(None)
+        if graph.value:
+            hip.hipGraphDestroy(graph)
+        hip.hipStreamDestroy(st)
+    c.plan.set(c.seqs, 2)
+    far.set(c.seqs, 2)
+    c.check(queries(np.random.default_rng(35), c))
+    m.buf.free()
+    far.free()
+    c.free()

@@ -528,14 +528,15 @@ static hipError_t tables_landed(const ftx_plan* pl) {
 // the tables' copy ahead of a call on another stream than its own, and of a
 // captured one on any: the copy is not in the graph, which may be launched on
 // another stream than the captured one, so the host waits
-static int plan_order(ftx_plan* pl, bool captures) {
+static int plan_order(ftx_plan* pl) {
     ftx_ctx* ctx = pl->ctx;
-    if (!captures) {
+    if (!capturing(ctx->stream)) {
         if (ctx->stream == pl->stream) return FTX_OK;
         FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
         pl->stream = ctx->stream;
         return FTX_OK;
     }
+    pl->captured = true;
     if (pl->landed) return FTX_OK;
     OnDevice od(ctx->device);
     hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
@@ -552,7 +553,7 @@ static int plan_order(ftx_plan* pl, bool captures) {
     return FTX_OK;
 }
 
-// what every call of a plan checks; *ld: 0 becomes `width`
+// what every call of a plan checks, before plan_order; *ld: 0 becomes `width`
 static int plan_call(ftx_plan* pl, int64_t layer, const void* x, int64_t* ldx, int64_t xw, const void* y,
                      int64_t* ldy, int64_t yw) {
     ftx_ctx* ctx = pl->ctx;
@@ -565,9 +566,7 @@ static int plan_call(ftx_plan* pl, int64_t layer, const void* x, int64_t* ldx, i
     if (((uintptr_t)x | (uintptr_t)y) & 3) return ftx_fail(ctx, FTX_E_INVALID, "rows must be 4-byte aligned");
     if (!on_device(ctx, x) || !on_device(ctx, y))
         return ftx_fail(ctx, FTX_E_INVALID, "rows must be memory of the context's device");
-    const bool captures = capturing(ctx->stream);
-    if (captures) pl->captured = true;
-    return plan_order(pl, captures);
+    return FTX_OK;
 }
 
 // whether n rows of w floats, ldx and ldy apart, at x and y share a float
@@ -718,7 +717,8 @@ int ftx_paged_write(ftx_plan* pl, int64_t layer, const float* k, int64_t ldk, co
     if (!pl) return FTX_E_INVALID;
     const int64_t w = pl->pool->n_kv * pl->pool->hd;
     if (pl->ready && pl->t.tokens == 0) return FTX_OK;
-    const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
+    int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
+    if (!rc) rc = plan_order(pl);
     return rc ? rc : paged_write_rows(pl, layer, k, ldk, v, ldv);
 }
 
@@ -727,13 +727,14 @@ int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t l
     const int64_t w = pl->pool->n_kv * pl->pool->hd;
     const int64_t n = context ? pl->t.rows : pl->t.tokens;
     if (pl->ready && n == 0) return FTX_OK;
-    const int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
+    int rc = plan_call(pl, layer, k, &ldk, w, v, &ldv, w);
     if (rc) return rc;
     if (context && !paged_grid_fits(pl->t.max_pages * 2 * pl->pool->n_kv, 256))
         return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: too many positions of one sequence");
     if (context && pl->t.absent) return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: a page is absent");
     if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_read: k and v overlap");
-    return paged_read_rows(pl, layer, context, k, ldk, v, ldv);
+    rc = plan_order(pl);
+    return rc ? rc : paged_read_rows(pl, layer, context, k, ldk, v, ldv);
 }
 
 int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out, int64_t ldo) {
@@ -741,11 +742,12 @@ int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq
     if (pl->ready && pl->t.n_head == 0) return ftx_fail(pl->ctx, FTX_E_INVALID, "the plan has no query heads");
     if (pl->ready && pl->t.tokens == 0) return FTX_OK;
     const int64_t w = pl->t.n_head * pl->pool->hd;
-    const int rc = plan_call(pl, layer, q, &ldq, w, out, &ldo, w);
+    int rc = plan_call(pl, layer, q, &ldq, w, out, &ldo, w);
     if (rc) return rc;
     if (rows_overlap(q, ldq, out, ldo, w, pl->t.tokens))
         return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_attention: q and out overlap");
-    return paged_attend_rows(pl, layer, q, ldq, out, ldo);
+    rc = plan_order(pl);
+    return rc ? rc : paged_attend_rows(pl, layer, q, ldq, out, ldo);
 }
 
 }  // extern "C"

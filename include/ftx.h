@@ -431,12 +431,13 @@ int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t l
 /* out[n][h] = sum_j softmax_j(q[n][h] . k_j / sqrt(head_dim)) v_j over the
  * slots that new token n sees (its own among them: ftx_paged_write first), kv
  * head h / (n_head / n_head_kv).  q, out: [sum of M][n_head * head_dim], not
- * overlapping.  Error against 64 bits some 2^-21 of sum_j p_j |v_j|, at most
- * 2^-20 of it more for each page seen, plus up to 2^-32 of the largest |v_j|
- * seen for each slot seen.  A score past fp32,
- * or of a k row from 2^112 up, may make its row NaN.  What a token does not
- * see does not change its rows by a bit.  Rows past the last token stay as they
- * are. */
+ * overlapping.  Error against 64 bits: a score's is some 2^-22, at most 2^-18,
+ * of sum_i |q_i k_ji| / sqrt(head_dim) and moves its weight by as much; beside
+ * that some 2^-21 of sum_j p_j |v_j|, at most 2^-20 of it more for each page
+ * seen, and up to 2^-32 of the largest |v_j| seen for each slot seen.  A score
+ * past fp32, or of a k row from 2^112 up, may make its row NaN.  What a token
+ * does not see does not change its rows by a bit.  Rows past the last token
+ * stay as they are. */
 int ftx_paged_attention(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, float* out,
                         int64_t ldo);
 

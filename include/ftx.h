@@ -76,8 +76,8 @@ enum {
     FTX_BF16 = 30
 };
 
-/* KV element types (FTX_KV_Q8: paged caches only) */
-enum { FTX_KV_F32 = 0, FTX_KV_F16 = 1, FTX_KV_Q8 = 2 };
+/* KV element types (FTX_KV_Q8, FTX_KV_Q4: paged caches only) */
+enum { FTX_KV_F32 = 0, FTX_KV_F16 = 1, FTX_KV_Q8 = 2, FTX_KV_Q4 = 3 };
 
 /* acceptance modes */
 enum {
@@ -362,11 +362,19 @@ int ftx_argmax_prob(ftx_ctx* ctx, const float* row, int64_t V, int32_t* token, f
  *               keep 11 bits)
  *   FTX_KV_Q8   q s with the scale s = float(a / 127) and q = 127 x / a
  *               rounded to the nearest integer, ties to even
- * A row with a < 2^-100 is stored as zeros; one that holds an infinity or a
- * NaN is NaN in every element. */
+ *   FTX_KV_Q4   float((q c) s), c one integer (0 .. 255) for each block of 32
+ *               dims and s one scale: in fp32, every operation rounded to
+ *               nearest (ties to even), t the block's largest of max(x, 0)
+ *               (1/7) (the float next to 1/7) and max(-x, 0) / 8, T the row's
+ *               largest t: s = T / 255, c = min(255, ceil(t (255 / T))),
+ *               q = x (1 / (c s)) to the nearest integer, ties to even, -8 .. 7
+ *               (0 where c is).  |q c| is at most 2040; head_dim / 2 +
+ *               head_dim / 32 + 4 bytes a row
+ * A row with a < 2^-100 (FTX_KV_Q4: T < 2^-103) is stored as zeros; one that
+ * holds an infinity or a NaN is NaN in every element. */
 enum { FTX_PAGE = 64 };
 /* n_pages (<= 2^24) pages for n_layer layers of n_head_kv heads; head_dim 64,
- * 128 or 256; kv_dtype FTX_KV_F16 or FTX_KV_Q8. */
+ * 128 or 256; kv_dtype FTX_KV_F16, FTX_KV_Q8 or FTX_KV_Q4. */
 int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t head_dim,
                     int64_t n_pages, int kv_dtype, ftx_pool** out);
 /* Frees the pool; FTX_E_INVALID while a plan or a paged cache of it lives. */

@@ -1,0 +1,319 @@
+"""Paged KV caches in 4 bits on the GPU: the stores bit for bit, and attention by
+the bounds of 8-bit rows (test_gpu_paged.py): what a row stands for is an integer
+of up to 2040, exact as a half, times one fp32 scale, as it is there.  The last
+term of the bound, up to 2^-34 of the largest |v| for each slot seen, counts the
+weights' lost low halves in values of the row's largest: here that is at least
+7 * 255 = 1785 of 2040 steps, so the largest |v| stands for any value but for a
+factor of 1.15, which the bound's own factor of two covers.
+"""
+import numpy as np
+import pytest
+
+import test_gpu_paged as P
+import test_gpu_paged_extremes
+import test_gpu_paged_levels
+import test_gpu_paged_long
+import test_gpu_paged_scores
+import test_gpu_paged_steps as S
+import test_gpu_paged_strides
+from test_gpu_paged import TILES, Cache, Rows, queries, tiles  # noqa: F401
+from xwfes_amd import ftx
+
+pytestmark = pytest.mark.gpu
+
+Q4 = ftx.KV_Q4
+F = np.float32
+
+
+def stored4(x, kvt=Q4):
+    """What rows [..., hd] stand for once stored, every operation rounded to fp32."""
+    assert kvt == Q4
+    x = np.asarray(x, F)
+    with np.errstate(all="ignore"):
+        b = x.reshape(x.shape[:-1] + (x.shape[-1] // 32, 32))
+        t = np.maximum(np.maximum(b, F(0)) * (F(1) / F(7)), np.maximum(-b, F(0)) / F(8)).max(-1)
+        T = t.max(-1, keepdims=True)
+        bad = ~np.isfinite(x).all(-1, keepdims=True)
+        none = bad | (T < 2.0 ** -103)
+        T = np.where(none, F(1), T).astype(F)
+        s = T / F(255)
+        c = np.minimum(np.ceil(t * (F(255) / T)), F(255))
+        r = F(1) / (c * s)
+        q = np.rint(b * r[..., None])
+        q = np.where((c > 0)[..., None], q, F(0))
+        assert none.any() or not q.size or (q.min() >= -8 and q.max() <= 7)
+        y = ((q * c[..., None]).reshape(x.shape) * s).astype(F)
+    return np.where(bad, F(np.nan), np.where(none, F(0), y)).astype(F)
+
+
+@pytest.fixture(autouse=True)
+def in_4_bits(monkeypatch):
+    for m in (P, test_gpu_paged_extremes, test_gpu_paged_levels, test_gpu_paged_long, test_gpu_paged_scores):
+        if hasattr(m, "stored"):
+            monkeypatch.setattr(m, "stored", stored4)
+
+
+def params(f, n=0):
+    """The cases of a test of the other types: its n-th parametrisation but the types'."""
+    marks = [m for m in f.pytestmark if m.name == "parametrize" and m.args[0] != "kvt"]
+    return pytest.mark.parametrize(marks[n].args[0], marks[n].args[1])
+
+
+# ---------------------------------------------------------------- stores
+
+
+@params(P.test_rows_come_back_as_they_are_stored)
+def test_rows_come_back_as_they_are_stored(gctx, hd, kv, seqs, pad, off):
+    P.test_rows_come_back_as_they_are_stored(gctx, Q4, hd, kv, seqs, pad, off)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("M", [1, 14, 90])
+def test_rows_of_every_size(gctx, hd, M):
+    """Zero, tiny, subnormal, huge and mixed rows; blocks far apart in size; values at the
+    borders of the rounding and their neighbours; rows that hold an infinity or a NaN.
+    Row by row and page by page."""
+    rng = np.random.default_rng(hd)
+    base = rng.standard_normal(hd).astype(F)
+    rows = [base * F(f) for f in (0, 2.0 ** -105, 2.0 ** -100, 2.0 ** -98, 1e-42, 1e30, 1.0, 1e-7)]
+    big = base / np.abs(base).max()
+    rows += [big * F(3.4e38), -big * F(3.4e38), np.abs(big), -np.abs(big)]
+    # T on both sides of 2^-103
+    for sign, most in ((1, 7), (-1, 8)):
+        for e in (0.99, 1.0, 1.01):
+            y = np.zeros(hd, F)
+            y[hd - 1] = F(sign * most * e * 2.0 ** -103)
+            rows.append(y)
+    # blocks from one end of the multipliers to the other, and below
+    y = base.copy()
+    for g in range(hd // 32):
+        y[32 * g:32 * g + 32] *= F(10.0 ** (-2 * g))
+    rows += [y, y[::-1].copy(), -y]
+    only = np.zeros(hd, F)
+    only[hd // 2 + 3] = -5
+    rows.append(only)
+    # every border of the rounding, n + 1/2 steps, and its neighbours
+    for step in (1.0, 0.37, 1e-3):
+        n = (np.arange(hd) % 15) - 7.5
+        y = (n * step).astype(F)
+        y[::32], y[1::32] = F(7 * step), F(-8 * step)
+        rows += [y, np.nextafter(y, F(np.inf)), np.nextafter(y, F(-np.inf))]
+    for bad in (np.inf, -np.inf, np.nan):
+        y = base.copy()
+        y[hd - 9] = bad
+        rows.append(y)
+    x = np.stack(rows).astype(F)[:, None, :]
+    x = np.concatenate([x] * (M // len(x) + 1))
+    for at in range(0, len(x), M):
+        part = x[at:at + M]
+        n = len(part)
+        c = Cache(gctx, rng, Q4, hd, 1, 0, [(7, n)],
+                  rows=([np.concatenate([x[:7], part])], [np.concatenate([x[:7], -part])]))
+        c.write_new()
+        for got, s in zip(c.read(), (1, -1)):
+            np.testing.assert_array_equal(got, stored4(s * part))
+        for got, s in zip(c.read(context=True), (1, -1)):
+            np.testing.assert_array_equal(got, stored4(np.concatenate([x[:7], s * part])))
+        c.free()
+
+
+def test_a_page_filled_token_by_token(gctx):
+    """Every token's bytes are its own: tokens one at a time and several at once into the
+    same page, others' rows as they were."""
+    rng = np.random.default_rng(31)
+    x = [rng.standard_normal((64, 2, 128)).astype(F) for _ in range(2)]
+    pool = gctx.pool(1, 2, 128, 1, Q4)
+    pages = pool.take(1)
+    c = Cache.__new__(Cache)
+    c.ctx, c.kvt, c.hd, c.kv, c.heads, c.layer, c.pool = gctx, Q4, 128, 2, 0, 0, pool
+    at = 0
+    for n in (1, 2, 1, 7, 15, 1, 20, 17):
+        plan = pool.plan([(pages, at, n)])
+        c.write(plan, [x[0][at:at + n]], [x[1][at:at + n]])
+        at += n
+        for got, y in zip(c.read(plan, context=True, n=at), x):
+            np.testing.assert_array_equal(got, stored4(y[:at]))
+        plan.free()
+    assert at == 64
+    pool.free()
+
+
+# ---------------------------------------------------------------- attention
+
+
+@TILES
+@params(P.test_chains)
+def test_chains(gctx, hd, kv, heads, seqs):
+    P.test_chains(gctx, Q4, hd, kv, heads, seqs)
+
+
+@TILES
+@params(P.test_windows)
+def test_windows(gctx, hd, kv, heads, seqs, window, sinks):
+    P.test_windows(gctx, Q4, hd, kv, heads, seqs, window, sinks)
+
+
+@TILES
+@params(P.test_trees)
+def test_trees(gctx, hd, kv, heads, seqs, window, sinks):
+    P.test_trees(gctx, Q4, hd, kv, heads, seqs, window, sinks)
+
+
+@TILES
+@params(P.test_values_of_every_size)
+def test_values_of_every_size(gctx, qs, ks, vs):
+    P.test_values_of_every_size(gctx, Q4, qs, ks, vs)
+
+
+@TILES
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("seqs,heads", [([(300, 1)], 4), ([(300, 3), (90, 1)], 2), ([(200, 9)], 8), ([(130, 40)], 2)])
+def test_blocks_of_every_size(gctx, hd, seqs, heads):
+    """Keys and values whose blocks of 32 dims lie far apart, rows far apart in size."""
+    rng = np.random.default_rng(hd + heads)
+    rows = []
+    for _ in range(2):
+        x = [rng.standard_normal((a + b, 1, hd)).astype(F) for a, b in seqs]
+        for y in x:
+            y *= np.repeat(F(10.0) ** rng.integers(-3, 1, (len(y), 1, hd // 32)), 32, -1).astype(F)
+            y *= F(10.0) ** rng.integers(-4, 2, (len(y), 1, 1)).astype(F)
+        rows.append(x)
+    c = Cache(gctx, rng, Q4, hd, 1, heads, seqs, rows=rows)
+    c.write_new()
+    c.check(queries(rng, c, 2.0))
+    c.free()
+
+
+@TILES
+def test_large_values_in_hidden_places_change_nothing(gctx):
+    P.test_large_values_in_hidden_places_change_nothing(gctx, Q4)
+
+
+@TILES
+def test_a_row_hidden_by_the_window(gctx):
+    P.test_a_row_hidden_by_the_window(gctx, Q4)
+
+
+@TILES
+def test_pages_that_held_other_things(gctx):
+    P.test_pages_that_held_other_things(gctx, Q4)
+
+
+@TILES
+@params(P.test_strides_and_alignment)
+def test_strides_and_alignment(gctx, pad, off):
+    P.test_strides_and_alignment(gctx, Q4, pad, off)
+
+
+@TILES
+def test_chunks_give_what_one_chunk_gives(gctx):
+    P.test_chunks_give_what_one_chunk_gives(gctx, Q4)
+
+
+@TILES
+def test_shared_prefix_pages(gctx):
+    P.test_shared_prefix_pages(gctx, Q4)
+
+
+def test_two_graphs_replayed(gctx):
+    P.test_two_graphs_replayed(gctx, Q4)
+
+
+@params(test_gpu_paged_strides.test_many_rows)
+def test_strides_of_many_rows(gctx, hd, kv, heads, seqs, rows):
+    test_gpu_paged_strides.test_many_rows(gctx, Q4, hd, kv, heads, seqs, rows)
+
+
+@params(test_gpu_paged_strides.test_joins)
+def test_joins(gctx, hd, kv, heads, seqs, rows, parts):
+    test_gpu_paged_strides.test_joins(gctx, Q4, hd, kv, heads, seqs, rows, parts)
+
+
+@params(test_gpu_paged_long.test_pages_past_the_first_64)
+def test_pages_past_the_first_64(gctx, M, rows):
+    test_gpu_paged_long.test_pages_past_the_first_64(gctx, Q4, M, rows)
+
+
+@params(test_gpu_paged_long.test_sums_of_alike_weights)
+def test_sums_of_alike_weights(gctx, M, rows):
+    test_gpu_paged_long.test_sums_of_alike_weights(gctx, Q4, M, rows)
+
+
+@TILES
+@params(test_gpu_paged_scores.test_scores_past_fp32_are_nan)
+def test_scores_past_fp32_are_nan(gctx, sign):
+    test_gpu_paged_scores.test_scores_past_fp32_are_nan(gctx, Q4, sign)
+
+
+def test_offsets_past_32_bits(gctx):
+    """A pool of 9.6 GB: the last pages of its last layer."""
+    rng = np.random.default_rng(19)
+    pages = 32600
+    pool = gctx.pool(4, 8, 128, pages, Q4)
+    ids = pool.take(pages)
+    c = Cache.__new__(Cache)
+    c.ctx, c.kvt, c.hd, c.kv, c.heads, c.window, c.sinks, c.layer, c.pool = gctx, Q4, 128, 8, 8, 0, 0, 3, pool
+    c.seqs, c.new = [(ids[-3:][::-1], 0, 150, None)], 150
+    c.k, c.v = ([rng.standard_normal((150, 8, 128)).astype(F)] for _ in range(2))
+    c.plan = pool.plan(c.seqs, 8)
+    c.write_new()
+    c.check(queries(rng, c))
+    c.free()
+
+
+# ---------------------------------------------------------------- verify steps
+
+
+@params(S.test_rows_of_a_step_are_stored_as_the_store_does)
+def test_rows_of_a_step_are_stored_as_the_store_does(gctx, orc, monkeypatch, cfg, neox, M):
+    monkeypatch.setattr(S, "stored", stored4)
+    S.test_rows_of_a_step_are_stored_as_the_store_does(gctx, orc, Q4, cfg, neox, M)
+
+
+def test_commit_of_a_tree_path(gctx, orc):
+    """A path's rows move to the next slots, across a page's end, byte for byte; the step
+    after it is the step after the chain of the path.
+
+    Projections of up to 8 tokens and of more differ by some 1e-4 of a row's size.  By that
+    one value in 1400 crosses its rounding (15 steps to four times the row's spread, 0.57 of
+    it a step): sqrt(1 / 1400) 0.57 = 1.5e-2.  One multiplier in 40 does (255 to T): its block
+    moves by up to 1/255 and one value in 60 of it with it: sqrt(1 / 40) (0.004 + sqrt(1 / 60)
+    0.57) = 1.2e-2.  Together 2e-2 of a row's size in the rows that differ, as a share of the
+    logits less, by the rows seen; 8-bit rows' 3e-3 are given 5 LOGIT_TOL."""
+    t = S.Setup(gctx, orc, S.CFG64, S.Q8, Q4)
+    toks = np.random.default_rng(3).integers(0, 300, 20).tolist()
+    par = [-1, -1, 0, 1, 2, 2, 3, 4, 5, 6, 7, 7, 8, 9, 10, 11, 12, 13, 14, 15]
+    path = [1, 3, 6, 9, 13, 17]
+    a, _, _ = t.context(60, 90)
+    b, _, _ = t.context(60, 90)
+    t.step([(a, toks, par, False)])
+    before = a.read()
+    a.commit(path)
+    for x, y in zip(before, a.read()):
+        np.testing.assert_array_equal(y[:, :60], x[:, :60])
+        np.testing.assert_array_equal(y[:, 60:66], x[:, [60 + j for j in path]])
+    t.step([(b, [toks[j] for j in path], None, True)])
+    assert a.pointers()[2] == b.pointers()[2] == 66
+    x, y = (t.step([(z, [7], None, True)])[0] for z in (a, b))
+    assert S.rel_err_rows(x, y) < 34 * S.LOGIT_TOL
+    t.free()
+
+
+def test_steps_near_those_of_halves(gctx, orc):
+    """Steps over 4-bit rows are steps over the rows that they stand for: a cache of halves
+    given those rows (they are within halves' reach) has the same logits, but for halves'
+    rounding of them and of the new rows that are kept in 4 bits here."""
+    t = S.Setup(gctx, orc, S.CFG64, S.Q8, Q4)
+    u = S.Setup(gctx, orc, S.CFG64, S.Q8, ftx.KV_F16)
+    kv, _, _ = t.context(200, 230)
+    k, v = kv.read()
+    half = u.gm.kv_paged(u.pool, 230)
+    u.kvs.append(half)
+    half.write(k, v)
+    half.truncate(200)
+    x, = t.step([(kv, [5], None, False)])
+    y, = u.step([(half, [5], None, False)])
+    # one new row of 201 in 4 bits: off by 0.08 of its size at most (a step of 0.27 of a block's
+    # spread, rounded evenly), a 201st part of what is seen, and halves' 2^-11 of every row
+    assert S.rel_err_rows(x, y) < 5 * S.LOGIT_TOL
+    t.free(), u.free()

@@ -329,8 +329,12 @@ __global__ void __launch_bounds__(64 * ROPE_HPW) k_rope_kv4(RopeBatch b) {
 // k_paged_write stores them): few tokens a sequence, whose store is then not a
 // launch of its own.  A step of one token over 2048
 // slots (8 layers of the 8B shape) 649 -> 633 us, of eight 667 -> 641.
-template <bool Q8>
+template <int KT>
 __global__ void __launch_bounds__(64 * ROPE_HPW) k_rope_paged(RopeBatch b, PagedView p) {
+    constexpr bool Q8 = KT == PT_Q8;
+    // 4-bit rows: a wave's k (v) row in the order of its dims, since their blocks
+    // and bytes are of other lanes' values
+    __shared__ float rows[KT == PT_Q4 ? ROPE_HPW : 1][KT == PT_Q4 ? 256 : 1];
     int s = 0;
     while (s + 1 < b.nseq && (int)blockIdx.x >= b.row0[s + 1]) ++s;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -340,18 +344,30 @@ __global__ void __launch_bounds__(64 * ROPE_HPW) k_rope_paged(RopeBatch b, Paged
                  [&](int64_t pos, int64_t kvh, const int64_t(&el)[2][2], const bool(&ok)[2], const float(&kept)[2][4]) {
         const int slot = (int)(pos % FTX_PAGE);
         uint8_t* blk = page_block(p, p.table[p.seqs[s].tab0 + pos / FTX_PAGE], (int)kvh);
-        const int64_t vb = paged_values_bytes(p.hd, Q8);
+        if constexpr (KT == PT_Q4) {
+            for (int v = 0; v < 2; ++v) {
+                // (one wave writes and reads its row: in order)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (ok[i >> 1]) rows[w][el[i >> 1][i & 1]] = kept[v][i];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                q4_store_row(blk, p.hd, slot, v, lane, [&](int d) { return rows[w][d]; });
+            }
+            return;
+        }
+        const int64_t vb = paged_values_bytes(p.hd, KT);
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
             const float* x = kept[v];
-            const RowForm<Q8> f(group_max<64>(max(max(mag(x[0]), mag(x[1])), max(mag(x[2]), mag(x[3])))));
+            const RowForm<KT> f(group_max<64>(max(max(mag(x[0]), mag(x[1])), max(mag(x[2]), mag(x[3])))));
             uint32_t bits[4];
             f.bits(kept[v], bits);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (!ok[i >> 1]) continue;
                 const int d = (int)el[i >> 1][i & 1];
-                uint8_t* t = blk + (v ? vb + paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8));
+                uint8_t* t = blk + (v ? vb + paged_v_at(slot, d, KT) : paged_k_at(slot, d, KT));
                 if constexpr (Q8)
                     *t = (uint8_t)bits[i];
                 else
@@ -425,7 +441,10 @@ hipError_t launch_rope_kv_batch(hipStream_t st, const RopeArgs* as, const int64_
     const dim3 grid4((unsigned)rows, (unsigned)((nh + ROPE_HPW - 1) / ROPE_HPW));
     if (pages && !regs) return hipErrorInvalidValue;
     if (pages)
-        hipLaunchKernelGGL(pages->q8 ? k_rope_paged<true> : k_rope_paged<false>, grid4, dim3(64 * ROPE_HPW), 0, st, b, *pages);
+        hipLaunchKernelGGL(pages->kt == PT_Q4   ? k_rope_paged<PT_Q4>
+                           : pages->kt == PT_Q8 ? k_rope_paged<PT_Q8>
+                                                : k_rope_paged<PT_F16>,
+                           grid4, dim3(64 * ROPE_HPW), 0, st, b, *pages);
     else if (regs)
         hipLaunchKernelGGL(k_rope_kv4, grid4, dim3(64 * ROPE_HPW), 0, st, b);
     else

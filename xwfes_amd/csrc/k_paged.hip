@@ -31,14 +31,16 @@ __device__ __forceinline__ void st4(float* p, v4f v, bool vec) {
 // that both sides of the copy are whole runs (32 lanes a row of 128 floats;
 // 16 bytes a thread of the page).
 struct PageRows {
+    uint8_t* blk;
     uint8_t* vals;  // the page's K or V values
     float* scale;
+    uint8_t* mult;  // (of 4-bit rows)
     int s0, s1;
     int64_t row;  // of slot 0 in the matrix (it may lie before its start)
     int col;      // the kv head's first float
     bool isv;
 };
-template <int HD, bool Q8>
+template <int HD, int KT>
 __device__ __forceinline__ PageRows page_rows(const PagedView& p, int context) {
     const PagedSeq sq = p.seqs[blockIdx.y];
     const int from = context ? 0 : sq.npast;
@@ -50,9 +52,10 @@ __device__ __forceinline__ PageRows page_rows(const PagedView& p, int context) {
     if (r.s0 >= r.s1) return r;
     const int kvh = z >> 1;
     r.isv = z & 1;
-    uint8_t* blk = page_block(p, p.table[sq.tab0 + first], kvh);
-    r.vals = blk + (r.isv ? paged_values_bytes(HD, Q8) : 0);
-    r.scale = (float*)(blk + 2 * paged_values_bytes(HD, Q8)) + (r.isv ? FTX_PAGE : 0);
+    r.blk = page_block(p, p.table[sq.tab0 + first], kvh);
+    r.vals = r.blk + (r.isv ? paged_values_bytes(HD, KT) : 0);
+    r.scale = (float*)(r.blk + 2 * paged_values_bytes(HD, KT)) + (r.isv ? FTX_PAGE : 0);
+    r.mult = r.blk + 2 * paged_values_bytes(HD, KT) + 2 * FTX_PAGE * 4 + (r.isv ? paged_mult_bytes(HD, KT) : 0);
     r.row = (int64_t)first * FTX_PAGE + (context ? sq.all0 : (int64_t)sq.tok0 - sq.npast);
     r.col = kvh * HD;
     return r;
@@ -72,19 +75,25 @@ __device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4)
 // rate and a launch that does nothing 2: bound by the latency of a workgroup's
 // one pass, load, maximum, LDS, barrier and store.  A kernel without the image
 // in LDS, its values written a row apart, took 24.
-template <int HD, bool Q8>
+template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
-    constexpr int E = HD / 64, D4 = HD / 4, EB = Q8 ? 1 : 2;
-    __shared__ uint4 img[HD * FTX_PAGE * EB / 16];
+    constexpr bool Q8 = KT == PT_Q8, Q4 = KT == PT_Q4;
+    constexpr int E = HD / 64, D4 = HD / 4, EB = Q8 ? 1 : 2, UNITS = paged_values_bytes(HD, KT) / 16;
+    __shared__ uint4 img[UNITS];
     __shared__ uint32_t amax[FTX_PAGE];
-    const PageRows pr = page_rows<HD, Q8>(p, 0);
+    __shared__ uint8_t mult[Q4 ? FTX_PAGE * HD / 32 : 1];
+    const PageRows pr = page_rows<HD, KT>(p, 0);
     if (pr.s0 >= pr.s1) return;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int64_t ld = pr.isv ? ldv : ldk;
     const float* src = (pr.isv ? v : k) + pr.row * ld + pr.col;
     if (pr.s1 - pr.s0 < ROWS_FEW) {
         for (int slot = pr.s0 + w; slot < pr.s1; slot += 4) {
+            if constexpr (Q4) {
+                q4_store_row(pr.blk, HD, slot, pr.isv, lane, [&](int d) { return src[slot * ld + d]; });
+                continue;
+            }
             float x[E];
             uint32_t a = 0;
 #pragma unroll
@@ -92,13 +101,13 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
                 x[e] = src[slot * ld + E * lane + e];
                 a = max(a, mag(x[e]));
             }
-            const RowForm<Q8> f(group_max<64>(a));
+            const RowForm<KT> f(group_max<64>(a));
             uint32_t b[E];
             f.bits(x, b);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int d = E * lane + e;
-                uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8));
+                uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, KT) : paged_k_at(slot, d, KT));
                 if constexpr (Q8)
                     *t = (uint8_t)b[e];
                 else
@@ -122,11 +131,46 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
             x[r] = slot >= pr.s0 && slot < pr.s1 ? ld4(src + slot * ld + d, vec) : v4f{0.f, 0.f, 0.f, 0.f};
         }
         uint32_t bits[4][4];
+        if constexpr (Q4) {
+            // (a block of 32 dims: eight threads)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                uint32_t t = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t = max(t, mag(q4_need(x[r][e])));
+                const uint32_t top = group_max<D4>(t);
+                const Q4Row f(top);
+                float by;
+                const int c = f.mult(group_max<8>(t), by);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bits[r][e] = f.bits(x[r][e], by);
+                if ((d & 31) == 0) mult[paged_c_at(4 * g + r, d >> 5)] = (uint8_t)c;
+                if (d == 0) amax[4 * g + r] = top;
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                // K: slot 4 g + r's eight dims about d, half of them the neighbour's;
+                // V: slots 4 g ..+3 of dim d + r and, from four threads on, d + r + 16
+                uint32_t word;
+                if (pr.isv) {
+                    word = (bits[0][r] | bits[1][r] << 16 | bits[2][r] << 8 | bits[3][r] << 24) << (d & 16 ? 4 : 0);
+                    word |= (uint32_t)__shfl_xor((int)word, 4, 64);
+                } else {
+                    word = (bits[r][0] | bits[r][1] << 16 | bits[r][2] << 4 | bits[r][3] << 20) << (d & 4 ? 8 : 0);
+                    word |= (uint32_t)__shfl_xor((int)word, 1, 64);
+                }
+                // (both threads of a word have it: each stores half of them)
+                if (pr.isv ? (r >> 1) == ((d >> 4) & 1) : (r >> 1) == ((d >> 2) & 1))
+                    *(uint32_t*)(im + (image_at(pr.isv ? paged_v_at(4 * g, d + r, KT) : paged_k_at(4 * g + r, d, KT)) &
+                                       ~3)) = word;
+            }
+            continue;
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const uint32_t a =
                 group_max<D4>(max(max(mag(x[r][0]), mag(x[r][1])), max(mag(x[r][2]), mag(x[r][3]))));
-            const RowForm<Q8> f(a);
+            const RowForm<Q4 ? PT_Q8 : KT> f(a);
             const float xr[4] = {x[r][0], x[r][1], x[r][2], x[r][3]};
             f.bits(xr, bits[r]);
             if (d == 0) amax[4 * g + r] = a;
@@ -137,7 +181,7 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
             uint32_t b[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) b[e] = pr.isv ? bits[e][r] : bits[r][e];
-            uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, Q8) : paged_k_at(4 * g + r, d, Q8));
+            uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, KT) : paged_k_at(4 * g + r, d, KT));
             if constexpr (Q8)
                 *(uint32_t*)t = __builtin_amdgcn_perm(__builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u),
                                                       __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), 0x05040100u);
@@ -146,11 +190,33 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
         }
     }
     __syncthreads();
-    if (tid >= pr.s0 && tid < pr.s1) pr.scale[tid] = RowForm<Q8>(amax[tid]).scale();
+    if constexpr (Q4) {
+        if (tid >= pr.s0 && tid < pr.s1) pr.scale[tid] = Q4Row(amax[tid]).scale();
+        for (int i = tid; i < FTX_PAGE * HD / 32; i += 256) {
+            const int slot = 16 * ((i >> 2) & 3) + 4 * ((i >> 4) & 3) + (i & 3);
+            if (slot >= pr.s0 && slot < pr.s1) pr.mult[i] = mult[i];
+        }
+    } else {
+        if (tid >= pr.s0 && tid < pr.s1) pr.scale[tid] = RowForm<KT>(amax[tid]).scale();
+    }
     const bool full = pr.s0 == 0 && pr.s1 == FTX_PAGE;
-    for (int u = tid; u < HD * FTX_PAGE * EB / 16; u += 256) {
+    for (int u = tid; u < UNITS; u += 256) {
         if (full) {
             ((uint4*)pr.vals)[u] = img[image_unit(u)];
+        } else if (Q4 && !pr.isv) {
+            // a unit holds two slots, 8 bytes each
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int slot = 16 * (2 * ((u >> 6) & 1) + x) + (u & 15);
+                if (slot >= pr.s0 && slot < pr.s1) ((uint2*)pr.vals)[2 * u + x] = ((const uint2*)img)[2 * image_unit(u) + x];
+            }
+        } else if (Q4) {
+            // 16: those of other tokens stay
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int slot = 16 * (x >> 2) + 4 * ((u >> 4) & 3) + ((x >> 1) & 1) + 2 * (x & 1);
+                if (slot >= pr.s0 && slot < pr.s1) pr.vals[u * 16 + x] = im[image_unit(u) * 16 + x];
+            }
         } else if (!pr.isv) {
             const int slot = 16 * ((u >> 6) & 3) + (u & 15);
             if (slot >= pr.s0 && slot < pr.s1) ((uint4*)pr.vals)[u] = img[image_unit(u)];
@@ -174,12 +240,13 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
 // x = (byte - 128) scale, or half scale.  Bound by HBM, mostly its writes: four
 // contexts of up to 16384 (57138 tokens in all, 8 heads of 128, 8-bit) 120 us,
 // 4.9 TB/s, a large copy's rate.
-template <int HD, bool Q8>
+template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, float* __restrict__ k, int64_t ldk,
                                                     float* __restrict__ v, int64_t ldv) {
-    constexpr int E = HD / 64, D4 = HD / 4, EB = Q8 ? 1 : 2;
-    __shared__ uint4 img[HD * FTX_PAGE * EB / 16];
-    const PageRows pr = page_rows<HD, Q8>(p, context);
+    constexpr bool Q8 = KT == PT_Q8, Q4 = KT == PT_Q4;
+    constexpr int E = HD / 64, D4 = HD / 4, UNITS = paged_values_bytes(HD, KT) / 16;
+    __shared__ uint4 img[UNITS];
+    const PageRows pr = page_rows<HD, KT>(p, context);
     if (pr.s0 >= pr.s1) return;
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
     const int64_t ld = pr.isv ? ldv : ldk;
@@ -190,14 +257,19 @@ __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, fl
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int d = E * lane + e;
-                const uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, Q8) : paged_k_at(slot, d, Q8));
+                const uint8_t* t = pr.vals + (pr.isv ? paged_v_at(slot, d, KT) : paged_k_at(slot, d, KT));
+                if constexpr (Q4) {
+                    const int n = (*t >> (d & (pr.isv ? 16 : 2) ? 4 : 0) & 15) - 8;
+                    dst[slot * ld + d] = (float)(n * (int)pr.mult[paged_c_at(slot, d >> 5)]) * sc;
+                    continue;
+                }
                 dst[slot * ld + d] = (Q8 ? (float)((int)*t - 128) : (float)*(const _Float16*)t) * sc;
             }
         }
         return;
     }
 #pragma unroll
-    for (int u = tid; u < HD * FTX_PAGE * EB / 16; u += 256) img[image_unit(u)] = ((const uint4*)pr.vals)[u];
+    for (int u = tid; u < UNITS; u += 256) img[image_unit(u)] = ((const uint4*)pr.vals)[u];
     __syncthreads();
     const bool vec = !(((uintptr_t)dst | (uintptr_t)(ld * 4)) & 15);
     const uint8_t* im = (const uint8_t*)img;
@@ -207,7 +279,18 @@ __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, fl
         float q[4][4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, Q8) : paged_k_at(4 * g + r, d, Q8));
+            const uint8_t* t = im + image_at(pr.isv ? paged_v_at(4 * g, d + r, KT) : paged_k_at(4 * g + r, d, KT));
+            if constexpr (Q4) {
+                // (the thread's first byte in the word: K's second four dims are the bytes above)
+                const uint32_t word = *(const uint32_t*)((uintptr_t)t & ~(uintptr_t)3) >>
+                                      (pr.isv ? d & 16 ? 4 : 0 : d & 4 ? 8 : 0);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at = pr.isv ? (e & 1) * 16 + (e >> 1) * 8 : (e & 1) * 16 + (e >> 1) * 4;
+                    q[r][e] = (float)((int)((word >> at) & 15) - 8);
+                }
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 q[r][e] = Q8 ? (float)((*(const uint32_t*)t >> (8 * e)) & 255) : (float)((const _Float16*)t)[e];
@@ -219,7 +302,10 @@ __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, fl
             const float sc = pr.scale[slot];
             v4f y;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = ((pr.isv ? q[e][r] : q[r][e]) - (Q8 ? 128.f : 0.f)) * sc;
+            for (int e = 0; e < 4; ++e) {
+                const float z = pr.isv ? q[e][r] : q[r][e];
+                y[e] = Q4 ? z * (float)pr.mult[paged_c_at(slot, d >> 5)] * sc : (z - (Q8 ? 128.f : 0.f)) * sc;
+            }
             st4(dst + slot * ld + d, y, vec);
         }
     }
@@ -232,18 +318,29 @@ __global__ void __launch_bounds__(256) k_paged_move(PagedMove m) {
     const int d = threadIdx.x;
     if (d >= m.hd) return;
     uint8_t* base = m.data + ((int64_t)blockIdx.y * m.n_pages * m.n_kv + blockIdx.x) * m.block;
-    const int64_t vb = paged_values_bytes(m.hd, m.q8), step = m.block * m.n_kv;
+    const int64_t vb = paged_values_bytes(m.hd, m.kt), step = m.block * m.n_kv;
+    const int64_t mb = paged_mult_bytes(m.hd, m.kt);
     for (int i = 0; i < m.n; ++i) {
         const int ss = m.src[i] % FTX_PAGE, ds = m.dst[i] % FTX_PAGE;
         const uint8_t* s = base + (m.src[i] / FTX_PAGE) * step;
         uint8_t* t = base + (m.dst[i] / FTX_PAGE) * step;
         if (m.src[i] == m.dst[i]) continue;
-        if (m.q8) {
-            t[paged_k_at(ds, d, 1)] = s[paged_k_at(ss, d, 1)];
-            t[vb + paged_v_at(ds, d, 1)] = s[vb + paged_v_at(ss, d, 1)];
+        if (m.kt == PT_Q4) {
+            if (d < m.hd / 2) {
+                const int kd = paged_k_dim(d), vd = paged_v_dim(d);
+                t[paged_k_at(ds, kd, PT_Q4)] = s[paged_k_at(ss, kd, PT_Q4)];
+                t[vb + paged_v_at(ds, vd, PT_Q4)] = s[vb + paged_v_at(ss, vd, PT_Q4)];
+            }
+            if (d < 2 * (m.hd / 32)) {
+                const int64_t at = 2 * vb + 2 * FTX_PAGE * 4 + (d & 1) * mb;
+                t[at + paged_c_at(ds, d >> 1)] = s[at + paged_c_at(ss, d >> 1)];
+            }
+        } else if (m.kt == PT_Q8) {
+            t[paged_k_at(ds, d, PT_Q8)] = s[paged_k_at(ss, d, PT_Q8)];
+            t[vb + paged_v_at(ds, d, PT_Q8)] = s[vb + paged_v_at(ss, d, PT_Q8)];
         } else {
-            *(uint16_t*)(t + paged_k_at(ds, d, 0)) = *(const uint16_t*)(s + paged_k_at(ss, d, 0));
-            *(uint16_t*)(t + vb + paged_v_at(ds, d, 0)) = *(const uint16_t*)(s + vb + paged_v_at(ss, d, 0));
+            *(uint16_t*)(t + paged_k_at(ds, d, PT_F16)) = *(const uint16_t*)(s + paged_k_at(ss, d, PT_F16));
+            *(uint16_t*)(t + vb + paged_v_at(ds, d, PT_F16)) = *(const uint16_t*)(s + vb + paged_v_at(ss, d, PT_F16));
         }
         if (d < 2) ((float*)(t + 2 * vb))[d * FTX_PAGE + ds] = ((const float*)(s + 2 * vb))[d * FTX_PAGE + ss];
     }
@@ -258,6 +355,33 @@ __device__ __forceinline__ v8h u8x8(uint32_t a, uint32_t b) {
     const v2h h2 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, 0x64646464u, 0x00050004u)) + o;
     const v2h h3 = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(b, 0x64646464u, 0x00070006u)) + o;
     return v8h{h0[0], h0[1], h1[0], h1[1], h2[0], h2[1], h3[0], h3[1]};
+}
+
+// 4-bit values under their multipliers as halves (exact: |q c| <= 2040).  A nibble
+// n = q + 8 under 0x64 is 1024 + n, four bits up under 0x54 it is 64 + n.
+__device__ __forceinline__ v2h q4_low(uint32_t x) {
+    return __builtin_bit_cast(v2h, (x & 0x000F000Fu) | 0x64006400u) + v2h{(_Float16)(-1032.f), (_Float16)(-1032.f)};
+}
+__device__ __forceinline__ v2h q4_high(uint32_t x) {
+    return __builtin_bit_cast(v2h, (x & 0x00F000F0u) | 0x54005400u) + v2h{(_Float16)(-72.f), (_Float16)(-72.f)};
+}
+__device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
+    return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+// a K word: eight dims of a slot
+__device__ __forceinline__ v8h q4x8(uint32_t x, v8h c) {
+    return join(q4_low(x), q4_high(x), q4_low(x >> 8), q4_high(x >> 8)) * c;
+}
+// two V words: four slots each of a dim's low nibbles or of another's high ones;
+// c0, c1: the slots' multipliers, a byte each
+__device__ __forceinline__ v8h q4x4x2(uint32_t x, uint32_t y, bool high, uint32_t c0, uint32_t c1) {
+    const v2h o = {(_Float16)(-1024.f), (_Float16)(-1024.f)};
+    const v2h a = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(c0, 0x64646464u, 0x00050004u)) + o;
+    const v2h b = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(c0, 0x64646464u, 0x00070006u)) + o;
+    const v2h c = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(c1, 0x64646464u, 0x00050004u)) + o;
+    const v2h d = __builtin_bit_cast(v2h, __builtin_amdgcn_perm(c1, 0x64646464u, 0x00070006u)) + o;
+    if (high) return join(q4_high(x) * a, q4_high(x >> 8) * b, q4_high(y) * c, q4_high(y >> 8) * d);
+    return join(q4_low(x) * a, q4_low(x >> 8) * b, q4_low(y) * c, q4_low(y >> 8) * d);
 }
 
 // A product rounded once, in a register: converted to halves in two places, it
@@ -318,8 +442,10 @@ __device__ __forceinline__ int ev_level(float vm) {
 // products of the sums so far, a third of a page's arithmetic, then fall to one
 // page in ten).  l = sum p, and P.V of p vs 2^-ev in two halves, ev the level
 // of the largest V scale that the row has seen.  out = 2^ev o / l.
-template <int HD, bool Q8>
+template <int HD, int KT>
 struct WaveAttn {
+    // values that are integers under a scale of any size (8 and 4 bits), or halves
+    static constexpr bool Q8 = KT != PT_F16;
     static constexpr int NDC = HD / 32, NDT = HD / 16;
     v8h qh[NDC], ql[NDC];
     v4f o[NDT];
@@ -334,7 +460,7 @@ struct WaveAttn {
         float a = 0.f;
 #pragma unroll
         for (int dc = 0; dc < NDC; ++dc) {
-            const int d0 = Q8 ? 64 * (dc >> 1) + 16 * kq + 8 * (dc & 1) : 32 * dc + 8 * kq;
+            const int d0 = KT == PT_Q8 ? 64 * (dc >> 1) + 16 * kq + 8 * (dc & 1) : 32 * dc + 8 * kq;
             x[dc][0] = ld4(q + d0, vec);
             x[dc][1] = ld4(q + d0 + 4, vec);
         }
@@ -368,9 +494,10 @@ struct WaveAttn {
 
     // A page's loads, issued together: the values of K (or V) as this lane's
     // operands, 16 bytes each, and the lane's 16 K and V scales
-    static constexpr int NL = HD / (Q8 ? 16 : 8);  // 16-byte loads of K or of V
+    static constexpr int NL = HD / (KT == PT_F16 ? 8 : KT == PT_Q8 ? 16 : 32);  // 16-byte loads of K or of V
     struct Vals {
         uint4 u[NL];
+        uint4 c[KT == PT_Q4 ? NDC : 1];  // 4 bits: the multipliers of each 32 dims
     };
     struct Scales {
         v4f k[4], v[4];
@@ -378,6 +505,11 @@ struct WaveAttn {
     static __device__ __forceinline__ void load_vals(Vals& x, const uint8_t* vals, int lane) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
+    }
+    // 4 bits: the multipliers of a page for the lane's K (kq: of slots 16 st + m) or V operands
+    static __device__ __forceinline__ void load_mults(Vals& x, const uint8_t* mult, int kq) {
+#pragma unroll
+        for (int g = 0; g < NDC; ++g) x.c[g] = *(const uint4*)(mult + 64 * g + 16 * kq);
     }
     static __device__ __forceinline__ void load_four(v4f (&x)[4], const float* at, int kq) {
 #pragma unroll
@@ -387,8 +519,16 @@ struct WaveAttn {
         load_four(x.k, k, kq);
         load_four(x.v, v, kq);
     }
-    static __device__ __forceinline__ v8h k_frag(const Vals& x, int st, int dc) {
-        if constexpr (Q8) {
+    static __device__ __forceinline__ uint32_t word(const uint4& u, int i) {
+        return i == 0 ? u.x : i == 1 ? u.y : i == 2 ? u.z : u.w;
+    }
+    // lane: of the wave
+    static __device__ __forceinline__ v8h k_frag(const Vals& x, int st, int dc, int lane) {
+        if constexpr (KT == PT_Q4) {
+            const uint32_t c = (word(x.c[dc], st) >> (8 * (lane & 3))) & 255;
+            const _Float16 h = (_Float16)(float)c;
+            return q4x8(word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1)), v8h{h, h, h, h, h, h, h, h});
+        } else if constexpr (Q8) {
             const uint4 u = x.u[(dc >> 1) * 4 + st];
             return dc & 1 ? u8x8(u.z, u.w) : u8x8(u.x, u.y);
         } else {
@@ -396,7 +536,10 @@ struct WaveAttn {
         }
     }
     static __device__ __forceinline__ v8h v_frag(const Vals& x, int dt, int sp) {
-        if constexpr (Q8) {
+        if constexpr (KT == PT_Q4) {
+            const uint32_t c0 = word(x.c[dt >> 1], 2 * sp), c1 = word(x.c[dt >> 1], 2 * sp + 1);
+            return q4x4x2(word(x.u[dt >> 1], 2 * sp), word(x.u[dt >> 1], 2 * sp + 1), dt & 1, c0, c1);
+        } else if constexpr (Q8) {
             const uint4 u = x.u[dt];
             return sp ? u8x8(u.z, u.w) : u8x8(u.x, u.y);
         } else {
@@ -686,10 +829,11 @@ struct RowSight {
 // of 131072 (halves) 104 us, the loads alone 104.  (Joining the partials in the
 // last workgroup of a list instead of a launch of their own: the same for
 // short lists, 14 us slower for one of 131072; by fences 60 us slower.)
-template <int HD, bool Q8, int NW>
+template <int HD, int KT, int NW>
 __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(PagedAttn a) {
-    using W = WaveAttn<HD, Q8>;
-    constexpr bool PRE = HD * (Q8 ? 1 : 2) <= 128, EARLY = PRE;  // as far as two waves a SIMD have the registers
+    using W = WaveAttn<HD, KT>;
+    constexpr bool Q8 = W::Q8;
+    constexpr bool PRE = paged_values_bytes(HD, KT) <= 8192, EARLY = PRE;  // as far as two waves a SIMD have the registers
     // the query's halves, of which the waves have the same: in LDS where
     // they would leave too few registers for the values in flight (halves of
     // 128 dims: 37 spilled, 129 us for one token over 131072; so 104)
@@ -741,17 +885,26 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         if ((j & 63) == 0 && j) ids = j + lane < n ? a.p.table[sq.tab0 + place(j + lane)] : 0;
         return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
     };
+    constexpr int64_t VB = paged_values_bytes(HD, KT), MB = paged_mult_bytes(HD, KT), MULT = 2 * VB + 2 * FTX_PAGE * 4;
+    auto load_k = [&](typename W::Vals& x, const uint8_t* b) {
+        W::load_vals(x, b, lane);
+        if constexpr (KT == PT_Q4) W::load_mults(x, b + MULT, col >> 2);
+    };
+    auto load_v = [&](typename W::Vals& x, const uint8_t* b) {
+        W::load_vals(x, b + VB, lane);
+        if constexpr (KT == PT_Q4) W::load_mults(x, b + MULT + MB, kq);
+    };
     typename W::Vals kv, vv;
     typename W::Scales sc;
     const uint8_t* blk = nullptr;
     if (n) {
         blk = block_of(0);
-        if (PRE) W::load_vals(kv, blk, lane);
+        if (PRE) load_k(kv, blk);
     }
     bool second = false;  // a page of large and small rows of halves: its small ones
     for (int j = 0; j < n;) {
-        if (!PRE) W::load_vals(kv, blk, lane);
-        const float* scale = (const float*)(blk + 2 * paged_values_bytes(HD, Q8));
+        if (!PRE) load_k(kv, blk);
+        const float* scale = (const float*)(blk + 2 * VB);
         float k1 = 0.f, v1 = 0.f;
         if constexpr (Q8) {
             W::load_scales(sc, scale, scale + FTX_PAGE, kq);
@@ -761,10 +914,10 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
             k1 = scale[lane];
             v1 = scale[FTX_PAGE + lane];
         }
-        if (EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
+        if (EARLY) load_v(vv, blk);
         __builtin_amdgcn_sched_barrier(0);
         v4f s[4];
-        auto kf = [&](int st, int dc) { return W::k_frag(kv, st, dc); };
+        auto kf = [&](int st, int dc) { return W::k_frag(kv, st, dc, lane); };
         if constexpr (QLDS) {
             asm volatile("" ::: "memory");  // (read again for every page)
             W::scores_of(s, kf, [&](int dc) { return qs[1][dc][lane]; }, [&](int dc) { return qs[0][dc][lane]; });
@@ -774,14 +927,14 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
         __builtin_amdgcn_sched_barrier(0);
         const bool ones = !Q8 && !__builtin_amdgcn_ballot_w64((k1 != 1.f) | (v1 != 1.f));
         if (!Q8 && !ones) W::load_scales(sc, scale, scale + FTX_PAGE, kq);
-        if (!EARLY) W::load_vals(vv, blk + paged_values_bytes(HD, Q8), lane);
+        if (!EARLY) load_v(vv, blk);
         const int p0 = place(j) * FTX_PAGE;
         const bool both = !Q8 && !ones && both_kinds(v1), again = both && !second;
         if (again) {
-            if (PRE) W::load_vals(kv, blk, lane);
+            if (PRE) load_k(kv, blk);
         } else if (++j < n) {
             blk = block_of(j);
-            if (PRE) W::load_vals(kv, blk, lane);
+            if (PRE) load_k(kv, blk);
         }
         __builtin_amdgcn_sched_barrier(0);
         const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
@@ -904,11 +1057,12 @@ template <int HD>
 constexpr int many_lo_bytes() {
     return HD <= 128 ? many_tiles<HD>() * PAGED_TR_MANY * HD * 2 : 0;
 }
-template <int HD, bool Q8>
+template <int HD, int KT>
 __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     constexpr int NW = NW_MANY, NT = many_tiles<HD>();
     constexpr bool QLO = many_lo_bytes<HD>() > 0;
-    using W = WaveAttn<HD, Q8>;
+    using W = WaveAttn<HD, KT>;
+    constexpr bool Q8 = W::Q8;
     constexpr int VB = FTX_PAGE * HD * 2;  // bytes of K's (V's) halves in LDS
     constexpr int BUF = many_buf_bytes<HD>();
     constexpr int NC = 2 * VB / 1024;  // KB of both
@@ -935,14 +1089,31 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
         return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
     };
     // the thread's share of the next page
-    constexpr int NQ = Q8 ? NC / (2 * NW) : 1;  // 16-byte units of 8-bit values
-    uint4 u[NQ];
+    constexpr int64_t PB = 2 * paged_values_bytes(HD, KT);  // bytes of K's and V's values in the page
+    constexpr int NQ = Q8 ? (PB / 16 + 64 * NW - 1) / (64 * NW) : 1;  // 16-byte units of 8- or 4-bit values
+    constexpr int UK = PB / 32;                                       // of K
+    uint4 u[NQ], um[KT == PT_Q4 ? NQ : 1];
     float sc1 = 0.f;
     auto stage = [&](int j) {
         const uint8_t* blk = block_of(j);
         uint8_t* dst = lds + (j & 1) * BUF;
-        if (tid < 2 * FTX_PAGE) sc1 = ((const float*)(blk + 2 * paged_values_bytes(HD, Q8)))[tid];
-        if constexpr (Q8) {
+        if (tid < 2 * FTX_PAGE) sc1 = ((const float*)(blk + PB))[tid];
+        if constexpr (KT == PT_Q4) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int x = i * 64 * NW + tid;
+                if (x >= 2 * UK) break;  // (heads of 64 dims: half of the threads)
+                u[i] = ((const uint4*)blk)[x];
+                const uint8_t* mult = blk + PB + 2 * FTX_PAGE * 4;
+                // K: the lane's four multipliers of two slots and blocks; V: those of its 16 slots
+                if (x < UK) {
+                    const uint8_t* t = mult + (x >> 7) * 128 + ((x >> 2) & 3) * 16 + (x >> 6 & 1) * 8 + (x & 3);
+                    um[i] = uint4{t[0], t[64], t[4], t[68]};
+                } else {
+                    um[i] = *(const uint4*)(mult + paged_mult_bytes(HD, KT) + ((x - UK) >> 6) * 64 + ((x >> 4) & 3) * 16);
+                }
+            }
+        } else if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < NQ; ++i) u[i] = ((const uint4*)blk)[i * 64 * NW + tid];
         } else {
@@ -962,7 +1133,29 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             const bool both = !Q8 && both_kinds(sc1);
             if (lane == 0) *(int*)(dst + 2 * VB + 3 * FTX_PAGE * 4) = both ? W::NO_LEVEL : pe;
         }
-        if constexpr (Q8) {
+        if constexpr (KT == PT_Q4) {
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int x = i * 64 * NW + tid, l = x & 63;
+                if (x >= 2 * UK) break;
+                if (x < UK) {
+                    // words: slot tile 2 sh + (w >> 1), dims 32 (2 dh + (w & 1)) ..
+                    const int sh = (x >> 6) & 1, dh = x >> 7;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const _Float16 h = (_Float16)(float)W::word(um[i], y);
+                        ((v8h*)dst)[((2 * dh + (y & 1)) * 4 + 2 * sh + (y >> 1)) * 64 + l] =
+                            q4x8(W::word(u[i], y), v8h{h, h, h, h, h, h, h, h});
+                    }
+                } else {
+                    v8h* t = (v8h*)(dst + VB) + ((x - UK) >> 6) * 256 + l;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)  // dim tile 2 g + (y >> 1), slots' half y & 1
+                        t[y * 64] = q4x4x2(W::word(u[i], 2 * (y & 1)), W::word(u[i], 2 * (y & 1) + 1), y >> 1,
+                                           W::word(um[i], 2 * (y & 1)), W::word(um[i], 2 * (y & 1) + 1));
+                }
+            }
+        } else if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 // unit x of K: dims' half (dc) and slot tile; of V: dim tile
@@ -1182,17 +1375,16 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
 
 }  // namespace
 
-// f<HD, Q8>() of the pool's head size and type
-#define PAGED_CASE(f, hd, q8)                                             \
-    ((hd) == 64 ? ((q8) ? f<64, true> : f<64, false>)                     \
-                : (hd) == 128 ? ((q8) ? f<128, true> : f<128, false>)     \
-                              : ((q8) ? f<256, true> : f<256, false>))
+// f<HD, KT> of the pool's head size and type
+#define PAGED_TYPE(f, hd, kt) ((kt) == PT_Q4 ? f<hd, PT_Q4> : (kt) == PT_Q8 ? f<hd, PT_Q8> : f<hd, PT_F16>)
+#define PAGED_CASE(f, hd, kt) \
+    ((hd) == 64 ? PAGED_TYPE(f, 64, kt) : (hd) == 128 ? PAGED_TYPE(f, 128, kt) : PAGED_TYPE(f, 256, kt))
 
 hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_new_pages, const float* k, int64_t ldk,
                               const float* v, int64_t ldv) {
     if (max_new_pages == 0) return hipSuccess;
     const dim3 grid((unsigned)(max_new_pages * 2 * p.n_kv), (unsigned)p.nseq);
-    ktimed_launch(PAGED_CASE(k_paged_write, p.hd, p.q8), grid, dim3(256), 0, st, p, k, ldk, v, ldv);
+    ktimed_launch(PAGED_CASE(k_paged_write, p.hd, p.kt), grid, dim3(256), 0, st, p, k, ldk, v, ldv);
     return hipGetLastError();
 }
 
@@ -1200,40 +1392,40 @@ hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pag
                              float* v, int64_t ldv) {
     if (max_pages == 0) return hipSuccess;
     const dim3 grid((unsigned)(max_pages * 2 * p.n_kv), (unsigned)p.nseq);
-    ktimed_launch(PAGED_CASE(k_paged_read, p.hd, p.q8), grid, dim3(256), 0, st, p, context, k, ldk, v, ldv);
+    ktimed_launch(PAGED_CASE(k_paged_read, p.hd, p.kt), grid, dim3(256), 0, st, p, context, k, ldk, v, ldv);
     return hipGetLastError();
 }
 
-template <int HD, bool Q8>
+template <int HD, int KT>
 static hipError_t launch_many(hipStream_t st, const PagedAttn& a) {
     static std::atomic<uint64_t> lds_set{0};
     constexpr size_t bytes = 2 * (size_t)many_buf_bytes<HD>() + many_lo_bytes<HD>();
-    const hipError_t e = lds_limit((const void*)k_paged_many<HD, Q8>, bytes, lds_set);
+    const hipError_t e = lds_limit((const void*)k_paged_many<HD, KT>, bytes, lds_set);
     if (e != hipSuccess) return e;
-    ktimed_launch(k_paged_many<HD, Q8>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(64 * NW_MANY),
+    ktimed_launch(k_paged_many<HD, KT>, dim3((unsigned)a.n_many * (unsigned)a.p.n_kv), dim3(64 * NW_MANY),
                   (uint32_t)bytes, st, a);
     return hipGetLastError();
 }
 
-template <int HD, bool Q8>
+template <int HD, int KT>
 static auto attn_four() {
-    return k_paged_attn<HD, Q8, 4>;
+    return k_paged_attn<HD, KT, 4>;
 }
-template <int HD, bool Q8>
+template <int HD, int KT>
 static auto attn_wide() {
-    return k_paged_attn<HD, Q8, HD <= 128 ? 8 : 4>;
+    return k_paged_attn<HD, KT, HD <= 128 ? 8 : 4>;
 }
 
 hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     hipError_t e = hipSuccess;
-    if (a.n_many) e = PAGED_CASE(launch_many, a.p.hd, a.p.q8)(st, a);
+    if (a.n_many) e = PAGED_CASE(launch_many, a.p.hd, a.p.kt)(st, a);
     if (e != hipSuccess) return e;
     if (a.n_few) {
         const dim3 grid((unsigned)a.n_few * (unsigned)a.p.n_kv);
         if (a.wide)
-            ktimed_launch(PAGED_CASE(attn_wide, a.p.hd, a.p.q8)(), grid, dim3(512), 0, st, a);
+            ktimed_launch(PAGED_CASE(attn_wide, a.p.hd, a.p.kt)(), grid, dim3(512), 0, st, a);
         else
-            ktimed_launch(PAGED_CASE(attn_four, a.p.hd, a.p.q8)(), grid, dim3(256), 0, st, a);
+            ktimed_launch(PAGED_CASE(attn_four, a.p.hd, a.p.kt)(), grid, dim3(256), 0, st, a);
     }
     e = hipGetLastError();
     if (e != hipSuccess || a.n_combs == 0) return e;

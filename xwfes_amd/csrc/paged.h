@@ -10,32 +10,55 @@
 
 // ---------------------------------------------------------------- page layout
 // One block per (layer, page, kv head): K values, V values, FTX_PAGE K scales,
-// FTX_PAGE V scales (fp32), all in the order the attention's MFMA operands are
-// loaded, so that every wave load of 16 bytes per lane is one contiguous KB.
+// FTX_PAGE V scales (fp32), and for 4-bit rows K's and V's multipliers (a byte
+// for each 32 dims of a slot), all in the order the attention's MFMA operands
+// are loaded, so that every wave load of 16 bytes per lane is one contiguous KB.
 // Slot of a page: slot = 16 st + m (K: row m of score tile st);
 // slot = 16 st + 4 kq + r (V: the slots whose scores lane (q row, kq) holds).
 //   halves: K unit (dc 4 + st) 64 + 16 kq + m: slot 16 st + m, dims 32 dc + 8 kq ..+7
 //           V unit (2 dt + sp) 64 + 16 kq + dl: dim 16 dt + dl, slots 16 (2 sp + i / 4) + 4 kq + i % 4
 //   8 bit:  K unit (4 j + st) 64 + 16 kq + m: slot 16 st + m, dims 64 j + 16 kq ..+15
 //           V unit 64 dt + 16 kq + dl: dim 16 dt + dl, byte 4 st + r: slot 16 st + 4 kq + r
-__host__ __device__ inline int64_t paged_values_bytes(int hd, int q8) {
-    return (int64_t)FTX_PAGE * hd * (q8 ? 1 : 2);
+//   4 bit:  K unit (2 (dc / 2) + st / 2) 64 + 16 kq + m, word 2 (st % 2) + dc % 2: slot 16 st + m,
+//             dims 32 dc + 8 kq ..+7 as nibbles 0 4 1 5 2 6 3 7 (nibble n + 4 in the high half)
+//           V unit 64 g + 16 kq + dl, word st, bytes of slots 16 st + 4 kq + 0 2 1 3:
+//             dim 32 g + dl in the low nibble, 32 g + 16 + dl in the high one
+//           (so that a row's bytes are its own, and a nibble of both halves of a word is two
+//           neighbours of an operand)
+//           multiplier of slot 16 st + 4 kq + r, dims 32 g ..+31: byte 64 g + 16 kq + 4 st + r
+enum { PT_F16 = 0, PT_Q8 = 1, PT_Q4 = 2 };
+__host__ __device__ constexpr int64_t paged_values_bytes(int hd, int kt) {
+    return (int64_t)FTX_PAGE * hd * (kt == PT_F16 ? 4 : kt == PT_Q8 ? 2 : 1) / 2;
 }
-__host__ __device__ inline int64_t paged_block_bytes(int hd, int q8) {
-    return 2 * paged_values_bytes(hd, q8) + 2 * FTX_PAGE * 4;
+__host__ __device__ constexpr int64_t paged_mult_bytes(int hd, int kt) {
+    return kt == PT_Q4 ? (int64_t)FTX_PAGE * hd / 32 : 0;
+}
+__host__ __device__ constexpr int64_t paged_block_bytes(int hd, int kt) {
+    return 2 * paged_values_bytes(hd, kt) + 2 * FTX_PAGE * 4 + 2 * paged_mult_bytes(hd, kt);
 }
 // byte offsets of element (slot, d) in the K and in the V values of a block
-__host__ __device__ inline int paged_k_at(int slot, int d, int q8) {
+__host__ __device__ inline int paged_k_at(int slot, int d, int kt) {
     const int st = slot >> 4, m = slot & 15;
-    return q8 ? (((d >> 6) * 4 + st) * 64 + ((d >> 4) & 3) * 16 + m) * 16 + (d & 15)
-              : ((((d >> 5) * 4 + st) * 64 + ((d >> 3) & 3) * 16 + m) * 8 + (d & 7)) * 2;
+    if (kt == PT_Q4)
+        return (((d >> 6) * 2 + (st >> 1)) * 64 + ((d >> 3) & 3) * 16 + m) * 16 + (st & 1) * 8 + ((d >> 5) & 1) * 4 +
+               (d & 1) * 2 + ((d >> 2) & 1);
+    return kt == PT_Q8 ? (((d >> 6) * 4 + st) * 64 + ((d >> 4) & 3) * 16 + m) * 16 + (d & 15)
+                       : ((((d >> 5) * 4 + st) * 64 + ((d >> 3) & 3) * 16 + m) * 8 + (d & 7)) * 2;
 }
-__host__ __device__ inline int paged_v_at(int slot, int d, int q8) {
+__host__ __device__ inline int paged_v_at(int slot, int d, int kt) {
     const int st = slot >> 4, kq = (slot >> 2) & 3, r = slot & 3;
     const int lane = kq * 16 + (d & 15);
-    return q8 ? ((d >> 4) * 64 + lane) * 16 + 4 * st + r
-              : ((((d >> 4) * 2 + (st >> 1)) * 64 + lane) * 8 + 4 * (st & 1) + r) * 2;
+    if (kt == PT_Q4) return ((d >> 5) * 64 + lane) * 16 + 4 * st + (r & 1) * 2 + (r >> 1);
+    return kt == PT_Q8 ? ((d >> 4) * 64 + lane) * 16 + 4 * st + r
+                       : ((((d >> 4) * 2 + (st >> 1)) * 64 + lane) * 8 + 4 * (st & 1) + r) * 2;
 }
+// of 4-bit rows: the byte of slot `slot`'s multiplier for dims 32 g ..+31, and the
+// dim in the low nibble of byte t of a row (the other is d + 2 in K, d + 16 in V)
+__host__ __device__ inline int paged_c_at(int slot, int g) {
+    return 64 * g + ((slot >> 2) & 3) * 16 + (slot >> 4) * 4 + (slot & 3);
+}
+__host__ __device__ inline int paged_k_dim(int t) { return (t >> 2) * 8 + ((t >> 1) & 1) + (t & 1) * 4; }
+__host__ __device__ inline int paged_v_dim(int t) { return (t >> 4) * 32 + (t & 15); }
 
 // ---------------------------------------------------------------- a plan's tables
 struct PagedSeq {
@@ -109,7 +132,7 @@ inline bool paged_grid_fits(int64_t workgroups, int64_t threads) { return workgr
 struct PagedView {
     uint8_t* data;  // the layer's first block
     int64_t block;  // bytes of a block
-    int n_kv, hd, q8;
+    int n_kv, hd, kt;
     const PagedSeq* seqs;
     const int32_t* table;
     int nseq;
@@ -142,7 +165,7 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a);
 struct PagedMove {
     uint8_t* data;
     int64_t block, n_pages;
-    int n_kv, hd, q8, n_layer, n;
+    int n_kv, hd, kt, n_layer, n;
     int32_t src[256], dst[256];
 };
 hipError_t launch_paged_move(hipStream_t st, const PagedMove& m);

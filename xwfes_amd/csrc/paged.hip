@@ -499,7 +499,7 @@ PagedView paged_view(const ftx_plan* pl, int64_t layer) {
     v.data = p->data + layer * p->n_pages * p->n_kv * p->block;
     v.n_kv = (int)p->n_kv;
     v.hd = (int)p->hd;
-    v.q8 = p->q8;
+    v.kt = p->kt;
     v.seqs = (const PagedSeq*)(pl->dev + pl->o_seq);
     v.table = (const int32_t*)(pl->dev + pl->o_tab);
     v.nseq = (int)pl->t.seqs.size();
@@ -590,8 +590,8 @@ int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t he
         return ftx_fail(ctx, FTX_E_INVALID, "pool: layers, kv heads or pages out of range");
     if (head_dim != 64 && head_dim != 128 && head_dim != 256)
         return ftx_fail(ctx, FTX_E_UNSUPPORTED, "pool: head_dim must be 64, 128 or 256");
-    if (kv_dtype != FTX_KV_F16 && kv_dtype != FTX_KV_Q8)
-        return ftx_fail(ctx, FTX_E_UNSUPPORTED, "pool: kv dtype must be F16 or Q8");
+    if (kv_dtype != FTX_KV_F16 && kv_dtype != FTX_KV_Q8 && kv_dtype != FTX_KV_Q4)
+        return ftx_fail(ctx, FTX_E_UNSUPPORTED, "pool: kv dtype must be F16, Q8 or Q4");
     OnDevice od(ctx->device);
     if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
     ftx_pool* p = new (std::nothrow) ftx_pool;
@@ -601,8 +601,8 @@ int ftx_pool_create(ftx_ctx* ctx, int64_t n_layer, int64_t n_head_kv, int64_t he
     p->n_kv = n_head_kv;
     p->hd = head_dim;
     p->n_pages = n_pages;
-    p->q8 = kv_dtype == FTX_KV_Q8;
-    p->block = paged_block_bytes((int)head_dim, p->q8);
+    p->kt = kv_dtype == FTX_KV_Q4 ? PT_Q4 : kv_dtype == FTX_KV_Q8 ? PT_Q8 : PT_F16;
+    p->block = paged_block_bytes((int)head_dim, p->kt);
     p->free_pages = n_pages;
     try {
         p->taken.assign((size_t)n_pages, 0);

@@ -10,7 +10,7 @@ struct ftx_plan;
 struct ftx_pool {
     ftx_ctx* ctx = nullptr;
     int64_t n_layer = 0, n_kv = 0, hd = 0, n_pages = 0;
-    int q8 = 0;
+    int kt = 0;  // how rows are stored (PT_F16, ..)
     int64_t block = 0;  // bytes of one (layer, page, kv head)
     uint8_t* data = nullptr;  // [n_layer][n_pages][n_kv] blocks
     std::vector<uint8_t> taken;

@@ -1171,7 +1171,7 @@ int ftx_kv_create_paged(ftx_ctx* ctx, const ftx_model* m, ftx_pool* p, int64_t c
     kv->hd = m->d.head_dim;
     kv->n_head = m->d.n_head;
     kv->mmax = m->Mmax;
-    kv->kv_f16 = !p->q8;
+    kv->kv_f16 = p->kt == PT_F16;
     kv->pool = p;
     kv->window = window;
     // (positions stay below 2^30; not cut to cap, which caches of one step need not share)
@@ -1384,7 +1384,7 @@ int ftx_kv_commit(ftx_kv* kv, const int32_t* nodes, int64_t n) {
         pm.n_pages = kv->pool->n_pages;
         pm.n_kv = (int)kv->n_kv;
         pm.hd = (int)kv->hd;
-        pm.q8 = kv->pool->q8;
+        pm.kt = kv->pool->kt;
         pm.n_layer = (int)kv->n_layer;
         pm.n = (int)n;
         auto at = [&](int64_t pos) {

@@ -17,7 +17,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "ftx.h")
 F32, F16, Q4_0, Q4_1, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 2, 3, 8, 12, 14, 30
 BLOCK = {F32: (1, 4), F16: (1, 2), BF16: (1, 2), Q4_0: (32, 18), Q4_1: (32, 20),
          Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
-KV_F32, KV_F16, KV_Q8 = 0, 1, 2
+KV_F32, KV_F16, KV_Q8, KV_Q4 = 0, 1, 2, 3
 PAGE = 64  # tokens of a page
 # the sampler state of seed 0 (include/ft/sampler.h:19)
 SAMPLER_SEED = 0x9E3779B97F4A7C15

@@ -418,6 +418,57 @@ int ftx_plan_create(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args* a, ftx_plan*
 int ftx_plan_set(ftx_plan* pl, const ftx_plan_args* a);
 int ftx_plan_free(ftx_plan* pl);
 
+/* A plan whose steps are built on the GPU, from lengths and tables that the GPU
+ * holds: nothing of a step passes the host, so that a loop of steps is one
+ * stream's work, or one HIP graph replayed.  `room` is what it has room for; its
+ * launches cover the room, so keep it near the steps' sizes.  Chains only.
+ * Until a build the plan holds no tokens. */
+typedef struct {
+    int64_t nseq;     /* 1 .. 4096 sequences */
+    int64_t tokens;   /* >= 1 new tokens of all sequences */
+    int64_t M;        /* 1 .. tokens of one sequence */
+    int64_t n_pages;  /* >= 1 pages of one sequence */
+    int64_t n_head, window, sinks;  /* as in ftx_plan_args */
+} ftx_plan_room;
+int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room, ftx_plan** out);
+/* All pointers are int32 device memory, 4-byte aligned; none may overlap another
+ * but used and used_after, which may be one. */
+typedef struct {
+    int64_t nseq;               /* 1 .. room.nseq sequences of this step */
+    const int32_t* npast;       /* [nseq] tokens in their pages */
+    const int32_t* M;           /* [nseq] new ones, >= 0 */
+    int32_t* tables;            /* [nseq][ldt]: sequence s's pages in order; entries from
+                                   ceil(npast / FTX_PAGE) to ceil((npast + M) / FTX_PAGE) - 1 are written */
+    int64_t ldt;
+    const int32_t* free_pages;  /* [n_free]: taken pages that no table names, for the new tokens */
+    int64_t n_free;
+    const int32_t* used;        /* [1]: how many of them are used up, in their order */
+    int32_t* used_after;        /* [1] */
+    int32_t* starts;            /* [nseq + 1] sequence s's first row in the packed new rows, or NULL */
+    int32_t* slots;             /* [room.tokens] page * FTX_PAGE + slot of each new token, or NULL */
+    int32_t* positions;         /* [room.tokens], or NULL; both -1 past the last token */
+    int32_t* status;            /* [1] FTX_OK or the step's fault */
+} ftx_build_args;
+/* Enqueues the building of a step's block tables, starts, slots, positions and
+ * the attention's division on the context's stream: new pages from the list,
+ * sequence after sequence, in order.  What cannot be seen from the host is told
+ * by `status`: FTX_E_RANGE (a length that is negative or past the room or ldt,
+ * used outside 0 .. n_free), FTX_E_NOMEM (the list is too short),
+ * FTX_E_INVALID (a page that a new token sees or goes to, without a window any
+ * page of a sequence, or a page of the list is none of the pool's), the lowest where there are
+ * several.  Then the tables stay as they were, used_after is used, starts are 0,
+ * slots and positions -1, and the plan holds no tokens.  That pages are taken
+ * and that no other sequence has a page that new tokens go to is the caller's
+ * to see to.
+ * The plan's calls (below; matrices of room.tokens rows, of which those past the
+ * last token are not touched) then go by these tables, of which the plan keeps
+ * its own; contexts are read back only without a window, k and v then as
+ * long as the lengths say.  A call that is recorded into a graph needs the build before
+ * it in the same capture (FTX_E_INVALID); a build on another stream than the
+ * plan's last call waits for the device.  Graphs and eager calls of one plan
+ * must not overlap. */
+int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a);
+
 /* The calls below enqueue on the context's stream and take device memory;
  * row n of a matrix is ld floats (0: dense) after row n - 1.  They may be
  * recorded into a HIP graph; ftx_plan_set is then refused for that plan, and

@@ -42,11 +42,16 @@ struct PageRows {
 };
 template <int HD, int KT>
 __device__ __forceinline__ PageRows page_rows(const PagedView& p, int context) {
-    const PagedSeq sq = p.seqs[blockIdx.y];
-    const int from = context ? 0 : sq.npast;
     const int z = blockIdx.x % (2 * p.n_kv);
-    const int first = from / FTX_PAGE + blockIdx.x / (2 * p.n_kv);  // the page's place in the table
     PageRows r{};
+    int2 to{(int)blockIdx.y, (int)(blockIdx.x / (2 * p.n_kv))};
+    if (p.touch && !context) {
+        to = p.touch[to.y];
+        if (to.x < 0) return r;
+    }
+    const PagedSeq sq = p.seqs[to.x];
+    const int from = context ? 0 : sq.npast;
+    const int first = p.touch && !context ? to.y : from / FTX_PAGE + to.y;  // the page's place in the table
     r.s0 = max(from - first * FTX_PAGE, 0);
     r.s1 = min(FTX_PAGE, sq.npast + sq.M - first * FTX_PAGE);
     if (r.s0 >= r.s1) return r;
@@ -843,6 +848,7 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
     __shared__ int se[NW][64];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
+    if (it.seq < 0) return;  // (of tables built on the GPU)
     const PagedSeq sq = it.q;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
@@ -1069,6 +1075,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[a.n_few + blockIdx.x / a.p.n_kv];
+    if (it.seq < 0) return;
     const PagedSeq sq = it.q;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, kq = lane >> 4;
@@ -1383,7 +1390,7 @@ __global__ void __launch_bounds__(256) k_paged_combine(PagedAttn a) {
 hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_new_pages, const float* k, int64_t ldk,
                               const float* v, int64_t ldv) {
     if (max_new_pages == 0) return hipSuccess;
-    const dim3 grid((unsigned)(max_new_pages * 2 * p.n_kv), (unsigned)p.nseq);
+    const dim3 grid((unsigned)((p.touch ? p.n_touch : max_new_pages) * 2 * p.n_kv), p.touch ? 1u : (unsigned)p.nseq);
     ktimed_launch(PAGED_CASE(k_paged_write, p.hd, p.kt), grid, dim3(256), 0, st, p, k, ldk, v, ldv);
     return hipGetLastError();
 }
@@ -1391,7 +1398,8 @@ hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_ne
 hipError_t launch_paged_read(hipStream_t st, const PagedView& p, int64_t max_pages, int context, float* k, int64_t ldk,
                              float* v, int64_t ldv) {
     if (max_pages == 0) return hipSuccess;
-    const dim3 grid((unsigned)(max_pages * 2 * p.n_kv), (unsigned)p.nseq);
+    const bool touch = p.touch && !context;
+    const dim3 grid((unsigned)((touch ? p.n_touch : max_pages) * 2 * p.n_kv), touch ? 1u : (unsigned)p.nseq);
     ktimed_launch(PAGED_CASE(k_paged_read, p.hd, p.kt), grid, dim3(256), 0, st, p, context, k, ldk, v, ldv);
     return hipGetLastError();
 }

@@ -87,6 +87,9 @@ struct PagedComb {
     int32_t seq, row0, part0, n, step, tok0, M, pad;
 };
 constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
+// Sequences of at least this many query rows a kv head may go to the kernel
+// that shares each page among 128 or 256 rows
+constexpr int PAGED_MANY = 65;
 
 struct PagedGeom {
     int64_t n_kv = 0, hd = 0, n_pages = 0;
@@ -125,6 +128,43 @@ extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int
 // from now on, 16, 128 or 256 (heads of 256 dims: 128), 0: by the estimate
 extern "C" void paged_force_rows(int rows);
 
+// ---------------------------------------------------------------- tables built on the GPU
+constexpr int PAGED_ROOM_SEQS = 4096;
+// What a plan of lengths that the GPU holds has room for
+struct PagedRoom {
+    int32_t nseq, tokens, most, n_pages;  // sequences, new tokens of all, of one; pages of one
+    int32_t pool_pages, n_kv, gqa;        // gqa = 0: no attention
+    int32_t window, sinks;
+    int32_t cut_few, cut_many;  // parts that lists are cut into beyond one each (seq_per)
+    int32_t wide;               // lists of few rows stay whole, for workgroups of eight waves
+    int32_t few, many, combs, parts, touch;  // entries
+};
+// from ftx_plan_room, or an FTX_E_* code and its message
+int paged_room(const PagedGeom& g, const ftx_plan_room& a, PagedRoom& r, std::string& err);
+
+struct PagedBuild {
+    PagedRoom r;
+    int nseq;
+    // the caller's
+    const int32_t *npast, *M, *free_pages, *used;
+    int32_t *tables, *used_after, *starts, *slots, *positions, *status;
+    int64_t ldt, n_free;
+    // the plan's
+    PagedSeq* seqs;
+    int32_t* table;  // [r.nseq][r.n_pages]
+    int2* touch;     // (sequence or -1, page of it) that new tokens go to
+    PagedItem* items;  // r.few, then r.many; seq = -1: none
+    PagedComb* combs;  // M = 0: none
+    int32_t* codes;    // [r.nseq]: what the first kernel says of each sequence, then the pages used before
+};
+hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b);
+
+// The same lists for plain arrays, no context and no device: items (r.few + r.many
+// of them) and joins (r.combs) of sequences whose lengths fit the room
+extern "C" int paged_build_probe(const ftx_plan_room* a, int64_t n_kv, int64_t hd, int64_t pool_pages, int cu,
+                                 const int32_t* npast, const int32_t* M, int64_t nseq, PagedRoom* room, PagedItem* items,
+                                 PagedComb* combs, int64_t max_out, char* msg, int64_t msg_bytes);
+
 // ---------------------------------------------------------------- launches
 // a launch has fewer than 2^32 threads along its x
 inline bool paged_grid_fits(int64_t workgroups, int64_t threads) { return workgroups * threads < (int64_t)1 << 32; }
@@ -136,6 +176,10 @@ struct PagedView {
     const PagedSeq* seqs;
     const int32_t* table;
     int nseq;
+    // of tables built on the GPU: the pages that new tokens go to, one after the
+    // other (else a launch covers every sequence's most such pages)
+    const int2* touch;
+    int n_touch;
 };
 hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_new_pages,
                               const float* k, int64_t ldk, const float* v, int64_t ldv);

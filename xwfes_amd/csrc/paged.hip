@@ -10,12 +10,10 @@
 #include <thread>
 
 #include "paged_pool.h"
+#include "plan_dev.h"
 
 // ---------------------------------------------------------------- plan tables
 
-// Sequences of at least this many query rows a kv head may go to the kernel
-// that shares each page among 128 or 256 rows
-constexpr int64_t PAGED_MANY = 65;
 // Row tiles beyond which such sequences do so without a look at tiles of 16
 constexpr int64_t FEW_MOST = 4096;
 // Pages of a list beyond which few rows are not given to eight waves unsplit
@@ -291,6 +289,115 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     return FTX_OK;
 }
 
+int paged_room(const PagedGeom& g, const ftx_plan_room& a, PagedRoom& r, std::string& err) {
+    auto fail = [&](int code, const char* what) {
+        err = std::string("plan: ") + what;
+        return code;
+    };
+    r = PagedRoom{};
+    constexpr int64_t FAR = (int64_t)1 << 30, LIM = (int64_t)1 << 31;
+    if (a.nseq < 1 || a.nseq > PAGED_ROOM_SEQS) return fail(FTX_E_INVALID, "nseq out of range (1 .. 4096)");
+    if (a.tokens < 1 || a.M < 1 || a.M > a.tokens || a.tokens > FAR)
+        return fail(FTX_E_INVALID, "room for tokens and M: 1 <= M <= tokens <= 2^30");
+    if (a.n_pages < 1 || a.n_pages > FAR / FTX_PAGE) return fail(FTX_E_INVALID, "room for n_pages out of range");
+    if (a.n_head < 0 || a.n_head % g.n_kv || a.n_head > 65535)
+        return fail(FTX_E_INVALID, "n_head must be a multiple of the pool's kv heads");
+    if (a.window < 0 || a.sinks < 0) return fail(FTX_E_INVALID, "negative window or sinks");
+    const int64_t gqa = a.n_head / g.n_kv, cu = std::max(g.cu, 1);
+    if (a.tokens * std::max<int64_t>(a.n_head, 1) >= LIM || a.nseq * a.n_pages >= LIM)
+        return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
+    r.nseq = (int32_t)a.nseq;
+    r.tokens = (int32_t)a.tokens;
+    r.most = (int32_t)a.M;
+    r.n_pages = (int32_t)a.n_pages;
+    r.pool_pages = (int32_t)g.n_pages;
+    r.n_kv = (int32_t)g.n_kv;
+    r.gqa = (int32_t)gqa;
+    r.window = (int32_t)std::min(a.window, FAR);
+    r.sinks = r.window ? (int32_t)std::min(a.sinks, FAR) : 0;
+    // (every page has a token; a sequence's first and last may be parts of one)
+    const int64_t touch = std::min(a.tokens, a.tokens / FTX_PAGE + 2 * a.nseq);
+    if (!paged_grid_fits(touch * 2 * g.n_kv, 256)) return fail(FTX_E_RANGE, "too many new tokens in one plan");
+    r.touch = (int32_t)touch;
+    if (gqa == 0) return FTX_OK;
+    // Tiles of 16 rows of sequences of fewer than PAGED_MANY rows, of 128 rows of
+    // the others
+    const int64_t longest = a.M * gqa, rows = a.tokens * gqa;
+    const int64_t each = (std::min<int64_t>(longest, PAGED_MANY - 1) + PAGED_TR - 1) / PAGED_TR;
+    const int64_t few = std::min(a.nseq * each, rows / PAGED_TR + std::min(a.nseq, a.tokens));
+    const int64_t big = longest >= PAGED_MANY ? std::min(a.nseq, rows / PAGED_MANY) : 0;
+    const int64_t many = big ? rows / PAGED_TR_MANY + big : 0;
+    // Lists are cut so that a launch has four (few rows) or two (many) workgroups a
+    // CU more than it has lists, as far as they have pages: a part has total / cut
+    // pages at least, so at most `cut` lists are cut, into 2 cut parts in all.
+    // Whole lists, for eight waves, by the rule of a step's own plan for lists as
+    // long as the room.
+    const double load = (double)(few * a.n_pages * g.n_kv) / (double)cu;
+    r.wide = g.hd <= 128 && a.n_pages > 4 && a.n_pages <= WIDE_MOST && few * g.n_kv <= cu && !r.window &&
+             (double)a.n_pages <= (g.hd == 64 ? 15 : 10) + 1.6 * load;
+    r.cut_few = r.wide ? 0 : (int32_t)(4 * cu / g.n_kv);
+    r.cut_many = big ? (int32_t)(2 * cu / g.n_kv) : 0;
+    constexpr int64_t B = PAGED_TR_MANY / PAGED_TR;
+    if (few + many + r.cut_few + r.cut_many >= LIM / 2 || !paged_grid_fits((few + r.cut_few) * g.n_kv, r.wide ? 512 : 256) ||
+        !paged_grid_fits((many + r.cut_many) * g.n_kv, 512))
+        return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
+    r.few = (int32_t)(few + r.cut_few);
+    r.many = (int32_t)(many + r.cut_many);
+    r.combs = (int32_t)(r.cut_few + B * r.cut_many);
+    r.parts = (int32_t)(2 * r.cut_few + 2 * B * r.cut_many);
+    return FTX_OK;
+}
+
+extern "C" int paged_build_probe(const ftx_plan_room* a, int64_t n_kv, int64_t hd, int64_t pool_pages, int cu,
+                                 const int32_t* npast, const int32_t* M, int64_t nseq, PagedRoom* room, PagedItem* items,
+                                 PagedComb* combs, int64_t max_out, char* msg, int64_t msg_bytes) {
+    try {
+        PagedGeom g;
+        g.n_kv = n_kv;
+        g.hd = hd;
+        g.n_pages = pool_pages;
+        g.cu = cu;
+        std::string err;
+        PagedRoom& r = *room;
+        int rc = paged_room(g, *a, r, err);
+        snprintf(msg, (size_t)msg_bytes, "%s", err.c_str());
+        if (rc) return rc;
+        if (r.few + r.many > max_out || r.combs > max_out || nseq > r.nseq) return FTX_E_RANGE;
+        int64_t total[2] = {0, 0}, tokens = 0;
+        for (int64_t s = 0; s < nseq; ++s) {
+            const SeqLoad l = seq_load(r, r.n_pages, npast[s], M[s]);
+            if (l.code) return l.code;
+            total[l.many] += (int64_t)l.tiles * l.n;
+            tokens += M[s];
+        }
+        if (tokens > r.tokens) return FTX_E_RANGE;
+        const int per[2] = {r.wide ? INT32_MAX : seq_per(total[0], r.cut_few, 4), seq_per(total[1], r.cut_many, 2)};
+        int64_t at[2] = {0, 0}, part = 0, comb = 0, tok = 0;
+        for (int64_t i = 0; i < r.few + r.many; ++i) items[i].seq = -1;
+        for (int64_t i = 0; i < r.combs; ++i) combs[i] = PagedComb{};
+        for (int64_t s = 0; s < nseq; ++s) {
+            const SeqLoad l = seq_load(r, r.n_pages, npast[s], M[s]);
+            const SeqCount c = seq_count(l, per[l.many]);
+            PagedSeq q{};
+            q.npast = npast[s];
+            q.M = M[s];
+            q.tok0 = (int32_t)tok;
+            q.tab0 = (int32_t)(s * r.n_pages);
+            q.dep0 = -1;
+            if (at[l.many] + c.items > (l.many ? r.many : r.few) || part + c.parts > r.parts || comb + c.combs > r.combs)
+                return FTX_E_NOMEM;  // (never: the room is for any lengths that fit it)
+            for (int e = 0; e < c.items; ++e)
+                items[(l.many ? r.few : 0) + at[l.many]++] = seq_item(r, q, (int)s, l.many, c.np, (int)part, e);
+            for (int e = 0; e < c.combs; ++e) combs[comb++] = seq_comb(r, q, (int)s, l.many, c.np, (int)part, e);
+            part += c.parts;
+            tok += M[s];
+        }
+        return FTX_OK;
+    } catch (...) {
+        return FTX_E_NOMEM;
+    }
+}
+
 extern "C" void paged_force_rows(int rows) { forced_rows = rows; }
 
 extern "C" int paged_probe(const ftx_plan_args* a, int64_t n_kv, int64_t hd, int64_t n_pages, const uint8_t* taken,
@@ -352,6 +459,17 @@ bool capturing(hipStream_t st) {
     return s != hipStreamCaptureStatusNone;
 }
 
+// the number of the capture that the stream is in, 0: none
+unsigned long long capture_id(hipStream_t st) {
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(st, &s, &id) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return s == hipStreamCaptureStatusActive ? id : 0;
+}
+
 // device memory of the context's own device
 bool on_device(const ftx_ctx* ctx, const void* p) {
     hipPointerAttribute_t at;
@@ -401,6 +519,12 @@ struct ftx_plan {
     size_t o_seq = 0, o_tab = 0, o_dep = 0, o_anc = 0, o_item = 0, o_comb = 0, o_serial = 0;
     size_t bytes = 0;     // of the last set's tables
     uint64_t serial = 0;  // its number
+    // tables built on the GPU: what there is room for, its entries, and the capture
+    // that the last build was recorded in
+    bool device = false;
+    PagedRoom room;
+    size_t o_touch = 0, o_code = 0;
+    unsigned long long capture = 0;
 };
 
 static void plan_release(ftx_plan* pl) {
@@ -502,7 +626,11 @@ PagedView paged_view(const ftx_plan* pl, int64_t layer) {
     v.kt = p->kt;
     v.seqs = (const PagedSeq*)(pl->dev + pl->o_seq);
     v.table = (const int32_t*)(pl->dev + pl->o_tab);
-    v.nseq = (int)pl->t.seqs.size();
+    v.nseq = pl->device ? pl->room.nseq : (int)pl->t.seqs.size();
+    if (pl->device) {
+        v.touch = (const int2*)(pl->dev + pl->o_touch);
+        v.n_touch = pl->room.touch;
+    }
     return v;
 }
 
@@ -532,8 +660,14 @@ static int plan_order(ftx_plan* pl) {
     ftx_ctx* ctx = pl->ctx;
     if (!capturing(ctx->stream)) {
         if (ctx->stream == pl->stream) return FTX_OK;
-        FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
+        if (pl->up) FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
         pl->stream = ctx->stream;
+        return FTX_OK;
+    }
+    if (pl->device) {
+        // (tables of a build outside of the graph: nothing would order the two)
+        if (pl->capture == 0 || capture_id(ctx->stream) != pl->capture)
+            return ftx_fail(ctx, FTX_E_INVALID, "plan: no build of it in this capture");
         return FTX_OK;
     }
     pl->captured = true;
@@ -664,6 +798,7 @@ int ftx_plan_set(ftx_plan* pl, const ftx_plan_args* a) {
     if (!pl) return FTX_E_INVALID;
     ftx_ctx* ctx = pl->ctx;
     if (!a) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    if (pl->device) return ftx_fail(ctx, FTX_E_INVALID, "plan: its steps are built on the GPU");
     if (pl->captured) return ftx_fail(ctx, FTX_E_INVALID, "plan: a graph holds calls of this plan");
     if (capturing(ctx->stream)) return ftx_fail(ctx, FTX_E_INVALID, "plan: set while the stream is captured");
     OnDevice od(ctx->device);
@@ -705,6 +840,139 @@ int ftx_plan_create(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_args* a, ftx_plan*
     return FTX_OK;
 }
 
+int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room, ftx_plan** out) {
+    if (!ctx || !p || !room || !out) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    *out = nullptr;
+    if (p->ctx != ctx) return ftx_fail(ctx, FTX_E_INVALID, "plan: the pool is another context's");
+    if (capturing(ctx->stream)) return ftx_fail(ctx, FTX_E_INVALID, "plan: created while the stream is captured");
+    OnDevice od(ctx->device);
+    if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
+    ftx_plan* pl = nullptr;
+    try {
+        PagedGeom g;
+        g.n_kv = p->n_kv;
+        g.hd = p->hd;
+        g.n_pages = p->n_pages;
+        g.cu = ctx->cu_count;
+        PagedRoom r;
+        std::string err;
+        const int rc = paged_room(g, *room, r, err);
+        if (rc) return ftx_fail(ctx, rc, err);
+        pl = new ftx_plan;
+        pl->ctx = ctx;
+        pl->pool = p;
+        ++p->users;
+        pl->device = true;
+        pl->room = r;
+        PagedTables& t = pl->t;
+        t.n_head = room->n_head;
+        t.window = r.window;
+        t.sinks = r.sinks;
+        t.tokens = r.tokens;
+        t.longest = r.most;
+        t.max_new_pages = r.touch;
+        t.max_pages = r.n_pages;
+        t.rows = (int64_t)r.nseq * r.n_pages * FTX_PAGE;
+        t.parts = r.parts;
+        t.few = r.few;
+        t.wide = r.wide;
+        // (a list of n pages is cut into parts of 4 and more)
+        t.comb_max = ((int64_t)r.n_pages + 1) / 2;
+        size_t at = 0;
+        auto place = [&](size_t& off, size_t bytes) {
+            off = at;
+            at += up256(bytes);
+        };
+        place(pl->o_seq, (size_t)r.nseq * sizeof(PagedSeq));
+        place(pl->o_tab, (size_t)r.nseq * (size_t)r.n_pages * 4);
+        place(pl->o_touch, (size_t)r.touch * sizeof(int2));
+        place(pl->o_item, ((size_t)r.few + (size_t)r.many) * sizeof(PagedItem));
+        place(pl->o_comb, (size_t)r.combs * sizeof(PagedComb));
+        place(pl->o_code, ((size_t)r.nseq + 1) * 4);
+        const size_t pf = (size_t)r.parts * p->n_kv * PAGED_TR * (p->hd + 2);
+        if (hipMalloc((void**)&pl->dev, at) != hipSuccess || (pf && hipMalloc((void**)&pl->part, pf * 4 + 256) != hipSuccess)) {
+            (void)hipGetLastError();
+            plan_release(pl);
+            return ftx_fail(ctx, FTX_E_NOMEM, "plan: device allocation failed");
+        }
+        // no tokens: items and pages of no sequence
+        if (hipMemset(pl->dev, 0, at) != hipSuccess || hipMemset(pl->dev + pl->o_touch, 0xFF, pl->o_comb - pl->o_touch) != hipSuccess ||
+            hipDeviceSynchronize() != hipSuccess) {
+            (void)hipGetLastError();
+            plan_release(pl);
+            return ftx_fail(ctx, FTX_E_DEVICE, "plan: clearing failed");
+        }
+        pl->stream = ctx->stream;
+        pl->ready = true;
+        *out = pl;
+        return FTX_OK;
+    } catch (...) {
+        if (pl) plan_release(pl);
+        return ftx_fail(ctx, FTX_E_NOMEM, "host allocation failed");
+    }
+}
+
+int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
+    if (!pl) return FTX_E_INVALID;
+    ftx_ctx* ctx = pl->ctx;
+    if (!a) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+    if (!pl->device) return ftx_fail(ctx, FTX_E_INVALID, "plan: its steps are set from the host");
+    const PagedRoom& r = pl->room;
+    if (a->nseq < 1 || a->nseq > r.nseq) return ftx_fail(ctx, FTX_E_RANGE, "build: more sequences than the plan has room for");
+    if (a->ldt < 1 || a->n_free < 0 || a->n_free > INT32_MAX) return ftx_fail(ctx, FTX_E_INVALID, "build: ldt or n_free out of range");
+    const struct {
+        const void* p;
+        bool need;
+    } mem[] = {{a->npast, true}, {a->M, true}, {a->tables, true}, {a->free_pages, a->n_free > 0}, {a->used, true},
+               {a->used_after, true}, {a->starts, false}, {a->slots, false}, {a->positions, false}, {a->status, true}};
+    for (const auto& m : mem) {
+        if (!m.p && !m.need) continue;
+        if (!m.p) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
+        if ((uintptr_t)m.p & 3) return ftx_fail(ctx, FTX_E_INVALID, "build: arrays must be 4-byte aligned");
+        if (!on_device(ctx, m.p)) return ftx_fail(ctx, FTX_E_INVALID, "build: arrays must be memory of the context's device");
+    }
+    OnDevice od(ctx->device);
+    if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
+    hipStream_t st = ctx->stream;
+    const bool cap = capturing(st);
+    // (calls of the plan on another stream may still read its tables)
+    if (!cap && pl->stream != st) FTX_HIP(ctx, hipDeviceSynchronize());
+    if (!cap && !pl->ev[0]) FTX_HIP(ctx, hipEventCreateWithFlags(&pl->ev[0], hipEventDisableTiming));
+    PagedBuild b{};
+    b.r = r;
+    b.nseq = (int)a->nseq;
+    b.npast = a->npast;
+    b.M = a->M;
+    b.free_pages = a->free_pages;
+    b.used = a->used;
+    b.tables = a->tables;
+    b.used_after = a->used_after;
+    b.starts = a->starts;
+    b.slots = a->slots;
+    b.positions = a->positions;
+    b.status = a->status;
+    b.ldt = a->ldt;
+    b.n_free = a->n_free;
+    b.seqs = (PagedSeq*)(pl->dev + pl->o_seq);
+    b.table = (int32_t*)(pl->dev + pl->o_tab);
+    b.touch = (int2*)(pl->dev + pl->o_touch);
+    b.items = (PagedItem*)(pl->dev + pl->o_item);
+    b.combs = (PagedComb*)(pl->dev + pl->o_comb);
+    b.codes = (int32_t*)(pl->dev + pl->o_code);
+    NoTrace nt(ctx, ctx->trace && cap);
+    TraceScope ts(ctx);
+    FTX_HIP(ctx, launch_paged_build(st, b));
+    ts.end(TK_PAGED_KV, 8.0 * ((double)r.nseq + r.tokens));
+    if (cap) {
+        pl->capture = capture_id(st);
+        return FTX_OK;
+    }
+    FTX_HIP(ctx, hipEventRecord(pl->ev[0], st));
+    pl->up = pl->ev[0];
+    pl->stream = st;
+    return FTX_OK;
+}
+
 int ftx_plan_free(ftx_plan* pl) {
     if (!pl) return FTX_OK;
     OnDevice od(pl->ctx->device);
@@ -731,8 +999,12 @@ int ftx_paged_read(ftx_plan* pl, int64_t layer, int context, float* k, int64_t l
     if (rc) return rc;
     if (context && !paged_grid_fits(pl->t.max_pages * 2 * pl->pool->n_kv, 256))
         return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: too many positions of one sequence");
+    if (context && pl->device && pl->t.window)
+        return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: contexts under a window of a plan built on the GPU");
     if (context && pl->t.absent) return ftx_fail(pl->ctx, FTX_E_RANGE, "paged_read: a page is absent");
-    if (rows_overlap(k, ldk, v, ldv, w, n)) return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_read: k and v overlap");
+    // (contexts of lengths that only the GPU holds: one row at least)
+    if (rows_overlap(k, ldk, v, ldv, w, context && pl->device ? 1 : n))
+        return ftx_fail(pl->ctx, FTX_E_INVALID, "paged_read: k and v overlap");
     rc = plan_order(pl);
     return rc ? rc : paged_read_rows(pl, layer, context, k, ldk, v, ldv);
 }
@@ -792,8 +1064,8 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.items = (const PagedItem*)(pl->dev + pl->o_item);
     a.combs = (const PagedComb*)(pl->dev + pl->o_comb);
     a.n_few = (int)t.few;
-    a.n_many = (int)((int64_t)t.items.size() - t.few);
-    a.n_combs = (int)t.combs.size();
+    a.n_many = pl->device ? pl->room.many : (int)((int64_t)t.items.size() - t.few);
+    a.n_combs = pl->device ? pl->room.combs : (int)t.combs.size();
     a.wide = t.wide;
     a.gqa = (int)(t.n_head / p->n_kv);
     a.rows_max = (int)(t.longest * a.gqa);

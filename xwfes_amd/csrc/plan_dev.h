@@ -1,0 +1,114 @@
+// plan_dev.h -- a step's tables from its lengths: what a sequence has to do, and
+// the entries of the attention's work lists, each from its number alone, so that
+// the threads that write them share nothing but running sums (device and host).
+#pragma once
+
+#include "paged.h"
+
+// What a sequence of p tokens and m new ones has to do, or an FTX_E_* code
+struct SeqLoad {
+    int code;
+    int have, need, touch;  // pages before and after, pages that new tokens go to
+    int many, tiles, n;     // its row tiles (PAGED_TR or PAGED_TR_MANY rows), at most n pages each
+};
+__host__ __device__ inline SeqLoad seq_load(const PagedRoom& r, int64_t ldt, int p, int m) {
+    SeqLoad l{};
+    const int64_t most = (int64_t)(ldt < r.n_pages ? ldt : r.n_pages) * FTX_PAGE;
+    if (p < 0 || m < 0 || m > r.most || (int64_t)p + m > most) {
+        l.code = FTX_E_RANGE;
+        return l;
+    }
+    l.have = (p + FTX_PAGE - 1) / FTX_PAGE;
+    l.need = (p + m + FTX_PAGE - 1) / FTX_PAGE;
+    l.touch = m ? l.need - p / FTX_PAGE : 0;
+    if (r.gqa && m) {
+        const int R = m * r.gqa;
+        l.many = R >= PAGED_MANY;
+        const int tr = l.many ? PAGED_TR_MANY : PAGED_TR;
+        l.tiles = (R + tr - 1) / tr;
+        l.n = l.need;
+        if (r.window) {
+            // (a tile's positions, its tokens' and the window before them, end inside pages on both sides)
+            const int64_t n = (int64_t)(r.sinks + FTX_PAGE - 1) / FTX_PAGE + ((int64_t)r.window + (tr - 1) / r.gqa + 1) / FTX_PAGE + 2;
+            l.n = n < l.n ? (int)n : l.n;
+        }
+    }
+    return l;
+}
+// Pages below have that have to be pages of the pool: [0, s) and [a, have).
+// Under a window those between are not read
+__host__ __device__ inline void seq_held(const PagedRoom& r, int p, int have, int& s, int& a) {
+    s = 0;
+    a = 0;
+    if (!r.window) return;
+    a = p - r.window + 1 > 0 ? (p - r.window + 1) / FTX_PAGE : 0;
+    s = (int)(((int64_t)r.sinks + FTX_PAGE - 1) / FTX_PAGE);
+    s = s < a ? s : a;
+    s = s < have ? s : have;
+    a = a < have ? a : have;
+}
+
+// The most pages of a part of lists of `total` pages in all: a launch then has
+// some cut / n_kv workgroups more than it has lists
+__host__ __device__ inline int seq_per(int64_t total, int cut, int least) {
+    if (cut <= 0) return INT32_MAX;
+    const int64_t per = (total + cut - 1) / cut;
+    return per < least ? least : per > INT32_MAX ? INT32_MAX : (int)per;
+}
+// Entries of a sequence: parts of a list, items, blocks of partials, joins
+struct SeqCount {
+    int np, items, parts, combs;
+};
+__host__ __device__ inline SeqCount seq_count(const SeqLoad& l, int per) {
+    SeqCount c{};
+    if (l.tiles == 0) return c;
+    const int b = l.many ? PAGED_TR_MANY / PAGED_TR : 1;
+    c.np = (int)(((int64_t)l.n + per - 1) / per);
+    c.items = l.tiles * c.np;
+    c.parts = c.np > 1 ? c.items * b : 0;
+    c.combs = c.np > 1 ? l.tiles * b : 0;
+    return c;
+}
+
+// The pages of the tile at row row0: [0, s) and then n - s from a on
+__host__ __device__ inline void tile_pages(const PagedRoom& r, int p, int m, int row0, int tr, int& s, int& a, int& n) {
+    const int R = m * r.gqa, t0 = row0 / r.gqa, t1 = ((R < row0 + tr ? R : row0 + tr) - 1) / r.gqa;
+    const int lo = r.window && p + t0 - r.window + 1 > 0 ? p + t0 - r.window + 1 : 0;
+    a = lo / FTX_PAGE;
+    s = r.window ? (int)(((int64_t)r.sinks + FTX_PAGE - 1) / FTX_PAGE) : 0;
+    s = s < a ? s : a;
+    n = s + (p + t1) / FTX_PAGE + 1 - a;
+}
+// Item e of sequence q (number s), its partials from part0 on; seq = -1: none (a
+// tile whose list is shorter than the sequence's longest)
+__host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq& q, int s, int many, int np, int part0, int e) {
+    const int tr = many ? PAGED_TR_MANY : PAGED_TR, tile = e / np, k = e % np;
+    PagedItem it{};
+    int n;
+    tile_pages(r, q.npast, q.M, tile * tr, tr, it.s, it.a, n);
+    const int npt = np < n ? np : n;
+    it.seq = k < npt ? s : -1;
+    it.row0 = tile * tr;
+    it.i0 = (int32_t)((int64_t)n * k / npt);
+    it.i1 = (int32_t)((int64_t)n * (k + 1) / npt);
+    it.part = np > 1 ? part0 + e * (tr / PAGED_TR) : -1;
+    it.nt = many;
+    it.q = q;
+    return it;
+}
+// Join c of it (M = 0: none)
+__host__ __device__ inline PagedComb seq_comb(const PagedRoom& r, const PagedSeq& q, int s, int many, int np, int part0, int c) {
+    const int tr = many ? PAGED_TR_MANY : PAGED_TR, b = tr / PAGED_TR, tile = c / b, row0 = c * PAGED_TR;
+    PagedComb o{};
+    if (row0 >= q.M * r.gqa) return o;
+    int ps, pa, n;
+    tile_pages(r, q.npast, q.M, tile * tr, tr, ps, pa, n);
+    o.seq = s;
+    o.row0 = row0;
+    o.part0 = part0 + tile * np * b + c % b;
+    o.n = np < n ? np : n;
+    o.step = b;
+    o.tok0 = q.tok0;
+    o.M = q.M;
+    return o;
+}

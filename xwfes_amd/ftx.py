@@ -90,6 +90,17 @@ class PlanArgs(C.Structure):
                 ("sinks", _i64)]
 
 
+class PlanRoom(C.Structure):
+    _fields_ = [("nseq", _i64), ("tokens", _i64), ("M", _i64), ("n_pages", _i64), ("n_head", _i64),
+                ("window", _i64), ("sinks", _i64)]
+
+
+class BuildArgs(C.Structure):
+    _fields_ = [("nseq", _i64), ("npast", _vp), ("M", _vp), ("tables", _vp), ("ldt", _i64),
+                ("free_pages", _vp), ("n_free", _i64), ("used", _vp), ("used_after", _vp),
+                ("starts", _vp), ("slots", _vp), ("positions", _vp), ("status", _vp)]
+
+
 class TraceEntry(C.Structure):
     _fields_ = [("name", C.c_char * 24), ("launches", C.c_int64), ("ms", C.c_double),
                 ("bytes", C.c_double), ("kernel_launches", C.c_int64), ("kernel_ms", C.c_double)]
@@ -153,6 +164,8 @@ def load(path=LIB_PATH):
         "ftx_plan_create": (C.c_int, [_vp, _vp, C.POINTER(PlanArgs), C.POINTER(_vp)]),
         "ftx_plan_set": (C.c_int, [_vp, C.POINTER(PlanArgs)]),
         "ftx_plan_free": (C.c_int, [_vp]),
+        "ftx_plan_create_device": (C.c_int, [_vp, _vp, C.POINTER(PlanRoom), C.POINTER(_vp)]),
+        "ftx_plan_build": (C.c_int, [_vp, C.POINTER(BuildArgs)]),
         "ftx_paged_write": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64]),
         "ftx_paged_read": (C.c_int, [_vp, _i64, C.c_int, _vp, _i64, _vp, _i64]),
         "ftx_paged_attention": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _i64]),
@@ -470,6 +483,14 @@ class Pool:
                                                     C.byref(h)))
         return Plan(self.ctx, h.value)
 
+    def device_plan(self, nseq, tokens, M, n_pages, n_head=0, window=0, sinks=0):
+        """A plan whose steps are built on the GPU (Plan.build), with room for nseq
+        sequences, `tokens` new tokens of all and M of one, n_pages pages of one."""
+        a, h = PlanRoom(nseq, tokens, M, n_pages, n_head, window, sinks), _vp()
+        self.ctx.check(self.ctx.lib.ftx_plan_create_device(self.ctx.h, self.handle, C.byref(a),
+                                                           C.byref(h)))
+        return Plan(self.ctx, h.value)
+
     def free(self):
         if self.handle:
             self.ctx.check(self.ctx.lib.ftx_pool_free(self.handle))
@@ -485,10 +506,21 @@ class Plan:
         L = ctx.lib  # (a step makes a few calls a layer: looked up once)
         self._write, self._read, self._attend = (L.ftx_paged_write, L.ftx_paged_read,
                                                  L.ftx_paged_attention)
+        self._build = L.ftx_plan_build
 
     def set(self, seqs, n_head=0, window=0, sinks=0):
         a, keep = plan_args(seqs, n_head, window, sinks)
         self.ctx.check(self.ctx.lib.ftx_plan_set(self.handle, C.byref(a)))
+
+    def build(self, npast_ptr, M_ptr, nseq, tables_ptr, ldt, free_ptr, n_free, used_ptr, after_ptr,
+              status_ptr, starts_ptr=None, slots_ptr=None, positions_ptr=None):
+        """A step's tables from int32 device arrays (ftx_plan_build; a plan of
+        Pool.device_plan)."""
+        a = BuildArgs(nseq, npast_ptr, M_ptr, tables_ptr, ldt, free_ptr, n_free, used_ptr, after_ptr,
+                      starts_ptr, slots_ptr, positions_ptr, status_ptr)
+        rc = self._build(self.handle, C.byref(a))
+        if rc:
+            self.ctx.check(rc)
 
     def write(self, layer, k_ptr, v_ptr, ldk=0, ldv=0):
         rc = self._write(self.handle, layer, k_ptr, ldk, v_ptr, ldv)

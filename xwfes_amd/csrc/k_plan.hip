@@ -1,4 +1,6 @@
 // k_plan.hip -- a step's tables built on the GPU (ftx_plan_build).
+#include <type_traits>
+
 #include "plan_dev.h"
 
 namespace {
@@ -30,37 +32,17 @@ __global__ void __launch_bounds__(256) k_plan_check(PagedBuild b) {
     if (lane == 0) b.codes[s] = c;
 }
 
-constexpr int NT = 1024, NW = NT / 64;
+// (four waves, one a SIMD: every wave forms the same sums, so that sixteen take
+// four times as long for it: 16 sequences 13.3 us)
+constexpr int NT = 256, NW = NT / 64;
+constexpr int ONE_MOST = 6144;  // table entries (and others) of a build by one workgroup
 
-// sums over the workgroup, in all threads
-template <typename T>
-__device__ __forceinline__ T group_sum(T v, T* red) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();  // (red may still be read)
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    T t = red[0];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) t += red[w];
-    return t;
-}
-// the sum over the threads before this one
-template <typename T>
-__device__ __forceinline__ T group_before(T v, T* red) {
-    T x = v;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const T y = __shfl_up(x, o, 64);
-        x += lane >= o ? y : T(0);
-    }
-    __syncthreads();
-    if (lane == 63) red[w] = x;
-    __syncthreads();
-    T t = x - v;
-    for (int i = 0; i < w; ++i) t += red[i];
-    return t;
+// Between the waves' uses of LDS: what is on its way to global memory is not
+// waited for (the stores, which no other wave reads)
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // The sequence that entry i belongs to: at[s] <= i < at[s + 1]
@@ -76,136 +58,253 @@ __device__ __forceinline__ int owner(const int* at, int n, int i) {
     return lo;
 }
 
+// Sums of non-negative numbers over the lanes up to this one, in registers, by
+// DPP; SAT: they stop at 2^31 - 1
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, 0x7FFFFFFFu); }
+template <bool SAT>
+__device__ __forceinline__ int wave_upto(int v) {
+    uint32_t x = (uint32_t)v;
+    auto step = [&](auto ctrl, auto rows) {
+        const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+        x = SAT ? sat_add(x, y) : x + y;
+    };
+    using std::integral_constant;
+    constexpr integral_constant<int, 0xF> all{};
+    step(integral_constant<int, 0x111>{}, all);  // from 1, 2, 4, 8 lanes before, in rows of 16
+    step(integral_constant<int, 0x112>{}, all);
+    step(integral_constant<int, 0x114>{}, all);
+    step(integral_constant<int, 0x118>{}, all);
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xA>{});  // rows 1 and 3: the last lane of the row before
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xC>{});  // rows 2 and 3: lane 31
+    return (int)x;
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_upto<true>(v), 63); }
+
 enum { S_TOK, S_FRESH, S_TOUCH, S_FEW, S_MANY, S_PART, S_COMB, N_SUMS };
 
 // Every workgroup forms all running sums itself (a sequence's lengths are eight
 // bytes), then writes its share of the entries.  CHECK: the only workgroup, which
-// looks at the tables too, where they are short.
+// looks at the tables too, where they are short: a launch less.  Bound by latency,
+// lengths, tables, list and entries one after the other: two exchanges between
+// the waves, the first of totals (how lists are cut follows from them), the second
+// of running sums and what the list of pages holds.
 template <bool CHECK>
 __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedRoom& r = b.r;
-    __shared__ int64_t red[NW];
-    const int tid = threadIdx.x, n1 = b.nseq + 1;
-    int64_t* const rows_at = (int64_t*)lds;            // [n1]
-    int* const sums = (int*)(lds + 8 * (size_t)n1);    // [N_SUMS][n1]
-    int* const codes = CHECK ? sums + N_SUMS * n1 : b.codes;
-    const int per = (b.nseq + NT - 1) / NT, s0 = min(tid * per, b.nseq), s1 = min(s0 + per, b.nseq);
+    enum { T_FEW, T_MANY, T_TOK, T_FRESH, T_CODE, N_TOT };  // (page lists' totals stay below 2^31: paged_room)
+    __shared__ int tot[NW][N_TOT], sum_of[NW][N_SUMS], rows_of[NW][2], bad_of[NW];
+    const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = b.nseq, n1 = n + 1;
+    int* const P = (int*)lds;  // [n] lengths
+    int* const M = P + n;      // (in the end the parts of a list)
+    int* const sums = M + n;   // [N_SUMS][n1] (CHECK: first have, s and a of seq_held)
+    const int per = (n + NT - 1) / NT, s0 = min(tid * per, n), s1 = min(s0 + per, n);
+    // The first loads, none of which waits for another: the lengths, the first
+    // table entries whether they are pages or not, and (next) the list from `used` on
+    // (a wave takes a sequence's entries 64 at a time, every NW-th sequence, so that
+    // all but the entry itself is the wave's)
+    constexpr int U = CHECK ? 12 : 1;  // loads of a wave in flight
+    const int chunks = (r.n_pages + 63) / 64, wv = __builtin_amdgcn_readfirstlane(w);
+    const int loads = wv < n ? ((n - 1 - wv) / NW + 1) * chunks : 0;
+    int id[U];
+    // the first load's sequence and chunk, and the next one's
+    auto next = [&](int& s, int& c) {
+        if (++c == chunks) {
+            c = 0;
+            s += NW;
+        }
+    };
+    int ls = wv, lc = 0;
+    auto load = [&](int e0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = 64 * lc + lane;
+            id[u] = e0 + u < loads && i < r.n_pages && i < b.ldt ? b.tables[ls * b.ldt + i] : 0;
+            next(ls, lc);
+        }
+    };
+    if constexpr (CHECK) load(0);
     const int base = CHECK ? b.used[0] : b.codes[r.nseq];
-    if constexpr (CHECK) {
-        for (int s = tid >> 6; s < b.nseq; s += NW) {
-            const int c = check_seq(b, s, tid & 63);
-            if ((tid & 63) == 0) codes[s] = c;
-        }
-        __syncthreads();
-    }
-    int64_t few = 0, many = 0, tok = 0, fresh = 0;
-    int code = base < 0 || base > b.n_free ? FTX_E_RANGE : FTX_OK;
+    int code = FTX_OK;
     for (int s = s0; s < s1; ++s) {
-        const SeqLoad l = seq_load(r, b.ldt, b.npast[s], b.M[s]);
-        code = min(code, codes[s]);
-        if (l.code) continue;
-        (l.many ? many : few) += (int64_t)l.tiles * l.n;
-        tok += b.M[s];
-        fresh += l.need - l.have;
-    }
-    few = group_sum(few, red);
-    many = group_sum(many, red);
-    tok = group_sum(tok, red);
-    fresh = group_sum(fresh, red);
-    if (tok > r.tokens) code = FTX_E_RANGE;
-    if (code == FTX_OK && fresh > b.n_free - base) code = FTX_E_NOMEM;
-    // (before the list is read past its end)
-    const bool fits = base >= 0 && base <= b.n_free && fresh <= b.n_free - base;
-    if (fits)
-        for (int64_t i = tid; i < fresh; i += NT) {
-            const int id = b.free_pages[base + i];
-            if (id < 0 || id >= r.pool_pages) code = min(code, FTX_E_INVALID);
+        P[s] = b.npast[s];
+        M[s] = b.M[s];
+        if constexpr (CHECK) {
+            const SeqLoad l = seq_load(r, b.ldt, P[s], M[s]);
+            int hs = 0, ha = 0;
+            if (!l.code) seq_held(r, P[s], l.have, hs, ha);
+            sums[s] = l.have;  // (0 with a code: nothing to look at)
+            sums[n1 + s] = hs;
+            sums[2 * n1 + s] = ha;
+        } else {
+            code = min(code, b.codes[s]);
         }
+    }
+    const int mine_at = base >= 0 && base <= b.n_free && tid < b.n_free - base ? b.free_pages[base + tid] : 0;
+    if constexpr (CHECK) {
+        lds_barrier();
+        int cs = wv, cc = 0;
+        for (int e0 = 0; e0 < loads;) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) code = min(code, __shfl_xor(code, o, 64));
-    __syncthreads();
-    if ((tid & 63) == 0) red[tid >> 6] = code;
-    __syncthreads();
+            for (int u = 0; u < U; ++u) {
+                if (e0 + u >= loads) break;
+                const int i = 64 * cc + lane, have = __builtin_amdgcn_readfirstlane(sums[cs]);
+                const int hs = __builtin_amdgcn_readfirstlane(sums[n1 + cs]), ha = __builtin_amdgcn_readfirstlane(sums[2 * n1 + cs]);
+                if (i < have && (i < hs || i >= ha)) {
+                    if ((uint32_t)id[u] >= (uint32_t)r.pool_pages) code = FTX_E_INVALID;
+                    b.table[cs * r.n_pages + i] = id[u];
+                }
+                next(cs, cc);
+            }
+            e0 += U;
+            if (e0 < loads) load(e0);
+        }
+    }
+    if (base < 0 || base > b.n_free) code = FTX_E_RANGE;
+    uint32_t t[N_TOT] = {};
+    for (int s = s0; s < s1; ++s) {
+        const SeqLoad l = seq_load(r, b.ldt, P[s], M[s]);
+        code = min(code, l.code);
+        if (l.code) continue;
+        const uint32_t pages = (uint32_t)(l.tiles * l.n);
+        t[T_FEW] = sat_add(t[T_FEW], l.many ? 0 : pages);
+        t[T_MANY] = sat_add(t[T_MANY], l.many ? pages : 0);
+        t[T_TOK] = sat_add(t[T_TOK], (uint32_t)M[s]);
+        t[T_FRESH] = sat_add(t[T_FRESH], (uint32_t)(l.need - l.have));
+    }
 #pragma unroll
-    for (int w = 0; w < NW; ++w) code = min(code, (int)red[w]);
-    const bool ok = code == FTX_OK;
-    const int per_few = r.wide ? INT32_MAX : seq_per(few, r.cut_few, 4), per_many = seq_per(many, r.cut_many, 2);
+    for (int x = 0; x < T_CODE; ++x) {
+        const int v = wave_total((int)t[x]);
+        if (lane == 0) tot[w][x] = v;
+    }
+    // (the lowest code: of 0, -1, -4, -5)
+    const auto seen = [&](int c) { return __builtin_amdgcn_ballot_w64(code == c) != 0; };
+    code = seen(FTX_E_RANGE) ? FTX_E_RANGE : seen(FTX_E_NOMEM) ? FTX_E_NOMEM : seen(FTX_E_INVALID) ? FTX_E_INVALID : FTX_OK;
+    if (lane == 0) tot[w][T_CODE] = code;
+    lds_barrier();
+#pragma unroll
+    for (int x = 0; x < T_CODE; ++x) {
+        t[x] = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) t[x] = sat_add(t[x], (uint32_t)tot[i][x]);
+    }
+#pragma unroll
+    for (int i = 0; i < NW; ++i) code = min(code, tot[i][T_CODE]);
+    if (t[T_TOK] > (uint32_t)r.tokens) code = FTX_E_RANGE;
+    bool bad = false;
+    if (base >= 0 && base <= b.n_free) {
+        const int fresh = (int)t[T_FRESH];
+        if (fresh > b.n_free - base)
+            code = min(code, FTX_E_NOMEM);
+        else
+            for (int i = tid; i < fresh; i += NT) {
+                const int pg = i < NT ? mine_at : b.free_pages[base + i];
+                bad |= pg < 0 || pg >= r.pool_pages;
+            }
+    }
+    const int per_few = r.wide ? INT32_MAX : seq_per((int)t[T_FEW], r.cut_few, 4);
+    const int per_many = seq_per((int)t[T_MANY], r.cut_many, 2);
     int mine[N_SUMS] = {};
     int64_t rows = 0;
-    auto add = [&](int s, auto&& each) {
-        const int m = b.M[s], p = b.npast[s];
-        const SeqLoad l = seq_load(r, b.ldt, p, m);
+    auto add = [&](int s, int (&to)[N_SUMS], int64_t& to_rows) -> int {
+        const SeqLoad l = seq_load(r, b.ldt, P[s], M[s]);
         const SeqCount c = seq_count(l, l.many ? per_many : per_few);
-        const int v[N_SUMS] = {m, l.need - l.have, l.touch, l.many ? 0 : c.items, l.many ? c.items : 0, c.parts, c.combs};
-        each(v, (int64_t)p + m);
-    };
-    if (ok)
-        for (int s = s0; s < s1; ++s)
-            add(s, [&](const int (&v)[N_SUMS], int64_t n) {
+        const int v[N_SUMS] = {M[s], l.need - l.have, l.touch, l.many ? 0 : c.items, l.many ? c.items : 0, c.parts, c.combs};
 #pragma unroll
-                for (int x = 0; x < N_SUMS; ++x) mine[x] += v[x];
-                rows += n;
-            });
+        for (int x = 0; x < N_SUMS; ++x) to[x] += v[x];
+        to_rows += (int64_t)P[s] + M[s];
+        return c.np;
+    };
+    int np = 0;
+    if (code == FTX_OK)
+        for (int s = s0; s < s1; ++s) np = add(s, mine, rows);
+    const int64_t own_rows = rows;
     int at[N_SUMS];
 #pragma unroll
-    for (int x = 0; x < N_SUMS; ++x) at[x] = (int)group_before<int64_t>(mine[x], red);
-    rows = group_before(rows, red);
-    for (int s = s0; s < s1; ++s) {
+    for (int x = 0; x < N_SUMS; ++x) at[x] = wave_upto<false>(mine[x]);
+    // (up to 2^30 positions a sequence: in two parts)
+    const int low = wave_upto<false>((int)(rows & 0xFFFF)), high = wave_upto<false>((int)(rows >> 16));
+    const bool any = __builtin_amdgcn_ballot_w64(bad);
+    if (lane == 63) {
 #pragma unroll
-        for (int x = 0; x < N_SUMS; ++x) sums[x * n1 + s] = at[x];
-        rows_at[s] = rows;
-        if (ok)
-            add(s, [&](const int (&v)[N_SUMS], int64_t n) {
-#pragma unroll
-                for (int x = 0; x < N_SUMS; ++x) at[x] += v[x];
-                rows += n;
-            });
-        if (s + 1 == b.nseq) {
-#pragma unroll
-            for (int x = 0; x < N_SUMS; ++x) sums[x * n1 + b.nseq] = at[x];
-            rows_at[b.nseq] = rows;
-        }
+        for (int x = 0; x < N_SUMS; ++x) sum_of[w][x] = at[x];
+        rows_of[w][0] = low;
+        rows_of[w][1] = high;
+        bad_of[w] = any;
     }
-    __syncthreads();
-    auto sum_at = [&](int x) { return sums + x * n1; };
-    auto total = [&](int x) { return sums[x * n1 + b.nseq]; };
-    auto record = [&](int s) {
+    lds_barrier();
+    rows = low + ((int64_t)high << 16) - rows;
+#pragma unroll
+    for (int x = 0; x < N_SUMS; ++x) at[x] -= mine[x];
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        if (bad_of[i]) code = min(code, FTX_E_INVALID);
+        if (i >= w) continue;
+        rows += rows_of[i][0] + ((int64_t)rows_of[i][1] << 16);
+#pragma unroll
+        for (int x = 0; x < N_SUMS; ++x) at[x] += sum_of[i][x];
+    }
+    const bool ok = code == FTX_OK;
+    auto record = [&](int s, int m, int tok0, int64_t all0) {
         PagedSeq q{};
-        q.npast = ok ? b.npast[s] : 0;
-        q.M = ok ? b.M[s] : 0;
-        q.tok0 = sum_at(S_TOK)[s];
+        q.npast = ok ? P[s] : 0;
+        q.M = ok ? m : 0;
+        q.tok0 = tok0;
         q.tab0 = s * r.n_pages;
         q.ntab = (q.npast + q.M + FTX_PAGE - 1) / FTX_PAGE;
         q.dep0 = -1;
-        q.all0 = rows_at[s];
+        q.all0 = all0;
         return q;
     };
+    for (int s = s0; s < s1; ++s) {
+#pragma unroll
+        for (int x = 0; x < N_SUMS; ++x) sums[x * n1 + s] = ok ? at[x] : 0;
+        if (blockIdx.x == 0) b.seqs[s] = record(s, M[s], ok ? at[S_TOK] : 0, ok ? rows : 0);
+        if (per == 1) {
+#pragma unroll
+            for (int x = 0; x < N_SUMS; ++x) at[x] += mine[x];
+            rows += own_rows;
+            M[s] = np;
+        } else if (ok) {
+            M[s] = add(s, at, rows);
+        }
+        if (s + 1 == n)
+#pragma unroll
+            for (int x = 0; x < N_SUMS; ++x) sums[x * n1 + n] = ok ? at[x] : 0;
+    }
+    lds_barrier();
+    auto sum_at = [&](int x) { return sums + x * n1; };
+    auto total = [&](int x) { return sums[x * n1 + n]; };
+    auto of = [&](int s) { return record(s, sum_at(S_TOK)[s + 1] - sum_at(S_TOK)[s], sum_at(S_TOK)[s], 0); };
     const int g0 = blockIdx.x * NT + tid, gs = gridDim.x * NT;
+    // (each kind's entries from another wave on, where they are few: side by side)
+    auto from = [&](int wave) {
+        const int o = 64 * wave % gs;
+        return g0 >= o ? g0 - o : g0 - o + gs;  // in [0, gs)
+    };
     if (g0 == 0) {
         b.used_after[0] = base + total(S_FRESH);
         b.status[0] = code;
     }
-    for (int s = g0; s < r.nseq; s += gs) {
+    for (int s = n + from(1); s < r.nseq; s += gs) {
         PagedSeq q{};
         q.dep0 = -1;
-        if (s < b.nseq) q = record(s);
         b.seqs[s] = q;
     }
     if (b.starts)
-        for (int s = g0; s < n1; s += gs) b.starts[s] = sum_at(S_TOK)[s];
-    for (int i = g0; i < total(S_FRESH); i += gs) {
-        const int s = owner(sum_at(S_FRESH), b.nseq, i), id = b.free_pages[base + i];
-        const int64_t col = (b.npast[s] + FTX_PAGE - 1) / FTX_PAGE + i - sum_at(S_FRESH)[s];
+        for (int s = from(2); s < n1; s += gs) b.starts[s] = sum_at(S_TOK)[s];
+    for (int i = from(3); i < total(S_FRESH); i += gs) {
+        const int s = owner(sum_at(S_FRESH), n, i), id = b.free_pages[base + i];
+        const int64_t col = (P[s] + FTX_PAGE - 1) / FTX_PAGE + i - sum_at(S_FRESH)[s];
         b.tables[s * b.ldt + col] = id;
         b.table[(int64_t)s * r.n_pages + col] = id;
     }
     if (b.slots || b.positions)
-        for (int i = g0; i < r.tokens; i += gs) {
+        for (int i = from(4); i < r.tokens; i += gs) {
             int slot = -1, pos = -1;
             if (i < total(S_TOK)) {
-                const int s = owner(sum_at(S_TOK), b.nseq, i), p = b.npast[s], have = (p + FTX_PAGE - 1) / FTX_PAGE;
-                pos = p + i - sum_at(S_TOK)[s];
+                const int s = owner(sum_at(S_TOK), n, i), have = (P[s] + FTX_PAGE - 1) / FTX_PAGE;
+                pos = P[s] + i - sum_at(S_TOK)[s];
                 const int pg = pos / FTX_PAGE;
                 const int id = pg < have ? b.tables[s * b.ldt + pg] : b.free_pages[base + sum_at(S_FRESH)[s] + pg - have];
                 slot = id * FTX_PAGE + pos % FTX_PAGE;
@@ -213,33 +312,29 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
             if (b.slots) b.slots[i] = slot;
             if (b.positions) b.positions[i] = pos;
         }
-    for (int i = g0; i < r.touch; i += gs) {
-        int2 t{-1, 0};
+    for (int i = from(5); i < r.touch; i += gs) {
+        int2 to{-1, 0};
         if (i < total(S_TOUCH)) {
-            t.x = owner(sum_at(S_TOUCH), b.nseq, i);
-            t.y = b.npast[t.x] / FTX_PAGE + i - sum_at(S_TOUCH)[t.x];
+            to.x = owner(sum_at(S_TOUCH), n, i);
+            to.y = P[to.x] / FTX_PAGE + i - sum_at(S_TOUCH)[to.x];
         }
-        b.touch[i] = t;
+        b.touch[i] = to;
     }
-    for (int i = g0; i < r.few + r.many; i += gs) {
+    for (int i = from(6); i < r.few + r.many; i += gs) {
         const int mn = i >= r.few, e = mn ? i - r.few : i, x = mn ? S_MANY : S_FEW;
         if (e >= total(x)) {
             b.items[i].seq = -1;
             continue;
         }
-        const int s = owner(sum_at(x), b.nseq, e);
-        const PagedSeq q = record(s);
-        const SeqCount c = seq_count(seq_load(r, b.ldt, q.npast, q.M), mn ? per_many : per_few);
-        b.items[i] = seq_item(r, q, s, mn, c.np, sum_at(S_PART)[s], e - sum_at(x)[s]);
+        const int s = owner(sum_at(x), n, e);
+        b.items[i] = seq_item(r, of(s), s, mn, M[s], sum_at(S_PART)[s], e - sum_at(x)[s]);
     }
-    for (int i = g0; i < r.combs; i += gs) {
+    for (int i = from(7); i < r.combs; i += gs) {
         PagedComb o{};
         if (i < total(S_COMB)) {
-            const int s = owner(sum_at(S_COMB), b.nseq, i);
-            const PagedSeq q = record(s);
-            const SeqLoad l = seq_load(r, b.ldt, q.npast, q.M);
-            const SeqCount c = seq_count(l, l.many ? per_many : per_few);
-            o = seq_comb(r, q, s, l.many, c.np, sum_at(S_PART)[s], i - sum_at(S_COMB)[s]);
+            const int s = owner(sum_at(S_COMB), n, i);
+            const PagedSeq q = of(s);
+            o = seq_comb(r, q, s, q.M * r.gqa >= PAGED_MANY, M[s], sum_at(S_PART)[s], i - sum_at(S_COMB)[s]);
         }
         b.combs[i] = o;
     }
@@ -250,8 +345,8 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
 hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b) {
     const PagedRoom& r = b.r;
     const int64_t entries = (int64_t)r.tokens + r.nseq + r.touch + r.few + r.many + r.combs;
-    const bool one = (int64_t)b.nseq * r.n_pages <= 8192 && entries <= 8192;
-    const size_t bytes = (size_t)(b.nseq + 1) * (8 + 4 * N_SUMS + (one ? 4 : 0));
+    const bool one = (int64_t)b.nseq * r.n_pages <= ONE_MOST && entries <= ONE_MOST;
+    const size_t bytes = (size_t)(b.nseq + 1) * (8 + 4 * N_SUMS);
     static std::atomic<uint64_t> set_one{0}, set_many{0};
     const size_t most = (size_t)(PAGED_ROOM_SEQS + 1) * (8 + 4 * N_SUMS);
     hipError_t e = lds_limit(one ? (const void*)k_plan_build<true> : (const void*)k_plan_build<false>, most,
@@ -263,7 +358,7 @@ hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b) {
     }
     hipLaunchKernelGGL(k_plan_check, dim3((unsigned)(b.nseq + 3) / 4), dim3(256), 0, st, b);
     if ((e = hipGetLastError()) != hipSuccess) return e;
-    const unsigned wgs = (unsigned)std::min<int64_t>(64, (entries + NT - 1) / NT);
+    const unsigned wgs = (unsigned)std::min<int64_t>(128, (entries + NT - 1) / NT);
     hipLaunchKernelGGL(k_plan_build<false>, dim3(wgs), dim3(NT), bytes, st, b);
     return hipGetLastError();
 }

@@ -335,10 +335,11 @@ int paged_room(const PagedGeom& g, const ftx_plan_room& a, PagedRoom& r, std::st
     const double load = (double)(few * a.n_pages * g.n_kv) / (double)cu;
     r.wide = g.hd <= 128 && a.n_pages > 4 && a.n_pages <= WIDE_MOST && few * g.n_kv <= cu && !r.window &&
              (double)a.n_pages <= (g.hd == 64 ? 15 : 10) + 1.6 * load;
-    r.cut_few = r.wide ? 0 : (int32_t)(4 * cu / g.n_kv);
-    r.cut_many = big ? (int32_t)(2 * cu / g.n_kv) : 0;
+    // (no more than all lists together have, of four and two pages)
+    r.cut_few = r.wide ? 0 : (int32_t)std::min(4 * cu / g.n_kv, few * a.n_pages / 4);
+    r.cut_many = big ? (int32_t)std::min(2 * cu / g.n_kv, many * a.n_pages / 2) : 0;
     constexpr int64_t B = PAGED_TR_MANY / PAGED_TR;
-    if (few + many + r.cut_few + r.cut_many >= LIM / 2 || !paged_grid_fits((few + r.cut_few) * g.n_kv, r.wide ? 512 : 256) ||
+    if (few * a.n_pages >= LIM || many * a.n_pages >= LIM || few + many + r.cut_few + r.cut_many >= LIM / 2 || !paged_grid_fits((few + r.cut_few) * g.n_kv, r.wide ? 512 : 256) ||
         !paged_grid_fits((many + r.cut_many) * g.n_kv, 512))
         return fail(FTX_E_RANGE, "too many tokens or pages in one plan");
     r.few = (int32_t)(few + r.cut_few);
@@ -371,7 +372,7 @@ extern "C" int paged_build_probe(const ftx_plan_room* a, int64_t n_kv, int64_t h
             tokens += M[s];
         }
         if (tokens > r.tokens) return FTX_E_RANGE;
-        const int per[2] = {r.wide ? INT32_MAX : seq_per(total[0], r.cut_few, 4), seq_per(total[1], r.cut_many, 2)};
+        const int per[2] = {r.wide ? INT32_MAX : seq_per((int)total[0], r.cut_few, 4), seq_per((int)total[1], r.cut_many, 2)};
         int64_t at[2] = {0, 0}, part = 0, comb = 0, tok = 0;
         for (int64_t i = 0; i < r.few + r.many; ++i) items[i].seq = -1;
         for (int64_t i = 0; i < r.combs; ++i) combs[i] = PagedComb{};

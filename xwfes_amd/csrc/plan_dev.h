@@ -50,10 +50,10 @@ __host__ __device__ inline void seq_held(const PagedRoom& r, int p, int have, in
 
 // The most pages of a part of lists of `total` pages in all: a launch then has
 // some cut / n_kv workgroups more than it has lists
-__host__ __device__ inline int seq_per(int64_t total, int cut, int least) {
+__host__ __device__ inline int seq_per(int total, int cut, int least) {
     if (cut <= 0) return INT32_MAX;
-    const int64_t per = (total + cut - 1) / cut;
-    return per < least ? least : per > INT32_MAX ? INT32_MAX : (int)per;
+    const int per = total ? (total - 1) / cut + 1 : 0;
+    return per < least ? least : per;
 }
 // Entries of a sequence: parts of a list, items, blocks of partials, joins
 struct SeqCount {
@@ -63,7 +63,7 @@ __host__ __device__ inline SeqCount seq_count(const SeqLoad& l, int per) {
     SeqCount c{};
     if (l.tiles == 0) return c;
     const int b = l.many ? PAGED_TR_MANY / PAGED_TR : 1;
-    c.np = (int)(((int64_t)l.n + per - 1) / per);
+    c.np = per >= l.n ? 1 : (l.n - 1) / per + 1;
     c.items = l.tiles * c.np;
     c.parts = c.np > 1 ? c.items * b : 0;
     c.combs = c.np > 1 ? l.tiles * b : 0;
@@ -82,15 +82,17 @@ __host__ __device__ inline void tile_pages(const PagedRoom& r, int p, int m, int
 // Item e of sequence q (number s), its partials from part0 on; seq = -1: none (a
 // tile whose list is shorter than the sequence's longest)
 __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq& q, int s, int many, int np, int part0, int e) {
-    const int tr = many ? PAGED_TR_MANY : PAGED_TR, tile = e / np, k = e % np;
+    const int tr = many ? PAGED_TR_MANY : PAGED_TR, tile = e / np, k = e - tile * np;
     PagedItem it{};
     int n;
     tile_pages(r, q.npast, q.M, tile * tr, tr, it.s, it.a, n);
     const int npt = np < n ? np : n;
     it.seq = k < npt ? s : -1;
     it.row0 = tile * tr;
-    it.i0 = (int32_t)((int64_t)n * k / npt);
-    it.i1 = (int32_t)((int64_t)n * (k + 1) / npt);
+    // (the first n % npt parts are a page longer)
+    const int len = n / npt, rem = n - len * npt;
+    it.i0 = k * len + (k < rem ? k : rem);
+    it.i1 = it.i0 + len + (k < rem);
     it.part = np > 1 ? part0 + e * (tr / PAGED_TR) : -1;
     it.nt = many;
     it.q = q;

@@ -1031,6 +1031,377 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
     }
 }
 
+// ---------------------------------------------------------------- few rows of 4 bits
+// A lane's value from lane `st` of its group of U (2 or 4), or from the lane across
+template <int U, int ST>
+__device__ __forceinline__ float of_lane(float x) {
+    constexpr int b = ST % U, ctrl = U == 4 ? b * 0x55 : b | b << 2 | (2 + b) << 4 | (2 + b) << 6;
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), ctrl, 0xF, 0xF, false));
+}
+template <int X>  // 1 or 2
+__device__ __forceinline__ float across(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), X == 1 ? 0xB1 : 0x4E,
+                                                                 0xF, 0xF, false));
+}
+
+// One wave's online softmax over pages of 4-bit rows for at most 16 / U query
+// rows: a product's 16 columns are U for each row, column U r + u that of row r
+// and of the blocks of 32 dims U j + u (the query is zero in the others' dims).
+//   Scores: column (r, u) sums q k over its blocks, times the slot's multiplier of
+//   the block once it is summed (a multiplier a slot and block, not one a value),
+//   and the U columns are added so that each lane keeps the scores of one slot
+//   tile (two of U = 2): the softmax of a page is 4 (8) weights a lane and not 16.
+//   Outputs: column (r, u) takes the weights times the slots' multipliers of block
+//   u: column u holds the output dims of its blocks (the others' are not used).
+// As the products of rows past the last are made in any case, this trades them for
+// vector instructions, some 600 a page instead of 950, where the bytes of a page
+// (9216 at 128 dims) are to be read in the time of 960 on every SIMD.
+// Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256.
+template <int HD, int U>
+struct FoldAttn {
+    static constexpr int NB = HD / 32, J = NB > U ? NB / U : 1, NDT = HD / 16, S = 4 / U, NL = HD / 32, OWN = 2 * J;
+    static constexpr int64_t VB = paged_values_bytes(HD, PT_Q4), MB = paged_mult_bytes(HD, PT_Q4);
+    v8h qh[NB], ql[NB];
+    v4f o[NDT];
+    float off = -INFINITY, l = 0.f, lp = 0.f, c2;
+    int ev = EV_MIN;
+
+    // the largest of a row's lanes
+    static __device__ __forceinline__ float row_top(float x) {
+        x = fmaxf(x, across<1>(x));
+        if constexpr (U == 4) x = fmaxf(x, across<2>(x));
+        return col_max(x);
+    }
+
+    // the query row at q
+    __device__ __forceinline__ void query(const float* q, int u, int kq, bool vec) {
+        v4f x[J][2];
+        float a = 0.f;
+        const bool any = u < NB;  // (heads of 64 dims have two blocks)
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const int d0 = 32 * (U * j + (any ? u : 0)) + 8 * kq;
+            x[j][0] = ld4(q + d0, vec);
+            x[j][1] = ld4(q + d0 + 4, vec);
+        }
+        const float by = 1.4426950408889634f / sqrtf((float)HD);
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = rounded(x[j][i >> 2][i & 3] * by);
+                x[j][i >> 2][i & 3] = y;
+                a = fabsf(y) <= FLT_BIG ? fmaxf(a, fabsf(y)) : a;
+            }
+        a = row_top(a);
+        const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 126) : 0;
+        const float qs = ldexpf(1.f, e);
+        c2 = ldexpf(1.f, -e);
+        v8h h[J], lo[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                v2h hh, ll;
+                split_hl2(rounded(x[j][i >> 2][i & 3] * qs), rounded(x[j][i >> 2][(i & 3) + 1] * qs), hh, ll);
+                h[j][i] = hh[0];
+                h[j][i + 1] = hh[1];
+                lo[j][i] = ll[0];
+                lo[j][i + 1] = ll[1];
+            }
+        const v8h none = {};
+#pragma unroll
+        for (int dc = 0; dc < NB; ++dc) {
+            const bool mine = dc % U == u;
+            qh[dc] = mine ? h[dc / U] : none;
+            ql[dc] = mine ? lo[dc / U] : none;
+        }
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // A page's loads of K or V: values, the lane's blocks' multipliers of its 16
+    // slots, the scales of the slots that it keeps
+    struct Vals {
+        uint4 u[NL], c[J];
+        v4f s[S];
+    };
+    static __device__ __forceinline__ void load(Vals& x, const uint8_t* blk, bool v, int u, int kq, int lane) {
+        const uint8_t* vals = blk + (v ? VB : 0);
+        const uint8_t* mult = blk + 2 * VB + 2 * FTX_PAGE * 4 + (v ? MB : 0);
+        const float* scale = (const float*)(blk + 2 * VB) + (v ? FTX_PAGE : 0);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
+#pragma unroll
+        for (int j = 0; j < J; ++j) x.c[j] = *(const uint4*)(mult + 64 * (U * j + u % NB) + 16 * kq);
+#pragma unroll
+        for (int a = 0; a < S; ++a) x.s[a] = *(const v4f*)(scale + 16 * (U * a + u) + 4 * kq);
+    }
+    static __device__ __forceinline__ uint32_t word(const uint4& x, int i) {
+        return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w;
+    }
+    // multiplier of slot 16 st + 4 kq + i
+    static __device__ __forceinline__ float mult(const uint4& c, int st, int i) {
+        return (float)((word(c, st) >> (8 * i)) & 255);
+    }
+
+    // the scores, by the K scales, of the lane's slots
+    __device__ __forceinline__ void scores(v4f (&s)[S], const Vals& x, int u) const {
+        v4f p[J][4];
+#pragma unroll
+        for (int dc = 0; dc < NB; ++dc)
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1));
+                const v8h k = join(q4_low(w), q4_high(w), q4_low(w >> 8), q4_high(w >> 8));
+                v4f& a = p[dc / U][st];
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[dc], dc % U ? a : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[dc], a, 0, 0, 0);
+            }
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float t = p[0][st][i] * mult(x.c[0], st, i);
+#pragma unroll
+                for (int j = 1; j < J; ++j) t = __builtin_fmaf(p[j][st][i], mult(x.c[j], st, i), t);
+                p[0][st][i] = t;
+            }
+        // the columns' sum, each lane its own slot tiles': U a + u
+        const bool odd = u & 1, upper = u & 2;
+        v4f t[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                t[a][i] = (odd ? p[0][2 * a + 1][i] : p[0][2 * a][i]) + across<1>(odd ? p[0][2 * a][i] : p[0][2 * a + 1][i]);
+        if constexpr (U == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[0][i] = (upper ? t[1][i] : t[0][i]) + across<2>(upper ? t[0][i] : t[1][i]);
+        } else {
+            s[0] = t[0];
+            s[1] = t[1];
+        }
+#pragma unroll
+        for (int a = 0; a < S; ++a) s[a] *= x.s[a];
+    }
+
+    __device__ __forceinline__ void raise(int en) {
+        const float f = ldexpf(1.f, max(ev - en, -126));
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[dt] *= f;
+        ev = en;
+    }
+
+    // the page's weights (as WaveAttn's soften) and their outputs
+    __device__ __forceinline__ void take(v4f (&s)[S], Vals& x, bool whole, uint64_t sight, int u, int kq) {
+        if (!whole) {
+            const uint64_t seen = sight >> (4 * kq);
+#pragma unroll
+            for (int a = 0; a < S; ++a)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!((seen >> (16 * (U * a + u) + i)) & 1)) {
+                        s[a][i] = -INFINITY;
+                        x.s[a][i] = 0.f;
+                    }
+        }
+        l += lp;
+        // (`maximum`, which hands NaN on, as in WaveAttn)
+        float mx = __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[0][0], s[0][1]),
+                                                 __builtin_elementwise_maximum(s[0][2], s[0][3]));
+        float top = fmaxf(fmaxf(x.s[0][0], x.s[0][1]), fmaxf(x.s[0][2], x.s[0][3]));
+        if constexpr (S == 2) {
+            mx = __builtin_elementwise_maximum(
+                mx, __builtin_elementwise_maximum(__builtin_elementwise_maximum(s[1][0], s[1][1]),
+                                                  __builtin_elementwise_maximum(s[1][2], s[1][3])));
+            top = fmaxf(top, fmaxf(fmaxf(x.s[1][0], x.s[1][1]), fmaxf(x.s[1][2], x.s[1][3])));
+        }
+        mx = row_top(mx);
+        const bool over = __builtin_fmaf(mx, c2, -off) > 15.f;
+        if (__builtin_amdgcn_ballot_w64(over)) {
+            float cand = __builtin_fmaf(mx, c2, -12.f);
+            if (__builtin_fmaf(mx, c2, -cand) > 15.f) cand = mx * c2;
+            if (cand > FLT_BIG) cand = __builtin_nanf("");
+            const float on = over ? cand : off;
+            const float al = off == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(off - on);
+            off = on;
+            l *= al;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) o[dt] *= al;
+        }
+        const float on = off == -INFINITY ? 0.f : off;
+        if (__builtin_amdgcn_ballot_w64(top > ldexpf(1.f, ev))) raise(max(ev, ev_level(row_top(fmaxf(top, 0.f)))));
+        const float f = ldexpf(1.f, -ev - 8);
+        lp = 0.f;
+        v4f w[S];
+#pragma unroll
+        for (int a = 0; a < S; ++a)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[a][i], c2, -on));
+                lp += p;
+                w[a][i] = p * (x.s[a][i] * f);
+            }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            v8h ph[2], pl[2];
+            auto tile = [&](auto st_) {
+                constexpr int st = decltype(st_)::value;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    v2h h, lo;
+                    split_hl2(rounded(of_lane<U, st>(w[st / U][i]) * mult(x.c[j], st, i)),
+                              rounded(of_lane<U, st>(w[st / U][i + 1]) * mult(x.c[j], st, i + 1)), h, lo);
+                    const int at = 4 * (st & 1) + i;
+                    ph[st >> 1][at] = h[0];
+                    ph[st >> 1][at + 1] = h[1];
+                    pl[st >> 1][at] = lo[0];
+                    pl[st >> 1][at + 1] = lo[1];
+                }
+            };
+            tile(std::integral_constant<int, 0>{});
+            tile(std::integral_constant<int, 1>{});
+            tile(std::integral_constant<int, 2>{});
+            tile(std::integral_constant<int, 3>{});
+            // the dims of blocks U j .. U j + U - 1
+#pragma unroll
+            for (int dt = 2 * U * j; dt < 2 * U * (j + 1) && dt < NDT; ++dt)
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp) {
+                    const uint32_t y = word(x.u[dt >> 1], 2 * sp), z = word(x.u[dt >> 1], 2 * sp + 1);
+                    const v8h v = dt & 1 ? join(q4_high(y), q4_high(y >> 8), q4_high(z), q4_high(z >> 8))
+                                         : join(q4_low(y), q4_low(y >> 8), q4_low(z), q4_low(z >> 8));
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[sp], o[dt], 0, 0, 0);
+                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[sp], o[dt], 0, 0, 0);
+                }
+        }
+    }
+
+    // the lane's own outputs: own[2 j + e], dim tile 2 (U j + u) + e
+    __device__ __forceinline__ void pick(v4f (&own)[OWN], int u) const {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                own[2 * j + e] = o[2 * U * j + e];
+#pragma unroll
+                for (int x = 1; x < U && U * j + x < NB; ++x)
+                    if (u == x) own[2 * j + e] = o[2 * (U * j + x) + e];
+            }
+    }
+};
+
+// As k_paged_attn, at most 16 / U query rows a sequence
+template <int HD, int U, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
+    using W = FoldAttn<HD, U>;
+    __shared__ v4f so[NW - 1][W::OWN][64];
+    __shared__ float sm[NW][64], sl[NW][64];
+    __shared__ int se[NW][64];
+    const int kvh = blockIdx.x % a.p.n_kv;
+    const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
+    if (it.seq < 0) return;
+    const PagedSeq sq = it.q;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, u = lane & (U - 1), rr = (lane & 15) / U, kq = lane >> 4;
+    const int R = sq.M * a.gqa, r = min(rr, R - 1), t = r / a.gqa;
+    const int64_t tok = sq.tok0 + t;
+    const int head = kvh * a.gqa + r % a.gqa;
+    // the pages of the wave, as in k_paged_attn
+    const int n = max(0, (it.i1 - it.i0 - w + NW - 1) / NW);
+    auto place = [&](int j) {
+        const int i = it.i0 + w + NW * j;
+        return i < it.s ? i : it.a + (i - it.s);
+    };
+    int ids = lane < n ? a.p.table[sq.tab0 + place(lane)] : 0;
+    auto block_of = [&](int j) {
+        if ((j & 63) == 0 && j) ids = j + lane < n ? a.p.table[sq.tab0 + place(j + lane)] : 0;
+        return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
+    };
+    W wa;
+    wa.query(a.q + tok * a.ldq + (int64_t)head * HD, u, kq, !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15));
+    const RowSight sight(a, sq, t);
+    int hi = sight.hi, lo = sight.lo;
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) {
+        hi = min(hi, __shfl_xor(hi, x, 64));
+        lo = max(lo, __shfl_xor(lo, x, 64));
+    }
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    typename W::Vals kv, vv;
+    const uint8_t* blk = nullptr;
+    if (n) {
+        blk = block_of(0);
+        W::load(kv, blk, false, u, kq, lane);
+    }
+    for (int j = 0; j < n; ++j) {
+        W::load(vv, blk, true, u, kq, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        v4f s[W::S];
+        wa.scores(s, kv, u);
+        __builtin_amdgcn_sched_barrier(0);
+        const int p0 = place(j) * FTX_PAGE;
+        if (j + 1 < n) {
+            blk = block_of(j + 1);
+            W::load(kv, blk, false, u, kq, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);
+        wa.take(s, vv, whole, whole ? 0 : sight.page(p0), u, kq);
+    }
+    wa.l += wa.lp;
+    wa.l += across<1>(wa.l);
+    if constexpr (U == 4) wa.l += across<2>(wa.l);
+    wa.l += __shfl_xor(wa.l, 16, 64);
+    wa.l += __shfl_xor(wa.l, 32, 64);
+    v4f own[W::OWN];
+    wa.pick(own, u);
+    sm[w][lane] = wa.off;
+    sl[w][lane] = wa.l;
+    se[w][lane] = wa.ev;
+    if (w)
+#pragma unroll
+        for (int x = 0; x < W::OWN; ++x) so[w - 1][x][lane] = own[x];
+    __syncthreads();
+    if (w) return;
+    float M = wa.off, f[NW], L = 0.f;
+    int EV = wa.ev;
+#pragma unroll
+    for (int x = 1; x < NW; ++x) {
+        M = fmaxf(M, sm[x][lane]);
+        EV = max(EV, se[x][lane]);
+    }
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+        const float mx = sm[x][lane];
+        f[x] = mx == M ? 1.f : __builtin_amdgcn_exp2f(mx - M);
+        L += f[x] * sl[x][lane];
+        f[x] = ldexpf(f[x], se[x][lane] - EV);
+    }
+    if (rr >= R || u >= W::NB) return;
+    const bool part = it.part >= 0;
+    const int64_t prow = ((int64_t)it.part * a.p.n_kv + kvh) * PAGED_TR + rr;
+    float* dst = part ? a.part + prow * HD : a.out + tok * a.ldo + (int64_t)head * HD;
+    const bool vec = part || !(((uintptr_t)a.out | (uintptr_t)(a.ldo * 4)) & 15);
+    const float inv = part && L == 0.f ? 0.f : 1.f / L;  // (as in k_paged_attn)
+#pragma unroll
+    for (int x = 0; x < W::OWN; ++x) {
+        v4f y = own[x] * f[0];
+#pragma unroll
+        for (int z = 1; z < NW; ++z) y += so[z - 1][x][lane] * f[z];
+#pragma unroll
+        for (int z = 0; z < 4; ++z) y[z] = ldexpf(y[z] * inv, EV + 8);
+        st4(dst + 32 * (U * (x >> 1) + u) + 16 * (x & 1) + 4 * kq, y, vec);
+    }
+    if (part && kq == 0 && u == 0) {
+        a.pml[2 * prow] = M;
+        a.pml[2 * prow + 1] = L;
+    }
+}
+
 typedef __attribute__((address_space(3))) void lds_void;
 
 // Many rows: workgroup = (item of 128 or 256 rows, kv head), eight waves of one
@@ -1424,13 +1795,28 @@ static auto attn_wide() {
     return k_paged_attn<HD, KT, HD <= 128 ? 8 : 4>;
 }
 
+// of 4-bit rows and heads of 64 or 128 dims, by the most query rows of a sequence
+typedef void (*paged_kernel)(PagedAttn);
+template <int U, int NW>
+static paged_kernel fold_hd(int hd) {
+    return hd == 64 ? k_paged_fold<64, U, NW> : k_paged_fold<128, U, NW>;
+}
+static paged_kernel fold_of(int rows, int hd, bool wide) {
+    if (rows <= 4) return wide ? fold_hd<4, 8>(hd) : fold_hd<4, 4>(hd);
+    if (rows <= 8) return wide ? fold_hd<2, 8>(hd) : fold_hd<2, 4>(hd);
+    return nullptr;
+}
+
 hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     hipError_t e = hipSuccess;
     if (a.n_many) e = PAGED_CASE(launch_many, a.p.hd, a.p.kt)(st, a);
     if (e != hipSuccess) return e;
     if (a.n_few) {
         const dim3 grid((unsigned)a.n_few * (unsigned)a.p.n_kv);
-        if (a.wide)
+        auto* fold = a.p.kt != PT_Q4 || a.p.hd == 256 ? nullptr : fold_of(a.rows_max, a.p.hd, a.wide);
+        if (fold)
+            ktimed_launch(fold, grid, dim3(a.wide ? 512 : 256), 0, st, a);
+        else if (a.wide)
             ktimed_launch(PAGED_CASE(attn_wide, a.p.hd, a.p.kt)(), grid, dim3(512), 0, st, a);
         else
             ktimed_launch(PAGED_CASE(attn_four, a.p.hd, a.p.kt)(), grid, dim3(256), 0, st, a);

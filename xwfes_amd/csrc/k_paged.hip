@@ -364,11 +364,22 @@ __device__ __forceinline__ v8h u8x8(uint32_t a, uint32_t b) {
 
 // 4-bit values under their multipliers as halves (exact: |q c| <= 2040).  A nibble
 // n = q + 8 under 0x64 is 1024 + n, four bits up under 0x54 it is 64 + n.
+// (the constants in registers, so that `and` and `or` are one instruction)
+__device__ __forceinline__ uint32_t in_sgpr(uint32_t x) {
+    asm("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
+    asm("" : "+v"(x));
+    return x;
+}
 __device__ __forceinline__ v2h q4_low(uint32_t x) {
-    return __builtin_bit_cast(v2h, (x & 0x000F000Fu) | 0x64006400u) + v2h{(_Float16)(-1032.f), (_Float16)(-1032.f)};
+    return __builtin_bit_cast(v2h, (x & in_sgpr(0x000F000Fu)) | in_vgpr(0x64006400u)) +
+           v2h{(_Float16)(-1032.f), (_Float16)(-1032.f)};
 }
 __device__ __forceinline__ v2h q4_high(uint32_t x) {
-    return __builtin_bit_cast(v2h, (x & 0x00F000F0u) | 0x54005400u) + v2h{(_Float16)(-72.f), (_Float16)(-72.f)};
+    return __builtin_bit_cast(v2h, (x & in_sgpr(0x00F000F0u)) | in_vgpr(0x54005400u)) +
+           v2h{(_Float16)(-72.f), (_Float16)(-72.f)};
 }
 __device__ __forceinline__ v8h join(v2h a, v2h b, v2h c, v2h d) {
     return v8h{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
@@ -1146,19 +1157,42 @@ struct FoldAttn {
         return (float)((word(c, st) >> (8 * i)) & 255);
     }
 
+    // Eight products, between each two of which go four or five of the vector
+    // instructions that make the next eight's operands
+    static __device__ __forceinline__ void beside() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);
+        }
+    }
+
     // the scores, by the K scales, of the lane's slots
     __device__ __forceinline__ void scores(v4f (&s)[S], const Vals& x, int u) const {
         v4f p[J][4];
-#pragma unroll
-        for (int dc = 0; dc < NB; ++dc)
+        v8h k[2][4];
+        auto make = [&](int dc) {
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
                 const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1));
-                const v8h k = join(q4_low(w), q4_high(w), q4_low(w >> 8), q4_high(w >> 8));
-                v4f& a = p[dc / U][st];
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[dc], dc % U ? a : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                a = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[dc], a, 0, 0, 0);
+                k[dc & 1][st] = join(q4_low(w), q4_high(w), q4_low(w >> 8), q4_high(w >> 8));
             }
+        };
+        make(0);
+#pragma unroll
+        for (int dc = 0; dc < NB; ++dc) {
+            if (dc + 1 < NB) make(dc + 1);
+            v4f(&a)[4] = p[dc / U];
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                a[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[dc & 1][st], ql[dc],
+                                                               dc % U ? a[st] : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                a[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[dc & 1][st], qh[dc], a[st], 0, 0, 0);
+            if (dc + 1 < NB) beside();
+            __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int st = 0; st < 4; ++st)
 #pragma unroll
@@ -1265,17 +1299,35 @@ struct FoldAttn {
             tile(std::integral_constant<int, 1>{});
             tile(std::integral_constant<int, 2>{});
             tile(std::integral_constant<int, 3>{});
-            // the dims of blocks U j .. U j + U - 1
-#pragma unroll
-            for (int dt = 2 * U * j; dt < 2 * U * (j + 1) && dt < NDT; ++dt)
+            // the dims of blocks U j .. U j + U - 1, two dim tiles each
+            constexpr int N = NB < U ? NB : U;
+            v8h v[2][2][2];  // [block's parity][dim tile][slots' half]
+            auto make = [&](int g) {
 #pragma unroll
                 for (int sp = 0; sp < 2; ++sp) {
-                    const uint32_t y = word(x.u[dt >> 1], 2 * sp), z = word(x.u[dt >> 1], 2 * sp + 1);
-                    const v8h v = dt & 1 ? join(q4_high(y), q4_high(y >> 8), q4_high(z), q4_high(z >> 8))
-                                         : join(q4_low(y), q4_low(y >> 8), q4_low(z), q4_low(z >> 8));
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[sp], o[dt], 0, 0, 0);
-                    o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[sp], o[dt], 0, 0, 0);
+                    const uint32_t y = word(x.u[U * j + g], 2 * sp), z = word(x.u[U * j + g], 2 * sp + 1);
+                    const uint32_t y8 = y >> 8, z8 = z >> 8;
+                    v[g & 1][0][sp] = join(q4_low(y), q4_low(y8), q4_low(z), q4_low(z8));
+                    v[g & 1][1][sp] = join(q4_high(y), q4_high(y8), q4_high(z), q4_high(z8));
                 }
+            };
+            make(0);
+#pragma unroll
+            for (int g = 0; g < N; ++g) {
+                if (g + 1 < N) make(g + 1);
+                v4f* const d = o + 2 * (U * j + g);
+#pragma unroll
+                for (int sp = 0; sp < 2; ++sp) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        d[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][e][sp], pl[sp], d[e], 0, 0, 0);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        d[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[g & 1][e][sp], ph[sp], d[e], 0, 0, 0);
+                }
+                if (g + 1 < N) beside();
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 

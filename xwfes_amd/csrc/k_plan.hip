@@ -92,7 +92,8 @@ template <bool CHECK>
 __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedRoom& r = b.r;
-    enum { T_FEW, T_MANY, T_TOK, T_FRESH, T_CODE, N_TOT };  // (page lists' totals stay below 2^31: paged_room)
+    enum { T_FEW, T_MANY, T_LISTS, T_TOK, T_FRESH, T_CODE, N_TOT };  // (page lists' totals stay below 2^31: paged_room)
+    __shared__ int parts_of[NW][FEW_TRIES];
     __shared__ int tot[NW][N_TOT], sum_of[NW][N_SUMS], rows_of[NW][2], bad_of[NW];
     const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, n = b.nseq, n1 = n + 1;
     int* const P = (int*)lds;  // [n] lengths
@@ -169,6 +170,7 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
         const uint32_t pages = (uint32_t)(l.tiles * l.n);
         t[T_FEW] = sat_add(t[T_FEW], l.many ? 0 : pages);
         t[T_MANY] = sat_add(t[T_MANY], l.many ? pages : 0);
+        t[T_LISTS] = sat_add(t[T_LISTS], l.many ? 0 : (uint32_t)l.tiles);
         t[T_TOK] = sat_add(t[T_TOK], (uint32_t)M[s]);
         t[T_FRESH] = sat_add(t[T_FRESH], (uint32_t)(l.need - l.have));
     }
@@ -202,7 +204,34 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
                 bad |= pg < 0 || pg >= r.pool_pages;
             }
     }
-    const int per_few = r.wide ? INT32_MAX : seq_per((int)t[T_FEW], r.cut_few, 4);
+    int per_few = INT32_MAX;
+    if (r.cut_few) {
+        // (parts of each try, of all lists)
+        uint32_t parts[FEW_TRIES] = {};
+        int tries[FEW_TRIES];
+#pragma unroll
+        for (int k = 0; k < FEW_TRIES; ++k) tries[k] = try_per((int)t[T_FEW], r.slots, (int)t[T_LISTS], k);
+        for (int s = s0; s < s1; ++s) {
+            const SeqLoad l = seq_load(r, b.ldt, P[s], M[s]);
+            if (l.many) continue;
+#pragma unroll
+            for (int k = 0; k < FEW_TRIES; ++k) parts[k] = sat_add(parts[k], (uint32_t)(l.tiles * seq_parts(l.n, tries[k])));
+        }
+#pragma unroll
+        for (int k = 0; k < FEW_TRIES; ++k) {
+            const int v = wave_total((int)parts[k]);
+            if (lane == 0) parts_of[w][k] = v;
+        }
+        lds_barrier();
+        per_few = else_per((int)t[T_FEW], r.slots, (int)t[T_LISTS]);
+#pragma unroll
+        for (int k = FEW_TRIES - 1; k >= 0; --k) {
+            uint32_t v = 0;
+#pragma unroll
+            for (int i = 0; i < NW; ++i) v = sat_add(v, (uint32_t)parts_of[i][k]);
+            if (v <= (uint32_t)r.slots && (int)t[T_LISTS] < r.slots) per_few = tries[k];
+        }
+    }
     const int per_many = seq_per((int)t[T_MANY], r.cut_many, 2);
     int mine[N_SUMS] = {};
     int64_t rows = 0;

@@ -95,6 +95,7 @@ struct PagedGeom {
     int64_t n_kv = 0, hd = 0, n_pages = 0;
     const uint8_t* taken = nullptr;
     int cu = 0;
+    int kt = PT_F16;
 };
 struct PagedTables {
     int64_t n_head = 0, window = 0, sinks = 0;
@@ -135,7 +136,9 @@ struct PagedRoom {
     int32_t nseq, tokens, most, n_pages;  // sequences, new tokens of all, of one; pages of one
     int32_t pool_pages, n_kv, gqa;        // gqa = 0: no attention
     int32_t window, sinks;
-    int32_t cut_few, cut_many;  // parts that lists are cut into beyond one each (seq_per)
+    // parts that lists of many rows are cut into beyond one each (seq_per); of few
+    // rows: workgroups a kv head that fill the chip, and the most such parts
+    int32_t cut_many, slots, cut_few;
     int32_t wide;               // lists of few rows stay whole, for workgroups of eight waves
     int32_t few, many, combs, parts, touch;  // entries
 };

@@ -61,6 +61,17 @@ struct LaunchCost {
     }
 };
 
+// plan_dev.h's division of lists of few rows; parts(per): of all lists
+template <typename F>
+int few_per(int total, int slots, int lists, F parts) {
+    if (slots == 0) return INT32_MAX;
+    for (int k = 0; k < FEW_TRIES && lists < slots; ++k) {
+        const int per = try_per(total, slots, lists, k);
+        if (parts(per) <= slots) return per;
+    }
+    return else_per(total, slots, lists);
+}
+
 }  // namespace
 
 int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_t>& mark,
@@ -204,7 +215,13 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
         if (g.hd <= 128 && longest > 4 && longest <= WIDE_MOST && (int64_t)tiles.size() * g.n_kv <= cu &&
             (double)longest <= (g.hd == 64 ? 15 : 10) + 1.6 * load)
             return Few{true, INT32_MAX, 6 + std::max((0.17 + 0.17 * (double)g.hd / 128) * (double)longest, 0.6 * load)};
-        const int64_t per = std::max<int64_t>(4, (total * g.n_kv + 4 * cu - 1) / (4 * cu));
+        int64_t per = std::max<int64_t>(4, (total * g.n_kv + 4 * cu - 1) / (4 * cu));
+        if (g.kt == PT_Q4 && total <= INT32_MAX)
+            per = few_per((int)total, (int)(2 * cu / g.n_kv), (int)tiles.size(), [&](int p) {
+                int64_t n = 0;
+                for (const Tile& t : tiles) n += seq_parts(t.n, p);
+                return n;
+            });
         return Few{false, per, LaunchCost{g.n_kv, g.hd, 2 * cu, 8, 0.8 * (double)g.hd / 128}(tiles, per)};
     };
     std::vector<Tile> tiles[2], big;  // of PAGED_TR rows, of many
@@ -327,8 +344,8 @@ int paged_room(const PagedGeom& g, const ftx_plan_room& a, PagedRoom& r, std::st
     const int64_t few = std::min(a.nseq * each, rows / PAGED_TR + std::min(a.nseq, a.tokens));
     const int64_t big = longest >= PAGED_MANY ? std::min(a.nseq, rows / PAGED_MANY) : 0;
     const int64_t many = big ? rows / PAGED_TR_MANY + big : 0;
-    // Lists are cut so that a launch has four (few rows) or two (many) workgroups a
-    // CU more than it has lists, as far as they have pages: a part has total / cut
+    // Lists are cut so that a launch has two workgroups a CU (few rows), or as many
+    // more than it has lists (many), as far as they have pages: a part has total / cut
     // pages at least, so at most `cut` lists are cut, into 2 cut parts in all.
     // Whole lists, for eight waves, by the rule of a step's own plan for lists as
     // long as the room.
@@ -336,7 +353,8 @@ int paged_room(const PagedGeom& g, const ftx_plan_room& a, PagedRoom& r, std::st
     r.wide = g.hd <= 128 && a.n_pages > 4 && a.n_pages <= WIDE_MOST && few * g.n_kv <= cu && !r.window &&
              (double)a.n_pages <= (g.hd == 64 ? 15 : 10) + 1.6 * load;
     // (no more than all lists together have, of four and two pages)
-    r.cut_few = r.wide ? 0 : (int32_t)std::min(4 * cu / g.n_kv, few * a.n_pages / 4);
+    r.slots = (int32_t)(2 * cu / g.n_kv);
+    r.cut_few = r.wide ? 0 : (int32_t)std::min<int64_t>(r.slots, few * a.n_pages / 4);
     r.cut_many = big ? (int32_t)std::min(2 * cu / g.n_kv, many * a.n_pages / 2) : 0;
     constexpr int64_t B = PAGED_TR_MANY / PAGED_TR;
     if (few * a.n_pages >= LIM || many * a.n_pages >= LIM || few + many + r.cut_few + r.cut_many >= LIM / 2 || !paged_grid_fits((few + r.cut_few) * g.n_kv, r.wide ? 512 : 256) ||
@@ -365,14 +383,24 @@ extern "C" int paged_build_probe(const ftx_plan_room* a, int64_t n_kv, int64_t h
         if (rc) return rc;
         if (r.few + r.many > max_out || r.combs > max_out || nseq > r.nseq) return FTX_E_RANGE;
         int64_t total[2] = {0, 0}, tokens = 0;
+        int lists = 0;
         for (int64_t s = 0; s < nseq; ++s) {
             const SeqLoad l = seq_load(r, r.n_pages, npast[s], M[s]);
             if (l.code) return l.code;
             total[l.many] += (int64_t)l.tiles * l.n;
+            lists += l.many ? 0 : l.tiles;
             tokens += M[s];
         }
         if (tokens > r.tokens) return FTX_E_RANGE;
-        const int per[2] = {r.wide ? INT32_MAX : seq_per((int)total[0], r.cut_few, 4), seq_per((int)total[1], r.cut_many, 2)};
+        const int few = r.cut_few == 0 ? INT32_MAX : few_per((int)total[0], r.slots, lists, [&](int p) {
+            int64_t n = 0;
+            for (int64_t s = 0; s < nseq; ++s) {
+                const SeqLoad l = seq_load(r, r.n_pages, npast[s], M[s]);
+                if (!l.many) n += (int64_t)l.tiles * seq_parts(l.n, p);
+            }
+            return n;
+        });
+        const int per[2] = {few, seq_per((int)total[1], r.cut_many, 2)};
         int64_t at[2] = {0, 0}, part = 0, comb = 0, tok = 0;
         for (int64_t i = 0; i < r.few + r.many; ++i) items[i].seq = -1;
         for (int64_t i = 0; i < r.combs; ++i) combs[i] = PagedComb{};
@@ -811,6 +839,7 @@ int ftx_plan_set(ftx_plan* pl, const ftx_plan_args* a) {
         g.n_pages = pl->pool->n_pages;
         g.taken = pl->pool->taken.data();
         g.cu = ctx->cu_count;
+        g.kt = pl->pool->kt;
         PagedTables t;
         std::string err;
         const int rc = paged_tables(g, *a, pl->mark, pl->epoch, t, err);

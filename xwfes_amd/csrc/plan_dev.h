@@ -55,6 +55,23 @@ __host__ __device__ inline int seq_per(int total, int cut, int least) {
     const int per = total ? (total - 1) / cut + 1 : 0;
     return per < least ? least : per;
 }
+// The most pages of a part where `lists` lists of few rows, `total` pages in all,
+// share a chip that takes `slots` workgroups a kv head at once, two a CU.  One round
+// is filled where that can be: parts of try_per pages, the first (finest) of FEW_TRIES
+// that gives at most `slots` parts; else what is left of a round for each page, or
+// half a round where that is less (long lists among many short ones).  16 sequences
+// over 820 to 8192 slots of 4 bits 25.2 us, by four workgroups a CU, in rounds, 30.1;
+// one over 131072 38.6 and 43.9; 64 over up to 2000, whole, 24.4, cut 32
+constexpr int FEW_TRIES = 3;
+__host__ __device__ inline int try_per(int total, int slots, int lists, int k) {
+    const int left = slots - (int)((int64_t)lists * (k + 1) / (FEW_TRIES + 1));
+    return lists < slots ? seq_per(total, left, 4) : INT32_MAX;
+}
+__host__ __device__ inline int else_per(int total, int slots, int lists) {
+    const int left = slots - lists;
+    return seq_per(total, left > slots / 2 ? left : slots / 2, 4);
+}
+__host__ __device__ inline int seq_parts(int n, int per) { return per >= n ? 1 : (n - 1) / per + 1; }
 // Entries of a sequence: parts of a list, items, blocks of partials, joins
 struct SeqCount {
     int np, items, parts, combs;
@@ -63,7 +80,7 @@ __host__ __device__ inline SeqCount seq_count(const SeqLoad& l, int per) {
     SeqCount c{};
     if (l.tiles == 0) return c;
     const int b = l.many ? PAGED_TR_MANY / PAGED_TR : 1;
-    c.np = per >= l.n ? 1 : (l.n - 1) / per + 1;
+    c.np = seq_parts(l.n, per);
     c.items = l.tiles * c.np;
     c.parts = c.np > 1 ? c.items * b : 0;
     c.combs = c.np > 1 ? l.tiles * b : 0;

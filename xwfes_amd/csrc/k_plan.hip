@@ -32,9 +32,13 @@ __global__ void __launch_bounds__(256) k_plan_check(PagedBuild b) {
     if (lane == 0) b.codes[s] = c;
 }
 
-// (four waves, one a SIMD: every wave forms the same sums, so that sixteen take
-// four times as long for it: 16 sequences 13.3 us)
-constexpr int NT = 256, NW = NT / 64;
+// Threads of a workgroup: the only one has its entries to write as well (us for 16
+// sequences 256: 13.5, 512: 13.1, 1024: 15.5), of several each the sums alone (512
+// sequences 18.0, 19.5)
+template <bool CHECK>
+constexpr int build_threads() {
+    return CHECK ? 512 : 256;
+}
 constexpr int ONE_MOST = 6144;  // table entries (and others) of a build by one workgroup
 
 // Between the waves' uses of LDS: what is on its way to global memory is not
@@ -89,7 +93,8 @@ enum { S_TOK, S_FRESH, S_TOUCH, S_FEW, S_MANY, S_PART, S_COMB, N_SUMS };
 // the waves, the first of totals (how lists are cut follows from them), the second
 // of running sums and what the list of pages holds.
 template <bool CHECK>
-__global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
+__global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuild b) {
+    constexpr int NT = build_threads<CHECK>(), NW = NT / 64;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const PagedRoom& r = b.r;
     enum { T_FEW, T_MANY, T_LISTS, T_TOK, T_FRESH, T_CODE, N_TOT };  // (page lists' totals stay below 2^31: paged_room)
@@ -100,6 +105,9 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     int* const M = P + n;      // (in the end the parts of a list)
     int* const sums = M + n;   // [N_SUMS][n1] (CHECK: first have, s and a of seq_held)
     const int per = (n + NT - 1) / NT, s0 = min(tid * per, n), s1 = min(s0 + per, n);
+    // waves that have sequences form their sums, the others wait: all would share the
+    // SIMDs (16 sequences, sixteen waves that all form sums: 13.3 us)
+    const bool busy = __builtin_amdgcn_readfirstlane(w) * 64 * per < n;
     // The first loads, none of which waits for another: the lengths, the first
     // table entries whether they are pages or not, and (next) the list from `used` on
     // (a wave takes a sequence's entries 64 at a time, every NW-th sequence, so that
@@ -108,20 +116,26 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     const int chunks = (r.n_pages + 63) / 64, wv = __builtin_amdgcn_readfirstlane(w);
     const int loads = wv < n ? ((n - 1 - wv) / NW + 1) * chunks : 0;
     int id[U];
-    // the first load's sequence and chunk, and the next one's
-    auto next = [&](int& s, int& c) {
-        if (++c == chunks) {
-            c = 0;
-            s += NW;
+    // (a place past the row's end reads its last entry)
+    const int row = (int)min((int64_t)r.n_pages, b.ldt);
+    struct Walk {
+        int s, c;  // sequence, chunk
+    };
+    auto next = [&](Walk& x) {
+        if (++x.c == chunks) {
+            x.c = 0;
+            x.s += NW;
         }
     };
-    int ls = wv, lc = 0;
+    Walk lw{wv, 0};
+    const int32_t* from_row = b.tables + wv * b.ldt;
     auto load = [&](int e0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int i = 64 * lc + lane;
-            id[u] = e0 + u < loads && i < r.n_pages && i < b.ldt ? b.tables[ls * b.ldt + i] : 0;
-            next(ls, lc);
+            if (e0 + u >= loads) break;
+            id[u] = from_row[min(64 * lw.c + lane, row - 1)];
+            next(lw);
+            if (lw.c == 0) from_row += NW * b.ldt;
         }
     };
     if constexpr (CHECK) load(0);
@@ -144,18 +158,25 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     const int mine_at = base >= 0 && base <= b.n_free && tid < b.n_free - base ? b.free_pages[base + tid] : 0;
     if constexpr (CHECK) {
         lds_barrier();
-        int cs = wv, cc = 0;
+        Walk x{wv, 0};
+        int have = 0, hs = 0, ha = 0;
+        int32_t* to_row = b.table + (int64_t)wv * r.n_pages;
         for (int e0 = 0; e0 < loads;) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if (e0 + u >= loads) break;
-                const int i = 64 * cc + lane, have = __builtin_amdgcn_readfirstlane(sums[cs]);
-                const int hs = __builtin_amdgcn_readfirstlane(sums[n1 + cs]), ha = __builtin_amdgcn_readfirstlane(sums[2 * n1 + cs]);
+                if (x.c == 0) {
+                    have = __builtin_amdgcn_readfirstlane(sums[x.s]);
+                    hs = __builtin_amdgcn_readfirstlane(sums[n1 + x.s]);
+                    ha = __builtin_amdgcn_readfirstlane(sums[2 * n1 + x.s]);
+                }
+                const int i = 64 * x.c + lane;
                 if (i < have && (i < hs || i >= ha)) {
                     if ((uint32_t)id[u] >= (uint32_t)r.pool_pages) code = FTX_E_INVALID;
-                    b.table[cs * r.n_pages + i] = id[u];
+                    to_row[i] = id[u];
                 }
-                next(cs, cc);
+                next(x);
+                if (x.c == 0) to_row += (int64_t)NW * r.n_pages;
             }
             e0 += U;
             if (e0 < loads) load(e0);
@@ -176,7 +197,7 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     }
 #pragma unroll
     for (int x = 0; x < T_CODE; ++x) {
-        const int v = wave_total((int)t[x]);
+        const int v = busy ? wave_total((int)t[x]) : 0;
         if (lane == 0) tot[w][x] = v;
     }
     // (the lowest code: of 0, -1, -4, -5)
@@ -185,11 +206,11 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     if (lane == 0) tot[w][T_CODE] = code;
     lds_barrier();
 #pragma unroll
-    for (int x = 0; x < T_CODE; ++x) {
-        t[x] = 0;
+    for (int x = 0; x < T_CODE; ++x) t[x] = (uint32_t)tot[0][x];
 #pragma unroll
-        for (int i = 0; i < NW; ++i) t[x] = sat_add(t[x], (uint32_t)tot[i][x]);
-    }
+    for (int i = 1; i < NW; ++i)
+#pragma unroll
+        for (int x = 0; x < T_CODE; ++x) t[x] = sat_add(t[x], (uint32_t)tot[i][x]);
 #pragma unroll
     for (int i = 0; i < NW; ++i) code = min(code, tot[i][T_CODE]);
     if (t[T_TOK] > (uint32_t)r.tokens) code = FTX_E_RANGE;
@@ -219,16 +240,16 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
         }
 #pragma unroll
         for (int k = 0; k < FEW_TRIES; ++k) {
-            const int v = wave_total((int)parts[k]);
+            const int v = busy ? wave_total((int)parts[k]) : 0;
             if (lane == 0) parts_of[w][k] = v;
         }
         lds_barrier();
         per_few = else_per((int)t[T_FEW], r.slots, (int)t[T_LISTS]);
 #pragma unroll
         for (int k = FEW_TRIES - 1; k >= 0; --k) {
-            uint32_t v = 0;
+            uint32_t v = (uint32_t)parts_of[0][k];
 #pragma unroll
-            for (int i = 0; i < NW; ++i) v = sat_add(v, (uint32_t)parts_of[i][k]);
+            for (int i = 1; i < NW; ++i) v = sat_add(v, (uint32_t)parts_of[i][k]);
             if (v <= (uint32_t)r.slots && (int)t[T_LISTS] < r.slots) per_few = tries[k];
         }
     }
@@ -248,11 +269,14 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
     if (code == FTX_OK)
         for (int s = s0; s < s1; ++s) np = add(s, mine, rows);
     const int64_t own_rows = rows;
-    int at[N_SUMS];
+    int at[N_SUMS] = {}, low = 0, high = 0;
+    if (busy) {
 #pragma unroll
-    for (int x = 0; x < N_SUMS; ++x) at[x] = wave_upto<false>(mine[x]);
-    // (up to 2^30 positions a sequence: in two parts)
-    const int low = wave_upto<false>((int)(rows & 0xFFFF)), high = wave_upto<false>((int)(rows >> 16));
+        for (int x = 0; x < N_SUMS; ++x) at[x] = wave_upto<false>(mine[x]);
+        // (up to 2^30 positions a sequence: in two parts)
+        low = wave_upto<false>((int)(rows & 0xFFFF));
+        high = wave_upto<false>((int)(rows >> 16));
+    }
     const bool any = __builtin_amdgcn_ballot_w64(bad);
     if (lane == 63) {
 #pragma unroll
@@ -266,8 +290,10 @@ __global__ void __launch_bounds__(NT) k_plan_build(PagedBuild b) {
 #pragma unroll
     for (int x = 0; x < N_SUMS; ++x) at[x] -= mine[x];
 #pragma unroll
-    for (int i = 0; i < NW; ++i) {
+    for (int i = 0; i < NW; ++i)
         if (bad_of[i]) code = min(code, FTX_E_INVALID);
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
         if (i >= w) continue;
         rows += rows_of[i][0] + ((int64_t)rows_of[i][1] << 16);
 #pragma unroll
@@ -382,11 +408,12 @@ hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b) {
                              one ? set_one : set_many);
     if (e != hipSuccess) return e;
     if (one) {
-        hipLaunchKernelGGL(k_plan_build<true>, dim3(1), dim3(NT), bytes, st, b);
+        hipLaunchKernelGGL(k_plan_build<true>, dim3(1), dim3(build_threads<true>()), bytes, st, b);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(k_plan_check, dim3((unsigned)(b.nseq + 3) / 4), dim3(256), 0, st, b);
     if ((e = hipGetLastError()) != hipSuccess) return e;
+    constexpr int NT = build_threads<false>();
     const unsigned wgs = (unsigned)std::min<int64_t>(128, (entries + NT - 1) / NT);
     hipLaunchKernelGGL(k_plan_build<false>, dim3(wgs), dim3(NT), bytes, st, b);
     return hipGetLastError();

@@ -5,6 +5,21 @@
 
 #include "paged.h"
 
+// a / b, a >= 0, b > 0.  On the device by a reciprocal, off by at most one below
+// 2^22 (8 instructions and not 40 one after the other: the build is their latency)
+__host__ __device__ inline int idiv(int a, int b) {
+#ifdef __HIP_DEVICE_COMPILE__
+    if (a < 1 << 22) {
+        int q = (int)((float)a * __builtin_amdgcn_rcpf((float)b));
+        const int rem = a - q * b;
+        q += rem >= b;
+        q -= rem < 0;
+        return q;
+    }
+#endif
+    return a / b;
+}
+
 // What a sequence of p tokens and m new ones has to do, or an FTX_E_* code
 struct SeqLoad {
     int code;
@@ -52,7 +67,7 @@ __host__ __device__ inline void seq_held(const PagedRoom& r, int p, int have, in
 // some cut / n_kv workgroups more than it has lists
 __host__ __device__ inline int seq_per(int total, int cut, int least) {
     if (cut <= 0) return INT32_MAX;
-    const int per = total ? (total - 1) / cut + 1 : 0;
+    const int per = total ? idiv(total - 1, cut) + 1 : 0;
     return per < least ? least : per;
 }
 // The most pages of a part where `lists` lists of few rows, `total` pages in all,
@@ -71,7 +86,7 @@ __host__ __device__ inline int else_per(int total, int slots, int lists) {
     const int left = slots - lists;
     return seq_per(total, left > slots / 2 ? left : slots / 2, 4);
 }
-__host__ __device__ inline int seq_parts(int n, int per) { return per >= n ? 1 : (n - 1) / per + 1; }
+__host__ __device__ inline int seq_parts(int n, int per) { return per >= n ? 1 : idiv(n - 1, per) + 1; }
 // Entries of a sequence: parts of a list, items, blocks of partials, joins
 struct SeqCount {
     int np, items, parts, combs;
@@ -89,7 +104,7 @@ __host__ __device__ inline SeqCount seq_count(const SeqLoad& l, int per) {
 
 // The pages of the tile at row row0: [0, s) and then n - s from a on
 __host__ __device__ inline void tile_pages(const PagedRoom& r, int p, int m, int row0, int tr, int& s, int& a, int& n) {
-    const int R = m * r.gqa, t0 = row0 / r.gqa, t1 = ((R < row0 + tr ? R : row0 + tr) - 1) / r.gqa;
+    const int R = m * r.gqa, t0 = idiv(row0, r.gqa), t1 = idiv((R < row0 + tr ? R : row0 + tr) - 1, r.gqa);
     const int lo = r.window && p + t0 - r.window + 1 > 0 ? p + t0 - r.window + 1 : 0;
     a = lo / FTX_PAGE;
     s = r.window ? (int)(((int64_t)r.sinks + FTX_PAGE - 1) / FTX_PAGE) : 0;
@@ -99,7 +114,7 @@ __host__ __device__ inline void tile_pages(const PagedRoom& r, int p, int m, int
 // Item e of sequence q (number s), its partials from part0 on; seq = -1: none (a
 // tile whose list is shorter than the sequence's longest)
 __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq& q, int s, int many, int np, int part0, int e) {
-    const int tr = many ? PAGED_TR_MANY : PAGED_TR, tile = e / np, k = e - tile * np;
+    const int tr = many ? PAGED_TR_MANY : PAGED_TR, tile = idiv(e, np), k = e - tile * np;
     PagedItem it{};
     int n;
     tile_pages(r, q.npast, q.M, tile * tr, tr, it.s, it.a, n);
@@ -107,7 +122,7 @@ __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq
     it.seq = k < npt ? s : -1;
     it.row0 = tile * tr;
     // (the first n % npt parts are a page longer)
-    const int len = n / npt, rem = n - len * npt;
+    const int len = idiv(n, npt), rem = n - len * npt;
     it.i0 = k * len + (k < rem ? k : rem);
     it.i1 = it.i0 + len + (k < rem);
     it.part = np > 1 ? part0 + e * (tr / PAGED_TR) : -1;

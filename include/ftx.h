@@ -464,8 +464,8 @@ typedef struct {
  * last token are not touched) then go by these tables, of which the plan keeps
  * its own; contexts are read back only without a window, k and v then as
  * long as the lengths say.  A call that is recorded into a graph needs the build before
- * it in the same capture (FTX_E_INVALID); a build on another stream than the
- * plan's last call waits for the device.  Graphs and eager calls of one plan
+ * it in the same capture (FTX_E_INVALID); an eager build or call on another
+ * stream than the plan's last one waits for the device.  Graphs and eager calls of one plan
  * must not overlap. */
 int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a);
 

@@ -44,24 +44,30 @@ template <int HD, int KT>
 __device__ __forceinline__ PageRows page_rows(const PagedView& p, int context) {
     const int z = blockIdx.x % (2 * p.n_kv);
     PageRows r{};
-    int2 to{(int)blockIdx.y, (int)(blockIdx.x / (2 * p.n_kv))};
+    int page;
     if (p.touch && !context) {
-        to = p.touch[to.y];
-        if (to.x < 0) return r;
+        const PagedTouch to = p.touch[blockIdx.x / (2 * p.n_kv)];
+        if (to.page < 0) return r;
+        r.s0 = to.s0;
+        r.s1 = to.s1;
+        r.row = to.row;
+        page = to.page;
+    } else {
+        const PagedSeq sq = p.seqs[blockIdx.y];
+        const int from = context ? 0 : sq.npast;
+        const int first = from / FTX_PAGE + blockIdx.x / (2 * p.n_kv);  // the page's place in the table
+        r.s0 = max(from - first * FTX_PAGE, 0);
+        r.s1 = min(FTX_PAGE, sq.npast + sq.M - first * FTX_PAGE);
+        if (r.s0 >= r.s1) return r;
+        r.row = (int64_t)first * FTX_PAGE + (context ? sq.all0 : (int64_t)sq.tok0 - sq.npast);
+        page = p.table[sq.tab0 + first];
     }
-    const PagedSeq sq = p.seqs[to.x];
-    const int from = context ? 0 : sq.npast;
-    const int first = p.touch && !context ? to.y : from / FTX_PAGE + to.y;  // the page's place in the table
-    r.s0 = max(from - first * FTX_PAGE, 0);
-    r.s1 = min(FTX_PAGE, sq.npast + sq.M - first * FTX_PAGE);
-    if (r.s0 >= r.s1) return r;
     const int kvh = z >> 1;
     r.isv = z & 1;
-    r.blk = page_block(p, p.table[sq.tab0 + first], kvh);
+    r.blk = page_block(p, page, kvh);
     r.vals = r.blk + (r.isv ? paged_values_bytes(HD, KT) : 0);
     r.scale = (float*)(r.blk + 2 * paged_values_bytes(HD, KT)) + (r.isv ? FTX_PAGE : 0);
     r.mult = r.blk + 2 * paged_values_bytes(HD, KT) + 2 * FTX_PAGE * 4 + (r.isv ? paged_mult_bytes(HD, KT) : 0);
-    r.row = (int64_t)first * FTX_PAGE + (context ? sq.all0 : (int64_t)sq.tok0 - sq.npast);
     r.col = kvh * HD;
     return r;
 }

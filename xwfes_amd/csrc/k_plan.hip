@@ -331,6 +331,11 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
     auto sum_at = [&](int x) { return sums + x * n1; };
     auto total = [&](int x) { return sums[x * n1 + n]; };
     auto of = [&](int s) { return record(s, sum_at(S_TOK)[s + 1] - sum_at(S_TOK)[s], sum_at(S_TOK)[s], 0); };
+    // a page that new tokens go to
+    auto page_of = [&](int s, int pg) {
+        const int have = (P[s] + FTX_PAGE - 1) / FTX_PAGE;
+        return pg < have ? b.tables[s * b.ldt + pg] : b.free_pages[base + sum_at(S_FRESH)[s] + pg - have];
+    };
     const int g0 = blockIdx.x * NT + tid, gs = gridDim.x * NT;
     // (each kind's entries from another wave on, where they are few: side by side)
     auto from = [&](int wave) {
@@ -358,20 +363,22 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
         for (int i = from(4); i < r.tokens; i += gs) {
             int slot = -1, pos = -1;
             if (i < total(S_TOK)) {
-                const int s = owner(sum_at(S_TOK), n, i), have = (P[s] + FTX_PAGE - 1) / FTX_PAGE;
+                const int s = owner(sum_at(S_TOK), n, i);
                 pos = P[s] + i - sum_at(S_TOK)[s];
-                const int pg = pos / FTX_PAGE;
-                const int id = pg < have ? b.tables[s * b.ldt + pg] : b.free_pages[base + sum_at(S_FRESH)[s] + pg - have];
-                slot = id * FTX_PAGE + pos % FTX_PAGE;
+                slot = page_of(s, pos / FTX_PAGE) * FTX_PAGE + pos % FTX_PAGE;
             }
             if (b.slots) b.slots[i] = slot;
             if (b.positions) b.positions[i] = pos;
         }
     for (int i = from(5); i < r.touch; i += gs) {
-        int2 to{-1, 0};
+        PagedTouch to{-1, 0, 0, 0, 0, 0};
         if (i < total(S_TOUCH)) {
-            to.x = owner(sum_at(S_TOUCH), n, i);
-            to.y = P[to.x] / FTX_PAGE + i - sum_at(S_TOUCH)[to.x];
+            const int s = owner(sum_at(S_TOUCH), n, i), p = P[s], pg = p / FTX_PAGE + i - sum_at(S_TOUCH)[s];
+            const int tok0 = sum_at(S_TOK)[s], m = sum_at(S_TOK)[s + 1] - tok0;
+            to.page = page_of(s, pg);
+            to.s0 = max(p - pg * FTX_PAGE, 0);
+            to.s1 = min(p + m - pg * FTX_PAGE, FTX_PAGE);
+            to.row = (int64_t)tok0 - p + (int64_t)pg * FTX_PAGE;
         }
         b.touch[i] = to;
     }

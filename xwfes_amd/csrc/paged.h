@@ -86,6 +86,12 @@ struct PagedItem {
 struct PagedComb {
     int32_t seq, row0, part0, n, step, tok0, M, pad;
 };
+// A page that new tokens go to, in tables built on the GPU: its id (-1: none), their
+// slots s0 .. s1 - 1 and the row that slot 0 would be in the packed new rows
+struct PagedTouch {
+    int32_t page, s0, s1, pad;
+    int64_t row, pad2;
+};
 constexpr int PAGED_TR = 16, PAGED_TR_MANY = 128;
 // Sequences of at least this many query rows a kv head may go to the kernel
 // that shares each page among 128 or 256 rows
@@ -155,7 +161,7 @@ struct PagedBuild {
     // the plan's
     PagedSeq* seqs;
     int32_t* table;  // [r.nseq][r.n_pages]
-    int2* touch;     // (sequence or -1, page of it) that new tokens go to
+    PagedTouch* touch;
     PagedItem* items;  // r.few, then r.many; seq = -1: none
     PagedComb* combs;  // M = 0: none
     int32_t* codes;    // [r.nseq]: what the first kernel says of each sequence, then the pages used before
@@ -181,7 +187,7 @@ struct PagedView {
     int nseq;
     // of tables built on the GPU: the pages that new tokens go to, one after the
     // other (else a launch covers every sequence's most such pages)
-    const int2* touch;
+    const PagedTouch* touch;
     int n_touch;
 };
 hipError_t launch_paged_write(hipStream_t st, const PagedView& p, int64_t max_new_pages,

@@ -657,7 +657,7 @@ PagedView paged_view(const ftx_plan* pl, int64_t layer) {
     v.table = (const int32_t*)(pl->dev + pl->o_tab);
     v.nseq = pl->device ? pl->room.nseq : (int)pl->t.seqs.size();
     if (pl->device) {
-        v.touch = (const int2*)(pl->dev + pl->o_touch);
+        v.touch = (const PagedTouch*)(pl->dev + pl->o_touch);
         v.n_touch = pl->room.touch;
     }
     return v;
@@ -689,7 +689,10 @@ static int plan_order(ftx_plan* pl) {
     ftx_ctx* ctx = pl->ctx;
     if (!capturing(ctx->stream)) {
         if (ctx->stream == pl->stream) return FTX_OK;
-        if (pl->up) FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
+        if (pl->device)  // (an event after every build would take 3 us on the device)
+            FTX_HIP(ctx, hipDeviceSynchronize());
+        else
+            FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
         pl->stream = ctx->stream;
         return FTX_OK;
     }
@@ -915,7 +918,7 @@ int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room,
         };
         place(pl->o_seq, (size_t)r.nseq * sizeof(PagedSeq));
         place(pl->o_tab, (size_t)r.nseq * (size_t)r.n_pages * 4);
-        place(pl->o_touch, (size_t)r.touch * sizeof(int2));
+        place(pl->o_touch, (size_t)r.touch * sizeof(PagedTouch));
         place(pl->o_item, ((size_t)r.few + (size_t)r.many) * sizeof(PagedItem));
         place(pl->o_comb, (size_t)r.combs * sizeof(PagedComb));
         place(pl->o_code, ((size_t)r.nseq + 1) * 4);
@@ -967,7 +970,6 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     const bool cap = capturing(st);
     // (calls of the plan on another stream may still read its tables)
     if (!cap && pl->stream != st) FTX_HIP(ctx, hipDeviceSynchronize());
-    if (!cap && !pl->ev[0]) FTX_HIP(ctx, hipEventCreateWithFlags(&pl->ev[0], hipEventDisableTiming));
     PagedBuild b{};
     b.r = r;
     b.nseq = (int)a->nseq;
@@ -985,7 +987,7 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     b.n_free = a->n_free;
     b.seqs = (PagedSeq*)(pl->dev + pl->o_seq);
     b.table = (int32_t*)(pl->dev + pl->o_tab);
-    b.touch = (int2*)(pl->dev + pl->o_touch);
+    b.touch = (PagedTouch*)(pl->dev + pl->o_touch);
     b.items = (PagedItem*)(pl->dev + pl->o_item);
     b.combs = (PagedComb*)(pl->dev + pl->o_comb);
     b.codes = (int32_t*)(pl->dev + pl->o_code);
@@ -997,8 +999,6 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
         pl->capture = capture_id(st);
         return FTX_OK;
     }
-    FTX_HIP(ctx, hipEventRecord(pl->ev[0], st));
-    pl->up = pl->ev[0];
     pl->stream = st;
     return FTX_OK;
 }

@@ -184,6 +184,61 @@ def test_blocks_of_every_size(gctx, hd, seqs, heads):
     c.free()
 
 
+@pytest.mark.parametrize("hd,kv,heads,seqs", [
+    (128, 1, 4, [(300, 1)]), (64, 1, 4, [(300, 1), (70, 1)]), (128, 1, 8, [(300, 1)]), (64, 2, 8, [(130, 2)]),
+    (128, 2, 16, [(900, 1)]), (128, 1, 1, [(200, 1)]), (128, 1, 6, [(64, 1), (200, 1)]), (256, 1, 4, [(200, 1)]), (128, 1, 16, [(200, 1)])])
+def test_blocks_of_one_value(gctx, hd, kv, heads, seqs):
+    """Keys whose blocks hold one value each, in dims where the query is small: what the
+    other dims, zeros held as 8 less 8, leave of a score is its rounding.
+
+    A block's sum starts at -8 sum q and takes nibbles of up to 15: partial sums of up to
+    23 sum |q|, rounded four times by 2^-23 (each product of 32 dims in up to two steps, for
+    both halves of q), in steps c s; the block's largest |k| is at least 3.5 of them (c is
+    less than twice what it covers): 4 * 23 / 3.5 2^-23 < 2^-18 of sum |q| max |k|."""
+    rng = np.random.default_rng(hd + heads)
+    g = heads // kv
+    ks, vs = [], []
+    for a, b in seqs:
+        k = np.zeros((a + b, kv, hd // 32, 32), F)
+        k[..., 5] = rng.standard_normal(k.shape[:-1]) * 3
+        ks.append(k.reshape(a + b, kv, hd))
+        vs.append(rng.standard_normal((a + b, kv, hd)).astype(F))
+    c = Cache(gctx, rng, Q4, hd, kv, heads, seqs, rows=(ks, vs))
+    c.write_new()
+    q = rng.standard_normal((c.new, heads, hd)).astype(F) * 4
+    q.reshape(c.new, heads, -1, 32)[..., 5] *= F(1 / 64)
+    got, at = c.attend(q.reshape(c.new, -1)), 0
+    for (_, npast, M, _), k, v in zip(c.seqs, ks, vs):
+        k64, v64 = (np.repeat(stored4(x).astype(np.float64), g, axis=1) for x in (k, v))
+        qs = q[at:at + M].astype(np.float64)
+        s = np.einsum("ihd,jhd->hij", qs, k64) / np.sqrt(hd)
+        top = np.abs(k64).reshape(npast + M, heads, -1, 32).max(-1)
+        mag = np.einsum("ihb,jhb->hij", np.abs(qs).reshape(M, heads, -1, 32).sum(-1), top).max() / np.sqrt(hd)
+        see = np.arange(npast + M) <= npast + np.arange(M)[:, None]
+        p = np.where(see, np.exp(s - s.max()), 0)
+        p /= p.sum(-1, keepdims=True)
+        want, b = (np.einsum("hij,jhd->ihd", p, x) for x in (v64, np.abs(v64)))
+        tol = 2 * 2.0 ** -18 * mag + 2.0 ** -20 + 5 * ((npast + M) // 64 + 1) * 2.0 ** -23
+        err = np.abs(got[at:at + M] - want)
+        assert (err <= np.expm1(tol) * b + (npast + M) * 2.0 ** -34 * np.abs(v64).max()).all()
+        at += M
+    c.free()
+
+
+def test_dims_of_zeros_stay_zero(gctx):
+    """An output dim over values that are all held as zero is zero, whatever lies beside it."""
+    rng = np.random.default_rng(77)
+    for hd, heads, M in ((128, 4, 1), (64, 8, 1), (128, 8, 1), (64, 4, 1), (128, 16, 1), (128, 4, 30), (256, 4, 1)):
+        v = rng.standard_normal((200 + M, 1, hd)).astype(F) * 100
+        zero = rng.permutation(hd)[:hd // 3]
+        v[:, :, zero] = rng.uniform(-1e-3, 1e-3, (200 + M, 1, len(zero)))
+        c = Cache(gctx, rng, Q4, hd, 1, heads, [(200, M)], rows=([rng.standard_normal((200 + M, 1, hd)).astype(F)], [v]))
+        c.write_new()
+        got = c.check(queries(rng, c))
+        assert not stored4(v)[:, :, zero].any() and not got[:, :, zero].any() and got.any()
+        c.free()
+
+
 @TILES
 def test_large_values_in_hidden_places_change_nothing(gctx):
     P.test_large_values_in_hidden_places_change_nothing(gctx, Q4)

@@ -1063,26 +1063,36 @@ __device__ __forceinline__ float across(float x) {
 }
 
 // One wave's online softmax over pages of 4-bit rows for at most 16 / U query
-// rows: a product's 16 columns are U for each row, column U r + u that of row r
-// and of the blocks of 32 dims U j + u (the query is zero in the others' dims).
-//   Scores: column (r, u) sums q k over its blocks, times the slot's multiplier of
-//   the block once it is summed (a multiplier a slot and block, not one a value),
-//   and the U columns are added so that each lane keeps the scores of one slot
-//   tile (two of U = 2): the softmax of a page is 4 (8) weights a lane and not 16.
-//   Outputs: column (r, u) takes the weights times the slots' multipliers of block
-//   u: column u holds the output dims of its blocks (the others' are not used).
-// As the products of rows past the last are made in any case, this trades them for
-// vector instructions, some 600 a page instead of 950, where the bytes of a page
-// (9216 at 128 dims) are to be read in the time of 960 on every SIMD.
+// rows: a product's 16 columns are U for each row, column U r + u of row r.
+//   Scores: slot tile st goes to column u = st % U (the others' query is zeros), so
+// that the tiles share their sums' registers and each lane keeps the scores of one
+// tile (two of U = 2): the softmax of a page is 4 (8) weights a lane and not 16.
+// K's operand is the nibbles n = q + 8 as they are, the low bits of halves (n 2^-24),
+// and the sums start at -8 sum q of the block; a slot's multiplier of a block is
+// applied once, to the block's sum.
+//   Outputs: column u takes the weights times the slots' multipliers of block U j + u
+// and so holds the output dims of its blocks (the others' are not used).  V's
+// operand is signed: a sum over unsigned values less 8 times the weights' would leave
+// a dim whose values are all zero with the rounding of that sum.
+// Bound by the SIMDs' vector instructions (82% of the cycles of long lists by 16-row
+// tiles; products run beside them) and, with lists long enough, by HBM: 64
+// sequences of 16384 slots (8 kv heads of 128, 4 query heads each) 223 us, 5.4 TB/s, which is what loads
+// alone take.  In 16-row tiles, 950 vector instructions a page, one token of 16 sequences over
+// 820 to 8192 slots takes 41.6 us; folded with signed K operands and the multipliers
+// on partial sums, 600 a page, 23.7; as here, 500, 23.5, and longer lists 5 to 10% less.
 // Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256.
 template <int HD, int U>
 struct FoldAttn {
     static constexpr int NB = HD / 32, J = NB > U ? NB / U : 1, NDT = HD / 16, S = 4 / U, NL = HD / 32, OWN = 2 * J;
     static constexpr int64_t VB = paged_values_bytes(HD, PT_Q4), MB = paged_mult_bytes(HD, PT_Q4);
-    v8h qh[NB], ql[NB];
+    float bias[NB];  // -8 sum q of the blocks
     v4f o[NDT];
     float off = -INFINITY, l = 0.f, lp = 0.f, c2;
     int ev = EV_MIN;
+    // the query's halves in LDS, [block][high, low][kq][row], and as many zeros behind
+    // them, which the lanes of the other slot tiles read
+    static constexpr int QROWS = 16 / U, QN = NB * 2 * 4 * QROWS;
+    typedef v8h Query[2 * QN];
 
     // the largest of a row's lanes
     static __device__ __forceinline__ float row_top(float x) {
@@ -1091,11 +1101,13 @@ struct FoldAttn {
         return col_max(x);
     }
 
-    // the query row at q
-    __device__ __forceinline__ void query(const float* q, int u, int kq, bool vec) {
+    // The query row at q, to LDS if `store`.  A nibble n as the low bits of a half is
+    // n 2^-24, four bits up n 2^-20: the dims of the former are taken 2^4 times.
+    __device__ __forceinline__ void query(const float* q, int u, int r, int kq, bool vec, bool store, v8h* qs) {
+        // (each lane the blocks U j + u; heads of 64 dims have two)
         v4f x[J][2];
         float a = 0.f;
-        const bool any = u < NB;  // (heads of 64 dims have two blocks)
+        const bool any = u < NB;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int d0 = 32 * (U * j + (any ? u : 0)) + 8 * kq;
@@ -1112,48 +1124,86 @@ struct FoldAttn {
                 a = fabsf(y) <= FLT_BIG ? fmaxf(a, fabsf(y)) : a;
             }
         a = row_top(a);
-        const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 126) : 0;
-        const float qs = ldexpf(1.f, e);
-        c2 = ldexpf(1.f, -e);
-        v8h h[J], lo[J];
+        const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 122) : 0;
+        const float qs1 = ldexpf(1.f, e);
+        c2 = ldexpf(1.f, 20 - e);
+        float own[J];
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < J; ++j) {
+            v8h h, lo;
+            double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
+                const float f = i & 2 ? qs1 : 16.f * qs1;
                 v2h hh, ll;
-                split_hl2(rounded(x[j][i >> 2][i & 3] * qs), rounded(x[j][i >> 2][(i & 3) + 1] * qs), hh, ll);
-                h[j][i] = hh[0];
-                h[j][i + 1] = hh[1];
-                lo[j][i] = ll[0];
-                lo[j][i + 1] = ll[1];
+                split_hl2(rounded(x[j][i >> 2][i & 3] * f), rounded(x[j][i >> 2][(i & 3) + 1] * f), hh, ll);
+                h[i] = hh[0];
+                h[i + 1] = hh[1];
+                lo[i] = ll[0];
+                lo[i + 1] = ll[1];
+                // (a half and its rest add up exactly)
+                const float y = ((float)hh[0] + (float)ll[0]) * (i & 2 ? 16.f : 1.f), z = ((float)hh[1] + (float)ll[1]) * (i & 2 ? 16.f : 1.f);
+                sum += (double)y + (double)z;
             }
-        const v8h none = {};
-#pragma unroll
-        for (int dc = 0; dc < NB; ++dc) {
-            const bool mine = dc % U == u;
-            qh[dc] = mine ? h[dc / U] : none;
-            ql[dc] = mine ? lo[dc / U] : none;
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            own[j] = (float)(sum * (-8.0 * 0x1p-24));
+            if (store && any) {
+                const int dc = U * j + u;
+                qs[((dc * 2 + 0) * 4 + kq) * QROWS + r] = h;
+                qs[((dc * 2 + 1) * 4 + kq) * QROWS + r] = lo;
+            }
         }
+        auto share = [&](auto u_) {
+            constexpr int x = decltype(u_)::value;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+                if (U * j + x < NB) bias[U * j + x] = of_lane<U, x>(own[j]);
+        };
+        share(std::integral_constant<int, 0>{});
+        share(std::integral_constant<int, 1>{});
+        if constexpr (U == 4) {
+            share(std::integral_constant<int, 2>{});
+            share(std::integral_constant<int, 3>{});
+        }
+        if (store)
+            for (int i = threadIdx.x & 63; i < QN; i += 64) qs[QN + i] = v8h{};
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
 
     // A page's loads of K or V: values, the lane's blocks' multipliers of its 16
     // slots, the scales of the slots that it keeps
-    struct Vals {
-        uint4 u[NL], c[J];
+    struct Keys {
+        uint4 u[NL];
+        uint32_t c[NB][S];  // the multipliers of the lane's slots
         v4f s[S];
     };
-    static __device__ __forceinline__ void load(Vals& x, const uint8_t* blk, bool v, int u, int kq, int lane) {
-        const uint8_t* vals = blk + (v ? VB : 0);
-        const uint8_t* mult = blk + 2 * VB + 2 * FTX_PAGE * 4 + (v ? MB : 0);
-        const float* scale = (const float*)(blk + 2 * VB) + (v ? FTX_PAGE : 0);
+    struct Vals {
+        uint4 u[NL], c[J];  // the lane's blocks' multipliers of its 16 slots
+        v4f s[S];
+    };
+    static __device__ __forceinline__ void load_scales(v4f (&s)[S], const float* scale, int u, int kq) {
 #pragma unroll
-        for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(vals + (i * 64 + lane) * 16);
+        for (int a = 0; a < S; ++a) s[a] = *(const v4f*)(scale + 16 * (U * a + u) + 4 * kq);
+    }
+    static __device__ __forceinline__ void load(Keys& x, const uint8_t* blk, int u, int kq, int lane) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(blk + (i * 64 + lane) * 16);
+        const uint8_t* mult = blk + 2 * VB + 2 * FTX_PAGE * 4;
+#pragma unroll
+        for (int g = 0; g < NB; ++g)
+#pragma unroll
+            for (int a = 0; a < S; ++a) x.c[g][a] = *(const uint32_t*)(mult + 64 * g + 16 * kq + 4 * (U * a + u));
+        load_scales(x.s, (const float*)(blk + 2 * VB), u, kq);
+    }
+    static __device__ __forceinline__ void load(Vals& x, const uint8_t* blk, int u, int kq, int lane) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) x.u[i] = *(const uint4*)(blk + VB + (i * 64 + lane) * 16);
+        const uint8_t* mult = blk + 2 * VB + 2 * FTX_PAGE * 4 + MB;
 #pragma unroll
         for (int j = 0; j < J; ++j) x.c[j] = *(const uint4*)(mult + 64 * (U * j + u % NB) + 16 * kq);
-#pragma unroll
-        for (int a = 0; a < S; ++a) x.s[a] = *(const v4f*)(scale + 16 * (U * a + u) + 4 * kq);
+        load_scales(x.s, (const float*)(blk + 2 * VB) + FTX_PAGE, u, kq);
     }
     static __device__ __forceinline__ uint32_t word(const uint4& x, int i) {
         return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w;
@@ -1173,55 +1223,40 @@ struct FoldAttn {
         }
     }
 
-    // the scores, by the K scales, of the lane's slots
-    __device__ __forceinline__ void scores(v4f (&s)[S], const Vals& x, int u) const {
-        v4f p[J][4];
+    // the scores, by the K scales, of the lane's slots: tile st's products take the
+    // query in the lanes that keep it and zeros in the others, so that a block's sums
+    // of all tiles share one accumulator (two of U = 2) and each lane has its own
+    // slots' alone
+    __device__ __forceinline__ void scores(v4f (&s)[S], const Keys& x, const v8h* qs, const int (&at)[U]) const {
         v8h k[2][4];
         auto make = [&](int dc) {
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
-                const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1));
-                k[dc & 1][st] = join(q4_low(w), q4_high(w), q4_low(w >> 8), q4_high(w >> 8));
+                const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1)), w8 = w >> 8;
+                const uint32_t low = in_sgpr(0x000F000Fu), high = in_sgpr(0x00F000F0u);
+                k[dc & 1][st] = __builtin_bit_cast(v8h, uint4{w & low, w & high, w8 & low, w8 & high});
             }
         };
         make(0);
 #pragma unroll
         for (int dc = 0; dc < NB; ++dc) {
             if (dc + 1 < NB) make(dc + 1);
-            v4f(&a)[4] = p[dc / U];
+            v4f acc[S];
 #pragma unroll
-            for (int st = 0; st < 4; ++st)
-                a[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[dc & 1][st], ql[dc],
-                                                               dc % U ? a[st] : v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            for (int a = 0; a < S; ++a) acc[a] = v4f{bias[dc], bias[dc], bias[dc], bias[dc]};
 #pragma unroll
-            for (int st = 0; st < 4; ++st)
-                a[st] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[dc & 1][st], qh[dc], a[st], 0, 0, 0);
-            if (dc + 1 < NB) beside();
-            __builtin_amdgcn_sched_barrier(0);
-        }
+            for (int hl = 1; hl >= 0; --hl)
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
+                for (int st = 0; st < 4; ++st)
+                    acc[st / U] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        k[dc & 1][st], qs[(dc * 2 + hl) * 4 * QROWS + at[st % U]], acc[st / U], 0, 0, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float t = p[0][st][i] * mult(x.c[0], st, i);
+            for (int a = 0; a < S; ++a)
 #pragma unroll
-                for (int j = 1; j < J; ++j) t = __builtin_fmaf(p[j][st][i], mult(x.c[j], st, i), t);
-                p[0][st][i] = t;
-            }
-        // the columns' sum, each lane its own slot tiles': U a + u
-        const bool odd = u & 1, upper = u & 2;
-        v4f t[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                t[a][i] = (odd ? p[0][2 * a + 1][i] : p[0][2 * a][i]) + across<1>(odd ? p[0][2 * a][i] : p[0][2 * a + 1][i]);
-        if constexpr (U == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[0][i] = (upper ? t[1][i] : t[0][i]) + across<2>(upper ? t[0][i] : t[1][i]);
-        } else {
-            s[0] = t[0];
-            s[1] = t[1];
+                for (int i = 0; i < 4; ++i) {
+                    const float c = (float)((x.c[dc][a] >> (8 * i)) & 255);
+                    s[a][i] = dc ? __builtin_fmaf(acc[a][i], c, s[a][i]) : acc[a][i] * c;
+                }
         }
 #pragma unroll
         for (int a = 0; a < S; ++a) s[a] *= x.s[a];
@@ -1358,6 +1393,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
     __shared__ v4f so[NW - 1][W::OWN][64];
     __shared__ float sm[NW][64], sl[NW][64];
     __shared__ int se[NW][64];
+    __shared__ typename W::Query qs;
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
     if (it.seq < 0) return;
@@ -1379,7 +1415,11 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
         return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
     };
     W wa;
-    wa.query(a.q + tok * a.ldq + (int64_t)head * HD, u, kq, !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15));
+    wa.query(a.q + tok * a.ldq + (int64_t)head * HD, u, rr, kq, !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15), w == 0, qs);
+    int at[U];  // slot tile st's query: the lane's row, or zeros
+#pragma unroll
+    for (int x = 0; x < U; ++x) at[x] = kq * W::QROWS + rr + (x == u ? 0 : W::QN);
+    __syncthreads();
     const RowSight sight(a, sq, t);
     int hi = sight.hi, lo = sight.lo;
 #pragma unroll
@@ -1389,22 +1429,24 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
     }
     hi = __builtin_amdgcn_readfirstlane(hi);
     lo = __builtin_amdgcn_readfirstlane(lo);
-    typename W::Vals kv, vv;
+    typename W::Keys kv;
+    typename W::Vals vv;
     const uint8_t* blk = nullptr;
     if (n) {
         blk = block_of(0);
-        W::load(kv, blk, false, u, kq, lane);
+        W::load(kv, blk, u, kq, lane);
     }
     for (int j = 0; j < n; ++j) {
-        W::load(vv, blk, true, u, kq, lane);
+        W::load(vv, blk, u, kq, lane);
         __builtin_amdgcn_sched_barrier(0);
         v4f s[W::S];
-        wa.scores(s, kv, u);
+        asm volatile("" ::: "memory");  // (the query is read again for every page)
+        wa.scores(s, kv, qs, at);
         __builtin_amdgcn_sched_barrier(0);
         const int p0 = place(j) * FTX_PAGE;
         if (j + 1 < n) {
             blk = block_of(j + 1);
-            W::load(kv, blk, false, u, kq, lane);
+            W::load(kv, blk, u, kq, lane);
         }
         __builtin_amdgcn_sched_barrier(0);
         const bool whole = p0 + FTX_PAGE - 1 <= hi && (p0 >= lo || p0 + FTX_PAGE <= a.sinks);

@@ -865,7 +865,6 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
     __shared__ int se[NW][64];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
-    if (it.seq < 0) return;  // (of tables built on the GPU)
     const PagedSeq sq = it.q;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, col = lane & 15, kq = lane >> 4;
@@ -898,6 +897,9 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 2 : 1) k_paged_attn(Paged
     // lanes.  A page's V loads are issued before its scores are formed, the
     // next page's K loads and scales (PRE) before its softmax, so that each
     // wait leaves the later loads in flight.
+    // (none, of tables built on the GPU: looked at here, where the item's other parts
+    // have been waited for; at the start it takes 0.3 us)
+    if (it.seq < 0) return;
     const int n = max(0, (it.i1 - it.i0 - w + NW - 1) / NW);
     auto place = [&](int j) {  // in the table
         const int i = it.i0 + w + NW * j;
@@ -1396,7 +1398,6 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
     __shared__ typename W::Query qs;
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[blockIdx.x / a.p.n_kv];
-    if (it.seq < 0) return;
     const PagedSeq sq = it.q;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63, u = lane & (U - 1), rr = (lane & 15) / U, kq = lane >> 4;
@@ -1414,6 +1415,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
         if ((j & 63) == 0 && j) ids = j + lane < n ? a.p.table[sq.tab0 + place(j + lane)] : 0;
         return page_block(a.p, __builtin_amdgcn_readlane(ids, j & 63), kvh);
     };
+    if (it.seq < 0) return;
     W wa;
     wa.query(a.q + tok * a.ldq + (int64_t)head * HD, u, rr, kq, !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15), w == 0, qs);
     int at[U];  // slot tile st's query: the lane's row, or zeros
@@ -1546,7 +1548,6 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int kvh = blockIdx.x % a.p.n_kv;
     const PagedItem it = a.items[a.n_few + blockIdx.x / a.p.n_kv];
-    if (it.seq < 0) return;
     const PagedSeq sq = it.q;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lane = tid & 63, col = lane & 15, kq = lane >> 4;
@@ -1652,6 +1653,7 @@ __global__ void __launch_bounds__(64 * NW_MANY) k_paged_many(PagedAttn a) {
             }
         }
     };
+    if (it.seq < 0) return;  // (before the first copy to LDS)
     stage(0);
     W wa[NT];
     v8h* const qlo = (v8h*)(lds + 2 * BUF) + (QLO ? w * (NT * W::NDC * 64) + lane : 0);

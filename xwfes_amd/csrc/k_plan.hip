@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
     for (int i = from(6); i < r.few + r.many; i += gs) {
         const int mn = i >= r.few, e = mn ? i - r.few : i, x = mn ? S_MANY : S_FEW;
         if (e >= total(x)) {
-            b.items[i].seq = -1;
+            b.items[i] = seq_none();
             continue;
         }
         const int s = owner(sum_at(x), n, e);
@@ -404,22 +404,25 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
 
 }  // namespace
 
+hipError_t paged_build_limits() {
+    static std::atomic<uint64_t> set_one{0}, set_many{0};
+    const size_t most = (size_t)(PAGED_ROOM_SEQS + 1) * (8 + 4 * N_SUMS);
+    const hipError_t e = lds_limit((const void*)k_plan_build<true>, most, set_one);
+    return e != hipSuccess ? e : lds_limit((const void*)k_plan_build<false>, most, set_many);
+}
+
 hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b) {
     const PagedRoom& r = b.r;
     const int64_t entries = (int64_t)r.tokens + r.nseq + r.touch + r.few + r.many + r.combs;
     const bool one = (int64_t)b.nseq * r.n_pages <= ONE_MOST && entries <= ONE_MOST;
     const size_t bytes = (size_t)(b.nseq + 1) * (8 + 4 * N_SUMS);
-    static std::atomic<uint64_t> set_one{0}, set_many{0};
-    const size_t most = (size_t)(PAGED_ROOM_SEQS + 1) * (8 + 4 * N_SUMS);
-    hipError_t e = lds_limit(one ? (const void*)k_plan_build<true> : (const void*)k_plan_build<false>, most,
-                             one ? set_one : set_many);
-    if (e != hipSuccess) return e;
     if (one) {
         hipLaunchKernelGGL(k_plan_build<true>, dim3(1), dim3(build_threads<true>()), bytes, st, b);
         return hipGetLastError();
     }
     hipLaunchKernelGGL(k_plan_check, dim3((unsigned)(b.nseq + 3) / 4), dim3(256), 0, st, b);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     constexpr int NT = build_threads<false>();
     const unsigned wgs = (unsigned)std::min<int64_t>(128, (entries + NT - 1) / NT);
     hipLaunchKernelGGL(k_plan_build<false>, dim3(wgs), dim3(NT), bytes, st, b);

@@ -162,11 +162,13 @@ struct PagedBuild {
     PagedSeq* seqs;
     int32_t* table;  // [r.nseq][r.n_pages]
     PagedTouch* touch;
-    PagedItem* items;  // r.few, then r.many; seq = -1: none
+    PagedItem* items;  // r.few, then r.many; seq = -1: none (seq_none)
     PagedComb* combs;  // M = 0: none
     int32_t* codes;    // [r.nseq]: what the first kernel says of each sequence, then the pages used before
 };
 hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b);
+// its kernels' LDS on the current device, before the first
+hipError_t paged_build_limits();
 
 // The same lists for plain arrays, no context and no device: items (r.few + r.many
 // of them) and joins (r.combs) of sequences whose lengths fit the room

@@ -402,7 +402,7 @@ extern "C" int paged_build_probe(const ftx_plan_room* a, int64_t n_kv, int64_t h
         });
         const int per[2] = {few, seq_per((int)total[1], r.cut_many, 2)};
         int64_t at[2] = {0, 0}, part = 0, comb = 0, tok = 0;
-        for (int64_t i = 0; i < r.few + r.many; ++i) items[i].seq = -1;
+        for (int64_t i = 0; i < r.few + r.many; ++i) items[i] = seq_none();
         for (int64_t i = 0; i < r.combs; ++i) combs[i] = PagedComb{};
         for (int64_t s = 0; s < nseq; ++s) {
             const SeqLoad l = seq_load(r, r.n_pages, npast[s], M[s]);
@@ -923,13 +923,21 @@ int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room,
         place(pl->o_comb, (size_t)r.combs * sizeof(PagedComb));
         place(pl->o_code, ((size_t)r.nseq + 1) * 4);
         const size_t pf = (size_t)r.parts * p->n_kv * PAGED_TR * (p->hd + 2);
+        if (paged_build_limits() != hipSuccess) {
+            (void)hipGetLastError();
+            plan_release(pl);
+            return ftx_fail(ctx, FTX_E_DEVICE, "plan: the build's kernels could not be prepared");
+        }
         if (hipMalloc((void**)&pl->dev, at) != hipSuccess || (pf && hipMalloc((void**)&pl->part, pf * 4 + 256) != hipSuccess)) {
             (void)hipGetLastError();
             plan_release(pl);
             return ftx_fail(ctx, FTX_E_NOMEM, "plan: device allocation failed");
         }
         // no tokens: items and pages of no sequence
-        if (hipMemset(pl->dev, 0, at) != hipSuccess || hipMemset(pl->dev + pl->o_touch, 0xFF, pl->o_comb - pl->o_touch) != hipSuccess ||
+        const std::vector<PagedItem> none((size_t)r.few + (size_t)r.many, seq_none());
+        if (hipMemset(pl->dev, 0, at) != hipSuccess || hipMemset(pl->dev + pl->o_touch, 0xFF, pl->o_item - pl->o_touch) != hipSuccess ||
+            (!none.empty() &&
+             hipMemcpy(pl->dev + pl->o_item, none.data(), none.size() * sizeof(PagedItem), hipMemcpyHostToDevice) != hipSuccess) ||
             hipDeviceSynchronize() != hipSuccess) {
             (void)hipGetLastError();
             plan_release(pl);

@@ -111,6 +111,14 @@ __host__ __device__ inline void tile_pages(const PagedRoom& r, int p, int m, int
     s = s < a ? s : a;
     n = s + (p + t1) / FTX_PAGE + 1 - a;
 }
+// No item: what a workgroup reads before it looks at seq is the first row's
+__host__ __device__ inline PagedItem seq_none() {
+    PagedItem it{};
+    it.seq = -1;
+    it.q.M = 1;
+    it.q.dep0 = -1;
+    return it;
+}
 // Item e of sequence q (number s), its partials from part0 on; seq = -1: none (a
 // tile whose list is shorter than the sequence's longest)
 __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq& q, int s, int many, int np, int part0, int e) {
@@ -119,7 +127,8 @@ __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq
     int n;
     tile_pages(r, q.npast, q.M, tile * tr, tr, it.s, it.a, n);
     const int npt = np < n ? np : n;
-    it.seq = k < npt ? s : -1;
+    if (k >= npt) return seq_none();
+    it.seq = s;
     it.row0 = tile * tr;
     // (the first n % npt parts are a page longer)
     const int len = idiv(n, npt), rem = n - len * npt;

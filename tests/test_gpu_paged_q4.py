@@ -372,3 +372,60 @@ def test_steps_near_those_of_halves(gctx, orc):
     # spread, rounded evenly), a 201st part of what is seen, and halves' 2^-11 of every row
     assert S.rel_err_rows(x, y) < 5 * S.LOGIT_TOL
     t.free(), u.free()
+
+
+def test_steps_of_a_batch_and_under_a_window(gctx, orc):
+    """Sequences of one batch as each by itself (their rows' last bits may differ by the
+    batch's width: the bound of test_commit_of_a_tree_path); a window leaves its pages behind."""
+    t = S.Setup(gctx, orc, S.CFG128, S.Q8, Q4)
+    kvs = [t.context(n, 230, seed=n)[0] for n in (10, 128, 200)]
+    alone = [t.step([(kv, [7, 9], None, False)])[0] for kv in kvs]
+    for x, y in zip(t.step([(kv, [7, 9], None, False) for kv in kvs]), alone):
+        assert S.rel_err_rows(x, y) < 34 * S.LOGIT_TOL
+    free = t.pool.available
+    kv = t.gm.kv_paged(t.pool, 400, window=70, sinks=4)
+    t.kvs.append(kv)
+    for i in range(6):
+        x, = t.step([(kv, list(range(i, i + 50)), None, True)])
+        assert np.isfinite(x).all()
+    # the last step's 250 before it and 50: the first page, and from 250 - 69 on
+    assert free - t.pool.available == 1 + 3
+    t.free()
+
+
+@pytest.mark.parametrize("hd,heads,kv,seqs", [
+    (64, 4, 1, [(300, 1), (5, 1)]), (128, 8, 2, [(300, 1)]), (128, 8, 1, [(1000, 1), (70, 1)]), (64, 6, 1, [(40, 1)]),
+    (128, 2, 2, [(700, 4)]), (64, 16, 2, [(2000, 1)]), (128, 1, 1, [(130, 8)])])
+def test_strides_of_few_rows(gctx, hd, heads, kv, seqs):
+    rng = np.random.default_rng(15)
+    c = Cache(gctx, rng, Q4, hd, kv, heads, seqs)
+    c.write_new()
+    q = queries(rng, c)
+    want = c.check(q)
+    for pad, off in test_gpu_paged_strides.WAYS:
+        c.write_new(pad=pad, off=off)
+        np.testing.assert_array_equal(c.attend(q, pad=pad, off=off), want)
+    c.free()
+
+
+@pytest.mark.parametrize("heads,M,window,sinks", [(1, 1, 0, 0), (4, 1, 0, 0), (3, 1, 100, 3), (8, 1, 0, 0), (2, 3, 0, 0), (2, 4, 40, 66),
+                                                  (1, 7, 0, 0), (5, 1, 1, 0), (7, 1, 64, 64)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_few_rows_of_every_number(gctx, hd, heads, M, window, sinks):
+    """One to eight query rows a kv head: sequences of no token to many, whole and cut lists."""
+    rng = np.random.default_rng(heads * 8 + M)
+    seqs = [(n, M) for n in (0, 1, 15, 16, 63 - M, 64, 191, 700, 3000)]
+    c = Cache(gctx, rng, Q4, hd, 1, heads, seqs, window, sinks)
+    c.write_new()
+    c.check(queries(rng, c, 2.0))
+    c.free()
+
+
+def test_many_sequences(gctx):
+    """More lists than the chip takes at once, long ones among short ones."""
+    rng = np.random.default_rng(41)
+    seqs = [(int(n), 1) for n in rng.integers(0, 130, 600)] + [(5000, 1), (2500, 1)]
+    c = Cache(gctx, rng, Q4, 64, 2, 4, seqs)
+    c.write_new()
+    c.check(queries(rng, c))
+    c.free()

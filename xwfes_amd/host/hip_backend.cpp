@@ -261,10 +261,10 @@ HipSequence::HipSequence(HipVerifier& ver, HipPool& pool, int64_t ctx_cap, int64
               "kv_create_paged");
 }
 
-HipPool::HipPool(HipVerifier& ver, int64_t n_pages, bool eight_bit) {
+HipPool::HipPool(HipVerifier& ver, int64_t n_pages, KvRows rows) {
     const ModelConfig& c = ver.config();
-    ver.be_.check(ftx_pool_create(ver.be_.ctx(), c.n_layer, c.n_head_kv, c.head_dim, n_pages,
-                                  eight_bit ? FTX_KV_Q8 : FTX_KV_F16, &pool_),
+    const int dtype = rows == KvRows::Bits4 ? FTX_KV_Q4 : rows == KvRows::Bits8 ? FTX_KV_Q8 : FTX_KV_F16;
+    ver.be_.check(ftx_pool_create(ver.be_.ctx(), c.n_layer, c.n_head_kv, c.head_dim, n_pages, dtype, &pool_),
                   "pool_create");
 }
 

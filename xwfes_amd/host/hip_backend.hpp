@@ -234,12 +234,17 @@ private:
     int64_t max_tokens_ = 0;
 };
 
+// How a paged cache holds its rows of K and V (FTX_KV_F16, FTX_KV_Q8, FTX_KV_Q4)
+enum class KvRows { Halves, Bits8, Bits4 };
+
 // Pages of paged caches for a HipVerifier's model (ftx_pool_create; no
-// counterpart in the reference): rows of K and V in 8 bits or halves.  Must
+// counterpart in the reference): rows of K and V in halves, 8 or 4 bits.  Must
 // outlive its sequences.
 class HipPool {
 public:
-    HipPool(HipVerifier& ver, int64_t n_pages, bool eight_bit = false);
+    HipPool(HipVerifier& ver, int64_t n_pages, bool eight_bit = false)
+        : HipPool(ver, n_pages, eight_bit ? KvRows::Bits8 : KvRows::Halves) {}
+    HipPool(HipVerifier& ver, int64_t n_pages, KvRows rows);
     ~HipPool();
     HipPool(const HipPool&) = delete;
     HipPool& operator=(const HipPool&) = delete;

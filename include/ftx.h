@@ -432,7 +432,7 @@ typedef struct {
 } ftx_plan_room;
 int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room, ftx_plan** out);
 /* All pointers are int32 device memory, 4-byte aligned; none may overlap another
- * but used and used_after, which may be one. */
+ * (FTX_E_INVALID) but used and used_after, which may be one. */
 typedef struct {
     int64_t nseq;               /* 1 .. room.nseq sequences of this step */
     const int32_t* npast;       /* [nseq] tokens in their pages */
@@ -464,7 +464,7 @@ typedef struct {
  * last token are not touched) then go by these tables, of which the plan keeps
  * its own; contexts are read back only without a window, k and v then as
  * long as the lengths say.  A call that is recorded into a graph needs the build before
- * it in the same capture (FTX_E_INVALID); an eager build or call on another
+ * it in the same capture, on the same stream (FTX_E_INVALID); an eager build or call on another
  * stream than the plan's last one waits for the device.  Graphs and eager calls of one plan
  * must not overlap. */
 int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a);

@@ -339,6 +339,16 @@ def test_refused_calls(gctx):
                        (5, None, -1), (6, -1, -1), (6, 1 << 31, -1), (7, None, -1), (8, host.ctypes.data, -1), (9, None, -1)):
         refused(code, plan.build, *[x if j == i else y for j, y in enumerate(a)])
     refused(-1, plan.build, *a, slots_ptr=host.ctypes.data)
+    refused(-1, plan.build, *a[:4], (1 << 40) + 1, *a[5:])
+    # arrays over each other, by one number (the table's two rows, the list, and the outputs)
+    end = ls.ptr("tables") + 4 * (ls.ldt + min(ls.ldt, 2))
+    for i, x in ((0, ls.ptr("M")), (7, end - 4), (8, ls.ptr("free")), (8, ls.ptr("npast") + 4), (9, ls.ptr("used"))):
+        refused(-1, plan.build, *[x if j == i else y for j, y in enumerate(a)])
+    for n in ("npast", "M", "tables", "free", "used", "after", "status"):
+        for opt in ("starts_ptr", "slots_ptr", "positions_ptr"):
+            refused(-1, plan.build, *a, **{opt: ls.ptr(n)})
+    refused(-1, plan.build, *a, slots_ptr=ls.ptr("slots"), positions_ptr=ls.ptr("slots") + 4 * 7)
+    refused(-1, plan.build, *a, starts_ptr=ls.ptr("slots") + 4 * 8 - 4, slots_ptr=ls.ptr("slots"))
     refused(-1, plan.set, [([0], 0, 1)], 2)
     plan.build(*a)
     assert ls.get()["status"][0] == 0
@@ -469,3 +479,106 @@ def test_build_and_calls_on_two_streams(gctx):
     for x in (bq, bo, qd, out):
         x.buf.free()
     none.free(), c.free(), busy.free()
+
+
+def test_captures_hold_their_builds(gctx):
+    """Two graphs of one plan, each with its own build and lengths, replayed in turn with eager
+    steps of the plan between; a capture without a build, and another stream of a capture than
+    the build's, are refused."""
+    hip = _hip()
+    rng = np.random.default_rng(41)
+    c = Built(gctx, rng, Q4, 128, 2, 8, [(900, 3), (62, 5), (0, 0)], room=1)
+    c.write_new()
+    q = queries(rng, c)
+    want = c.check(q)
+    # the same sequences some tokens shorter: other tables of the same pages
+    less = Lists(gctx, [899, 60, 0], [3, 6, 0], c.lists.host["tables"], c.lists.host["free"], 0, c.room)
+    less.host["tables"][1, 0] = c.tables[1][0]
+    less.reset()
+    pair = [c.lists, less]
+    qd = Rows(gctx, c.pad(q, np.nan))
+    out = Rows(gctx, np.full((c.room, c.heads * c.hd), 9.0))
+
+    def step(ls):
+        ls.build(c.plan)
+        c.plan.attend(0, qd.ptr, out.ptr)
+
+    def taken():
+        got = out.get()
+        out.buf.write(out.host)
+        return got
+
+    eager = []
+    for ls in pair:
+        out.buf.write(out.host)
+        step(ls)
+        gctx.sync()
+        eager.append(taken())
+    np.testing.assert_array_equal(eager[0][:c.new].reshape(want.shape), want)
+    assert (eager[1] != eager[0]).any() and (eager[1][9:] == 9).all()
+    st, side, forked, joined = (ctypes.c_void_p() for _ in range(4))
+    graphs, exes = [ctypes.c_void_p() for _ in pair], [ctypes.c_void_p() for _ in pair]
+    for x in (st, side):
+        assert hip.hipStreamCreate(ctypes.byref(x)) == 0
+    for x in (forked, joined):
+        assert hip.hipEventCreate(ctypes.byref(x)) == 0
+    try:
+        for ls, g, e in zip(pair, graphs, exes):
+            gctx.set_stream(st.value)
+            assert hip.hipStreamBeginCapture(st, 2) == 0
+            refused(-1, c.plan.attend, 0, qd.ptr, out.ptr)
+            step(ls)
+            assert hip.hipEventRecord(forked, st) == 0
+            assert hip.hipStreamWaitEvent(side, forked, 0) == 0
+            gctx.set_stream(side.value)
+            refused(-1, c.plan.attend, 0, qd.ptr, out.ptr)
+            refused(-1, ls.build, c.plan)
+            assert hip.hipEventRecord(joined, side) == 0
+            assert hip.hipStreamWaitEvent(st, joined, 0) == 0
+            assert hip.hipStreamEndCapture(st, ctypes.byref(g)) == 0
+            assert hip.hipGraphInstantiate(ctypes.byref(e), g, None, None, 0) == 0
+            gctx.set_stream(None)
+        for i in (0, 1, 1, 0, 0, 1):
+            out.buf.write(out.host)
+            assert hip.hipGraphLaunch(exes[i], st) == 0
+            assert hip.hipStreamSynchronize(st) == 0
+            np.testing.assert_array_equal(taken(), eager[i])
+            step(pair[1 - i])
+            gctx.sync()
+            np.testing.assert_array_equal(taken(), eager[1 - i])
+    finally:
+        gctx.set_stream(None)
+        hip.hipStreamSynchronize(st)
+        for e in exes:
+            if e:
+                hip.hipGraphExecDestroy(e)
+        for g in graphs:
+            if g:
+                hip.hipGraphDestroy(g)
+        for x in (forked, joined):
+            hip.hipEventDestroy(x)
+        for x in (st, side):
+            hip.hipStreamDestroy(x)
+    for x in (qd, out):
+        x.buf.free()
+    less.free(), c.free()
+
+
+def test_a_page_twice_in_a_table(gctx):
+    """Sequences that share their first pages, and one that has a page in two places."""
+    rng = np.random.default_rng(43)
+    for kvt in (F16, Q8, Q4):
+        c = Built(gctx, rng, kvt, 64, 1, 4, [(256, 2), (200, 1)])
+        t = c.lists.host["tables"].copy()
+        t[0, 2] = t[0, 0]
+        t[1, :2] = t[0, :2]
+        for s, src, at in ((0, 0, 2), (1, 0, 0), (1, 1, 1)):
+            for x in (c.k, c.v):
+                x[s][at * 64:at * 64 + 64] = x[0][src * 64:src * 64 + 64]
+            c.tables[s][at] = t[s, at]
+        c.lists.reset(tables=t)
+        c.lists.build(c.plan)
+        c.lists.check()
+        c.write_new()
+        c.check(queries(rng, c, 2.0))
+        c.free()

@@ -429,3 +429,24 @@ def test_many_sequences(gctx):
     c.write_new()
     c.check(queries(rng, c))
     c.free()
+
+
+@pytest.mark.parametrize("hd,heads,M", [(64, 4, 1), (128, 4, 1), (128, 3, 1), (64, 8, 1), (128, 8, 1), (128, 2, 4), (128, 16, 1),
+                                        (256, 4, 1), (64, 2, 50)])
+def test_queries_that_are_no_numbers(gctx, hd, heads, M):
+    """A query row that holds an infinity or a NaN is NaN, the others are what they were bit
+    for bit, also those whose products share its instructions."""
+    rng = np.random.default_rng(hd + heads + M)
+    c = Cache(gctx, rng, Q4, hd, 1, heads, [(700, M), (40, M)])
+    c.write_new()
+    q = queries(rng, c)
+    want = c.check(q)
+    rows = q.reshape(-1, hd)
+    for n, bad in enumerate((np.nan, np.inf, -np.inf)):
+        for r in (0, len(rows) // 2, len(rows) - 1):
+            x = rows.copy()
+            x[r, (37 * n + 5 * r) % hd] = bad
+            got = c.attend(x.reshape(q.shape)).reshape(-1, hd)
+            assert np.isnan(got[r]).all()
+            np.testing.assert_array_equal(np.delete(got, r, 0), np.delete(want.reshape(-1, hd), r, 0))
+    c.free()

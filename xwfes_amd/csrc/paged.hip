@@ -549,11 +549,12 @@ struct ftx_plan {
     size_t bytes = 0;     // of the last set's tables
     uint64_t serial = 0;  // its number
     // tables built on the GPU: what there is room for, its entries, and the capture
-    // that the last build was recorded in
+    // that the last build was recorded in, on its stream
     bool device = false;
     PagedRoom room;
     size_t o_touch = 0, o_code = 0;
     unsigned long long capture = 0;
+    hipStream_t capture_stream = nullptr;
 };
 
 static void plan_release(ftx_plan* pl) {
@@ -697,9 +698,10 @@ static int plan_order(ftx_plan* pl) {
         return FTX_OK;
     }
     if (pl->device) {
-        // (tables of a build outside of the graph: nothing would order the two)
-        if (pl->capture == 0 || capture_id(ctx->stream) != pl->capture)
-            return ftx_fail(ctx, FTX_E_INVALID, "plan: no build of it in this capture");
+        // (tables of a build outside of the graph, or on another stream of it: nothing
+        // would have to order the two)
+        if (pl->capture == 0 || capture_id(ctx->stream) != pl->capture || ctx->stream != pl->capture_stream)
+            return ftx_fail(ctx, FTX_E_INVALID, "plan: no build of it in this capture on this stream");
         return FTX_OK;
     }
     pl->captured = true;
@@ -960,22 +962,42 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     if (!pl->device) return ftx_fail(ctx, FTX_E_INVALID, "plan: its steps are set from the host");
     const PagedRoom& r = pl->room;
     if (a->nseq < 1 || a->nseq > r.nseq) return ftx_fail(ctx, FTX_E_RANGE, "build: more sequences than the plan has room for");
-    if (a->ldt < 1 || a->n_free < 0 || a->n_free > INT32_MAX) return ftx_fail(ctx, FTX_E_INVALID, "build: ldt or n_free out of range");
+    if (a->ldt < 1 || a->ldt > (int64_t)1 << 40 || a->n_free < 0 || a->n_free > INT32_MAX)
+        return ftx_fail(ctx, FTX_E_INVALID, "build: ldt or n_free out of range");
     const struct {
         const void* p;
         bool need;
-    } mem[] = {{a->npast, true}, {a->M, true}, {a->tables, true}, {a->free_pages, a->n_free > 0}, {a->used, true},
-               {a->used_after, true}, {a->starts, false}, {a->slots, false}, {a->positions, false}, {a->status, true}};
+        int64_t n;  // (of the tables: from the first row's first entry that counts to the last's last)
+    } mem[] = {{a->npast, true, a->nseq},
+               {a->M, true, a->nseq},
+               {a->tables, true, (a->nseq - 1) * a->ldt + std::min<int64_t>(a->ldt, r.n_pages)},
+               {a->free_pages, a->n_free > 0, a->n_free},
+               {a->used, true, 1},
+               {a->used_after, true, 1},
+               {a->starts, false, a->nseq + 1},
+               {a->slots, false, r.tokens},
+               {a->positions, false, r.tokens},
+               {a->status, true, 1}};
     for (const auto& m : mem) {
         if (!m.p && !m.need) continue;
         if (!m.p) return ftx_fail(ctx, FTX_E_INVALID, "null argument");
         if ((uintptr_t)m.p & 3) return ftx_fail(ctx, FTX_E_INVALID, "build: arrays must be 4-byte aligned");
         if (!on_device(ctx, m.p)) return ftx_fail(ctx, FTX_E_INVALID, "build: arrays must be memory of the context's device");
+        // (a page is looked at before it is taken for one of the pool's: no write may come between)
+        for (const auto& o : mem) {
+            if (&o == &m) break;
+            if (!o.p || o.n == 0 || m.n == 0 || (o.p == a->used && m.p == o.p && &m == &o + 1)) continue;
+            const uintptr_t x = (uintptr_t)m.p, y = (uintptr_t)o.p;
+            if (x < y + 4 * (uintptr_t)o.n && y < x + 4 * (uintptr_t)m.n)
+                return ftx_fail(ctx, FTX_E_INVALID, "build: arrays overlap");
+        }
     }
     OnDevice od(ctx->device);
     if (!od.ok) return ftx_fail(ctx, FTX_E_DEVICE, "the context's device could not be made current");
     hipStream_t st = ctx->stream;
     const bool cap = capturing(st);
+    if (cap && pl->capture && pl->capture_stream != st && pl->capture == capture_id(st))
+        return ftx_fail(ctx, FTX_E_INVALID, "plan: built on another stream in this capture");
     // (calls of the plan on another stream may still read its tables)
     if (!cap && pl->stream != st) FTX_HIP(ctx, hipDeviceSynchronize());
     PagedBuild b{};
@@ -1005,6 +1027,7 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     ts.end(TK_PAGED_KV, 8.0 * ((double)r.nseq + r.tokens));
     if (cap) {
         pl->capture = capture_id(st);
+        pl->capture_stream = st;
         return FTX_OK;
     }
     pl->stream = st;

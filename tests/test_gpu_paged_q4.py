@@ -450,3 +450,20 @@ def test_queries_that_are_no_numbers(gctx, hd, heads, M):
             assert np.isnan(got[r]).all()
             np.testing.assert_array_equal(np.delete(got, r, 0), np.delete(want.reshape(-1, hd), r, 0))
     c.free()
+
+
+@pytest.mark.parametrize("qe,ke", [(117, -98), (120, -60), (126, -98), (126, -20), (-126, 110), (-140, 100)])
+@pytest.mark.parametrize("hd,heads,M", [(64, 4, 1), (128, 4, 1), (64, 8, 1), (128, 8, 1), (128, 16, 1), (64, 2, 40), (256, 3, 1)])
+def test_queries_of_every_size(gctx, hd, heads, M, qe, ke):
+    """The largest and smallest queries over rows that are all alike: whatever the score, an
+    output is the mean of the values seen."""
+    rng = np.random.default_rng(qe + 200)
+    k = np.repeat(rng.uniform(-1, 1, (1, 1, hd)).astype(F) * F(2.0 ** ke), 300 + M, 0)
+    v = rng.standard_normal((300 + M, 1, hd)).astype(F)
+    c = Cache(gctx, rng, Q4, hd, 1, heads, [(300, M)], rows=([k], [v]))
+    c.write_new()
+    got = c.attend((rng.uniform(-1, 1, (M, heads * hd)) * 2.0 ** qe).astype(F))
+    want = np.cumsum(stored4(v).astype(np.float64), 0)[300:] / np.arange(301, 301 + M)[:, None, None]
+    # (the weights are alike to a bit: what is left are the sums of six pages, 2^-20 each of the mean |v|)
+    assert (np.abs(got - want) <= 2.0 ** -16 * np.abs(v).max()).all()
+    c.free()

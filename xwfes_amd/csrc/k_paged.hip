@@ -1069,9 +1069,13 @@ __device__ __forceinline__ float across(float x) {
 //   Scores: slot tile st goes to column u = st % U (the others' query is zeros), so
 // that the tiles share their sums' registers and each lane keeps the scores of one
 // tile (two of U = 2): the softmax of a page is 4 (8) weights a lane and not 16.
-// K's operand is the nibbles n = q + 8 as they are, the low bits of halves (n 2^-24),
-// and the sums start at -8 sum q of the block; a slot's multiplier of a block is
-// applied once, to the block's sum.
+// K's operand is the nibbles n = q + 8, bits 4 to 7 of halves (n 2^-20), and the sums
+// start at -8 sum q of the block; a slot's multiplier of a block is applied once, to
+// the block's sum.  A product's sum keeps some 24 bits below the largest that its
+// operands' exponents allow, so a nibble needs its place near the top of a half's bits:
+// as the low bits, 2^-24, with two shifts less for eight dims, outputs are off by
+// 6.8e-6 of their size and not 5.6e-7 (in bits 6 to 9, a shift more, 4.8e-7; 131072
+// slots 35.5, 36.3 and 36.5 us).
 //   Outputs: column u takes the weights times the slots' multipliers of block U j + u
 // and so holds the output dims of its blocks (the others' are not used).  V's
 // operand is signed: a sum over unsigned values less 8 times the weights' would leave
@@ -1081,12 +1085,13 @@ __device__ __forceinline__ float across(float x) {
 // sequences of 16384 slots (8 kv heads of 128, 4 query heads each) 223 us, 5.4 TB/s, which is what loads
 // alone take.  In 16-row tiles, 950 vector instructions a page, one token of 16 sequences over
 // 820 to 8192 slots takes 41.6 us; folded with signed K operands and the multipliers
-// on partial sums, 600 a page, 23.7; as here, 500, 23.5, and longer lists 5 to 10% less.
+// on partial sums, 600 a page, 23.7; as here, 530, 23.5, and longer lists 4 to 8% less.
 // Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256.
 template <int HD, int U>
 struct FoldAttn {
     static constexpr int NB = HD / 32, J = NB > U ? NB / U : 1, NDT = HD / 16, S = 4 / U, NL = HD / 32, OWN = 2 * J;
     static constexpr int64_t VB = paged_values_bytes(HD, PT_Q4), MB = paged_mult_bytes(HD, PT_Q4);
+    static constexpr float NIBBLE = 0x1p-20f;  // what a nibble of K's operand counts
     float bias[NB];  // -8 sum q of the blocks
     v4f o[NDT];
     float off = -INFINITY, l = 0.f, lp = 0.f, c2;
@@ -1103,8 +1108,7 @@ struct FoldAttn {
         return col_max(x);
     }
 
-    // The query row at q, to LDS if `store`.  A nibble n as the low bits of a half is
-    // n 2^-24, four bits up n 2^-20: the dims of the former are taken 2^4 times.
+    // The query row at q, to LDS if `store`
     __device__ __forceinline__ void query(const float* q, int u, int r, int kq, bool vec, bool store, v8h* qs) {
         // (each lane the blocks U j + u; heads of 64 dims have two)
         v4f x[J][2];
@@ -1126,9 +1130,9 @@ struct FoldAttn {
                 a = fabsf(y) <= FLT_BIG ? fmaxf(a, fabsf(y)) : a;
             }
         a = row_top(a);
-        const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 122) : 0;
+        const int e = a > 0.f ? min(max(6 - f_exp(a), -121), 126) : 0;
         const float qs1 = ldexpf(1.f, e);
-        c2 = ldexpf(1.f, 20 - e);
+        c2 = ldexpf(1.f, -e);
         float own[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
@@ -1136,20 +1140,18 @@ struct FoldAttn {
             double sum = 0.0;
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                const float f = i & 2 ? qs1 : 16.f * qs1;
                 v2h hh, ll;
-                split_hl2(rounded(x[j][i >> 2][i & 3] * f), rounded(x[j][i >> 2][(i & 3) + 1] * f), hh, ll);
+                split_hl2(rounded(x[j][i >> 2][i & 3] * qs1), rounded(x[j][i >> 2][(i & 3) + 1] * qs1), hh, ll);
                 h[i] = hh[0];
                 h[i + 1] = hh[1];
                 lo[i] = ll[0];
                 lo[i + 1] = ll[1];
                 // (a half and its rest add up exactly)
-                const float y = ((float)hh[0] + (float)ll[0]) * (i & 2 ? 16.f : 1.f), z = ((float)hh[1] + (float)ll[1]) * (i & 2 ? 16.f : 1.f);
-                sum += (double)y + (double)z;
+                sum += (double)((float)hh[0] + (float)ll[0]) + (double)((float)hh[1] + (float)ll[1]);
             }
             sum += __shfl_xor(sum, 16, 64);
             sum += __shfl_xor(sum, 32, 64);
-            own[j] = (float)(sum * (-8.0 * 0x1p-24));
+            own[j] = (float)(sum * (-8.0 * NIBBLE));
             if (store && any) {
                 const int dc = U * j + u;
                 qs[((dc * 2 + 0) * 4 + kq) * QROWS + r] = h;
@@ -1234,9 +1236,9 @@ struct FoldAttn {
         auto make = [&](int dc) {
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
-                const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1)), w8 = w >> 8;
-                const uint32_t low = in_sgpr(0x000F000Fu), high = in_sgpr(0x00F000F0u);
-                k[dc & 1][st] = __builtin_bit_cast(v8h, uint4{w & low, w & high, w8 & low, w8 & high});
+                const uint32_t w = word(x.u[(dc >> 1) * 2 + (st >> 1)], (st & 1) * 2 + (dc & 1));
+                const uint32_t bits = in_sgpr(0x00F000F0u);
+                k[dc & 1][st] = __builtin_bit_cast(v8h, uint4{w << 4 & bits, w & bits, w >> 4 & bits, w >> 8 & bits});
             }
         };
         make(0);
@@ -1261,7 +1263,7 @@ struct FoldAttn {
                 }
         }
 #pragma unroll
-        for (int a = 0; a < S; ++a) s[a] *= x.s[a];
+        for (int a = 0; a < S; ++a) s[a] = s[a] * (1.f / NIBBLE) * x.s[a];
     }
 
     __device__ __forceinline__ void raise(int en) {

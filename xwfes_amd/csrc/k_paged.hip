@@ -85,7 +85,8 @@ __device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4)
 // tokens of 8 heads of 128, 8-bit: 8.0 us, where the bytes take 4.2 at a copy's
 // rate and a launch that does nothing 2: bound by the latency of a workgroup's
 // one pass, load, maximum, LDS, barrier and store.  A kernel without the image
-// in LDS, its values written a row apart, took 24.
+// in LDS, its values written a row apart, took 24.  4 bits (q4_store_row's, paged_dev.h):
+// 7.7 of 3.9.
 template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* _
 // ---------------------------------------------------------------- read back
 // x = (byte - 128) scale, or half scale.  Bound by HBM, mostly its writes: four
 // contexts of up to 16384 (57138 tokens in all, 8 heads of 128, 8-bit) 120 us,
-// 4.9 TB/s, a large copy's rate.
+// 4.9 TB/s, a large copy's rate; 4 bits 109 us, the same.
 template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_paged_read(PagedView p, int context, float* __restrict__ k, int64_t ldk,
                                                     float* __restrict__ v, int64_t ldv) {
@@ -848,7 +849,14 @@ struct RowSight {
 // Four waves take a part of a list, eight a whole one where that is faster.  For one token a sequence bound by HBM, the pages
 // straight to registers: 16 sequences of 820 to 8192 slots (8-bit, 8 kv heads
 // of 128) 35 us, where a kernel of the loads alone takes 31.4 (5.3 TB/s); one
-// of 131072 (halves) 104 us, the loads alone 104.  (Joining the partials in the
+// of 131072 (halves) 104 us, the loads alone 104.  Of 4 bits, rows that do not fit
+// FoldAttn's columns: 16 sequences of 8 tokens under a window of 4096 (64 dims, 32
+// rows a kv head) 28.3 us a call with the join, 507 vector instructions a page and tile,
+// the vector units busy for 65% of the cycles, the rest the start and the end of short
+// lists; two tiles a wave that share their operands: 64 dims 28.3 ->
+// 26.8, 128 dims 34.3 -> 38.2 (28 registers spilled) and one sequence of 8 tokens 10.8
+// -> 16.1, so not; nibbles as FoldAttn takes them 28.0 -> 27.7 and, with 67 spilled,
+// 33.9 -> 50.4.  (Joining the partials in the
 // last workgroup of a list instead of a launch of their own: the same for
 // short lists, 14 us slower for one of 131072; by fences 60 us slower.)
 template <int HD, int KT, int NW>
@@ -1511,16 +1519,17 @@ typedef __attribute__((address_space(3))) void lds_void;
 // Many rows: workgroup = (item of 128 or 256 rows, kv head), eight waves of one
 // or two tiles of 16 rows, the low halves of the queries in LDS (but for heads
 // of 256 dims, where LDS holds the pages alone and a wave has one tile).
-// Each page goes to LDS as the halves that the operands are (8-bit values
-// converted once, by all waves), one page ahead in the other buffer: halves by
-// direct copies, 8-bit values through registers, their loads issued before the
-// current page's work and written after it.
+// Each page goes to LDS as the halves that the operands are (8- and 4-bit values
+// converted once, by all waves, these under their multipliers), one page ahead in the
+// other buffer: halves by direct copies, the others through registers, their loads
+// issued before the current page's work and written after it.
 // Bound by the SIMDs' issue: queries and weights in two halves make it two
 // products of 16x16x32 for each of the formula's, 16 cycles each; three chunks
 // of 1500 tokens after 1600 to 4000 (8-bit, 128 dims) take 467 us call after
 // call, the CUs busy for 88% of it, in that time products for 48% and other
 // vector instructions for 45% of the SIMDs' cycles (a wave's products run beside
-// another's vector instructions in part).  On the lower clock of a trace, where
+// another's vector instructions in part); 4 bits 513, for whose conversion it issues
+// 7% more vector instructions and twice the loads.  On the lower clock of a trace, where
 // the kernel takes 539 and took 557: one tile a wave reads twice the
 // LDS for a product: 656 us, LDS as busy as the products.  Tried and slower:
 // both tiles' low halves in registers (73 spilled, 680), the waves' halves kept

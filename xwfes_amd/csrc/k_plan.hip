@@ -32,9 +32,9 @@ __global__ void __launch_bounds__(256) k_plan_check(PagedBuild b) {
     if (lane == 0) b.codes[s] = c;
 }
 
-// Threads of a workgroup: the only one has its entries to write as well (us for 16
-// sequences 256: 13.5, 512: 13.1, 1024: 15.5), of several each the sums alone (512
-// sequences 18.0, 19.5)
+// Threads of a workgroup: the only one has its entries to write as well (us a call for
+// 16 sequences 256: 11.6, 512: 10.8, 1024: 12.4), of several each its share (512
+// sequences of 48 new tokens, 128: 18.2, 256: 15.6, 512: 16.3)
 template <bool CHECK>
 constexpr int build_threads() {
     return CHECK ? 512 : 256;
@@ -91,7 +91,9 @@ enum { S_TOK, S_FRESH, S_TOUCH, S_FEW, S_MANY, S_PART, S_COMB, N_SUMS };
 // looks at the tables too, where they are short: a launch less.  Bound by latency,
 // lengths, tables, list and entries one after the other: two exchanges between
 // the waves, the first of totals (how lists are cut follows from them), the second
-// of running sums and what the list of pages holds.
+// of running sums and what the list of pages holds.  16 sequences: 9.5 us of kernel
+// for 370 bytes, 730 vector instructions a wave; sums by one wave, with 40
+// instructions a division, 23.8.  512 sequences of 48 tokens: 4.1 and 14.2 us.
 template <bool CHECK>
 __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuild b) {
     constexpr int NT = build_threads<CHECK>(), NW = NT / 64;
@@ -106,7 +108,7 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
     int* const sums = M + n;   // [N_SUMS][n1] (CHECK: first have, s and a of seq_held)
     const int per = (n + NT - 1) / NT, s0 = min(tid * per, n), s1 = min(s0 + per, n);
     // waves that have sequences form their sums, the others wait: all would share the
-    // SIMDs (16 sequences, sixteen waves that all form sums: 13.3 us)
+    // SIMDs
     const bool busy = __builtin_amdgcn_readfirstlane(w) * 64 * per < n;
     // The first loads, none of which waits for another: the lengths, the first
     // table entries whether they are pages or not, and (next) the list from `used` on

@@ -1106,8 +1106,9 @@ struct FoldAttn {
     int ev = EV_MIN;
     // the query's halves in LDS, [block][high, low][kq][row], and as many zeros behind
     // them, which the lanes of the other slot tiles read
-    static constexpr int QROWS = 16 / U, QN = NB * 2 * 4 * QROWS;
-    typedef v8h Query[2 * QN];
+    // (in the banks beside those of the same lanes' halves)
+    static constexpr int QROWS = 16 / U, QN = NB * 2 * 4 * QROWS, QZ = QN + QROWS;
+    typedef v8h Query[QN + QZ];
 
     // the largest of a row's lanes
     static __device__ __forceinline__ float row_top(float x) {
@@ -1179,7 +1180,7 @@ struct FoldAttn {
             share(std::integral_constant<int, 3>{});
         }
         if (store)
-            for (int i = threadIdx.x & 63; i < QN; i += 64) qs[QN + i] = v8h{};
+            for (int i = threadIdx.x & 63; i < QZ; i += 64) qs[QN + i] = v8h{};
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[dt] = v4f{0.f, 0.f, 0.f, 0.f};
     }
@@ -1430,7 +1431,7 @@ __global__ void __launch_bounds__(64 * NW, 2) k_paged_fold(PagedAttn a) {
     wa.query(a.q + tok * a.ldq + (int64_t)head * HD, u, rr, kq, !(((uintptr_t)a.q | (uintptr_t)(a.ldq * 4)) & 15), w == 0, qs);
     int at[U];  // slot tile st's query: the lane's row, or zeros
 #pragma unroll
-    for (int x = 0; x < U; ++x) at[x] = kq * W::QROWS + rr + (x == u ? 0 : W::QN);
+    for (int x = 0; x < U; ++x) at[x] = kq * W::QROWS + rr + (x == u ? 0 : W::QZ);
     __syncthreads();
     const RowSight sight(a, sq, t);
     int hi = sight.hi, lo = sight.lo;

@@ -467,3 +467,27 @@ def test_queries_of_every_size(gctx, hd, heads, M, qe, ke):
     # (the weights are alike to a bit: what is left are the sums of six pages, 2^-20 each of the mean |v|)
     assert (np.abs(got - want) <= 2.0 ** -16 * np.abs(v).max()).all()
     c.free()
+
+
+@pytest.mark.parametrize("hd,kv,heads", [(64, 2, 8), (128, 2, 8), (128, 1, 8), (64, 1, 1)])
+def test_scores_of_two_slots(gctx, hd, kv, heads):
+    """Two slots, where an output is off by what a score is.  Query elements of 2^6 to 2^7
+    times nibbles of up to 15 2^-20 keep 24 bits below 2^7 2^-14, 2^-18 |q|max of a nibble's unit a
+    product; a block's sum |q_i| max |k| is some 32 / 3 |q|max times 7 units, so that its two
+    products and the sums in fp32 stay below 2^-22 of it."""
+    rng = np.random.default_rng(hd + heads)
+    c = Cache(gctx, rng, Q4, hd, kv, heads, [(1, 1)] * 200)
+    c.write_new()
+    q = queries(rng, c)
+    got = c.attend(q).reshape(200, kv, heads // kv, hd)
+    q64 = np.asarray(q, np.float64).reshape(200, kv, heads // kv, hd) / np.sqrt(hd)
+    k, v = (np.stack([stored4(x) for x in y]).astype(np.float64) for y in (c.k, c.v))  # [200][2 slots][kv][hd]
+    s = np.einsum("skhd,sjkd->skhj", q64, k)
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    big = np.repeat(np.abs(k).reshape(200, 2, kv, hd // 32, 32).max(-1), 32, -1)
+    mag = np.einsum("skhd,sjkd->skhj", np.abs(q64), big).max(-1)[..., None]
+    err = np.abs(got - np.einsum("skhj,sjkd->skhd", p, v))
+    tol = (np.expm1(2 * 2.0 ** -22 * mag) + 2.0 ** -20 + 5 * 2.0 ** -23) * np.einsum("skhj,sjkd->skhd", p, np.abs(v))
+    assert (err <= tol).all(), (err - tol).max()
+    c.free()

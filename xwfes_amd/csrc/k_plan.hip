@@ -12,7 +12,7 @@ __device__ __forceinline__ int check_seq(const PagedBuild& b, int s, int lane) {
     const SeqLoad l = seq_load(b.r, b.ldt, p, m);
     if (l.code) return l.code;
     int hs, ha;
-    seq_held(b.r, p, l.have, hs, ha);
+    seq_held(b.r, p, m, l.have, hs, ha);
     const int32_t* from = b.tables + s * b.ldt;
     int32_t* to = b.table + (int64_t)s * b.r.n_pages;
     bool bad = false;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
         if constexpr (CHECK) {
             const SeqLoad l = seq_load(r, b.ldt, P[s], M[s]);
             int hs = 0, ha = 0;
-            if (!l.code) seq_held(r, P[s], l.have, hs, ha);
+            if (!l.code) seq_held(r, P[s], M[s], l.have, hs, ha);
             sums[s] = l.have;  // (0 with a code: nothing to look at)
             sums[n1 + s] = hs;
             sums[2 * n1 + s] = ha;

@@ -51,11 +51,16 @@ __host__ __device__ inline SeqLoad seq_load(const PagedRoom& r, int64_t ldt, int
     return l;
 }
 // Pages below have that have to be pages of the pool: [0, s) and [a, have).
-// Under a window those between are not read
-__host__ __device__ inline void seq_held(const PagedRoom& r, int p, int have, int& s, int& a) {
+// Under a window those between are not read, nor any of a sequence without new
+// tokens (contexts are not read back then)
+__host__ __device__ inline void seq_held(const PagedRoom& r, int p, int m, int have, int& s, int& a) {
     s = 0;
     a = 0;
     if (!r.window) return;
+    if (m == 0) {
+        a = have;
+        return;
+    }
     a = p - r.window + 1 > 0 ? (p - r.window + 1) / FTX_PAGE : 0;
     s = (int)(((int64_t)r.sinks + FTX_PAGE - 1) / FTX_PAGE);
     s = s < a ? s : a;

@@ -110,7 +110,9 @@ int ftx_destroy(ftx_ctx* ctx);
 int ftx_device_info(ftx_ctx* ctx, ftx_device_info_t* out);
 const char* ftx_last_error(ftx_ctx* ctx);
 /* Enqueue all following work on `stream` (a hipStream_t; NULL = the
- * context's own stream). */
+ * context's own stream).  A stream that a plan of ftx_plan_create_device was
+ * built or called on has to live until the context leaves it (left while it is
+ * being captured: until that plan's next build or call). */
 int ftx_set_stream(ftx_ctx* ctx, void* stream);
 int ftx_sync(ftx_ctx* ctx);
 
@@ -465,7 +467,8 @@ typedef struct {
  * its own; contexts are read back only without a window, k and v then as
  * long as the lengths say.  A call that is recorded into a graph needs the build before
  * it in the same capture, on the same stream (FTX_E_INVALID); an eager build or call on another
- * stream than the plan's last one waits for the device.  Graphs and eager calls of one plan
+ * stream than the plan's last one waits there for what the plan has on that one, and is refused while that one
+ * is being captured and was left so (FTX_E_INVALID).  Graphs and eager calls of one plan
  * must not overlap. */
 int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a);
 

@@ -147,6 +147,8 @@ int ftx_destroy(ftx_ctx* ctx) {
     if (ctx->ws) (void)hipFree(ctx->ws);
     if (ctx->pinned) (void)hipHostFree(ctx->pinned);
     for (hipEvent_t e : ctx->events) (void)hipEventDestroy(e);
+    if (ctx->mark) (void)hipEventDestroy(ctx->mark);
+    if (ctx->marks) (void)hipStreamDestroy(ctx->marks);
     if (ctx->own_stream) (void)hipStreamDestroy(ctx->own_stream);
     delete ctx;
     return FTX_OK;
@@ -169,7 +171,9 @@ const char* ftx_last_error(ftx_ctx* ctx) { return ctx ? ctx->err.c_str() : "no c
 
 int ftx_set_stream(ftx_ctx* ctx, void* stream) {
     if (!ctx) return FTX_E_INVALID;
-    ctx->stream = stream ? (hipStream_t)stream : ctx->own_stream;
+    hipStream_t st = stream ? (hipStream_t)stream : ctx->own_stream;
+    if (st != ctx->stream) paged_leave(ctx);
+    ctx->stream = st;
     return FTX_OK;
 }
 

@@ -77,6 +77,8 @@ inline hipError_t lds_limit(const void* kern, size_t bytes, std::atomic<uint64_t
     return e;
 }
 
+struct ftx_plan;
+
 struct ftx_ctx {
     int device = 0;
     // trace: events around launches, resolved by ftx_trace_read
@@ -108,7 +110,17 @@ struct ftx_ctx {
     // device address of the no-allocation entry points' scratch array on
     // this context's device
     float* noalloc_scratch = nullptr;
+    // plans whose steps are built on the GPU, a stream on which nothing waits but
+    // the marks of their work on streams that the context has left, and an event
+    // between the two (paged_leave)
+    std::vector<ftx_plan*> built;
+    hipStream_t marks = nullptr;
+    hipEvent_t mark = nullptr;
 };
+
+// Ahead of another stream of the context's: what its plans built on the GPU have
+// enqueued is marked (paged.hip)
+void paged_leave(ftx_ctx* ctx);
 
 struct ftx_tensor {
     ftx_ctx* ctx = nullptr;

@@ -555,9 +555,17 @@ struct ftx_plan {
     size_t o_touch = 0, o_code = 0;
     unsigned long long capture = 0;
     hipStream_t capture_stream = nullptr;
+    // behind its eager work on `stream`, from when the context leaves that stream
+    // (after every build it would take 3 us on the device); marked: it is, and
+    // there is no work since
+    hipEvent_t left = nullptr;
+    bool marked = false;
 };
 
 static void plan_release(ftx_plan* pl) {
+    auto& built = pl->ctx->built;
+    built.erase(std::remove(built.begin(), built.end(), pl), built.end());
+    if (pl->left) (void)hipEventDestroy(pl->left);
     if (pl->dev) (void)hipFree(pl->dev);
     if (pl->part) (void)hipFree(pl->part);
     for (int i = 0; i < ftx_plan::RING; ++i) {
@@ -683,17 +691,51 @@ static hipError_t tables_landed(const ftx_plan* pl) {
     return e;
 }
 
+// The plan's event behind its work on its stream, by way of a stream that is never
+// captured: HIP refuses to wait for an event whose stream is being captured, also
+// where it was recorded before.  (Nor is the left stream needed any more.)
+static hipError_t plan_mark(ftx_plan* pl) {
+    ftx_ctx* ctx = pl->ctx;
+    hipError_t e = hipEventRecord(ctx->mark, pl->stream);
+    if (e == hipSuccess) e = hipStreamWaitEvent(ctx->marks, ctx->mark, 0);
+    if (e == hipSuccess) e = hipEventRecord(pl->left, ctx->marks);
+    pl->marked = e == hipSuccess;
+    return e;
+}
+
+void paged_leave(ftx_ctx* ctx) {
+    for (ftx_plan* pl : ctx->built)
+        if (pl->stream == ctx->stream && !pl->marked && !capturing(ctx->stream) && plan_mark(pl) != hipSuccess)
+            (void)hipGetLastError();
+}
+
+// An eager build or call of a plan built on the GPU: behind what the plan has on
+// the stream that it was on.  By an event and not by the host: other streams go
+// on, and one that is being captured stays as it is
+static int plan_follow(ftx_plan* pl) {
+    ftx_ctx* ctx = pl->ctx;
+    if (pl->stream != ctx->stream) {
+        if (!pl->marked) {  // (left while it was being captured)
+            if (capturing(pl->stream))
+                return ftx_fail(ctx, FTX_E_INVALID, "plan: the stream of its last call is being captured");
+            FTX_HIP(ctx, plan_mark(pl));
+        }
+        FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->left, 0));
+        pl->stream = ctx->stream;
+    }
+    pl->marked = false;
+    return FTX_OK;
+}
+
 // the tables' copy ahead of a call on another stream than its own, and of a
 // captured one on any: the copy is not in the graph, which may be launched on
 // another stream than the captured one, so the host waits
 static int plan_order(ftx_plan* pl) {
     ftx_ctx* ctx = pl->ctx;
     if (!capturing(ctx->stream)) {
+        if (pl->device) return plan_follow(pl);
         if (ctx->stream == pl->stream) return FTX_OK;
-        if (pl->device)  // (an event after every build would take 3 us on the device)
-            FTX_HIP(ctx, hipDeviceSynchronize());
-        else
-            FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
+        FTX_HIP(ctx, hipStreamWaitEvent(ctx->stream, pl->up, 0));
         pl->stream = ctx->stream;
         return FTX_OK;
     }
@@ -897,6 +939,7 @@ int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room,
         pl->ctx = ctx;
         pl->pool = p;
         ++p->users;
+        ctx->built.push_back(pl);
         pl->device = true;
         pl->room = r;
         PagedTables& t = pl->t;
@@ -944,6 +987,13 @@ int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room,
             (void)hipGetLastError();
             plan_release(pl);
             return ftx_fail(ctx, FTX_E_DEVICE, "plan: clearing failed");
+        }
+        if (hipEventCreateWithFlags(&pl->left, hipEventDisableTiming) != hipSuccess ||
+            (!ctx->mark && hipEventCreateWithFlags(&ctx->mark, hipEventDisableTiming) != hipSuccess) ||
+            (!ctx->marks && hipStreamCreateWithFlags(&ctx->marks, hipStreamNonBlocking) != hipSuccess)) {
+            (void)hipGetLastError();
+            plan_release(pl);
+            return ftx_fail(ctx, FTX_E_DEVICE, "plan: its events could not be created");
         }
         pl->stream = ctx->stream;
         pl->ready = true;
@@ -999,7 +1049,8 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     if (cap && pl->capture && pl->capture_stream != st && pl->capture == capture_id(st))
         return ftx_fail(ctx, FTX_E_INVALID, "plan: built on another stream in this capture");
     // (calls of the plan on another stream may still read its tables)
-    if (!cap && pl->stream != st) FTX_HIP(ctx, hipDeviceSynchronize());
+    const int rc = cap ? FTX_OK : plan_follow(pl);
+    if (rc) return rc;
     PagedBuild b{};
     b.r = r;
     b.nseq = (int)a->nseq;
@@ -1028,9 +1079,7 @@ int ftx_plan_build(ftx_plan* pl, const ftx_build_args* a) {
     if (cap) {
         pl->capture = capture_id(st);
         pl->capture_stream = st;
-        return FTX_OK;
     }
-    pl->stream = st;
     return FTX_OK;
 }
 

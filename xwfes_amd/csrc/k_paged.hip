@@ -1909,7 +1909,8 @@ static auto attn_wide() {
     return k_paged_attn<HD, KT, HD <= 128 ? 8 : 4>;
 }
 
-// of 4-bit rows and heads of 64 or 128 dims, by the most query rows of a sequence
+// of 4-bit rows and heads of 64 or 128 dims, by the most query rows of a sequence that
+// has few (a chunk in the same step goes to the kernel of many)
 typedef void (*paged_kernel)(PagedAttn);
 template <int U, int NW>
 static paged_kernel fold_hd(int hd) {
@@ -1927,7 +1928,7 @@ hipError_t launch_paged_attention(hipStream_t st, const PagedAttn& a) {
     if (e != hipSuccess) return e;
     if (a.n_few) {
         const dim3 grid((unsigned)a.n_few * (unsigned)a.p.n_kv);
-        auto* fold = a.p.kt != PT_Q4 || a.p.hd == 256 ? nullptr : fold_of(a.rows_max, a.p.hd, a.wide);
+        auto* fold = a.p.kt != PT_Q4 || a.p.hd == 256 ? nullptr : fold_of(a.few_rows, a.p.hd, a.wide);
         if (fold)
             ktimed_launch(fold, grid, dim3(a.wide ? 512 : 256), 0, st, a);
         else if (a.wide)

@@ -276,6 +276,7 @@ int paged_tables(const PagedGeom& g, const ftx_plan_args& a, std::vector<uint32_
     const Few few = few_plan(tiles[0]);
     per[0] = few.per;
     o.wide = few.wide;
+    for (const Tile& t : tiles[0]) o.few_rows = std::max(o.few_rows, o.seqs[(size_t)t.seq].M * gqa);
     o.pages_read = 0;
     for (int many = 0; many < 2; ++many) {
         for (const Tile& t : tiles[many]) {
@@ -953,6 +954,8 @@ int ftx_plan_create_device(ftx_ctx* ctx, ftx_pool* p, const ftx_plan_room* room,
         t.rows = (int64_t)r.nseq * r.n_pages * FTX_PAGE;
         t.parts = r.parts;
         t.few = r.few;
+        // (the room's, not a step's: what k_paged_fold holds is known before a build)
+        t.few_rows = std::min<int64_t>((int64_t)r.most * r.gqa, PAGED_MANY - 1);
         t.wide = r.wide;
         // (a list of n pages is cut into parts of 4 and more)
         t.comb_max = ((int64_t)r.n_pages + 1) / 2;
@@ -1179,6 +1182,7 @@ int paged_attend_rows(ftx_plan* pl, int64_t layer, const float* q, int64_t ldq, 
     a.wide = t.wide;
     a.gqa = (int)(t.n_head / p->n_kv);
     a.rows_max = (int)(t.longest * a.gqa);
+    a.few_rows = (int)t.few_rows;
     a.comb_max = (int)std::min<int64_t>(t.comb_max, INT32_MAX);
     a.window = (int)t.window;
     a.sinks = (int)t.sinks;

@@ -39,7 +39,14 @@ template <bool CHECK>
 constexpr int build_threads() {
     return CHECK ? 512 : 256;
 }
-constexpr int ONE_MOST = 6144;  // table entries (and others) of a build by one workgroup
+// The most sequences, table entries and other entries of a build by one workgroup, which
+// looks at the tables itself.  One / several and the launch before, us in a graph, heads 8 a pool
+// if not said: sequences of some 100 pages 16 8.9 / 10.2, 32 9.5 / 10.4, 48 10.1 / 10.0, 64
+// 10.3 / 9.6; of 63 64 9.3 / 9.4, 96 11.0 / 10.7, 128 11.8 / 10.7; of 16 192 14.5 / 11.7, 256 16.8 /
+// 12.2; of 8 512 27.4 / 14.4; 16 sequences with 5008 table entries 9.6 / 10.0, 7504 10.4 / 10.3; with
+// 1206 other entries 9.9 / 11.0, 2097 10.5 / 10.9, 3374 12.2 / 11.1 (one kv head, whose lists are
+// cut finest, 1072 10.8 / 10.7, 1280 12.5 / 10.8)
+constexpr int ONE_SEQS = 64, ONE_TABLE = 6144, ONE_ENTRIES = 2048;
 
 // Between the waves' uses of LDS: what is on its way to global memory is not
 // waited for (the stores, which no other wave reads)
@@ -407,16 +414,15 @@ __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuil
 }  // namespace
 
 hipError_t paged_build_limits() {
-    static std::atomic<uint64_t> set_one{0}, set_many{0};
-    const size_t most = (size_t)(PAGED_ROOM_SEQS + 1) * (8 + 4 * N_SUMS);
-    const hipError_t e = lds_limit((const void*)k_plan_build<true>, most, set_one);
-    return e != hipSuccess ? e : lds_limit((const void*)k_plan_build<false>, most, set_many);
+    // (k_plan_build<true>, of ONE_SEQS sequences, needs no limit set)
+    static std::atomic<uint64_t> set{0};
+    return lds_limit((const void*)k_plan_build<false>, (size_t)(PAGED_ROOM_SEQS + 1) * (8 + 4 * N_SUMS), set);
 }
 
 hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b) {
     const PagedRoom& r = b.r;
     const int64_t entries = (int64_t)r.tokens + r.nseq + r.touch + r.few + r.many + r.combs;
-    const bool one = (int64_t)b.nseq * r.n_pages <= ONE_MOST && entries <= ONE_MOST;
+    const bool one = b.nseq <= ONE_SEQS && (int64_t)b.nseq * r.n_pages <= ONE_TABLE && entries <= ONE_ENTRIES;
     const size_t bytes = (size_t)(b.nseq + 1) * (8 + 4 * N_SUMS);
     if (one) {
         hipLaunchKernelGGL(k_plan_build<true>, dim3(1), dim3(build_threads<true>()), bytes, st, b);

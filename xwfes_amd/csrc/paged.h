@@ -168,7 +168,7 @@ struct PagedBuild {
     int32_t* codes;    // [r.nseq]: what the first kernel says of each sequence, then the pages used before
 };
 hipError_t launch_paged_build(hipStream_t st, const PagedBuild& b);
-// its kernels' LDS on the current device, before the first
+// its kernel's LDS on the current device, before the first
 hipError_t paged_build_limits();
 
 // The same lists for plain arrays, no context and no device: items (r.few + r.many

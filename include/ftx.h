@@ -423,7 +423,12 @@ int ftx_plan_free(ftx_plan* pl);
 /* A plan whose steps are built on the GPU, from lengths and tables that the GPU
  * holds: nothing of a step passes the host, so that a loop of steps is one
  * stream's work, or one HIP graph replayed.  `room` is what it has room for; its
- * launches cover the room, so keep it near the steps' sizes.  Chains only.
+ * launches cover the room, and its kernels are chosen by it, so keep it near the
+ * steps' sizes: of FTX_KV_Q4 rows, room.M n_head / n_head_kv <= 8 takes the fastest
+ * for single tokens (heads of 64 and 128 dims).  Query rows of a kv head go in tiles
+ * of 16, of sequences with more than 64 in tiles of 128, where plans set from the host
+ * choose 16, 128 or 256 by the step: chunks take up to twice as long, least over
+ * long contexts that fill the chip.  Chains only.
  * Until a build the plan holds no tokens. */
 typedef struct {
     int64_t nseq;     /* 1 .. 4096 sequences */

@@ -1094,7 +1094,9 @@ __device__ __forceinline__ float across(float x) {
 // alone take.  In 16-row tiles, 950 vector instructions a page, one token of 16 sequences over
 // 820 to 8192 slots takes 41.6 us; folded with signed K operands and the multipliers
 // on partial sums, 600 a page, 23.7; as here, 530, 23.5, and longer lists 4 to 8% less.
-// Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256.
+// Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256, rounded by
+// their scale and again by their multiplier (2^-24 each, where WaveAttn's integers are
+// the products): one rounding more of the some 2^-21 that an output is off by.
 template <int HD, int U>
 struct FoldAttn {
     static constexpr int NB = HD / 32, J = NB > U ? NB / U : 1, NDT = HD / 16, S = 4 / U, NL = HD / 32, OWN = 2 * J;

@@ -81,7 +81,14 @@ __host__ __device__ inline int seq_per(int total, int cut, int least) {
 // that gives at most `slots` parts; else what is left of a round for each page, or
 // half a round where that is less (long lists among many short ones).  16 sequences
 // over 820 to 8192 slots of 4 bits 25.2 us, by four workgroups a CU, in rounds, 30.1;
-// one over 131072 38.6 and 43.9; 64 over up to 2000, whole, 24.4, cut 32
+// one over 131072 38.6 and 43.9; 64 over up to 2000, whole, 24.4, cut 32.  Lists of more
+// rows, by this and by that rule: 16 sequences of 8 tokens, 32 rows a kv head, over 820 to
+// 8192 49.4 / 55.0 (64 dims 32.8 / 34.0, under a window of 4096 28.3 / 27.5), one of 8 over
+// 2048 11.4 / 11.4, over 16384 19.6 / 25.8, 4 of 16 29.1 / 39.0, 64 of 4 over up to 2000 29.2 /
+// 37.4.  Of heads of 256 dims a CU takes one workgroup at a time (453 registers), so that
+// this fills two rounds: this rule / slots for one a CU / that rule 16 of one token (16 query
+// heads over 8) 64 / 64 / 98, 32 over up to 4000 60 / 72 / 87, 16 of 8 (32 over 8) 104 / 136 /
+// 139, but one over 8192 26 / 20 / 26, 4 over 8192 43 / 32 / 64, one of 8 36 / 24 / 40
 constexpr int FEW_TRIES = 3;
 __host__ __device__ inline int try_per(int total, int slots, int lists, int k) {
     const int left = slots - (int)((int64_t)lists * (k + 1) / (FEW_TRIES + 1));
@@ -140,6 +147,9 @@ __host__ __device__ inline PagedItem seq_item(const PagedRoom& r, const PagedSeq
     it.i0 = k * len + (k < rem ? k : rem);
     it.i1 = it.i0 + len + (k < rem);
     it.part = np > 1 ? part0 + e * (tr / PAGED_TR) : -1;
+    // (one row tile a wave: the host's choice of 16, 128 or 256 rows follows from an estimate
+    // over all lists.  Chunks of 64 tokens over 300, 4000, 8-bit, 32 query heads over 8: 18.5
+    // and 48.2 us, by the host's plan 9.6 and 23.3; three of 1500 each over 1600 to 4000 686 and 644)
     it.nt = many;
     it.q = q;
     return it;

@@ -44,9 +44,9 @@ constexpr int build_threads() {
 // if not said: sequences of some 100 pages 16 8.9 / 10.2, 32 9.5 / 10.4, 48 10.1 / 10.0, 64
 // 10.3 / 9.6; of 63 64 9.3 / 9.4, 96 11.0 / 10.7, 128 11.8 / 10.7; of 16 192 14.5 / 11.7, 256 16.8 /
 // 12.2; of 8 512 27.4 / 14.4; 16 sequences with 5008 table entries 9.6 / 10.0, 7504 10.4 / 10.3; with
-// 1206 other entries 9.9 / 11.0, 2097 10.5 / 10.9, 3374 12.2 / 11.1 (one kv head, whose lists are
-// cut finest, 1072 10.8 / 10.7, 1280 12.5 / 10.8)
-constexpr int ONE_SEQS = 64, ONE_TABLE = 6144, ONE_ENTRIES = 2048;
+// 1206 other entries 9.9 / 11.0, 2097 10.3 / 11.1, 3374 12.2 / 11.1, one with 1709 9.2 / 9.8, 2709
+// 10.0 / 9.8 (one kv head, whose lists are cut finest, 16 with 1072 10.8 / 10.7, 64 with 1280 12.5 / 10.8)
+constexpr int ONE_SEQS = 64, ONE_TABLE = 6144, ONE_ENTRIES = 2560;
 
 // Between the waves' uses of LDS: what is on its way to global memory is not
 // waited for (the stores, which no other wave reads)

@@ -86,7 +86,7 @@ __device__ __forceinline__ int image_at(int byte) { return image_unit(byte >> 4)
 // rate and a launch that does nothing 2: bound by the latency of a workgroup's
 // one pass, load, maximum, LDS, barrier and store.  A kernel without the image
 // in LDS, its values written a row apart, took 24.  4 bits (q4_store_row's, paged_dev.h):
-// 7.7 of 3.9.
+// 9.2 of 3.9.
 template <int HD, int KT>
 __global__ void __launch_bounds__(256) k_paged_write(PagedView p, const float* __restrict__ k, int64_t ldk,
                                                      const float* __restrict__ v, int64_t ldv) {
@@ -1094,9 +1094,9 @@ __device__ __forceinline__ float across(float x) {
 // alone take.  In 16-row tiles, 950 vector instructions a page, one token of 16 sequences over
 // 820 to 8192 slots takes 41.6 us; folded with signed K operands and the multipliers
 // on partial sums, 600 a page, 23.7; as here, 530, 23.5, and longer lists 4 to 8% less.
-// Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256, rounded by
-// their scale and again by their multiplier (2^-24 each, where WaveAttn's integers are
-// the products): one rounding more of the some 2^-21 that an output is off by.
+// Sums, offsets and V levels as in WaveAttn; weights are taken times c / 256, rounded
+// with the scale and again with the multiplier (WaveAttn's once: its operands are the
+// integers q c): 2^-24 more beside the 2^-22 of their two halves.
 template <int HD, int U>
 struct FoldAttn {
     static constexpr int NB = HD / 32, J = NB > U ? NB / U : 1, NDT = HD / 16, S = 4 / U, NL = HD / 32, OWN = 2 * J;

@@ -98,9 +98,9 @@ enum { S_TOK, S_FRESH, S_TOUCH, S_FEW, S_MANY, S_PART, S_COMB, N_SUMS };
 // looks at the tables too, where they are short: a launch less.  Bound by latency,
 // lengths, tables, list and entries one after the other: two exchanges between
 // the waves, the first of totals (how lists are cut follows from them), the second
-// of running sums and what the list of pages holds.  16 sequences: 9.5 us of kernel
-// for 370 bytes, 730 vector instructions a wave; sums by one wave, with 40
-// instructions a division, 23.8.  512 sequences of 48 tokens: 4.1 and 14.2 us.
+// of running sums and what the list of pages holds.  16 sequences: 11.8 us of kernel
+// for 370 bytes (10.7 a build in a graph), 730 vector instructions a wave; sums by one
+// wave, with 40 instructions a division, 23.8.  512 sequences of 48 tokens: 4.0 and 13.3 us.
 template <bool CHECK>
 __global__ void __launch_bounds__(build_threads<CHECK>()) k_plan_build(PagedBuild b) {
     constexpr int NT = build_threads<CHECK>(), NW = NT / 64;
